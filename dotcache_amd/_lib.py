@@ -54,6 +54,24 @@ class MergeItem(C.Structure):
     _fields_ = [("seq", C.c_int32), ("kv_head", C.c_int32), ("partial_begin", C.c_int32), ("count", C.c_int32)]
 
 
+class TokenRows(C.Structure):
+    _fields_ = [("data", C.c_void_p), ("token_stride", C.c_int64), ("head_stride", C.c_int64), ("n_heads", C.c_int32),
+                ("dtype", C.c_int32)]
+
+
+class Norm(C.Structure):
+    _fields_ = [("weight", C.c_void_p), ("dtype", C.c_int32), ("head_stride", C.c_int32), ("eps", C.c_float)]
+
+
+class Rotary(C.Structure):
+    _fields_ = [("table", C.c_void_p), ("n_positions", C.c_int32), ("rotary_dim", C.c_int32), ("interleaved", C.c_int32)]
+
+
+class TokenDest(C.Structure):
+    _fields_ = [("k_pages", C.c_void_p), ("v_pages", C.c_void_p), ("row", C.c_void_p), ("token", C.c_void_p),
+                ("n_rows", C.c_int32), ("n_pages", C.c_int32), ("page_tokens", C.c_int32)]
+
+
 assert C.sizeof(PageDesc) == 8 and C.sizeof(WorkItem) == 32 and C.sizeof(MergeItem) == 16
 
 # name -> (restype, argtypes); this table is also the list of exported
@@ -72,6 +90,12 @@ SIGNATURES = {
     "dc_encode_streams_kv": (C.c_int, [C.c_void_p, C.c_void_p, C.c_int32, C.c_int32, C.c_int32, C.c_int64, C.c_void_p,
                                        C.c_void_p, C.c_int32, C.c_int32, C.c_int32, Pool, Pool, C.c_void_p, C.c_void_p,
                                        C.c_int32, C.c_void_p]),
+    "dc_norm_rotate": (C.c_int, [C.c_int64, C.c_int32, C.c_void_p, Rotary, TokenRows, Norm, TokenRows, TokenRows, Norm,
+                                 TokenRows, C.c_void_p]),
+    "dc_append_rotary": (C.c_int, [C.c_int64, C.c_void_p, Rotary, TokenRows, Norm, TokenRows, TokenRows, Norm, TokenRows,
+                                   TokenDest, Pool, Pool, C.c_void_p, C.c_void_p, C.c_void_p, C.c_int32, C.c_int32,
+                                   C.c_void_p]),
+    "dc_read_tokens": (C.c_int, [C.c_int64, TokenDest, Pool, Pool, TokenRows, TokenRows, C.c_void_p]),
     "dc_set_encode_path": (C.c_int, [C.c_int32]),
     "dc_score_pages": (C.c_int, [Pool, C.c_void_p, C.c_void_p, C.c_int32, C.c_void_p, C.c_int32, C.c_void_p, C.c_int64, C.c_void_p]),
     "dc_mix_pages": (C.c_int, [Pool, C.c_void_p, C.c_void_p, C.c_int32, C.c_void_p, C.c_int32, C.c_int64, C.c_void_p, C.c_int32, C.c_void_p]),

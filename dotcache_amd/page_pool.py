@@ -88,6 +88,20 @@ def current_stream_ptr() -> int:
     return int(_torch().cuda.current_stream().cuda_stream)
 
 
+def call_on(device, fn, what: str, *args) -> None:
+    """``fn(*args, stream)`` on the current stream of the tensors' device
+    (which need not be the current device), its status checked."""
+    cuda = _torch().cuda
+    if device.type != "cuda":
+        raise ValueError(f"{what}: tensors must be on a GPU")
+    if device.index == cuda.current_device():
+        st = fn(*args, current_stream_ptr())
+    else:
+        with cuda.device(device):
+            st = fn(*args, current_stream_ptr())
+    _lib.check(st, what)
+
+
 @dataclass(frozen=True)
 class PoolGeometry:
     head_dim: int
@@ -602,6 +616,116 @@ class DevicePagePool:
             self.c_pool(), v_pool.c_pool(), C.c_void_p(keep[0].data_ptr() if keep else 0),
             C.c_void_p(keep[1].data_ptr() if keep else 0), int(keep_from), C.c_void_p(current_stream_ptr()))
         _lib.check(st, "dc_encode_streams_kv")
+
+    # ---- new tokens by page table -------------------------------------------
+    def _token_dest(self, v_pool: "DevicePagePool", tables, row, token):
+        """``dc_token_dest`` of page tables ``[2, rows, heads, pages]`` and
+        each token's row and index, and the tensors it points into."""
+        from .rotary import index_tensor
+
+        torch = _torch()
+        g, vg = self.geometry, v_pool.geometry
+        if (vg.head_dim, vg.page_capacity) != (g.head_dim, g.page_capacity):
+            raise ValueError("key and value pools must share head_dim and page_capacity")
+        device = self.arena.device
+        if v_pool.arena.device != device or tables.device != device:
+            raise ValueError(f"pools and tables must be on {device}")
+        if tables.dtype != torch.int32 or tables.dim() != 4 or tables.shape[0] != 2 or not tables.is_contiguous():
+            raise ValueError("tables must be contiguous int32 [2, rows, heads, pages]")
+        _, R, H, W = tables.shape
+        if R == 0 or H == 0 or W == 0:
+            raise ValueError("tables must name at least one page")
+        row = index_tensor(row, "row", len(row), device)
+        token = index_tensor(token, "token", int(row.shape[0]), device)
+        at = tables.data_ptr()
+        dest = _lib.TokenDest(at, at + 4 * R * H * W, row.data_ptr(), token.data_ptr(), R, W, g.page_capacity)
+        return dest, (row, token)
+
+    def append_rotary_with(self, v_pool: "DevicePagePool", queries, keys, values, positions, rotary, tables, row, token, *,
+                           q_weight=None, k_weight=None, eps: float = 1e-6, keep=None, out=None):
+        """New tokens of a layer in one launch (``dc_append_rotary``): queries
+        ``[T, Hq, hd]`` (or None) normed and rotated to the returned tensor,
+        keys ``[T, H, hd]`` normed, rotated and encoded into this pool, values
+        ``[T, H, hd]`` encoded into ``v_pool``, all token-major with any token
+        and head stride.
+
+        Token t of head h goes to slot ``token[t] % capacity`` of page
+        ``tables[kind, row[t], h, token[t] // capacity]`` (int32 device
+        tables ``[2, rows, heads, pages]``, keys first; ``row`` and ``token``
+        int32 or int64 per token): a row is a sequence of a page table, or a
+        block of a block cache.  No two tokens of a call may share a slot.  A
+        token < 0 (padding), an index outside the table or a page id that the
+        pool does not hold is not written; its query row is still made.
+        ``positions``, ``rotary``, ``q_weight``, ``k_weight`` and ``eps`` as in
+        :func:`~dotcache_amd.rotary.norm_rotate`.
+
+        ``keep = (k_rows, v_rows, row, head_stride)`` also stores the fp32 rows
+        at row ``row[t] + h * head_stride`` (``row[t]`` < 0: not; no row
+        twice) of two fp32 buffers ``[m, hd]``.  Pages' token counts are not changed.  ``out``
+        takes the queries (their dtype or fp32; may be ``queries`` itself)."""
+        from .rotary import _NO_NORM, _NO_ROWS, head_norm, index_tensor, token_rows
+
+        torch = _torch()
+        hd, device = self.geometry.head_dim, self.arena.device
+        dest, held = self._token_dest(v_pool, tables, row, token)
+        T, H = int(held[0].shape[0]), int(tables.shape[2])
+        for x, name in ((keys, "keys"), (values, "values")):
+            if x.dim() != 3 or x.shape[0] != T or x.shape[1] != H or x.dtype != keys.dtype:
+                raise ValueError(f"{name} must have shape [{T}, {H}, {hd}] and the keys' dtype")
+        if rotary is not None:
+            if rotary.head_dim != hd or rotary.table.device != device:
+                raise ValueError("the rotary table is for another head_dim or device")
+            positions = index_tensor(positions, "positions", T, device, rotary.n_positions)
+        q_args = (_NO_ROWS, _NO_NORM, _NO_ROWS)
+        if queries is not None:
+            if queries.dim() != 3 or queries.shape[0] != T or queries.dtype != keys.dtype:
+                raise ValueError("queries must have the keys' tokens and dtype")
+            if out is None:
+                out = torch.empty(queries.shape, dtype=queries.dtype, device=device)
+            elif out.shape != queries.shape or out.dtype not in (queries.dtype, torch.float32):
+                raise ValueError("out must have the queries' shape, in their dtype or fp32")
+            q_args = (token_rows(queries, "queries", hd, device),
+                      head_norm(q_weight, "queries' weight", queries.shape[1], hd, eps, device),
+                      token_rows(out, "out", hd, device))
+        keep_args = (None, None, None, 0, 0)
+        if keep is not None:
+            for t in keep[:2]:
+                if t.dim() != 2 or t.shape != keep[0].shape or t.shape[1] != hd or t.dtype != torch.float32 or \
+                        not t.is_contiguous() or t.device != device:
+                    raise ValueError("kept rows must be two contiguous fp32 tensors [m, head_dim]")
+            keep_row = index_tensor(keep[2], "kept rows' index", T, device)
+            held += (keep_row,)
+            keep_args = (keep[0].data_ptr(), keep[1].data_ptr(), keep_row.data_ptr(), int(keep[3]), int(keep[0].shape[0]))
+        args = (positions.data_ptr() if rotary is not None else None,
+                rotary.c() if rotary is not None else _lib.Rotary(), *q_args, token_rows(keys, "keys", hd, device),
+                head_norm(k_weight, "keys' weight", H, hd, eps, device), token_rows(values, "values", hd, device), dest,
+                self.c_pool(), v_pool.c_pool(), *keep_args)
+        if T:
+            call_on(device, _lib.lib().dc_append_rotary, "dc_append_rotary", T, *args)
+        return out if queries is not None else None
+
+    def read_tokens_with(self, v_pool: "DevicePagePool", tables, row, token, *, dtype=None, out=None):
+        """Keys and values of tokens as dense rows ``[T, heads, hd]`` each, the
+        values their pages stand for (``dc_read_tokens``), for tokens named as
+        in :meth:`append_rotary_with`; a token without a page gives zeros.
+        ``dtype``: fp32 (default), fp16 or bf16; ``out = (keys, values)``
+        takes them instead.  The pages of one prefix handed to another
+        engine, or to attention over dense rows, need no host round trip."""
+        from .rotary import token_rows
+
+        torch = _torch()
+        hd, device = self.geometry.head_dim, self.arena.device
+        dest, held = self._token_dest(v_pool, tables, row, token)
+        shape = (int(held[0].shape[0]), int(tables.shape[2]), hd)
+        if out is None:
+            out = tuple(torch.empty((2, *shape), dtype=dtype or torch.float32, device=device))
+        for y in out:
+            if tuple(y.shape) != shape or y.dtype != out[0].dtype or (dtype is not None and y.dtype != dtype):
+                raise ValueError(f"out must be two tensors {list(shape)} of one dtype")
+        args = (dest, self.c_pool(), v_pool.c_pool(), token_rows(out[0], "out", hd, device), token_rows(out[1], "out", hd, device))
+        if shape[0]:
+            call_on(device, _lib.lib().dc_read_tokens, "dc_read_tokens", shape[0], *args)
+        return out
 
     def read_bytes(self, page_ids) -> int:
         """Compressed bytes a reader fetches for these pages (valid tokens only)."""

@@ -216,6 +216,88 @@ int dc_encode_streams_kv(const void* k_values, const void* v_values, int32_t val
  * (for cross-checking the two).  Host only; not thread-safe. */
 int dc_set_encode_path(int32_t path);
 
+/* ---- rows of new tokens ------------------------------------------------ */
+
+/* Token-major rows [n_tokens][n_heads][head_dim] of one dtype: element
+ * strides between tokens and heads, channels contiguous, so views of one
+ * projection's output need no copy.  n_heads 0 stands for none. */
+typedef struct dc_token_rows {
+  void* data; /* device                                                    */
+  int64_t token_stride;
+  int64_t head_stride;
+  int32_t n_heads;
+  int32_t dtype;
+} dc_token_rows;
+
+/* Per-head norm y = x / sqrt(mean(x^2) + eps) * weight over head_dim.
+ * weight: device [head_dim], or [n_heads][head_dim] with a head stride
+ * (elements; 0: one weight for all heads); NULL: no norm. */
+typedef struct dc_norm {
+  const void* weight;
+  int32_t dtype;
+  int32_t head_stride;
+  float eps;
+} dc_norm;
+
+/* Position rotation: device fp32 table [n_positions][rotary_dim], a position's
+ * rotary_dim / 2 cosines and then its sines; channel pairs (i, i + rotary_dim
+ * / 2), or (2 i, 2 i + 1) with interleaved; channels past rotary_dim stay.
+ * rotary_dim 0: no rotation.  The table is 16-byte aligned. */
+typedef struct dc_rotary {
+  const float* table;
+  int32_t n_positions;
+  int32_t rotary_dim;
+  int32_t interleaved;
+} dc_rotary;
+
+/* Where tokens live in pages: token t, head h is slot token[t] % page_tokens
+ * of page k_pages / v_pages[row[t]][h][token[t] / page_tokens] (device int32
+ * [n_rows][n_heads][n_pages]; row: a sequence of a cache, a block of a block
+ * cache).  A token < 0, a row or page index outside the table and a page id
+ * outside the pool name no page. */
+typedef struct dc_token_dest {
+  const int32_t* k_pages;
+  const int32_t* v_pages;
+  const int32_t* row;   /* device [n_tokens] */
+  const int32_t* token; /* device [n_tokens] */
+  int32_t n_rows;
+  int32_t n_pages;
+  int32_t page_tokens;
+} dc_token_dest;
+
+/* Queries and keys of new tokens normed per head and rotated to positions
+ * [n_tokens], in one launch: fp32 arithmetic, one rounding to the output
+ * dtype (the input's or DC_F32).  Either may be absent (n_heads 0).  An output
+ * may be its input.  A position outside the table gives NaN rows.  The
+ * reference's models hand rows over normed and rotated
+ * (dotcache/integrations/llama.py:345-358, _project_qkv). */
+int dc_norm_rotate(int64_t n_tokens, int32_t head_dim, const int32_t* positions, dc_rotary rotary, dc_token_rows q,
+                   dc_norm q_norm, dc_token_rows q_out, dc_token_rows k, dc_norm k_norm, dc_token_rows k_out,
+                   dc_stream_t stream);
+
+/* The same on the way into the pages, in one launch: queries (if any) to
+ * q_out, keys normed, rotated and encoded into their pages, values encoded as
+ * they are, each page as dc_encode_rows would write the fp32 rows.  Keys are
+ * computed in fp64 and rounded to fp32 once, so a page does not depend on the
+ * order of a norm's sum.  A token without a page, or whose position is outside
+ * the table, is not written.  k_keep / v_keep (NULL: none): the fp32 rows are
+ * also stored at row keep_row[t] + h * keep_head_stride of buffers of
+ * keep_rows rows (keep_row[t] < 0: not).  Does not change desc.tokens.
+ * Replaces the rotation ahead of reference dotcache/model_kv_cache.py:3830-3902
+ * (append_step) and that append. */
+int dc_append_rotary(int64_t n_tokens, const int32_t* positions, dc_rotary rotary, dc_token_rows q, dc_norm q_norm,
+                     dc_token_rows q_out, dc_token_rows k, dc_norm k_norm, dc_token_rows v, dc_token_dest dest,
+                     dc_pool k_pool, dc_pool v_pool, float* k_keep, float* v_keep, const int32_t* keep_row,
+                     int32_t keep_head_stride, int32_t keep_rows, dc_stream_t stream);
+
+/* Tokens of pages as dense rows, the values that codes, scales and biases
+ * stand for (fp32, rounded once to the output dtype): keys to k_out and values
+ * to v_out, one launch.  A token without a page gives zeros.  Slots are read
+ * up to the page's capacity, whatever desc.tokens says.  Replaces reference
+ * dotcache/modes/m0_affine.py:15-90 (dequantize_groups) over a page list. */
+int dc_read_tokens(int64_t n_tokens, dc_token_dest src, dc_pool k_pool, dc_pool v_pool, dc_token_rows k_out,
+                   dc_token_rows v_out, dc_stream_t stream);
+
 /* ---- read path: per-page entry points (score_page / mix_page) ------- */
 
 /* logits[q, token_offsets[i] + t] = score of query q against token t of
