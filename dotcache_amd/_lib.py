@@ -72,6 +72,9 @@ class TokenDest(C.Structure):
                 ("n_rows", C.c_int32), ("n_pages", C.c_int32), ("page_tokens", C.c_int32)]
 
 
+CHUNK_ITEM_FIELDS = ("seq", "kv_head", "q_begin", "row_begin", "row_end", "first", "kv_begin", "kv_end", "partial")
+CHUNK_MERGE_FIELDS = ("kv_head", "q_begin", "row_begin", "row_end", "partial_begin", "count")
+
 assert C.sizeof(PageDesc) == 8 and C.sizeof(WorkItem) == 32 and C.sizeof(MergeItem) == 16
 
 # name -> (restype, argtypes); this table is also the list of exported
@@ -96,6 +99,13 @@ SIGNATURES = {
                                    TokenDest, Pool, Pool, C.c_void_p, C.c_void_p, C.c_void_p, C.c_int32, C.c_int32,
                                    C.c_void_p]),
     "dc_read_tokens": (C.c_int, [C.c_int64, TokenDest, Pool, Pool, TokenRows, TokenRows, C.c_void_p]),
+    "dc_plan_chunk": (C.c_int, [C.c_void_p, C.c_void_p, C.c_int32, C.c_int32, C.c_int32, C.c_int32, C.c_int32, C.c_void_p,
+                                C.c_int32, C.POINTER(C.c_int32), C.c_void_p, C.c_int32, C.POINTER(C.c_int32),
+                                C.POINTER(C.c_int32)]),
+    "dc_chunk_workspace_bytes": (C.c_int64, [C.c_int32, C.c_int32]),
+    "dc_attend_chunk": (C.c_int, [Pool, Pool, C.c_void_p, C.c_void_p, C.c_int32, C.c_void_p, C.c_int32, C.c_void_p,
+                                  C.c_int32, C.c_int32, C.c_int32, C.c_int32, C.c_int64, TokenRows, C.c_float, TokenRows,
+                                  C.c_void_p, C.c_int64, C.c_void_p]),
     "dc_set_encode_path": (C.c_int, [C.c_int32]),
     "dc_score_pages": (C.c_int, [Pool, C.c_void_p, C.c_void_p, C.c_int32, C.c_void_p, C.c_int32, C.c_void_p, C.c_int64, C.c_void_p]),
     "dc_mix_pages": (C.c_int, [Pool, C.c_void_p, C.c_void_p, C.c_int32, C.c_void_p, C.c_int32, C.c_int64, C.c_void_p, C.c_int32, C.c_void_p]),

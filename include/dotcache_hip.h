@@ -543,6 +543,73 @@ int dc_decode_paged_noalloc(dc_pool k_pool, dc_pool v_pool, const int32_t* k_tab
 /* Bytes of the static scratch array dc_decode_paged_noalloc uses (host only). */
 int64_t dc_decode_noalloc_scratch_bytes(void);
 
+/* ---- read path: attention of a chunk of new tokens ----------------------- */
+
+/* Query rows [row_begin, row_end) (at most 128) of one (sequence, kv_head)
+ * against the sequence's tokens [kv_begin, kv_end).  Row r is head r % n_q of
+ * the sequence's new token r / n_q, whose row of the queries is q_begin + r /
+ * n_q; it attends tokens up to first + r / n_q.  partial < 0: the item writes
+ * the output; otherwise partial result slot `partial`.  row_end <= row_begin:
+ * an empty item. */
+typedef struct dc_chunk_item {
+  int32_t seq;
+  int32_t kv_head;
+  int32_t q_begin;
+  int32_t row_begin;
+  int32_t row_end;
+  int32_t first;
+  int32_t kv_begin;
+  int32_t kv_end;
+  int32_t partial;
+} dc_chunk_item;
+
+/* Join of partial results [partial_begin, partial_begin + count) of rows
+ * [row_begin, row_end). */
+typedef struct dc_chunk_merge {
+  int32_t kv_head;
+  int32_t q_begin;
+  int32_t row_begin;
+  int32_t row_end;
+  int32_t partial_begin;
+  int32_t count;
+} dc_chunk_merge;
+
+/* Host-only planner of dc_attend_chunk: new_tokens[b] new tokens (0 or more,
+ * none for a sequence that waits) of a context of context[b] tokens with them,
+ * packed one sequence after another in the queries.  Row tiles are cut into
+ * token ranges until about target_items items of near-equal length exist (at
+ * least min_tokens tokens each), and ordered so that items of one stream run
+ * on one die, the longest first.  DC_ESPACE if the output arrays are too small
+ * (counts are still written).  No reference counterpart: the reference decodes
+ * one token (dotcache/integrations/llama.py:424-425). */
+int dc_plan_chunk(const int32_t* new_tokens, const int32_t* context, int32_t n_seqs, int32_t n_kv_heads, int32_t n_q,
+                  int32_t target_items, int32_t min_tokens, dc_chunk_item* items, int32_t max_items, int32_t* n_items,
+                  dc_chunk_merge* merges, int32_t max_merges, int32_t* n_merges, int32_t* n_partials);
+
+/* Bytes of dc_attend_chunk's workspace. */
+int64_t dc_chunk_workspace_bytes(int32_t n_partials, int32_t head_dim);
+
+/* Causal attention of the new tokens of a batch over their sequences' pages
+ * (the new tokens' own rows among them: append first), in one launch and one
+ * more where rows were split.
+ *   q, out : [n_tokens][n_kv_heads * n_q][head_dim] rows of one dtype; query
+ *            head h reads KV head h / n_q.  out must not overlap q.
+ *   tables : device int32 [n_seqs][n_kv_heads][table_stride]; token u of a
+ *            sequence is slot u % page_capacity of its page u / page_capacity
+ *            (every page but a sequence's last is full)
+ *   workspace : at least dc_chunk_workspace_bytes(n_partials, head_dim)
+ * With 16-bit queries the matrix operands are fp16: queries, the pages' values
+ * and the softmax weights are each rounded to it once (values beyond +-65504
+ * overflow, as in fp16 pages), products and sums are fp32.  With DC_F32
+ * everything is fp32.  A token whose page the table does not name or that its
+ * page does not hold is left out; a row that sees no token gives zeros.
+ * head_dim <= 256.  Replaces, token by token, reference
+ * dotcache/attention_runtime.py:179-315. */
+int dc_attend_chunk(dc_pool k_pool, dc_pool v_pool, const int32_t* k_table, const int32_t* v_table, int32_t table_stride,
+                    const dc_chunk_item* items, int32_t n_items, const dc_chunk_merge* merges, int32_t n_merges,
+                    int32_t n_partials, int32_t n_seqs, int32_t n_kv_heads, int64_t n_tokens, dc_token_rows q,
+                    float query_scale, dc_token_rows out, void* workspace, int64_t workspace_bytes, dc_stream_t stream);
+
 /* Process-wide decode kernel choice: 0 (default) runs the MFMA kernel when
  * every page format (M3 fp16 keys and values, M0 4- or 8-bit keys of group
  * 32, M0 4- or 8-bit values of group 32 or 64), head_dim (64/128/256) and
