@@ -45,7 +45,7 @@ class ChunkPlan:
     merges: object           # device int32 [n_merges, 6]: dc_chunk_merge
     n_items: int
     n_merges: int
-    n_partials: int
+    n_partials: int          # rows of partial results
     host_items: np.ndarray
     host_merges: np.ndarray
     new: np.ndarray          # new tokens of every sequence
@@ -82,7 +82,7 @@ def plan_chunk(pool: DevicePagePool, v_pool: DevicePagePool | None, new, context
         raise ValueError("a sequence's context includes its new tokens")
     if int(kv_heads) <= 0 or int(q_per_kv) <= 0:
         raise ValueError("kv_heads and q_per_kv must be positive")
-    target = default_target_items() // 2 if target_items is None else int(target_items)
+    target = default_target_items() // 4 if target_items is None else int(target_items)
     if target <= 0:
         raise ValueError("target_items must be positive")
     L = _lib.lib()

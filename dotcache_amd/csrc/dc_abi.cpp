@@ -257,8 +257,8 @@ int64_t dc_decode_workspace_bytes(int32_t n_partials, int32_t n_q, int32_t head_
 }
 
 int64_t dc_chunk_workspace_bytes(int32_t n_partials, int32_t head_dim) {
-  // per partial: o [kChunkRows][head_dim] fp32, then (m, l) [kChunkRows][2] fp32
-  return int64_t(n_partials) * dc::kChunkRows * (head_dim + 2) * 4;
+  // per partial row: o [head_dim] fp32, then (m, l) fp32
+  return int64_t(n_partials) * (head_dim + 2) * 4;
 }
 
 int dc_plan_chunk(const int32_t* new_tokens, const int32_t* context, int32_t n_seqs, int32_t n_kv_heads, int32_t n_q,
@@ -293,13 +293,13 @@ int dc_plan_chunk(const int32_t* new_tokens, const int32_t* context, int32_t n_s
         for (int32_t r = 0; r < rows; r += dc::kChunkRows) {
           const int32_t r1 = std::min(r + dc::kChunkRows, rows);
           const int64_t len = steps(b, r1), n = (len + per - 1) / per;
+          if (parts + n * (r1 - r) > INT32_MAX) return dc::fail(DC_EINVAL, "dc_plan_chunk: too many partial results");
           const int32_t end = first + (r1 - 1) / n_q + 1;
           if (n > 1) joins.push_back({h, q_begin, r, r1, int32_t(parts), int32_t(n)});
           for (int64_t i = 0; i < n; ++i)
             all.push_back({b, h, q_begin, r, r1, first, int32_t(len * i / n * step),
-                           int32_t(std::min<int64_t>(len * (i + 1) / n * step, end)), n > 1 ? int32_t(parts + i) : -1});
-          if (n > 1) parts += n;
-          if (parts > INT32_MAX / dc::kChunkRows) return dc::fail(DC_EINVAL, "dc_plan_chunk: too many partial results");
+                           int32_t(std::min<int64_t>(len * (i + 1) / n * step, end)), n > 1 ? int32_t(parts + i * (r1 - r)) : -1});
+          if (n > 1) parts += n * (r1 - r);
         }
       q_begin += new_tokens[b];
     }

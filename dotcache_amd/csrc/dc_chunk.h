@@ -6,7 +6,7 @@
 
 namespace dc {
 
-constexpr int kChunkRows = 128;   // query rows of a work item
+constexpr int kChunkRows = 256;   // query rows of a work item
 constexpr int kChunkStep = 128;   // token ranges begin at multiples of this (a multiple of every tile)
 constexpr int kChunkXcds = 8;     // consecutive blocks go to consecutive dies, each with an L2 of its own
 
@@ -25,8 +25,10 @@ struct ChunkArgs {
   float scale;
   void* out;
   int64_t o_token_stride, o_head_stride;
-  float* part_o;   // [n_partials][kChunkRows][head_dim]
-  float* part_ml;  // [n_partials][kChunkRows][2]
+  float* part_o;   // [n_partials][head_dim]
+  float* part_ml;  // [n_partials][2]
+  uint32_t page_mul, page_shift;
+  int32_t q_vec, o_vec;  // rows start at multiples of 16 (8) bytes
 };
 
 // A work item outside the call's shapes is skipped, not read: a fault guard
@@ -35,14 +37,14 @@ __device__ __forceinline__ bool chunk_item_ok(const dc_chunk_item& it, const Chu
   return it.seq >= 0 && it.seq < a.n_seqs && it.kv_head >= 0 && it.kv_head < a.n_kv_heads && it.row_begin >= 0 &&
          it.row_begin < it.row_end && it.row_end - it.row_begin <= kChunkRows && it.q_begin >= 0 &&
          int64_t(it.q_begin) + (it.row_end - 1) / a.n_q < a.n_tokens && it.kv_begin >= 0 && it.first >= 0 &&
-         it.partial < a.n_partials;
+         int64_t(it.partial) + (it.partial >= 0 ? it.row_end - it.row_begin : 0) <= a.n_partials;
 }
 
 __device__ __forceinline__ bool chunk_merge_ok(const dc_chunk_merge& m, const ChunkArgs& a) {
   return m.kv_head >= 0 && m.kv_head < a.n_kv_heads && m.row_begin >= 0 && m.row_begin < m.row_end &&
          m.row_end - m.row_begin <= kChunkRows && m.q_begin >= 0 &&
          int64_t(m.q_begin) + (m.row_end - 1) / a.n_q < a.n_tokens && m.partial_begin >= 0 && m.count > 0 &&
-         int64_t(m.partial_begin) + m.count <= a.n_partials;
+         int64_t(m.partial_begin) + int64_t(m.count) * (m.row_end - m.row_begin) <= a.n_partials;
 }
 
 __device__ __forceinline__ void store_value(void* p, int32_t dtype, int64_t i, float x) {

@@ -4,11 +4,11 @@
 //
 //   o_r = sum_u p_ru v_u / sum_u p_ru,  p_ru = exp(scale q_r . k_u),  u <= last token that row r sees
 //
-// A work item is a tile of 128 query rows (token-major, the n_q heads of a KV
+// A work item is a tile of up to 256 query rows (token-major, the n_q heads of a KV
 // head next to each other, so they share every key and value) of one
-// (sequence, KV head) against a range of its tokens.  Four wavefronts of 32
-// rows each walk the range in tiles of KT tokens: the block turns a tile's
-// page rows into dense rows in LDS once, for all 128 query rows, and every
+// (sequence, KV head) against a range of its tokens.  Wavefronts of 32 rows
+// each walk the range in tiles of KT tokens: the block turns a tile's
+// page rows into dense rows in LDS once, for all its query rows, and every
 // wavefront then takes
 //   S^T = K Q^T   tokens x rows, so a lane holds one row's logits and the
 //                 softmax needs one exchange between the two half-wavefronts;
@@ -43,13 +43,15 @@ __device__ __forceinline__ int lds_at(int t, int ch) {
   return (t * CH + (ch ^ x)) * 16;
 }
 
-// This lane's value and that of lane ^ 32 (in one order or the other).
-__device__ __forceinline__ float2 both_halves(float v) {
-  const uint32_t u = __builtin_bit_cast(uint32_t, v);
-  const auto r = __builtin_amdgcn_permlane32_swap(u, u, false, false);
+// {a, b} of lanes 0 .. 31 and {a, b} of lanes 32 .. 63, exchanged to {a of the
+// first half, b of the first} and {a of the second, b of the second}: x is
+// what the first, y what the second half held, a in lanes 0 .. 31, b in 32 .. 63.
+__device__ __forceinline__ float2 swap_halves(float a, float b) {
+  const auto r = __builtin_amdgcn_permlane32_swap(__builtin_bit_cast(uint32_t, a), __builtin_bit_cast(uint32_t, b), false, false);
   const uint32_t x = r[0], y = r[1];  // (bit casts of vector elements would all take the first)
   return float2{__builtin_bit_cast(float, x), __builtin_bit_cast(float, y)};
 }
+__device__ __forceinline__ float2 both_halves(float v) { return swap_halves(v, v); }
 __device__ __forceinline__ float half_max(float v) {
   const float2 b = both_halves(v);
   return fmaxf(b.x, b.y);
@@ -92,6 +94,23 @@ __device__ __forceinline__ void page_values16(const dc_pool& pool, const dc_page
   }
 }
 
+// Whether the page d describes lies in the pool and holds token slot `slot`.
+__device__ __forceinline__ bool page_holds(const dc_pool& pool, const dc_page_desc& d, int slot) {
+  return slot < d.tokens && d.tokens <= pool.geometry.page_capacity &&
+         (int64_t(d.block) << 8) + blob_layout(d.format, d.bits, pool.geometry).total <= pool.arena_bytes;
+}
+
+// Narrows an item to this block's `rows` rows (blockIdx.y); false: none left.
+__device__ __forceinline__ bool block_rows(dc_chunk_item& it, int rows, int n_q) {
+  const int skip = rows * int(blockIdx.y);
+  if (it.row_begin + skip >= it.row_end) return false;
+  it.row_begin += skip;
+  if (it.partial >= 0) it.partial += skip;
+  it.row_end = min(it.row_end, it.row_begin + rows);
+  it.kv_end = max(min(it.kv_end, it.first + (it.row_end - 1) / n_q + 1), it.kv_begin);
+  return true;
+}
+
 }  // namespace
 
 // T: the matrix operands, _Float16 or float.  HDP: head_dim rounded up to the
@@ -109,8 +128,9 @@ __global__ void __launch_bounds__(256, sizeof(T) == 4 && HDP == 256 ? 1 : 2) att
   __shared__ uint32_t poison[TB];  // it has a value that is not finite (in a tile that some row does not see whole)
   __shared__ float odd[HDP];       // such a token's values
 
-  const dc_chunk_item it = a.items[blockIdx.x];
+  dc_chunk_item it = a.items[blockIdx.x];
   if (!chunk_item_ok(it, a)) return;
+  if (!block_rows(it, 128, a.n_q)) return;
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int col = lane & 31, half = lane >> 5;
   const int hd = a.kpool.geometry.head_dim, P = a.kpool.geometry.page_capacity;
@@ -158,58 +178,49 @@ __global__ void __launch_bounds__(256, sizeof(T) == 4 && HDP == 256 ? 1 : 2) att
     if (tid < TB) live[tid] = poison[tid] = 0;
     __syncthreads();
     const bool border = u0 + KT - 1 > it.first + it.row_begin / a.n_q;  // (uniform)
-    for (int i = tid; i < KT * (HDP / 16); i += 256) {
-      const int t = i % KT, c0 = i / KT * 16, u = u0 + t;
+    // (keys first, then values: KT HDP / 16 is a multiple of the block, so the side is uniform)
+    for (int i = tid; i < KT * (HDP / 8); i += 256) {
+      const bool vals = i >= KT * (HDP / 16);
+      const int t = i % KT, c0 = (i / KT - (vals ? HDP / 16 : 0)) * 16, u = u0 + t;
       const int page = u / P, slot = u - page * P;
-      float kv[16], vv[16];
+      const dc_pool& pool = vals ? a.vpool : a.kpool;
+      float x[16];
 #pragma unroll
-      for (int k = 0; k < 16; ++k) kv[k] = vv[k] = 0.f;
+      for (int k = 0; k < 16; ++k) x[k] = 0.f;
       if (u < it.kv_end && page < a.table_stride) {
         const int32_t kid = a.k_table[table + page], vid = a.v_table[table + page];
         if (uint32_t(kid) < uint32_t(a.kpool.n_descs) && uint32_t(vid) < uint32_t(a.vpool.n_descs)) {
           const dc_page_desc kd = a.kpool.descs[kid], vd = a.vpool.descs[vid];
-          const BlobLayout kl = blob_layout(kd.format, kd.bits, a.kpool.geometry);
-          const BlobLayout vl = blob_layout(vd.format, vd.bits, a.vpool.geometry);
-          if (slot < kd.tokens && slot < vd.tokens && kd.tokens <= P && vd.tokens <= P &&
-              (int64_t(kd.block) << 8) + kl.total <= a.kpool.arena_bytes &&
-              (int64_t(vd.block) << 8) + vl.total <= a.vpool.arena_bytes) {
-            if (c0 < hd) {
-              page_values16(a.kpool, kd, slot, c0, k_chunks, kv);
-              page_values16(a.vpool, vd, slot, c0, v_chunks, vv);
-              if (border) {
-                // a weight of 0 times an infinity or NaN would reach rows that do not see the token:
-                // such values are left out here, and added to the rows that see it below
-                bool bad = false;
+          if (page_holds(a.kpool, kd, slot) && page_holds(a.vpool, vd, slot)) {
+            if (c0 < hd) page_values16(pool, vals ? vd : kd, slot, c0, vals ? v_chunks : k_chunks, x);
+            if (vals && border) {
+              // a weight of 0 times an infinity or NaN would reach rows that do not see the token:
+              // such values are left out here, and added to the rows that see it below
+              bool bad = false;
 #pragma unroll
-                for (int k = 0; k < 16; ++k) {
-                  const bool fin = __builtin_isfinite(float(T(vv[k])));
-                  bad = bad || !fin;
-                  vv[k] = fin ? vv[k] : 0.f;
-                }
-                if (bad) atomicOr(&poison[t >> 5], 1u << (t & 31));
+              for (int k = 0; k < 16; ++k) {
+                const bool fin = __builtin_isfinite(float(T(x[k])));
+                bad = bad || !fin;
+                x[k] = fin ? x[k] : 0.f;
               }
+              if (bad) atomicOr(&poison[t >> 5], 1u << (t & 31));
             }
-            if (c0 == 0) atomicOr(&live[t >> 5], 1u << (t & 31));
+            if (!vals && c0 == 0) atomicOr(&live[t >> 5], 1u << (t & 31));
           }
         }
       }
+      uint8_t* const tile = vals ? vt : kt;
       if constexpr (F32) {
 #pragma unroll
-        for (int k = 0; k < 4; ++k) {
-          *reinterpret_cast<float4*>(kt + lds_at<CH>(t, c0 / 4 + k)) = float4{kv[4 * k], kv[4 * k + 1], kv[4 * k + 2], kv[4 * k + 3]};
-          *reinterpret_cast<float4*>(vt + lds_at<CH>(t, c0 / 4 + k)) = float4{vv[4 * k], vv[4 * k + 1], vv[4 * k + 2], vv[4 * k + 3]};
-        }
+        for (int k = 0; k < 4; ++k)
+          *reinterpret_cast<float4*>(tile + lds_at<CH>(t, c0 / 4 + k)) = float4{x[4 * k], x[4 * k + 1], x[4 * k + 2], x[4 * k + 3]};
       } else {
 #pragma unroll
         for (int k = 0; k < 2; ++k) {
-          h8v x, y;
+          h8v y;
 #pragma unroll
-          for (int j = 0; j < 8; ++j) {
-            x[j] = _Float16(kv[8 * k + j]);
-            y[j] = _Float16(vv[8 * k + j]);
-          }
-          *reinterpret_cast<h8v*>(kt + lds_at<CH>(t, c0 / 8 + k)) = x;
-          *reinterpret_cast<h8v*>(vt + lds_at<CH>(t, c0 / 8 + k)) = y;
+          for (int j = 0; j < 8; ++j) y[j] = _Float16(x[8 * k + j]);
+          *reinterpret_cast<h8v*>(tile + lds_at<CH>(t, c0 / 8 + k)) = y;
         }
       }
     }
@@ -329,7 +340,7 @@ __global__ void __launch_bounds__(256, sizeof(T) == 4 && HDP == 256 ? 1 : 2) att
   if (!has_row) return;
   l = half_sum(l);
   if (it.partial >= 0) {
-    const int64_t r = int64_t(it.partial) * kChunkRows + 32 * wave + col;
+    const int64_t r = int64_t(it.partial) + 32 * wave + col;
     float* po = a.part_o + r * hd;
 #pragma unroll
     for (int i = 0; i < CB; ++i)
@@ -355,23 +366,472 @@ __global__ void __launch_bounds__(256, sizeof(T) == 4 && HDP == 256 ? 1 : 2) att
     }
 }
 
-// Joins the partial results of a tile's token ranges: a wavefront per row,
+// ---- 16-bit queries, 32-channel groups ------------------------------------
+
+namespace {
+
+// Channels of an 8-channel group in the order in which LDS rows hold them: a
+// 4-bit word gives the pairs (0, 4), (1, 5), (2, 6), (3, 7) with one mask
+// each.  Keys and queries share the order, and the output's is undone at the
+// end, so it costs nothing.
+constexpr int kAhead = 4;  // matrix operands read ahead
+constexpr int kPerm[8] = {0, 4, 1, 5, 2, 6, 3, 7};
+
+__device__ __forceinline__ uint32_t twice(uint32_t h) { return h | (h << 16); }
+
+// Where a thread's 16 channels lie in the pages of a pool: the wavefront's
+// part (page layout) and the thread's (its channels, and its token where the
+// wavefront's share a page).  Byte offsets are those of 4-bit codes; 8-bit
+// ones are twice as far.
+struct Side {
+  const uint8_t* arena;
+  const dc_page_desc* descs;
+  const int32_t* table;
+  int64_t arena_bytes;
+  int32_t n_descs;
+  uint32_t token4, scales4, gap, f16_bytes, row2, groups2;
+  uint32_t at4, scale_at, f16_at;
+};
+
+__device__ __forceinline__ Side make_side(const dc_pool& p, const int32_t* table, uint32_t lt, uint32_t c0) {
+  const dc_page_geometry& geo = p.geometry;
+  Side x;
+  x.arena = reinterpret_cast<const uint8_t*>(p.arena);
+  x.descs = p.descs;
+  x.table = table;
+  x.arena_bytes = p.arena_bytes;
+  x.n_descs = p.n_descs;
+  const uint32_t C = geo.page_capacity, G = num_groups(geo), gs = geo.group_size, row = gs / 2, g = c0 / gs;
+  x.token4 = geo.layout == 0 ? row : G * row;
+  x.scales4 = G * C * row;
+  x.gap = (C * G * 2 + 15u) & ~15u;
+  x.f16_bytes = C * geo.head_dim * 2;
+  x.row2 = 2 * geo.head_dim;
+  x.groups2 = 2 * G;
+  x.at4 = lt * x.token4 + g * (geo.layout == 0 ? C * row : row) + (c0 - g * gs) / 2;
+  x.scale_at = (lt * G + g) * 2;
+  x.f16_at = (lt * geo.head_dim + c0) * 2;
+  return x;
+}
+
+enum UnitKind { U_NONE = 0, U_F16, U_B4, U_B8 };
+
+// Kind of a page's units, or U_NONE: no such page in the pool, or its first
+// token wanted is not in it.
+__device__ __forceinline__ int unit_kind(const Side& x, const dc_page_desc& d, int capacity, int slot) {
+  const bool m0 = d.format == DC_FMT_M0_AFFINE || d.format == DC_FMT_M0_SYMMETRIC;
+  const bool b8 = d.bits == 8;
+  const uint32_t codes = b8 ? 2 * x.scales4 : x.scales4;
+  const uint32_t bytes = m0 ? codes + (d.format == DC_FMT_M0_AFFINE ? 2 * x.gap : x.gap) : x.f16_bytes;
+  const bool ok = slot < d.tokens && d.tokens <= capacity && (int64_t(d.block) << 8) + bytes <= x.arena_bytes;
+  return !ok ? U_NONE : d.format == DC_FMT_M3_F16 ? U_F16 : !m0 ? U_NONE : b8 ? U_B8 : d.bits == 4 ? U_B4 : U_NONE;
+}
+
+// The unit's bytes: r, and scale and bias (0 where there is none).
+__device__ __forceinline__ void load_unit(const Side& x, const dc_page_desc& d, int kind, uint32_t slot, uint32_t (&r)[8],
+                                          uint32_t& scale, uint32_t& bias) {
+  const uint8_t* blob = x.arena + (uint64_t(d.block) << 8);
+  auto put4 = [&](int i, const uint8_t* p) __attribute__((always_inline)) {
+    const uint4 v = *reinterpret_cast<const uint4*>(p);
+    r[i] = v.x; r[i + 1] = v.y; r[i + 2] = v.z; r[i + 3] = v.w;
+  };
+  if (kind == U_F16) {
+    const uint8_t* p = blob + slot * x.row2 + x.f16_at;
+    put4(0, p);
+    put4(4, p + 16);
+  } else if (kind != U_NONE) {
+    const uint32_t sh = kind == U_B8;
+    const uint8_t* p = blob + ((slot * x.token4) << sh) + (x.at4 << sh);
+    if (kind == U_B8) {
+      put4(0, p);
+    } else {
+      const uint2 v = *reinterpret_cast<const uint2*>(p);
+      r[0] = v.x; r[1] = v.y;
+    }
+    const uint8_t* sp = blob + (x.scales4 << sh) + slot * x.groups2 + x.scale_at;
+    const bool affine = d.format == DC_FMT_M0_AFFINE;
+    scale = *reinterpret_cast<const uint16_t*>(sp);
+    const uint32_t b = *reinterpret_cast<const uint16_t*>(sp + (affine ? x.gap : 0));
+    bias = affine ? b : 0;
+  }
+}
+
+__device__ __forceinline__ uint32_t scaled(uint32_t codes, uint32_t zero, h2v s, h2v b) {
+  const h2v h = __builtin_bit_cast(h2v, codes | 0x64006400u) + __builtin_bit_cast(h2v, zero);  // exact
+  return __builtin_bit_cast(uint32_t, __builtin_elementwise_fma(h, s, b));
+}
+
+// The unit's 16 values as fp16 in LDS order, two chunks of 16 bytes.
+__device__ __forceinline__ void unit_values(int kind, bool affine, const uint32_t (&r)[8], uint32_t scale, uint32_t bias,
+                                            uint32_t (&y)[8]) {
+  if (kind == U_F16) {
+#pragma unroll
+    for (int i = 0; i < 8; ++i)
+      y[i] = __builtin_amdgcn_perm(r[4 * (i / 4) + 2 + (i % 4) / 2], r[4 * (i / 4) + (i % 4) / 2], i & 1 ? 0x07060302u : 0x05040100u);
+    return;
+  }
+  const h2v s = __builtin_bit_cast(h2v, twice(scale)), b = __builtin_bit_cast(h2v, twice(bias));
+  // -(1024 + zero point): 0xe400 is -1024, one unit per code
+  const uint32_t zero = twice(affine ? 0xe400u : kind == U_B4 ? 0xe407u : 0xe47fu);
+  if (kind == U_B4) {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) y[i] = scaled((r[i / 4] >> (4 * (i % 4))) & 0x000f000fu, zero, s, b);
+  } else {
+#pragma unroll
+    for (int i = 0; i < 8; ++i)
+      y[i] = scaled(__builtin_amdgcn_perm(r[2 * (i / 4) + 1], r[2 * (i / 4)], 0x0c040c00u + 0x00010001u * (i % 4)), zero, s, b);
+  }
+}
+
+// OR over the wavefront's parts of a token: bit t of the result is token t of
+// the wavefront's N tokens (lane t + N part).
+template <int N>
+__device__ __forceinline__ uint32_t fold_tokens(uint64_t b) {
+#pragma unroll
+  for (int n = 32; n >= N; n >>= 1) b |= b >> n;
+  return uint32_t(b) & ((1u << N) - 1u);
+}
+
+}  // namespace
+
+// fp16 operands where head_dim and both group sizes are multiples of 32 and the
+// pools hold 4- and 8-bit codes and fp16 rows.  Eight wavefronts of 32 rows
+// share a tile; a thread turns 16 channels of one token's key and of its value
+// into LDS (unit_values; packed fp16 arithmetic), two tiles in turn: while the
+// matrix instructions take tile i, tile i + 1 is written from registers, the
+// page rows of tile i + 2 are on their way to registers, and the descriptors
+// and page ids of the tiles after it likewise, so that no load is waited for
+// where it was issued.
+// UNI: the NT tokens that a wavefront turns always lie in one page, whose id,
+// descriptor and addresses are then the wavefront's.
+// CS: wavefronts that share 32 rows, each with a part of the output's channels
+// (head_dim 256, whose queries and output of 32 rows fill the registers).
+template <int HDP, int KT, bool UNI, int CS>
+__global__ void __launch_bounds__(512, 2) attend_chunk16_kernel(ChunkArgs a) {
+  constexpr int CH = HDP / 8, TB = KT / 32, CB = HDP / 32 / CS, TILE = KT * HDP * 2, QW = HDP / 16;
+  constexpr int NT = KT < 64 ? 8 : KT / 8;  // tokens a wavefront turns
+  constexpr int TW = KT / NT, PG = 8 / TW;  // wavefronts to a tile's tokens; parts of the channels that groups of TW take
+  static_assert(KT * HDP == 512 * 16, "one key and one value unit per thread");
+  extern __shared__ __attribute__((aligned(16))) uint8_t lds[];  // [2] keys, then [2] values
+  __shared__ __attribute__((aligned(4))) uint8_t live[2][KT / 8], poison[2][PG][KT / 8];  // one bit per token, as in attend_chunk_kernel
+  __shared__ float odd[HDP];
+
+  dc_chunk_item it = a.items[blockIdx.x];
+  if (!chunk_item_ok(it, a)) return;
+  if constexpr (CS > 1) {
+    if (!block_rows(it, 256 / CS, a.n_q)) return;
+  }
+  const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int col = lane & 31, half = lane >> 5;
+  const int hd = a.kpool.geometry.head_dim, P = a.kpool.geometry.page_capacity;
+
+  const int rows_at = 32 * (wave % (8 / CS)), cb0 = CS > 1 ? CB * (wave / (8 / CS)) : 0;  // (cb0: first channel block)
+  const int row = it.row_begin + rows_at + col;
+  const bool wave_rows = it.row_begin + rows_at < it.row_end;  // (uniform)
+  const bool has_row = row < it.row_end;
+  const int tok = row / a.n_q, head = it.kv_head * a.n_q + (row - tok * a.n_q);
+  const int sees = has_row ? it.first + tok : -1;
+  const int sees_all = it.first + (it.row_begin + rows_at) / a.n_q;
+  const int sees_block = it.first + it.row_begin / a.n_q;
+
+  // ---- the tiles' way from the pages to LDS
+  const int tw = wave % TW, pg = wave / TW;
+  const int ut = tw * NT + lane % NT, uc = 16 * (lane / NT) + HDP / PG * pg;  // this thread's token of a tile, first channel
+  const int lt = UNI ? lane % NT : 0;                           // token within the wavefront's, where they share a page
+  const int u_first = it.kv_begin + (UNI ? tw * NT : ut);     // first token of this wavefront's (thread's) of tile 0
+  const int64_t table = (int64_t(it.seq) * a.n_kv_heads + it.kv_head) * a.table_stride;
+  const int tiles = (it.kv_end - it.kv_begin + KT - 1) / KT;
+  const bool has = uc < hd;
+  const Side ks = make_side(a.kpool, a.k_table + table, lt, uc), vs = make_side(a.vpool, a.v_table + table, lt, uc);
+  auto uni = [](int x) { return UNI ? __builtin_amdgcn_readfirstlane(x) : x; };
+  auto page_of = [&](int tile) { return uint32_t((uint64_t(uint32_t(u_first + tile * KT)) * a.page_mul) >> a.page_shift); };
+  int32_t kid = -1, vid = -1;
+  uint2 kd{}, vd{};  // dc_page_desc
+  uint32_t kr[8], vr[8], k_scale = 0, k_bias = 0, v_scale = 0, v_bias = 0;
+  int k_kind = U_NONE, v_kind = U_NONE;  // of the raw units
+  bool k_affine = false, v_affine = false, counts = false;
+#pragma unroll
+  for (int i = 0; i < 8; ++i) kr[i] = vr[i] = 0;
+  auto load_ids = [&](int tile) __attribute__((always_inline)) {
+    const uint32_t page = page_of(tile);
+    const bool in = u_first + tile * KT < it.kv_end && page < uint32_t(a.table_stride);
+    kid = ks.table[in ? page : 0];
+    vid = vs.table[in ? page : 0];
+    if (!in) kid = -1;
+  };
+  auto load_descs = [&]() __attribute__((always_inline)) {
+    const int ki = uni(kid), vi = uni(vid);
+    const bool in = uint32_t(ki) < uint32_t(ks.n_descs) && uint32_t(vi) < uint32_t(vs.n_descs);
+    kd = reinterpret_cast<const uint2*>(ks.descs)[in ? ki : 0];
+    vd = reinterpret_cast<const uint2*>(vs.descs)[in ? vi : 0];
+    if (!in) kd.y &= 0xffff0000u;  // (no tokens)
+  };
+  auto load_units = [&](int tile) __attribute__((always_inline)) {
+    const int u = u_first + tile * KT, slot = u - int(page_of(tile)) * P;
+    const auto k = __builtin_bit_cast(dc_page_desc, uint2{uint32_t(uni(kd.x)), uint32_t(uni(kd.y))});
+    const auto v = __builtin_bit_cast(dc_page_desc, uint2{uint32_t(uni(vd.x)), uint32_t(uni(vd.y))});
+    k_kind = unit_kind(ks, k, P, slot);
+    v_kind = unit_kind(vs, v, P, slot);
+    k_affine = k.format == DC_FMT_M0_AFFINE;
+    v_affine = v.format == DC_FMT_M0_AFFINE;
+    // (tokens of the page behind its last and behind kv_end lie in its blob, but do not count)
+    const int end = min(min(int(k.tokens), int(v.tokens)), slot + it.kv_end - u);
+    const bool ok = k_kind != U_NONE && v_kind != U_NONE;
+    counts = ok && slot + lt < end;
+    if (ok && has) {
+      load_unit(ks, k, k_kind, slot, kr, k_scale, k_bias);
+      load_unit(vs, v, v_kind, slot, vr, v_scale, v_bias);
+    }
+  };
+  const int w_at[2] = {lds_at<CH>(ut, uc / 8), lds_at<CH>(ut, uc / 8 + 1)};  // of the unit's chunks in a tile
+  auto write_tile = [&](int tile) __attribute__((always_inline)) {
+    const int buf = tile & 1;
+    const bool zero = !(counts && has), border = it.kv_begin + (tile + 1) * KT - 1 > sees_block;  // (border: uniform)
+    uint32_t y[8];
+    auto put = [&](uint8_t* to) __attribute__((always_inline)) {
+#pragma unroll
+      for (int k = 0; k < 8; ++k) y[k] = zero ? 0 : y[k];
+#pragma unroll
+      for (int k = 0; k < 2; ++k) *reinterpret_cast<uint4*>(to + w_at[k]) = uint4{y[4 * k], y[4 * k + 1], y[4 * k + 2], y[4 * k + 3]};
+    };
+    unit_values(k_kind, k_affine, kr, k_scale, k_bias, y);
+    put(lds + buf * TILE);
+    unit_values(v_kind, v_affine, vr, v_scale, v_bias, y);
+    if (border) {
+      uint32_t any = 0;
+#pragma unroll
+      for (int k = 0; k < 8; ++k) {
+        const uint32_t e = ((y[k] & 0x7fff7fffu) + 0x04000400u) & 0x80008000u;  // sign bits: not finite
+        any |= e;
+        y[k] &= ~((e >> 15) * 0xffffu);
+      }
+      const uint32_t bits = fold_tokens<NT>(__ballot(any != 0 && !zero));
+      if (lane < NT / 8) poison[buf][pg][tw * (NT / 8) + lane] = uint8_t(bits >> (8 * lane));
+    }
+    put(lds + (2 + buf) * TILE);
+    const uint32_t bits = fold_tokens<NT>(__ballot(counts));
+    if (pg == 0 && lane < NT / 8) live[buf][tw * (NT / 8) + lane] = uint8_t(bits >> (8 * lane));
+  };
+  load_ids(0);
+  load_descs();
+  load_ids(1);
+  load_units(0);
+  load_descs();
+  load_ids(2);
+
+  // ---- queries: row col, channels 16 k + 8 half .. + 7 in LDS order
+  h8v q[QW];
+  {
+    const uint16_t* p = reinterpret_cast<const uint16_t*>(a.q) + int64_t(it.q_begin + tok) * a.q_token_stride +
+                        int64_t(head) * a.q_head_stride;
+#pragma unroll
+    for (int k = 0; k < QW; ++k) {
+      const int ch = 16 * k + 8 * half;
+      uint32_t w[4] = {0, 0, 0, 0};
+      if (has_row && ch < hd) {
+        if (a.q_vec) {
+          const uint4 x = *reinterpret_cast<const uint4*>(p + ch);
+          w[0] = x.x; w[1] = x.y; w[2] = x.z; w[3] = x.w;
+        } else {
+#pragma unroll
+          for (int i = 0; i < 4; ++i) w[i] = p[ch + 2 * i] | uint32_t(p[ch + 2 * i + 1]) << 16;
+        }
+      }
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        const uint32_t bits = w[kPerm[i] / 2] >> (16 * (kPerm[i] % 2));
+        q[k][i] = a.dtype == DC_F16 ? __builtin_bit_cast(_Float16, uint16_t(bits)) : _Float16(__builtin_bit_cast(float, bits << 16));
+      }
+    }
+  }
+  const float c = a.scale * kLog2e;
+  float m = -INFINITY, l = 0.f;
+  f32x16 o[CB];
+#pragma unroll
+  for (int i = 0; i < CB; ++i)
+#pragma unroll
+    for (int v = 0; v < 16; ++v) o[i][v] = 0.f;
+
+  write_tile(0);
+  load_units(1);
+  load_descs();
+  load_ids(3);
+  __syncthreads();
+  for (int i = 0; i < tiles; ++i) {
+    if (i + 1 < tiles) {
+      write_tile(i + 1);
+      load_units(i + 2);
+      load_descs();
+      load_ids(i + 4);
+    }
+    const uint8_t* const kt = lds + (i & 1) * TILE;
+    const uint8_t* const vt = lds + (2 + (i & 1)) * TILE;
+    const int u0 = it.kv_begin + i * KT;
+    if (u0 + KT - 1 > sees_block) {
+      const uint32_t* const bad = reinterpret_cast<const uint32_t*>(poison[i & 1][0]);
+#pragma unroll 1
+      for (int tb = 0; tb < TB; ++tb)
+#pragma unroll 1
+        for (uint32_t bits = bad[tb] | (PG > 1 ? bad[TB + tb] : 0); bits != 0; bits &= bits - 1) {
+          const int u = u0 + 32 * tb + __builtin_ctz(bits), page = u / P;
+          __syncthreads();
+          if (tid < HDP) {
+            const dc_page_desc d = a.vpool.descs[a.v_table[table + page]];
+            const BlobLayout L = blob_layout(d.format, d.bits, a.vpool.geometry);
+            const float x = tid < hd ? page_value(blob_ptr(a.vpool.arena, d), d, L, a.vpool.geometry, u - page * P, tid) : 0.f;
+            odd[tid] = float(_Float16(x));
+          }
+          __syncthreads();
+#pragma unroll
+          for (int j = 0; j < CB; ++j)
+#pragma unroll
+            for (int v = 0; v < 16; ++v) {
+              const float x = odd[32 * (cb0 + j) + 8 * (v / 4) + kPerm[4 * half + v % 4]];
+              if (u <= sees && !__builtin_isfinite(x)) o[j][v] += x;
+            }
+        }
+    }
+    if (wave_rows) {
+      const uint32_t* const on = reinterpret_cast<const uint32_t*>(live[i & 1]);
+      f32x16 s[TB];
+#pragma unroll
+      for (int tb = 0; tb < TB; ++tb)
+#pragma unroll
+        for (int v = 0; v < 16; ++v) s[tb][v] = 0.f;
+      // (operands are read kAhead instructions ahead; the scheduler would read them one ahead)
+      auto key = [&](int n) { return *reinterpret_cast<const h8v*>(kt + lds_at<CH>(32 * (n % TB) + col, 2 * (n / TB) + half)); };
+      h8v ka[kAhead];
+#pragma unroll
+      for (int n = 0; n < kAhead; ++n) ka[n] = key(n);
+#pragma unroll
+      for (int n = 0; n < QW * TB; ++n) {
+        __builtin_amdgcn_sched_barrier(0);
+        s[n % TB] = __builtin_amdgcn_mfma_f32_32x32x16_f16(ka[n % kAhead], q[n / TB], s[n % TB], 0, 0, 0);
+        if (n + kAhead < QW * TB) ka[n % kAhead] = key(n + kAhead);
+      }
+      bool masked = u0 + KT - 1 > sees_all;
+#pragma unroll
+      for (int tb = 0; tb < TB; ++tb) masked = masked || on[tb] != ~0u;
+      if (masked) {
+#pragma unroll
+        for (int tb = 0; tb < TB; ++tb) {
+          const uint32_t bits = on[tb] >> (4 * half);
+#pragma unroll
+          for (int v = 0; v < 16; ++v) {
+            const int t = 8 * (v / 4) + v % 4;
+            s[tb][v] = ((bits >> t) & 1) && u0 + 32 * tb + t + 4 * half <= sees ? s[tb][v] : -INFINITY;
+          }
+        }
+      }
+      float top = -INFINITY;
+#pragma unroll
+      for (int tb = 0; tb < TB; ++tb)
+#pragma unroll
+        for (int v = 0; v < 16; ++v) top = fmaxf(top, s[tb][v]);
+      top = half_max(top) * c;
+      if (__any(top > m + kLazy || (m == -INFINITY && top > m))) {
+        const float mn = fmaxf(m, top);
+        const float f = mn == -INFINITY ? 1.f : __builtin_amdgcn_exp2f(m - mn);
+        m = mn;
+        l *= f;
+#pragma unroll
+        for (int j = 0; j < CB; ++j)
+#pragma unroll
+          for (int v = 0; v < 16; ++v) o[j][v] *= f;
+      }
+      const float mu = m == -INFINITY ? 0.f : m;
+#pragma unroll
+      for (int tb = 0; tb < TB; ++tb)
+#pragma unroll
+        for (int v = 0; v < 16; ++v) s[tb][v] = __builtin_amdgcn_exp2f(fmaf(s[tb][v], c, -mu));
+      auto value = [&](int n) {
+        const int t = 16 * (n / CB) + 4 * half + ((lane & 15) >> 2), ch = 32 * (cb0 + n % CB) + (lane & 16) + 4 * (lane & 3);
+        s4v x[2];
+#pragma unroll
+        for (int e = 0; e < 2; ++e)
+          x[e] = __builtin_amdgcn_ds_read_tr16_b64_v4i16(
+              (__attribute__((address_space(3))) s4v*)(vt + lds_at<CH>(t + 8 * e, ch / 8) + 2 * (ch % 8)));
+        return __builtin_bit_cast(h8v, __builtin_shufflevector(x[0], x[1], 0, 1, 2, 3, 4, 5, 6, 7));
+      };
+      h8v va[kAhead];
+#pragma unroll
+      for (int n = 0; n < kAhead; ++n) va[n] = value(n);
+#pragma unroll
+      for (int st = 0; st < 2 * TB; ++st) {
+        h8v p;
+#pragma unroll
+        for (int k = 0; k < 8; k += 2) {
+          // (the sum takes the rounded weights, which are those the values get)
+          const h2v e = {(_Float16)s[st / 2][8 * (st % 2) + k], (_Float16)s[st / 2][8 * (st % 2) + k + 1]};
+          l = __builtin_amdgcn_fdot2(e, h2v{(_Float16)1.f, (_Float16)1.f}, l, false);
+          p[k] = e[0];
+          p[k + 1] = e[1];
+        }
+#pragma unroll
+        for (int j = 0; j < CB; ++j) {
+          const int n = st * CB + j;
+          __builtin_amdgcn_sched_barrier(0x6);  // (vector and scalar arithmetic may cross)
+          o[j] = __builtin_amdgcn_mfma_f32_32x32x16_f16(va[n % kAhead], p, o[j], 0, 0, 0);
+          if (n + kAhead < 2 * TB * CB) va[n % kAhead] = value(n + kAhead);
+        }
+      }
+    }
+    __syncthreads();
+  }
+  if (!has_row) return;
+  l = half_sum(l);
+  const bool part = it.partial >= 0;
+  const float inv = part ? 1.f : l == 0.f ? 0.f : 1.f / l;
+  const int64_t pr = int64_t(it.partial) + rows_at + col;
+  if (part && half == 0 && cb0 == 0) {
+    a.part_ml[2 * pr] = m;
+    a.part_ml[2 * pr + 1] = l;
+  }
+  uint16_t* const out = reinterpret_cast<uint16_t*>(a.out) + int64_t(it.q_begin + tok) * a.o_token_stride + int64_t(head) * a.o_head_stride;
+#pragma unroll
+  for (int j = 0; j < CB; ++j)
+#pragma unroll
+    for (int v = 0; v < 16; v += 4) {
+      // this half's channels 4 half .. + 3 of the group, from the LDS order
+      const float2 x = swap_halves(o[j][v], o[j][v + 1]), y = swap_halves(o[j][v + 2], o[j][v + 3]);
+      const float r[4] = {x.x * inv, y.x * inv, x.y * inv, y.y * inv};
+      const int ch = 32 * (cb0 + j) + 2 * v + 4 * half;
+      if (ch >= hd) continue;
+      if (part) {
+        *reinterpret_cast<float4*>(a.part_o + pr * hd + ch) = float4{r[0], r[1], r[2], r[3]};
+        continue;
+      }
+      uint32_t w[2];
+#pragma unroll
+      for (int k = 0; k < 2; ++k)
+        w[k] = a.dtype == DC_F16 ? __builtin_bit_cast(uint32_t, h2v{(_Float16)r[2 * k], (_Float16)r[2 * k + 1]})
+                                 : __builtin_bit_cast(uint32_t, b2v{(__bf16)r[2 * k], (__bf16)r[2 * k + 1]});
+      if (a.o_vec) {
+        *reinterpret_cast<uint2*>(out + ch) = uint2{w[0], w[1]};
+      } else {
+#pragma unroll
+        for (int k = 0; k < 4; ++k) out[ch + k] = uint16_t(w[k / 2] >> (16 * (k % 2)));
+      }
+    }
+}
+
+// Joins the partial results of a row tile's token ranges: a wavefront per row,
 // channels over its lanes.
 __global__ void __launch_bounds__(256) merge_chunk_kernel(ChunkArgs a, const dc_chunk_merge* merges) {
   const dc_chunk_merge mg = merges[blockIdx.x];
   if (!chunk_merge_ok(mg, a)) return;
   const int lane = threadIdx.x & 63, r = int(blockIdx.y) * 4 + int(threadIdx.x >> 6), row = mg.row_begin + r;
   if (row >= mg.row_end) return;
-  const int hd = a.kpool.geometry.head_dim;
+  const int hd = a.kpool.geometry.head_dim, rows = mg.row_end - mg.row_begin;
   const int tok = row / a.n_q, head = mg.kv_head * a.n_q + (row - tok * a.n_q);
   float top = -INFINITY;
-  for (int i = 0; i < mg.count; ++i) top = fmaxf(top, a.part_ml[2 * (int64_t(mg.partial_begin + i) * kChunkRows + r)]);
+  for (int i = 0; i < mg.count; ++i) top = fmaxf(top, a.part_ml[2 * (int64_t(mg.partial_begin) + int64_t(i) * rows + r)]);
   const float mu = top == -INFINITY ? 0.f : top;
   const int64_t off = int64_t(mg.q_begin + tok) * a.o_token_stride + int64_t(head) * a.o_head_stride;
   for (int ch = lane; ch < hd; ch += 64) {
     float sum = 0.f, l = 0.f;
     for (int i = 0; i < mg.count; ++i) {
-      const int64_t at = int64_t(mg.partial_begin + i) * kChunkRows + r;
+      const int64_t at = int64_t(mg.partial_begin) + int64_t(i) * rows + r;
       const float w = exp2f(a.part_ml[2 * at] - mu);
       l = fmaf(w, a.part_ml[2 * at + 1], l);
       sum = fmaf(w, a.part_o[at * hd + ch], sum);
@@ -386,8 +846,34 @@ static int launch_chunk(const ChunkArgs& a, hipStream_t stream) {
   static const hipError_t set = hipFuncSetAttribute(reinterpret_cast<const void*>(&attend_chunk_kernel<T, HDP, KT>),
                                                     hipFuncAttributeMaxDynamicSharedMemorySize, bytes);
   if (int rc = check_hip(set, "attend_chunk_kernel LDS")) return rc;
-  hipLaunchKernelGGL((attend_chunk_kernel<T, HDP, KT>), dim3(a.n_items), dim3(256), bytes, stream, a);
+  hipLaunchKernelGGL((attend_chunk_kernel<T, HDP, KT>), dim3(a.n_items, kChunkRows / 128), dim3(256), bytes, stream, a);
   return check_hip(hipGetLastError(), "attend_chunk_kernel launch");
+}
+
+template <int HDP, int KT, bool UNI, int CS>
+static int launch_chunk16_as(const ChunkArgs& a, hipStream_t stream) {
+  constexpr int bytes = 4 * KT * HDP * 2;
+  static const hipError_t set = hipFuncSetAttribute(reinterpret_cast<const void*>(&attend_chunk16_kernel<HDP, KT, UNI, CS>),
+                                                    hipFuncAttributeMaxDynamicSharedMemorySize, bytes);
+  if (int rc = check_hip(set, "attend_chunk16_kernel LDS")) return rc;
+  hipLaunchKernelGGL((attend_chunk16_kernel<HDP, KT, UNI, CS>), dim3(a.n_items, CS), dim3(512), bytes, stream, a);
+  return check_hip(hipGetLastError(), "attend_chunk16_kernel launch");
+}
+
+template <int HDP, int KT, int CS>
+static int launch_chunk16(const ChunkArgs& a, hipStream_t stream) {
+  return a.kpool.geometry.page_capacity % (KT < 64 ? 8 : KT / 8) == 0 ? launch_chunk16_as<HDP, KT, true, CS>(a, stream)
+                                                        : launch_chunk16_as<HDP, KT, false, CS>(a, stream);
+}
+
+// Whether a thread's 32 channels share a scale and lie at 16-byte multiples,
+// with offsets in a blob that fit 32 bits, in the formats that load_raw takes.
+static bool units32(const dc_pool& p) {
+  const dc_page_geometry& g = p.geometry;
+  uint64_t takes = uint64_t(1) << (DC_FMT_M3_F16 * 9);
+  for (int f : {DC_FMT_M0_AFFINE, DC_FMT_M0_SYMMETRIC})
+    for (int bits : {4, 8}) takes |= uint64_t(1) << (f * 9 + bits);
+  return p.format_mask != 0 && (p.format_mask & ~takes) == 0 && g.head_dim % 32 == 0 && g.group_size % 32 == 0 && chunk16_geometry(g);
 }
 
 }  // namespace dc
@@ -413,19 +899,28 @@ extern "C" int dc_attend_chunk(dc_pool k_pool, dc_pool v_pool, const int32_t* k_
   if (q.dtype != DC_F32 && q.dtype != DC_F16 && q.dtype != DC_BF16) return dc::fail(DC_EINVAL, "%s: queries must be DC_F32, DC_F16 or DC_BF16", who);
   if (out.dtype != q.dtype || out.n_heads != q.n_heads || q.n_heads <= 0 || q.n_heads % n_kv_heads)
     return dc::fail(DC_EINVAL, "%s: the output needs the queries' dtype and heads, a multiple of the KV heads", who);
-  const int64_t rows = int64_t(n_partials) * dc::kChunkRows;
   if (workspace_bytes < dc_chunk_workspace_bytes(n_partials, hd) || (n_partials && !workspace))
     return dc::fail(DC_ESPACE, "%s: workspace too small", who);
   dc::ChunkArgs a{k_pool, v_pool, k_table, v_table, table_stride, items, n_items, n_seqs, n_kv_heads, q.n_heads / n_kv_heads,
                   n_tokens, n_partials, q.data, q.token_stride, q.head_stride, q.dtype, query_scale, out.data, out.token_stride,
-                  out.head_stride, static_cast<float*>(workspace), static_cast<float*>(workspace) + rows * hd};
+                  out.head_stride, static_cast<float*>(workspace), static_cast<float*>(workspace) + int64_t(n_partials) * hd};
   const hipStream_t st = hipStream_t(stream);
+  a.q_vec = reinterpret_cast<uintptr_t>(q.data) % 16 == 0 && q.token_stride % 8 == 0 && q.head_stride % 8 == 0;
+  a.o_vec = reinterpret_cast<uintptr_t>(out.data) % 8 == 0 && out.token_stride % 4 == 0 && out.head_stride % 4 == 0;
+  const int merge_rows = dc::kChunkRows;
+  // u / page_capacity = u * page_mul >> page_shift for u < 2^31
+  const uint32_t P = uint32_t(k_pool.geometry.page_capacity);
+  a.page_shift = 31;
+  while ((1u << (a.page_shift - 31)) < P) ++a.page_shift;
+  a.page_mul = uint32_t(((uint64_t(1) << a.page_shift) + P - 1) / P);
   int rc;
-  if (q.dtype == DC_F32)
+  if (q.dtype != DC_F32 && dc::units32(k_pool) && dc::units32(v_pool))
+    rc = hd <= 64 ? dc::launch_chunk16<64, 128, 1>(a, st) : hd <= 128 ? dc::launch_chunk16<128, 64, 1>(a, st) : dc::launch_chunk16<256, 32, 2>(a, st);
+  else if (q.dtype == DC_F32)
     rc = hd <= 64 ? dc::launch_chunk<float, 64, 64>(a, st) : hd <= 128 ? dc::launch_chunk<float, 128, 32>(a, st) : dc::launch_chunk<float, 256, 32>(a, st);
   else
     rc = hd <= 64 ? dc::launch_chunk<_Float16, 64, 128>(a, st) : hd <= 128 ? dc::launch_chunk<_Float16, 128, 64>(a, st) : dc::launch_chunk<_Float16, 256, 32>(a, st);
   if (rc != DC_OK || n_merges == 0) return rc;
-  hipLaunchKernelGGL(dc::merge_chunk_kernel, dim3(n_merges, dc::kChunkRows / 4), dim3(256), 0, st, a, merges);
+  hipLaunchKernelGGL(dc::merge_chunk_kernel, dim3(n_merges, uint32_t(merge_rows + 3) / 4), dim3(256), 0, st, a, merges);
   return dc::check_hip(hipGetLastError(), "merge_chunk_kernel launch");
 }

@@ -545,12 +545,12 @@ int64_t dc_decode_noalloc_scratch_bytes(void);
 
 /* ---- read path: attention of a chunk of new tokens ----------------------- */
 
-/* Query rows [row_begin, row_end) (at most 128) of one (sequence, kv_head)
+/* Query rows [row_begin, row_end) (at most 256) of one (sequence, kv_head)
  * against the sequence's tokens [kv_begin, kv_end).  Row r is head r % n_q of
  * the sequence's new token r / n_q, whose row of the queries is q_begin + r /
  * n_q; it attends tokens up to first + r / n_q.  partial < 0: the item writes
- * the output; otherwise partial result slot `partial`.  row_end <= row_begin:
- * an empty item. */
+ * the output; otherwise its rows' partial results from partial row `partial`.
+ * row_end <= row_begin: an empty item. */
 typedef struct dc_chunk_item {
   int32_t seq;
   int32_t kv_head;
@@ -563,8 +563,8 @@ typedef struct dc_chunk_item {
   int32_t partial;
 } dc_chunk_item;
 
-/* Join of partial results [partial_begin, partial_begin + count) of rows
- * [row_begin, row_end). */
+/* Join of the count partial results of rows [row_begin, row_end), one after
+ * another from partial row partial_begin. */
 typedef struct dc_chunk_merge {
   int32_t kv_head;
   int32_t q_begin;
@@ -586,7 +586,7 @@ int dc_plan_chunk(const int32_t* new_tokens, const int32_t* context, int32_t n_s
                   int32_t target_items, int32_t min_tokens, dc_chunk_item* items, int32_t max_items, int32_t* n_items,
                   dc_chunk_merge* merges, int32_t max_merges, int32_t* n_merges, int32_t* n_partials);
 
-/* Bytes of dc_attend_chunk's workspace. */
+/* Bytes of dc_attend_chunk's workspace for n_partials partial rows. */
 int64_t dc_chunk_workspace_bytes(int32_t n_partials, int32_t head_dim);
 
 /* Causal attention of the new tokens of a batch over their sequences' pages

@@ -34,26 +34,29 @@ def test_items_cover_every_row_and_token_once(new, ctx, target):
     for x in items:
         b = x["seq"]
         assert 0 <= x["kv_head"] < H and x["q_begin"] == start[b] and x["first"] == ctx[b] - new[b]
-        assert x["row_begin"] % 128 == 0 and x["row_end"] == min(x["row_begin"] + 128, new[b] * n_q)
+        assert x["row_begin"] % 256 == 0 and x["row_end"] == min(x["row_begin"] + 256, new[b] * n_q)
+        n_rows = x["row_end"] - x["row_begin"]
         seen.setdefault((b, x["kv_head"], x["row_begin"]), []).append((x["kv_begin"], x["kv_end"], x["partial"]))
         if x["partial"] >= 0:
-            assert x["partial"] < plan.n_partials and x["partial"] not in slots
-            slots.add(x["partial"])
+            mine = set(range(x["partial"], x["partial"] + n_rows))
+            assert max(mine) < plan.n_partials and not mine & slots
+            slots |= mine
     assert len(slots) == plan.n_partials
-    assert len(seen) == sum(-(-n * n_q // 128) for n in new) * H
+    assert len(seen) == sum(-(-n * n_q // 256) for n in new) * H
     merges = {(h, q, r): (p, n) for h, q, r, _, p, n in plan.host_merges.tolist()}
     for (b, h, r), parts in seen.items():
         parts.sort()
-        last = ctx[b] - new[b] + (min(r + 128, new[b] * n_q) - 1) // n_q
+        last = ctx[b] - new[b] + (min(r + 256, new[b] * n_q) - 1) // n_q
         assert parts[0][0] == 0 and parts[-1][1] == last + 1
         assert all(x[1] == y[0] for x, y in zip(parts, parts[1:])) and all(x[0] % 128 == 0 and x[1] > x[0] for x in parts)
         if len(parts) == 1:
             assert parts[0][2] == -1
         else:
             assert merges[h, int(start[b]), r] == (parts[0][2], len(parts))
-            assert [x[2] for x in parts] == list(range(parts[0][2], parts[0][2] + len(parts)))
+            rows = min(256, new[b] * n_q - r)
+            assert [x[2] for x in parts] == list(range(parts[0][2], parts[0][2] + rows * len(parts), rows))
     assert len(merges) == sum(len(x) > 1 for x in seen.values()) == plan.n_merges
-    assert plan.n_tokens == sum(new) and workspace_bytes(plan, 64) == plan.n_partials * 128 * 66 * 4
+    assert plan.n_tokens == sum(new) and workspace_bytes(plan, 64) == plan.n_partials * 66 * 4
 
 
 def test_equal_work_on_every_die():
