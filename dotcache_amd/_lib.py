@@ -99,12 +99,12 @@ SIGNATURES = {
                                    TokenDest, Pool, Pool, C.c_void_p, C.c_void_p, C.c_void_p, C.c_int32, C.c_int32,
                                    C.c_void_p]),
     "dc_read_tokens": (C.c_int, [C.c_int64, TokenDest, Pool, Pool, TokenRows, TokenRows, C.c_void_p]),
-    "dc_plan_chunk": (C.c_int, [C.c_void_p, C.c_void_p, C.c_int32, C.c_int32, C.c_int32, C.c_int32, C.c_int32, C.c_void_p,
-                                C.c_int32, C.POINTER(C.c_int32), C.c_void_p, C.c_int32, C.POINTER(C.c_int32),
-                                C.POINTER(C.c_int32)]),
+    "dc_plan_chunk": (C.c_int, [C.c_void_p, C.c_void_p, C.c_int32, C.c_int32, C.c_int32, C.c_int32, C.c_int32, C.c_int32,
+                                C.c_void_p, C.c_int32, C.POINTER(C.c_int32), C.POINTER(C.c_int32), C.POINTER(C.c_int32),
+                                C.c_void_p, C.c_int32, C.POINTER(C.c_int32), C.POINTER(C.c_int32)]),
     "dc_chunk_workspace_bytes": (C.c_int64, [C.c_int32, C.c_int32]),
-    "dc_attend_chunk": (C.c_int, [Pool, Pool, C.c_void_p, C.c_void_p, C.c_int32, C.c_void_p, C.c_int32, C.c_void_p,
-                                  C.c_int32, C.c_int32, C.c_int32, C.c_int32, C.c_int64, TokenRows, C.c_float, TokenRows,
+    "dc_attend_chunk": (C.c_int, [Pool, Pool, C.c_void_p, C.c_void_p, C.c_int32, C.c_void_p, C.c_int32, C.c_int32,
+                                  C.c_int32, C.c_void_p, C.c_int32, C.c_int32, C.c_int32, C.c_int32, C.c_int64, TokenRows, C.c_float, TokenRows,
                                   C.c_void_p, C.c_int64, C.c_void_p]),
     "dc_set_encode_path": (C.c_int, [C.c_int32]),
     "dc_score_pages": (C.c_int, [Pool, C.c_void_p, C.c_void_p, C.c_int32, C.c_void_p, C.c_int32, C.c_void_p, C.c_int64, C.c_void_p]),

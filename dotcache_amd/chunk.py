@@ -44,6 +44,8 @@ class ChunkPlan:
     items: object            # device int32 [n_items, 9]: dc_chunk_item
     merges: object           # device int32 [n_merges, 6]: dc_chunk_merge
     n_items: int
+    n_few: int               # the first of them: sequences of few rows, at most few_rows each
+    few_rows: int
     n_merges: int
     n_partials: int          # rows of partial results
     host_items: np.ndarray
@@ -86,24 +88,25 @@ def plan_chunk(pool: DevicePagePool, v_pool: DevicePagePool | None, new, context
     if target <= 0:
         raise ValueError("target_items must be positive")
     L = _lib.lib()
-    counts = [C.c_int32() for _ in range(3)]
+    counts = [C.c_int32() for _ in range(5)]  # items, few, few rows, merges, partial rows
 
     def plan(items, merges):
-        return L.dc_plan_chunk(n.ctypes.data, ctx.ctypes.data, n.size, int(kv_heads), int(q_per_kv), target, MIN_SPLIT_TOKENS,
-                               items.ctypes.data, items.shape[0], C.byref(counts[0]), merges.ctypes.data, merges.shape[0],
-                               C.byref(counts[1]), C.byref(counts[2]))
+        return L.dc_plan_chunk(n.ctypes.data, ctx.ctypes.data, n.size, int(kv_heads), int(q_per_kv), pool.geometry.head_dim,
+                               target, MIN_SPLIT_TOKENS, items.ctypes.data, items.shape[0], *(C.byref(c) for c in counts[:3]),
+                               merges.ctypes.data, merges.shape[0], *(C.byref(c) for c in counts[3:]))
 
     empty = [np.zeros((0, len(f)), dtype=np.int32) for f in (_lib.CHUNK_ITEM_FIELDS, _lib.CHUNK_MERGE_FIELDS)]
     st = plan(*empty)
     if st != _lib.DC_ESPACE:
         _lib.check(st, "dc_plan_chunk")
-    items, merges = (np.zeros((c.value, e.shape[1]), dtype=np.int32) for c, e in zip(counts, empty))
+    items, merges = (np.zeros((c.value, e.shape[1]), dtype=np.int32) for c, e in zip((counts[0], counts[3]), empty))
     _lib.check(plan(items, merges), "dc_plan_chunk")
     both = torch.from_numpy(np.concatenate([items.ravel(), merges.ravel()])).to(pool.arena.device)
     busy = ctx[n > 0]
     return ChunkPlan(items=both[: items.size].view(items.shape), merges=both[items.size:].view(merges.shape),
-                     n_items=items.shape[0], n_merges=merges.shape[0], n_partials=counts[2].value, host_items=items,
-                     host_merges=merges, new=n, context=ctx, kv_heads=int(kv_heads), q_per_kv=int(q_per_kv),
+                     n_items=items.shape[0], n_few=counts[1].value, few_rows=counts[2].value, n_merges=merges.shape[0],
+                     n_partials=counts[4].value, host_items=items, host_merges=merges,
+                     new=n, context=ctx, kv_heads=int(kv_heads), q_per_kv=int(q_per_kv),
                      n_tokens=int(n.sum(dtype=np.int64)), max_context=int(busy.max()) if busy.size else 0)
 
 
@@ -172,7 +175,7 @@ def attend_chunk(pool: DevicePagePool, k_table, v_pool: DevicePagePool | None, v
         raise ValueError(f"workspace must be contiguous, {need} bytes at least, on {device}")
     if plan.n_items:
         call_on(device, _lib.lib().dc_attend_chunk, "dc_attend_chunk", pool.c_pool(), vpool.c_pool(), k_table.data_ptr(),
-                v_table.data_ptr(), shape[2], plan.items.data_ptr(), plan.n_items, plan.merges.data_ptr(), plan.n_merges,
+                v_table.data_ptr(), shape[2], plan.items.data_ptr(), plan.n_items, plan.n_few, plan.few_rows, plan.merges.data_ptr(), plan.n_merges,
                 plan.n_partials, B, plan.kv_heads, plan.n_tokens, q_rows, float(query_scale), out_rows,
                 workspace.data_ptr() if need else None, need)
     return out

@@ -262,67 +262,84 @@ int64_t dc_chunk_workspace_bytes(int32_t n_partials, int32_t head_dim) {
 }
 
 int dc_plan_chunk(const int32_t* new_tokens, const int32_t* context, int32_t n_seqs, int32_t n_kv_heads, int32_t n_q,
-                  int32_t target_items, int32_t min_tokens, dc_chunk_item* items, int32_t max_items, int32_t* n_items,
-                  dc_chunk_merge* merges, int32_t max_merges, int32_t* n_merges, int32_t* n_partials) {
-  if (!new_tokens || !context || n_seqs <= 0 || n_kv_heads <= 0 || n_q <= 0 || target_items <= 0 || min_tokens <= 0 ||
-      !n_items || !n_merges || !n_partials)
+                  int32_t head_dim, int32_t target_items, int32_t min_tokens, dc_chunk_item* items, int32_t max_items,
+                  int32_t* n_items, int32_t* n_few, int32_t* few_rows, dc_chunk_merge* merges, int32_t max_merges,
+                  int32_t* n_merges, int32_t* n_partials) {
+  if (!new_tokens || !context || n_seqs <= 0 || n_kv_heads <= 0 || n_q <= 0 || head_dim <= 0 || target_items <= 0 || min_tokens <= 0 ||
+      !n_items || !n_few || !few_rows || !n_merges || !n_partials)
     return dc::fail(DC_EINVAL, "dc_plan_chunk: bad arguments");
   try {
     const int64_t step = dc::kChunkStep;
-    int64_t q_tokens = 0, total = 0;  // total: steps of every tile's token range
-    auto steps = [&](int32_t b, int64_t row_end) {
-      return (int64_t(context[b]) - new_tokens[b] + (row_end - 1) / n_q + 1 + step - 1) / step;
-    };
+    int64_t q_tokens = 0;
     for (int32_t b = 0; b < n_seqs; ++b) {
       if (new_tokens[b] < 0 || context[b] < new_tokens[b])
         return dc::fail(DC_EINVAL, "dc_plan_chunk: sequence %d has %d new tokens in a context of %d", b, new_tokens[b], context[b]);
-      const int64_t rows = int64_t(new_tokens[b]) * n_q;
-      if (rows > INT32_MAX - dc::kChunkRows) return dc::fail(DC_EINVAL, "dc_plan_chunk: sequence %d has too many new tokens", b);
-      for (int64_t r = 0; r < rows; r += dc::kChunkRows) total += steps(b, std::min<int64_t>(r + dc::kChunkRows, rows)) * n_kv_heads;
+      if (int64_t(new_tokens[b]) * n_q > INT32_MAX - dc::kChunkRows) return dc::fail(DC_EINVAL, "dc_plan_chunk: sequence %d has too many new tokens", b);
       q_tokens += new_tokens[b];
     }
     if (q_tokens > INT32_MAX) return dc::fail(DC_EINVAL, "dc_plan_chunk: too many new tokens");
-    const int64_t per = std::max<int64_t>((total + target_items - 1) / target_items, (min_tokens + step - 1) / step);
-    std::vector<dc_chunk_item> all;
+    std::vector<dc_chunk_item> order;
     std::vector<dc_chunk_merge> joins;
     int64_t parts = 0;
-    int32_t q_begin = 0;
-    for (int32_t b = 0; b < n_seqs; ++b) {
-      const int32_t rows = new_tokens[b] * n_q, first = context[b] - new_tokens[b];
-      for (int32_t h = 0; h < n_kv_heads; ++h)
-        for (int32_t r = 0; r < rows; r += dc::kChunkRows) {
-          const int32_t r1 = std::min(r + dc::kChunkRows, rows);
-          const int64_t len = steps(b, r1), n = (len + per - 1) / per;
-          if (parts + n * (r1 - r) > INT32_MAX) return dc::fail(DC_EINVAL, "dc_plan_chunk: too many partial results");
-          const int32_t end = first + (r1 - 1) / n_q + 1;
-          if (n > 1) joins.push_back({h, q_begin, r, r1, int32_t(parts), int32_t(n)});
-          for (int64_t i = 0; i < n; ++i)
-            all.push_back({b, h, q_begin, r, r1, first, int32_t(len * i / n * step),
-                           int32_t(std::min<int64_t>(len * (i + 1) / n * step, end)), n > 1 ? int32_t(parts + i * (r1 - r)) : -1});
-          if (n > 1) parts += n * (r1 - r);
-        }
-      q_begin += new_tokens[b];
+    *few_rows = 0;
+    *n_few = 0;
+    // the sequences of few rows, then the others: a launch each, each with items for the whole card
+    for (const bool few : {true, false}) {
+      auto takes = [&](int32_t b) {
+        return new_tokens[b] > 0 && (int64_t(new_tokens[b]) * n_q <= dc::few_row_limit(head_dim)) == few;
+      };
+      auto steps = [&](int32_t b, int64_t row_end) {
+        return (int64_t(context[b]) - new_tokens[b] + (row_end - 1) / n_q + 1 + step - 1) / step;
+      };
+      int64_t total = 0;  // steps of every row tile's token range
+      for (int32_t b = 0; b < n_seqs; ++b) {
+        if (!takes(b)) continue;
+        const int64_t rows = int64_t(new_tokens[b]) * n_q;
+        if (few) *few_rows = std::max<int32_t>(*few_rows, int32_t(rows));
+        for (int64_t r = 0; r < rows; r += dc::kChunkRows) total += steps(b, std::min<int64_t>(r + dc::kChunkRows, rows)) * n_kv_heads;
+      }
+      // (two blocks of the few-row kernel share a compute unit)
+      const int64_t target = few ? 2 * int64_t(target_items) - 1 : target_items;
+      const int64_t per = std::max<int64_t>((total + target - 1) / target, (min_tokens + step - 1) / step);
+      std::vector<dc_chunk_item> all;
+      int32_t q_begin = 0;
+      for (int32_t b = 0; b < n_seqs; q_begin += new_tokens[b], ++b) {
+        if (!takes(b)) continue;
+        const int32_t rows = new_tokens[b] * n_q, first = context[b] - new_tokens[b];
+        for (int32_t h = 0; h < n_kv_heads; ++h)
+          for (int32_t r = 0; r < rows; r += dc::kChunkRows) {
+            const int32_t r1 = std::min(r + dc::kChunkRows, rows);
+            const int64_t len = steps(b, r1), n = (len + per - 1) / per;
+            if (n > 1 && parts + n * (r1 - r) > INT32_MAX) return dc::fail(DC_EINVAL, "dc_plan_chunk: too many partial results");
+            const int32_t end = first + (r1 - 1) / n_q + 1;
+            if (n > 1) joins.push_back({h, q_begin, r, r1, int32_t(parts), int32_t(n)});
+            for (int64_t i = 0; i < n; ++i)
+              all.push_back({b, h, q_begin, r, r1, first, int32_t(len * i / n * step),
+                             int32_t(std::min<int64_t>(len * (i + 1) / n * step, end)), n > 1 ? int32_t(parts + i * (r1 - r)) : -1});
+            if (n > 1) parts += n * (r1 - r);
+          }
+      }
+      // A die takes a run of items of equal total length, streams kept together,
+      // the longest first; block i runs on die i % kChunkXcds.
+      auto length = [](const dc_chunk_item& x) { return int64_t(x.kv_end - x.kv_begin); };
+      int64_t sum = 0, seen = 0;
+      for (const auto& x : all) sum += length(x);
+      std::vector<std::vector<dc_chunk_item>> die(dc::kChunkXcds);
+      for (const auto& x : all) {
+        die[std::min<int64_t>((seen + length(x) / 2) * dc::kChunkXcds / std::max<int64_t>(sum, 1), dc::kChunkXcds - 1)].push_back(x);
+        seen += length(x);
+      }
+      size_t most = 0;
+      for (auto& d : die) {
+        std::stable_sort(d.begin(), d.end(), [&](const dc_chunk_item& x, const dc_chunk_item& y) { return length(x) > length(y); });
+        most = std::max(most, d.size());
+      }
+      for (size_t i = 0; i < most; ++i)
+        for (auto& d : die) order.push_back(i < d.size() ? d[i] : dc_chunk_item{-1, 0, 0, 0, 0, 0, 0, 0, -1});
+      while (!order.empty() && order.back().seq < 0) order.pop_back();
+      if (order.size() > INT32_MAX) return dc::fail(DC_EINVAL, "dc_plan_chunk: too many items");
+      if (few) *n_few = int32_t(order.size());
     }
-    // A die takes a run of items of equal total length, streams kept together,
-    // the longest first; block i runs on die i % kChunkXcds.
-    auto length = [](const dc_chunk_item& x) { return int64_t(x.kv_end - x.kv_begin); };
-    int64_t sum = 0, seen = 0;
-    for (const auto& x : all) sum += length(x);
-    std::vector<std::vector<dc_chunk_item>> die(dc::kChunkXcds);
-    for (const auto& x : all) {
-      die[std::min<int64_t>((seen + length(x) / 2) * dc::kChunkXcds / std::max<int64_t>(sum, 1), dc::kChunkXcds - 1)].push_back(x);
-      seen += length(x);
-    }
-    size_t most = 0;
-    for (auto& d : die) {
-      std::stable_sort(d.begin(), d.end(), [&](const dc_chunk_item& x, const dc_chunk_item& y) { return length(x) > length(y); });
-      most = std::max(most, d.size());
-    }
-    std::vector<dc_chunk_item> order;
-    for (size_t i = 0; i < most; ++i)
-      for (auto& d : die) order.push_back(i < d.size() ? d[i] : dc_chunk_item{-1, 0, 0, 0, 0, 0, 0, 0, -1});
-    while (!order.empty() && order.back().seq < 0) order.pop_back();
-    if (order.size() > INT32_MAX) return dc::fail(DC_EINVAL, "dc_plan_chunk: too many items");
     *n_items = int32_t(order.size());
     *n_merges = int32_t(joins.size());
     *n_partials = int32_t(parts);

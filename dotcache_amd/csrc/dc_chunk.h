@@ -10,6 +10,9 @@ constexpr int kChunkRows = 256;   // query rows of a work item
 constexpr int kChunkStep = 128;   // token ranges begin at multiples of this (a multiple of every tile)
 constexpr int kChunkXcds = 8;     // consecutive blocks go to consecutive dies, each with an L2 of its own
 
+// Rows of one item of the few-row kernel at most, by what its registers hold.
+constexpr int few_row_limit(int head_dim) { return head_dim <= 64 ? 64 : head_dim <= 128 ? 48 : 16; }
+
 struct ChunkArgs {
   dc_pool kpool, vpool;
   const int32_t* k_table;

@@ -43,6 +43,16 @@ __device__ __forceinline__ int lds_at(int t, int ch) {
   return (t * CH + (ch ^ x)) * 16;
 }
 
+// An address that the compiler takes for a new one here: what is derived from
+// it by one exclusive or is then computed where it is used, not kept in a
+// register for each use across the loop.  (Chunks are exchanged by exclusive
+// or within a row, so a chunk's address is its row's, the chunk's number
+// joined in by exclusive or too, where the numbers share no bits.)
+__device__ __forceinline__ int fresh(int x) {
+  asm volatile("" : "+v"(x));
+  return x;
+}
+
 // {a, b} of lanes 0 .. 31 and {a, b} of lanes 32 .. 63, exchanged to {a of the
 // first half, b of the first} and {a of the second, b of the second}: x is
 // what the first, y what the second half held, a in lanes 0 .. 31, b in 32 .. 63.
@@ -699,7 +709,8 @@ __global__ void __launch_bounds__(512, 2) attend_chunk16_kernel(ChunkArgs a) {
 #pragma unroll
         for (int v = 0; v < 16; ++v) s[tb][v] = 0.f;
       // (operands are read kAhead instructions ahead; the scheduler would read them one ahead)
-      auto key = [&](int n) { return *reinterpret_cast<const h8v*>(kt + lds_at<CH>(32 * (n % TB) + col, 2 * (n / TB) + half)); };
+      const int k_at = fresh(lds_at<CH>(col, half));
+      auto key = [&](int n) { return *reinterpret_cast<const h8v*>(kt + (k_at ^ (32 * (n / TB))) + 32 * (n % TB) * CH * 16); };
       h8v ka[kAhead];
 #pragma unroll
       for (int n = 0; n < kAhead; ++n) ka[n] = key(n);
@@ -744,13 +755,15 @@ __global__ void __launch_bounds__(512, 2) attend_chunk16_kernel(ChunkArgs a) {
       for (int tb = 0; tb < TB; ++tb)
 #pragma unroll
         for (int v = 0; v < 16; ++v) s[tb][v] = __builtin_amdgcn_exp2f(fmaf(s[tb][v], c, -mu));
+      const int v_at = fresh(lds_at<CH>(4 * half + ((lane & 15) >> 2), 4 * cb0 + ((lane & 16) >> 3) + ((lane & 3) >> 1)) + 8 * (lane & 1));
       auto value = [&](int n) {
-        const int t = 16 * (n / CB) + 4 * half + ((lane & 15) >> 2), ch = 32 * (cb0 + n % CB) + (lane & 16) + 4 * (lane & 3);
+        // token 16 (n / CB) + 4 half + lane % 16 / 4 (+ 8), channel 32 (cb0 + n % CB) + lane / 16 % 2 * 16 + 4 (lane % 4):
+        // eight tokens on, the row's chunks are exchanged by 2 more
         s4v x[2];
 #pragma unroll
         for (int e = 0; e < 2; ++e)
           x[e] = __builtin_amdgcn_ds_read_tr16_b64_v4i16(
-              (__attribute__((address_space(3))) s4v*)(vt + lds_at<CH>(t + 8 * e, ch / 8) + 2 * (ch % 8)));
+              (__attribute__((address_space(3))) s4v*)(vt + (v_at ^ (64 * (n % CB) + 32 * e)) + (16 * (n / CB) + 8 * e) * CH * 16));
         return __builtin_bit_cast(h8v, __builtin_shufflevector(x[0], x[1], 0, 1, 2, 3, 4, 5, 6, 7));
       };
       h8v va[kAhead];
@@ -815,6 +828,582 @@ __global__ void __launch_bounds__(512, 2) attend_chunk16_kernel(ChunkArgs a) {
     }
 }
 
+// ---- few rows -----------------------------------------------------------------
+
+namespace {
+
+typedef float f32x4 __attribute__((ext_vector_type(4)));
+constexpr int kFewTile = 32;   // tokens a wavefront takes at a time
+constexpr int kFewWaves = 4;
+
+// Loads from a page: the page's and the wavefront's part of the address in
+// scalar registers and the lane's in one vector register where the wavefront
+// shares the page (a buffer load; pointers would take two registers for each
+// load), or by pointer where each lane has its own.
+template <bool UNI>
+struct PageLoad {
+  const uint8_t* base;
+  __device__ __forceinline__ uint32_t u16(uint32_t off, uint32_t lane) const {
+    if constexpr (UNI) return uint16_t(__builtin_amdgcn_raw_buffer_load_b16(rsrc(), int(lane), int(off), 0));
+    return *reinterpret_cast<const uint16_t*>(base + off + lane);
+  }
+  __device__ __forceinline__ uint32_t u32(uint32_t off, uint32_t lane) const {
+    if constexpr (UNI) return __builtin_amdgcn_raw_buffer_load_b32(rsrc(), int(lane), int(off), 0);
+    return *reinterpret_cast<const uint32_t*>(base + off + lane);
+  }
+  __device__ __forceinline__ uint4 u128(uint32_t off, uint32_t lane) const {
+    if constexpr (UNI) return __builtin_bit_cast(uint4, __builtin_amdgcn_raw_buffer_load_b128(rsrc(), int(lane), int(off), 0));
+    return *reinterpret_cast<const uint4*>(base + off + lane);
+  }
+
+ private:
+  __device__ __forceinline__ auto rsrc() const {
+    return __builtin_amdgcn_make_buffer_rsrc(const_cast<uint8_t*>(base), 0, 0x7fffffff, 0x00027000);
+  }
+};
+
+// As lds_at, for tiles whose reads take two chunks of eight tokens at once.
+template <int CH>
+__device__ __forceinline__ int few_at(int t, int ch) {
+  const int x = CH >= 16 ? ((t & 3) << 2) | (((t >> 2) & 1) << 1) | ((t >> 3) & 1)
+                         : (((t >> 1) & 1) << 2) | (((t >> 2) & 1) << 1) | ((t >> 3) & 1);
+  return (t * CH + (ch ^ x)) * 16;
+}
+
+// Maximum over the four lanes of equal lane % 16, in all of them.
+__device__ __forceinline__ float quarter_max(float v) {
+  const uint32_t u = __builtin_bit_cast(uint32_t, v);
+  const auto r = __builtin_amdgcn_permlane16_swap(u, u, false, false);
+  const uint32_t x = r[0], y = r[1];
+  return half_max(fmaxf(__builtin_bit_cast(float, x), __builtin_bit_cast(float, y)));
+}
+__device__ __forceinline__ float quarter_sum(float v) {
+  const uint32_t u = __builtin_bit_cast(uint32_t, v);
+  const auto r = __builtin_amdgcn_permlane16_swap(u, u, false, false);
+  const uint32_t x = r[0], y = r[1];
+  return half_sum(__builtin_bit_cast(float, x) + __builtin_bit_cast(float, y));
+}
+
+// Eight values of a 4-bit word, of two 8-bit words or of four fp16 words, in LDS order.
+__device__ __forceinline__ void eight4(uint32_t r, uint32_t zero, h2v s, h2v b, uint32_t (&y)[4]) {
+#pragma unroll
+  for (int i = 0; i < 4; ++i) y[i] = scaled((r >> (4 * i)) & 0x000f000fu, zero, s, b);
+}
+__device__ __forceinline__ void eight8(uint32_t r0, uint32_t r1, uint32_t zero, h2v s, h2v b, uint32_t (&y)[4]) {
+#pragma unroll
+  for (int i = 0; i < 4; ++i) y[i] = scaled(__builtin_amdgcn_perm(r1, r0, 0x0c040c00u + 0x00010001u * i), zero, s, b);
+}
+__device__ __forceinline__ void eight_halves(uint4 r, uint32_t (&y)[4]) {
+  y[0] = __builtin_amdgcn_perm(r.z, r.x, 0x05040100u);
+  y[1] = __builtin_amdgcn_perm(r.z, r.x, 0x07060302u);
+  y[2] = __builtin_amdgcn_perm(r.w, r.y, 0x05040100u);
+  y[3] = __builtin_amdgcn_perm(r.w, r.y, 0x07060302u);
+}
+__device__ __forceinline__ uint32_t zero_of(int kind, bool affine) {
+  return twice(affine ? 0xe400u : kind == U_B4 ? 0xe407u : 0xe47fu);
+}
+
+}  // namespace
+
+// A few query rows (at most 16 NB: a decode's, or drafted tokens') against a
+// long range: bound by reading the pages, so the four wavefronts split the
+// range among them, 32 tokens at a time, and never wait for each other until
+// they join at the end.  Keys go from the page's words to the matrix operand
+// in registers (a lane's eight channels are one 4-bit word); values pass
+// through the wavefront's own LDS to be read transposed.  While a tile is
+// worked on, the next one's words are on their way.  16-row operands: S^T =
+// K Q^T leaves a row's logits in four lanes, again in the order in which the
+// values' operand is read.
+// KW: words of a key operand that are read ahead (4: also fp16 rows; 2: codes
+// only, and fp16 rows when they are needed).  UNI: a tile's tokens lie in one page.
+template <int HDP, int NB, int KW, bool UNI>
+__global__ void __launch_bounds__(64 * kFewWaves, 2) attend_few_kernel(ChunkArgs a) {
+  constexpr int CH = HDP / 8, KS = HDP / 32, CB = HDP / 16, TILE = kFewTile * HDP * 2;
+  constexpr int VC = HDP / 2, VU = VC / 32;  // a lane's value channels, in units of 32
+  constexpr int PB = UNI ? 1 : 2;            // pages that a lane follows: its tokens of each 16
+  constexpr int COMB = HDP + 4;
+  constexpr bool QL = NB * HDP >= 256;       // the queries stay in LDS (registers are for the output and the next tile)
+  extern __shared__ __attribute__((aligned(16))) uint8_t lds[];  // values of each wavefront, then queries; at the end the joined rows
+  __shared__ float ml[kFewWaves][16 * NB][2];
+  __shared__ float odd[kFewWaves][HDP];
+
+  const dc_chunk_item it = a.items[blockIdx.x];
+  if (!chunk_item_ok(it, a) || it.row_end - it.row_begin > 16 * NB) return;
+  const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int col = lane & 15, g = lane >> 4;
+  const int hd = a.kpool.geometry.head_dim, P = a.kpool.geometry.page_capacity;
+  const int rows = it.row_end - it.row_begin;
+
+  int sees[NB];
+  h8v q[QL ? 1 : NB][QL ? 1 : KS];
+  uint8_t* const ql = lds + kFewWaves * TILE;
+#pragma unroll
+  for (int n = 0; n < NB; ++n) {
+    const int row = it.row_begin + 16 * n + col;
+    const bool has_row = row < it.row_end;
+    const int tok = row / a.n_q, head = it.kv_head * a.n_q + (row - tok * a.n_q);
+    sees[n] = has_row ? it.first + tok : -1;
+    const uint16_t* p = reinterpret_cast<const uint16_t*>(a.q) + int64_t(it.q_begin + tok) * a.q_token_stride +
+                        int64_t(head) * a.q_head_stride;
+#pragma unroll
+    for (int k = 0; k < KS; ++k) {
+      const int ch = 32 * k + 8 * g;
+      uint32_t w[4] = {0, 0, 0, 0};
+      if (has_row && ch < hd) {
+        if (a.q_vec) {
+          const uint4 x = *reinterpret_cast<const uint4*>(p + ch);
+          w[0] = x.x; w[1] = x.y; w[2] = x.z; w[3] = x.w;
+        } else {
+#pragma unroll
+          for (int i = 0; i < 4; ++i) w[i] = p[ch + 2 * i] | uint32_t(p[ch + 2 * i + 1]) << 16;
+        }
+      }
+      h8v x;
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        const uint32_t bits = w[kPerm[i] / 2] >> (16 * (kPerm[i] % 2));
+        x[i] = a.dtype == DC_F16 ? __builtin_bit_cast(_Float16, uint16_t(bits)) : _Float16(__builtin_bit_cast(float, bits << 16));
+      }
+      if constexpr (!QL)
+        q[n][k] = x;
+      else if (wave == 0)
+        *reinterpret_cast<h8v*>(ql + lds_at<CH>(16 * n + col, 4 * k + g)) = x;
+    }
+  }
+  if constexpr (QL) __syncthreads();
+  auto query = [&](int n, int k, int q_at) {
+    if constexpr (QL)
+      return *reinterpret_cast<const h8v*>(ql + (q_at ^ (64 * k)) + 16 * n * CH * 16);
+    else
+      return q[n][k];
+  };
+  const int sees_first = it.first + it.row_begin / a.n_q;  // the least of the rows'
+
+  // ---- the pages: keys of token 16 b + col, channels 32 k + 8 g .. + 7; values of
+  // token lane % 32, channels VC (lane / 32) ..
+  const int64_t table = (int64_t(it.seq) * a.n_kv_heads + it.kv_head) * a.table_stride;
+  const int kt0 = UNI ? col : 0, vt0 = UNI ? (lane & 31) : 0;
+  const Side ks = make_side(a.kpool, a.k_table + table, 0, 0), vs = make_side(a.vpool, a.v_table + table, 0, 0);
+  const uint32_t kgs = a.kpool.geometry.group_size, vgs = a.vpool.geometry.group_size;
+  const uint32_t k_plane = a.kpool.geometry.layout == 0 ? P * kgs / 2 : kgs / 2;  // from a group's codes to the next one's
+  const uint32_t v_plane = a.vpool.geometry.layout == 0 ? P * vgs / 2 : vgs / 2;
+  auto uni = [](int x) { return UNI ? __builtin_amdgcn_readfirstlane(x) : x; };
+  auto token = [&](int tile, int b) { return it.kv_begin + tile * kFewTile + (UNI ? 0 : 16 * b + col); };
+  auto page_of = [&](int u) { return uint32_t((uint64_t(uint32_t(u)) * a.page_mul) >> a.page_shift); };
+  int32_t kid[PB], vid[PB];
+  uint2 kd[PB], vd[PB];
+  auto load_ids = [&](int tile) __attribute__((always_inline)) {
+#pragma unroll
+    for (int b = 0; b < PB; ++b) {
+      const int u = token(tile, b);
+      const uint32_t page = page_of(u);
+      const bool in = u < it.kv_end && page < uint32_t(a.table_stride);
+      kid[b] = ks.table[in ? page : 0];
+      vid[b] = vs.table[in ? page : 0];
+      if (!in) kid[b] = -1;
+    }
+  };
+  auto load_descs = [&]() __attribute__((always_inline)) {
+#pragma unroll
+    for (int b = 0; b < PB; ++b) {
+      const int ki = uni(kid[b]), vi = uni(vid[b]);
+      const bool in = uint32_t(ki) < uint32_t(ks.n_descs) && uint32_t(vi) < uint32_t(vs.n_descs);
+      kd[b] = reinterpret_cast<const uint2*>(ks.descs)[in ? ki : 0];
+      vd[b] = reinterpret_cast<const uint2*>(vs.descs)[in ? vi : 0];
+      if (!in) kd[b].y &= 0xffff0000u;  // (no tokens)
+    }
+  };
+  // The raw tile: where it is and what its pages hold (of the lane's tokens 16 b + col, or of all where UNI) ...
+  struct Place { const uint8_t *k, *v; int k_kind, v_kind, slot, end; bool k_affine, v_affine; };
+  Place at[PB];
+  uint32_t on = 0;  // one bit per token: it counts
+  auto locate = [&](int tile) __attribute__((always_inline)) {
+#pragma unroll
+    for (int b = 0; b < PB; ++b) {
+      const int u = token(tile, b);
+      const auto k = __builtin_bit_cast(dc_page_desc, uint2{uint32_t(uni(kd[b].x)), uint32_t(uni(kd[b].y))});
+      const auto v = __builtin_bit_cast(dc_page_desc, uint2{uint32_t(uni(vd[b].x)), uint32_t(uni(vd[b].y))});
+      Place& x = at[b];
+      x.slot = u - int(page_of(u)) * P;
+      x.k_kind = unit_kind(ks, k, P, x.slot);
+      x.v_kind = unit_kind(vs, v, P, x.slot);
+      // (tokens of the page behind its last and behind kv_end lie in its blob, but do not count)
+      x.end = min(min(int(k.tokens), int(v.tokens)) - x.slot, it.kv_end - u);
+      if (x.k_kind == U_NONE || x.v_kind == U_NONE || x.end <= 0) {
+        x.k_kind = x.v_kind = U_NONE;
+        x.end = 0;
+      }
+      x.k_affine = k.format == DC_FMT_M0_AFFINE;
+      x.v_affine = v.format == DC_FMT_M0_AFFINE;
+      x.k = ks.arena + (uint64_t(k.block) << 8);
+      x.v = vs.arena + (uint64_t(v.block) << 8);
+    }
+    if constexpr (UNI)
+      on = at[0].end >= 32 ? ~0u : (1u << at[0].end) - 1u;
+    else
+      on = uint32_t(__ballot(at[0].end > 0) & 0xffffu) | uint32_t(__ballot(at[PB - 1].end > 0) & 0xffffu) << 16;
+  };
+  // the place of the lane's value token, which is one of its key tokens: 16 (lane / 16 % 2) + col
+  auto value_place = [&]() __attribute__((always_inline)) {
+    Place x = at[0];
+    if constexpr (!UNI) {
+      const bool second = (lane & 16) != 0;
+      const Place& y = at[PB - 1];
+      x.v = second ? y.v : x.v;
+      x.v_kind = second ? y.v_kind : x.v_kind;
+      x.slot = second ? y.slot : x.slot;
+      x.v_affine = second ? y.v_affine : x.v_affine;
+    }
+    return x;
+  };
+  // ... and its words
+  uint32_t kr[2][KS][KW], vr[VU][8], k_scale[2][KS], v_scale[VU];  // (scale: fp16 scale, bias above it)
+#pragma unroll
+  for (int b = 0; b < 2; ++b)
+#pragma unroll
+    for (int k = 0; k < KS; ++k) {
+      k_scale[b][k] = 0;
+#pragma unroll
+      for (int w = 0; w < KW; ++w) kr[b][k][w] = 0;
+    }
+#pragma unroll
+  for (int u = 0; u < VU; ++u) {
+    v_scale[u] = 0;
+#pragma unroll
+    for (int w = 0; w < 8; ++w) vr[u][w] = 0;
+  }
+  // the lane's offsets in a page, from its tile's first token (from its own where its tokens lie in several pages)
+  const uint32_t k4 = kt0 * ks.token4 + 4 * g, k_sc = kt0 * ks.groups2, k16 = kt0 * ks.row2 + 16 * g;
+  const uint32_t vc0 = VC * (lane >> 5), v16 = vt0 * vs.row2 + 2 * vc0;
+  uint32_t v4[VU], v_sc[VU];
+#pragma unroll
+  for (int u = 0; u < VU; ++u) {
+    const uint32_t c = vc0 + 32 * u, gr = c / vgs;
+    v4[u] = vt0 * vs.token4 + gr * v_plane + (c - gr * vgs) / 2;
+    v_sc[u] = vt0 * vs.groups2 + 2 * gr;
+  }
+  auto load_keys = [&]() __attribute__((always_inline)) {
+#pragma unroll
+    for (int b = 0; b < 2; ++b) {
+      const Place& x = at[UNI ? 0 : b];
+      const uint32_t slot = x.slot + (UNI ? 16 * b : 0);
+      if (x.k_kind == U_F16) {
+        if constexpr (KW == 4) {
+          const PageLoad<UNI> p{x.k};
+#pragma unroll
+          for (int k = 0; k < KS; ++k)
+            if (32 * k < hd) {
+              const uint4 r = p.u128(slot * ks.row2 + 64 * k, k16);
+              kr[b][k][0] = r.x; kr[b][k][1] = r.y; kr[b][k][2] = r.z; kr[b][k][3] = r.w;
+            }
+        }
+      } else if (x.k_kind != U_NONE) {
+        const uint32_t sh = x.k_kind == U_B8, off = k4 << sh;
+        const PageLoad<UNI> p{x.k};
+        const uint32_t codes = (slot * ks.token4) << sh, scales = (ks.scales4 << sh) + slot * ks.groups2;
+        const uint32_t gap = x.k_affine ? ks.gap : 0, keep = x.k_affine ? 0xffff0000u : 0u;
+#pragma unroll
+        for (int k = 0; k < KS; ++k)
+          if (32 * k < hd) {
+            const uint32_t gr = 32 * k / kgs, o = (gr * k_plane + (32 * k - gr * kgs) / 2) << sh;
+            // (no else: stores that two branches make to different words would keep the array in memory)
+            kr[b][k][0] = p.u32(codes + o, off);
+            if (sh) kr[b][k][1] = p.u32(codes + o + 4, off);
+            const uint32_t s = p.u16(scales + 2 * gr, k_sc), z = p.u16(scales + 2 * gr + gap, k_sc);
+            k_scale[b][k] = s | ((z << 16) & keep);
+          }
+      }
+    }
+  };
+  auto load_values = [&]() __attribute__((always_inline)) {
+    const Place x = value_place();
+    if (x.v_kind == U_NONE || x.v_kind == U_F16) return;
+    const uint32_t sh = x.v_kind == U_B8;
+    const PageLoad<UNI> p{x.v};
+    const uint32_t codes = (x.slot * vs.token4) << sh, scales = (vs.scales4 << sh) + x.slot * vs.groups2;
+    const uint32_t gap = x.v_affine ? vs.gap : 0, keep = x.v_affine ? 0xffff0000u : 0u;
+#pragma unroll
+    for (int u = 0; u < VU; ++u)
+      if (int(vc0 + 32 * u) < hd) {
+        const uint4 r = p.u128(codes, v4[u] << sh);
+        vr[u][0] = r.x; vr[u][1] = r.y; vr[u][2] = r.z; vr[u][3] = r.w;
+        if (sh) {
+          const uint4 y = p.u128(codes + 16, v4[u] << 1);
+          vr[u][4] = y.x; vr[u][5] = y.y; vr[u][6] = y.z; vr[u][7] = y.w;
+        }
+        const uint32_t s = p.u16(scales, v_sc[u]), z = p.u16(scales + gap, v_sc[u]);
+        v_scale[u] = s | ((z << 16) & keep);
+      }
+  };
+
+  const int all = (it.kv_end - it.kv_begin + kFewTile - 1) / kFewTile;
+  uint8_t* const vt = lds + wave * TILE;
+  const float c = a.scale * kLog2e;
+  float m[NB], l[NB];
+  f32x4 o[NB][CB];
+#pragma unroll
+  for (int n = 0; n < NB; ++n) {
+    m[n] = -INFINITY;
+    l[n] = 0.f;
+#pragma unroll
+    for (int j = 0; j < CB; ++j) o[n][j] = f32x4{0.f, 0.f, 0.f, 0.f};
+  }
+  load_ids(wave);
+  load_descs();
+  locate(wave);
+  load_values();
+  load_keys();
+  load_ids(wave + kFewWaves);
+  load_descs();
+  load_ids(wave + 2 * kFewWaves);
+  for (int i = wave; i < all; i += kFewWaves) {
+    const int u0 = it.kv_begin + i * kFewTile;
+    const bool border = u0 + kFewTile - 1 > sees_first;  // (uniform)
+    const uint32_t live = on;
+    // ---- values to LDS
+    uint32_t bad = 0;
+    {
+      const Place x = value_place();
+      const bool counts = ((live >> (lane & 31)) & 1) != 0;
+      const uint32_t zero = zero_of(x.v_kind, x.v_affine);
+      const int w_at = fresh(few_at<CH>(lane & 31, vc0 / 8));
+#pragma unroll
+      for (int u = 0; u < VU; ++u) {
+        uint32_t y[4][4];
+        const bool in = int(vc0 + 32 * u) < hd;
+        const h2v s = __builtin_bit_cast(h2v, twice(v_scale[u] & 0xffffu)), b = __builtin_bit_cast(h2v, twice(v_scale[u] >> 16));
+        if (x.v_kind == U_B4) {
+#pragma unroll
+          for (int e = 0; e < 4; ++e) eight4(vr[u][e], zero, s, b, y[e]);
+        } else if (x.v_kind == U_B8) {
+#pragma unroll
+          for (int e = 0; e < 4; ++e) eight8(vr[u][2 * e], vr[u][2 * e + 1], zero, s, b, y[e]);
+        } else if (x.v_kind == U_F16 && in) {
+          const PageLoad<UNI> p{x.v};
+#pragma unroll
+          for (int e = 0; e < 4; ++e) eight_halves(p.u128(x.slot * vs.row2 + 64 * u + 16 * e, v16), y[e]);
+        } else {
+#pragma unroll
+          for (int e = 0; e < 4; ++e) y[e][0] = y[e][1] = y[e][2] = y[e][3] = 0;
+        }
+        if (live != ~0u || HDP > hd) {
+          const bool keep = counts && in;
+#pragma unroll
+          for (int e = 0; e < 4; ++e)
+#pragma unroll
+            for (int k = 0; k < 4; ++k) y[e][k] = keep ? y[e][k] : 0;
+        }
+        if (border) {
+#pragma unroll
+          for (int e = 0; e < 4; ++e)
+#pragma unroll
+            for (int k = 0; k < 4; ++k) {
+              const uint32_t f = ((y[e][k] & 0x7fff7fffu) + 0x04000400u) & 0x80008000u;  // sign bits: not finite
+              bad |= f;
+              y[e][k] &= ~((f >> 15) * 0xffffu);
+            }
+        }
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+          *reinterpret_cast<uint4*>(vt + (w_at ^ (64 * u + 16 * e))) = uint4{y[e][0], y[e][1], y[e][2], y[e][3]};
+      }
+    }
+    // ---- S^T
+    uint32_t y[2][KS][4];  // the keys' operands
+#pragma unroll
+    for (int b = 0; b < 2; ++b) {
+      const Place& x = at[UNI ? 0 : b];
+      const uint32_t zero = zero_of(x.k_kind, x.k_affine);
+      if (x.k_kind == U_B4) {
+#pragma unroll
+        for (int k = 0; k < KS; ++k)
+          eight4(kr[b][k][0], zero, __builtin_bit_cast(h2v, twice(k_scale[b][k] & 0xffffu)), __builtin_bit_cast(h2v, twice(k_scale[b][k] >> 16)), y[b][k]);
+      } else if (x.k_kind == U_B8) {
+#pragma unroll
+        for (int k = 0; k < KS; ++k)
+          eight8(kr[b][k][0], kr[b][k][1], zero, __builtin_bit_cast(h2v, twice(k_scale[b][k] & 0xffffu)),
+                 __builtin_bit_cast(h2v, twice(k_scale[b][k] >> 16)), y[b][k]);
+      } else if (x.k_kind == U_F16) {
+        if constexpr (KW == 4) {
+#pragma unroll
+          for (int k = 0; k < KS; ++k) eight_halves(uint4{kr[b][k][0], kr[b][k][1], kr[b][k][2], kr[b][k][3]}, y[b][k]);
+        } else {
+          const PageLoad<UNI> p{x.k};
+          const uint32_t rows = (x.slot + (UNI ? 16 * b : 0)) * ks.row2;
+#pragma unroll
+          for (int k = 0; k < KS; ++k) eight_halves(p.u128(rows + (32 * k < hd ? 64 * k : 0), k16), y[b][k]);
+        }
+      } else {
+#pragma unroll
+        for (int k = 0; k < KS; ++k) y[b][k][0] = y[b][k][1] = y[b][k][2] = y[b][k][3] = 0;
+      }
+    }
+    const int q_at = fresh(lds_at<CH>(col, g));
+    f32x4 s[NB][2];
+#pragma unroll
+    for (int n = 0; n < NB; ++n) s[n][0] = s[n][1] = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+    for (int k = 0; k < KS; ++k) {
+      if (HDP > 64 && 32 * k >= hd) break;  // (uniform; channels past head_dim)
+#pragma unroll
+      for (int n = 0; n < NB; ++n) {
+        const h8v x = query(n, k, q_at);
+#pragma unroll
+        for (int b = 0; b < 2; ++b)
+          s[n][b] = __builtin_amdgcn_mfma_f32_16x16x32_f16(
+              __builtin_bit_cast(h8v, uint4{y[b][k][0], y[b][k][1], y[b][k][2], y[b][k][3]}), x, s[n][b], 0, 0, 0);
+      }
+    }
+    locate(i + kFewWaves);
+    load_values();
+    load_keys();
+    load_descs();
+    load_ids(i + 3 * kFewWaves);
+    // ---- softmax: tokens 16 b + 4 g + v of row col of each block
+    h8v p[NB];
+#pragma unroll
+    for (int n = 0; n < NB; ++n) {
+      if (border || live != ~0u) {
+#pragma unroll
+        for (int b = 0; b < 2; ++b)
+#pragma unroll
+          for (int v = 0; v < 4; ++v) {
+            const int t = 16 * b + 4 * g + v;
+            s[n][b][v] = ((live >> t) & 1) && u0 + t <= sees[n] ? s[n][b][v] : -INFINITY;
+          }
+      }
+      float top = fmaxf(fmaxf(fmaxf(s[n][0][0], s[n][0][1]), fmaxf(s[n][0][2], s[n][0][3])),
+                        fmaxf(fmaxf(s[n][1][0], s[n][1][1]), fmaxf(s[n][1][2], s[n][1][3])));
+      top = quarter_max(top) * c;
+      if (__any(top > m[n] + kLazy || (m[n] == -INFINITY && top > m[n]))) {
+        const float mn = fmaxf(m[n], top);
+        const float f = mn == -INFINITY ? 1.f : __builtin_amdgcn_exp2f(m[n] - mn);
+        m[n] = mn;
+        l[n] *= f;
+#pragma unroll
+        for (int j = 0; j < CB; ++j) o[n][j] *= f;
+      }
+      const float mu = m[n] == -INFINITY ? 0.f : m[n];
+#pragma unroll
+      for (int v = 0; v < 8; v += 2) {
+        const h2v e = {(_Float16)__builtin_amdgcn_exp2f(fmaf(s[n][v / 4][v % 4], c, -mu)),
+                       (_Float16)__builtin_amdgcn_exp2f(fmaf(s[n][v / 4][v % 4 + 1], c, -mu))};
+        l[n] = __builtin_amdgcn_fdot2(e, h2v{(_Float16)1.f, (_Float16)1.f}, l[n], false);
+        p[n][v] = e[0];
+        p[n][v + 1] = e[1];
+      }
+    }
+    // ---- values that are not finite, to the rows that see them
+    if (border) {
+      uint64_t who = __ballot(bad != 0);
+      for (uint32_t bits = uint32_t(who) | uint32_t(who >> 32); bits != 0; bits &= bits - 1) {
+        const int u = u0 + __builtin_ctz(bits), page = u / P;
+        const dc_page_desc d = a.vpool.descs[vs.table[page]];
+        const BlobLayout L = blob_layout(d.format, d.bits, a.vpool.geometry);
+        for (int ch = lane; ch < HDP; ch += 64)
+          odd[wave][ch] = ch < hd ? float(_Float16(page_value(blob_ptr(a.vpool.arena, d), d, L, a.vpool.geometry, u - page * P, ch))) : 0.f;
+        __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+#pragma unroll
+        for (int j = 0; j < CB; ++j)
+#pragma unroll
+          for (int v = 0; v < 4; ++v) {
+            const float x = odd[wave][16 * j + 8 * (g / 2) + kPerm[4 * (g % 2) + v]];
+#pragma unroll
+            for (int n = 0; n < NB; ++n)
+              if (u <= sees[n] && !__builtin_isfinite(x)) o[n][j][v] += x;
+          }
+        __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+      }
+    }
+    // ---- O^T
+    const int v_at = fresh(few_at<CH>(4 * g + ((lane & 15) >> 2), (lane & 3) >> 1) + 8 * (lane & 1));
+    auto value = [&](int j) {  // tokens 4 g .. + 3 and 16 on, channels 16 j ..
+      s4v x[2];
+#pragma unroll
+      for (int e = 0; e < 2; ++e)
+        x[e] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s4v*)(vt + (v_at ^ (32 * j)) + 16 * e * CH * 16));
+      return __builtin_bit_cast(h8v, __builtin_shufflevector(x[0], x[1], 0, 1, 2, 3, 4, 5, 6, 7));
+    };
+    h8v va[kAhead];
+#pragma unroll
+    for (int j = 0; j < kAhead; ++j) va[j] = value(j);
+#pragma unroll
+    for (int j = 0; j < CB; ++j) {
+      __builtin_amdgcn_sched_barrier(0x6);  // (vector and scalar arithmetic may cross)
+#pragma unroll
+      for (int n = 0; n < NB; ++n) o[n][j] = __builtin_amdgcn_mfma_f32_16x16x32_f16(va[j % kAhead], p[n], o[n][j], 0, 0, 0);
+      if (j + kAhead < CB) va[j % kAhead] = value(j + kAhead);
+    }
+  }
+  // ---- join the wavefronts, in order
+  float* const comb = reinterpret_cast<float*>(lds);
+#pragma unroll
+  for (int n = 0; n < NB; ++n) {
+    l[n] = quarter_sum(l[n]);
+    if (g == 0) {
+      ml[wave][16 * n + col][0] = m[n];
+      ml[wave][16 * n + col][1] = l[n];
+    }
+  }
+  __syncthreads();
+  for (int w = 0; w < kFewWaves; ++w) {
+    if (wave == w) {
+#pragma unroll
+      for (int n = 0; n < NB; ++n) {
+        const int r = 16 * n + col;
+        const float top = fmaxf(fmaxf(ml[0][r][0], ml[1][r][0]), fmaxf(ml[2][r][0], ml[3][r][0]));
+        const float f = m[n] == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(m[n] - top);
+#pragma unroll
+        for (int j = 0; j < CB; ++j)
+#pragma unroll
+          for (int v = 0; v < 4; ++v) {
+            float& x = comb[r * COMB + 16 * j + 8 * (g / 2) + kPerm[4 * (g % 2) + v]];
+            // (a wavefront that saw no token holds zeros, or what a value that is not finite left)
+            const float y = m[n] == -INFINITY ? o[n][j][v] : o[n][j][v] * f;
+            x = w == 0 ? y : x + y;
+          }
+      }
+    }
+    __syncthreads();
+  }
+  const bool part = it.partial >= 0;
+  for (int i = tid; i < rows * (HDP / 4); i += 64 * kFewWaves) {
+    const int r = i / (HDP / 4), ch = 4 * (i % (HDP / 4));
+    if (ch >= hd) continue;
+    const float top = fmaxf(fmaxf(ml[0][r][0], ml[1][r][0]), fmaxf(ml[2][r][0], ml[3][r][0]));
+    float sum = 0.f;
+#pragma unroll
+    for (int w = 0; w < kFewWaves; ++w)
+      sum += ml[w][r][0] == -INFINITY ? ml[w][r][1] : ml[w][r][1] * __builtin_amdgcn_exp2f(ml[w][r][0] - top);
+    const float4 x = *reinterpret_cast<const float4*>(comb + r * COMB + ch);
+    if (part) {
+      const int64_t pr = int64_t(it.partial) + r;
+      *reinterpret_cast<float4*>(a.part_o + pr * hd + ch) = x;
+      if (ch == 0) {
+        a.part_ml[2 * pr] = top;
+        a.part_ml[2 * pr + 1] = sum;
+      }
+      continue;
+    }
+    const float inv = sum == 0.f ? 0.f : 1.f / sum;
+    const int row = it.row_begin + r, tok = row / a.n_q, head = it.kv_head * a.n_q + (row - tok * a.n_q);
+    uint16_t* const out = reinterpret_cast<uint16_t*>(a.out) + int64_t(it.q_begin + tok) * a.o_token_stride +
+                          int64_t(head) * a.o_head_stride + ch;
+    const float v[4] = {x.x * inv, x.y * inv, x.z * inv, x.w * inv};
+    uint32_t w[2];
+#pragma unroll
+    for (int k = 0; k < 2; ++k)
+      w[k] = a.dtype == DC_F16 ? __builtin_bit_cast(uint32_t, h2v{(_Float16)v[2 * k], (_Float16)v[2 * k + 1]})
+                               : __builtin_bit_cast(uint32_t, b2v{(__bf16)v[2 * k], (__bf16)v[2 * k + 1]});
+    if (a.o_vec) {
+      *reinterpret_cast<uint2*>(out) = uint2{w[0], w[1]};
+    } else {
+#pragma unroll
+      for (int k = 0; k < 4; ++k) out[k] = uint16_t(w[k / 2] >> (16 * (k % 2)));
+    }
+  }
+}
+
 // Joins the partial results of a row tile's token ranges: a wavefront per row,
 // channels over its lanes.
 __global__ void __launch_bounds__(256) merge_chunk_kernel(ChunkArgs a, const dc_chunk_merge* merges) {
@@ -866,6 +1455,22 @@ static int launch_chunk16(const ChunkArgs& a, hipStream_t stream) {
                                                         : launch_chunk16_as<HDP, KT, false, CS>(a, stream);
 }
 
+template <int HDP, int NB, int KW, bool UNI>
+static int launch_few_as(const ChunkArgs& a, hipStream_t stream) {
+  constexpr int tiles = kFewWaves * kFewTile * HDP * 2 + (NB * HDP >= 256 ? 16 * NB * HDP * 2 : 0), joined = 16 * NB * (HDP + 4) * 4, bytes = tiles > joined ? tiles : joined;
+  static const hipError_t set = hipFuncSetAttribute(reinterpret_cast<const void*>(&attend_few_kernel<HDP, NB, KW, UNI>),
+                                                    hipFuncAttributeMaxDynamicSharedMemorySize, bytes);
+  if (int rc = check_hip(set, "attend_few_kernel LDS")) return rc;
+  hipLaunchKernelGGL((attend_few_kernel<HDP, NB, KW, UNI>), dim3(a.n_items), dim3(64 * kFewWaves), bytes, stream, a);
+  return check_hip(hipGetLastError(), "attend_few_kernel launch");
+}
+
+template <int HDP, int NB, int KW>
+static int launch_few(const ChunkArgs& a, hipStream_t stream) {
+  return a.kpool.geometry.page_capacity % kFewTile == 0 ? launch_few_as<HDP, NB, KW, true>(a, stream)
+                                                        : launch_few_as<HDP, NB, KW, false>(a, stream);
+}
+
 // Whether a thread's 32 channels share a scale and lie at 16-byte multiples,
 // with offsets in a blob that fit 32 bits, in the formats that load_raw takes.
 static bool units32(const dc_pool& p) {
@@ -879,7 +1484,7 @@ static bool units32(const dc_pool& p) {
 }  // namespace dc
 
 extern "C" int dc_attend_chunk(dc_pool k_pool, dc_pool v_pool, const int32_t* k_table, const int32_t* v_table,
-                               int32_t table_stride, const dc_chunk_item* items, int32_t n_items,
+                               int32_t table_stride, const dc_chunk_item* items, int32_t n_items, int32_t n_few, int32_t few_rows,
                                const dc_chunk_merge* merges, int32_t n_merges, int32_t n_partials, int32_t n_seqs,
                                int32_t n_kv_heads, int64_t n_tokens, dc_token_rows q, float query_scale, dc_token_rows out,
                                void* workspace, int64_t workspace_bytes, dc_stream_t stream) {
@@ -890,6 +1495,8 @@ extern "C" int dc_attend_chunk(dc_pool k_pool, dc_pool v_pool, const int32_t* k_
   if (v_pool.geometry.head_dim != hd || v_pool.geometry.page_capacity != k_pool.geometry.page_capacity)
     return dc::fail(DC_EINVAL, "%s: key and value pools must share head_dim and page_capacity", who);
   if (hd > 256) return dc::fail(DC_EINVAL, "%s: head_dim above 256", who);
+  if (n_few < 0 || n_few > n_items || (n_few && (few_rows <= 0 || few_rows > dc::few_row_limit(hd))))
+    return dc::fail(DC_EINVAL, "%s: n_few must lie in [0, n_items], their rows in [1, %d]", who, dc::few_row_limit(hd));
   if (n_items < 0 || n_merges < 0 || n_partials < 0 || n_seqs <= 0 || n_kv_heads <= 0 || n_tokens < 0 || table_stride <= 0)
     return dc::fail(DC_EINVAL, "%s: bad counts", who);
   if (n_items == 0) return DC_OK;
@@ -913,8 +1520,22 @@ extern "C" int dc_attend_chunk(dc_pool k_pool, dc_pool v_pool, const int32_t* k_
   a.page_shift = 31;
   while ((1u << (a.page_shift - 31)) < P) ++a.page_shift;
   a.page_mul = uint32_t(((uint64_t(1) << a.page_shift) + P - 1) / P);
-  int rc;
-  if (q.dtype != DC_F32 && dc::units32(k_pool) && dc::units32(v_pool))
+  int rc = DC_OK;
+  const bool units = q.dtype != DC_F32 && dc::units32(k_pool) && dc::units32(v_pool);
+  if (units && n_few) {
+    dc::ChunkArgs f = a;
+    f.n_items = n_few;
+    const bool one = few_rows <= 16;
+    rc = hd <= 64    ? (one ? dc::launch_few<64, 1, 4>(f, st) : dc::launch_few<64, 4, 4>(f, st))
+         : hd <= 128 ? (one ? dc::launch_few<128, 1, 4>(f, st) : few_rows <= 32 ? dc::launch_few<128, 2, 4>(f, st) : dc::launch_few<128, 3, 2>(f, st))
+                     : dc::launch_few<256, 1, 2>(f, st);
+    a.items += n_few;
+    a.n_items -= n_few;
+  }
+  if (rc != DC_OK) return rc;
+  if (a.n_items == 0)
+    ;
+  else if (units)
     rc = hd <= 64 ? dc::launch_chunk16<64, 128, 1>(a, st) : hd <= 128 ? dc::launch_chunk16<128, 64, 1>(a, st) : dc::launch_chunk16<256, 32, 2>(a, st);
   else if (q.dtype == DC_F32)
     rc = hd <= 64 ? dc::launch_chunk<float, 64, 64>(a, st) : hd <= 128 ? dc::launch_chunk<float, 128, 32>(a, st) : dc::launch_chunk<float, 256, 32>(a, st);

@@ -29,6 +29,8 @@ def test_items_cover_every_row_and_token_once(new, ctx, target):
     plan = _plan(new, ctx, H, n_q, target_items=target)
     start = np.concatenate([[0], np.cumsum(new)])
     items = [dict(zip(_lib.CHUNK_ITEM_FIELDS, x)) for x in plan.host_items.tolist()]
+    assert all(x["row_end"] <= plan.few_rows <= 64 for x in items[: plan.n_few])
+    assert all(x["row_end"] - x["row_begin"] > 64 or x["row_begin"] > 0 for x in items[plan.n_few:] if x["seq"] >= 0)
     items = [x for x in items if x["seq"] >= 0]
     seen, slots = {}, set()
     for x in items:
@@ -61,10 +63,12 @@ def test_items_cover_every_row_and_token_once(new, ctx, target):
 
 def test_equal_work_on_every_die():
     """Consecutive items go to consecutive dies: each takes an equal share."""
-    plan = _plan([2048], [16384], 4, 7, target_items=512)
+    plan = _plan([2048, 3], [16384, 20000], 4, 7, target_items=512)
     length = plan.host_items[:, 7] - plan.host_items[:, 6]
-    share = [int(length[i::8].sum()) for i in range(8)]
-    assert max(share) - min(share) <= 2 * int(length.max())
+    assert 0 < plan.n_few < plan.n_items and plan.few_rows == 21
+    for part in (length[: plan.n_few], length[plan.n_few:]):
+        share = [int(part[i::8].sum()) for i in range(8)]
+        assert max(share) - min(share) <= 2 * int(part.max())
 
 
 def test_plan_refusals():
@@ -78,12 +82,13 @@ def test_plan_refusals():
     with pytest.raises(ValueError):
         plan_chunk(_pools()[0], _pools(P=32)[0], [1], [1], kv_heads=1, q_per_kv=1)
     n = np.ones(1, dtype=np.int32)
-    c = [C.c_int32() for _ in range(3)]
-    tail = (C.byref(c[0]), None, 0, C.byref(c[1]), C.byref(c[2]))
+    c = [C.c_int32() for _ in range(5)]
+    tail = (*(C.byref(x) for x in c[:3]), None, 0, C.byref(c[3]), C.byref(c[4]))
     plan = _lib.lib().dc_plan_chunk
-    assert plan(n.ctypes.data, n.ctypes.data, 1, 2, 3, 8, 256, None, 0, *tail) == _lib.DC_ESPACE and c[0].value >= 2
-    assert plan(None, n.ctypes.data, 1, 2, 3, 8, 256, None, 0, *tail) == _lib.DC_EINVAL
-    assert plan(n.ctypes.data, n.ctypes.data, 1, 2, 3, 8, 0, None, 0, *tail) == _lib.DC_EINVAL
+    assert plan(n.ctypes.data, n.ctypes.data, 1, 2, 3, 64, 8, 256, None, 0, *tail) == _lib.DC_ESPACE and c[0].value >= 2
+    assert plan(None, n.ctypes.data, 1, 2, 3, 64, 8, 256, None, 0, *tail) == _lib.DC_EINVAL
+    assert plan(n.ctypes.data, n.ctypes.data, 1, 2, 3, 64, 8, 0, None, 0, *tail) == _lib.DC_EINVAL
+    assert plan(n.ctypes.data, n.ctypes.data, 1, 2, 3, 0, 8, 256, None, 0, *tail) == _lib.DC_EINVAL
 
 
 def test_attend_refusals():
@@ -113,16 +118,16 @@ def test_c_entry_refusals():
     pool = lambda **kw: _lib.Pool(**(dict(arena=4096, arena_bytes=1 << 20, descs=4096, n_descs=4, geometry=geo) | kw))  # noqa: E731
     rows = lambda **kw: _lib.TokenRows(**(dict(data=4096, token_stride=64, head_stride=64, n_heads=2, dtype=1) | kw))  # noqa: E731
 
-    def go(kp=pool(), vp=pool(), kt=4096, vt=4096, stride=1, items=4096, n_items=0, merges=None, n_merges=0, parts=0, B=1, H=1, T=1,
+    def go(kp=pool(), vp=pool(), kt=4096, vt=4096, stride=1, items=4096, n_items=0, few=0, few_rows=0, merges=None, n_merges=0, parts=0, B=1, H=1, T=1,
            q=rows(), out=rows(), ws=None, size=0):
-        return _lib.lib().dc_attend_chunk(kp, vp, kt, vt, stride, items, n_items, merges, n_merges, parts, B, H, T, q, 1.0, out, ws, size, None)
+        return _lib.lib().dc_attend_chunk(kp, vp, kt, vt, stride, items, n_items, few, few_rows, merges, n_merges, parts, B, H, T, q, 1.0, out, ws, size, None)
 
     assert go() == _lib.DC_OK
     for bad in (dict(kp=pool(geometry=_lib.geometry(512, 32, 16)), vp=pool(geometry=_lib.geometry(512, 32, 16))),
                 dict(vp=pool(geometry=_lib.geometry(32, 32, 16))), dict(vp=pool(geometry=_lib.geometry(64, 32, 32))), dict(n_items=-1),
                 dict(B=0), dict(stride=0), dict(n_items=1, kt=None), dict(n_items=1, items=None), dict(n_items=1, n_merges=1),
                 dict(n_items=1, q=rows(dtype=4)), dict(n_items=1, out=rows(dtype=0)), dict(n_items=1, out=rows(n_heads=1)),
-                dict(n_items=1, H=3), dict(n_items=1, kp=pool(descs=None))):
+                dict(n_items=1, H=3), dict(n_items=1, few=2, few_rows=1), dict(n_items=1, few=1), dict(n_items=1, few=1, few_rows=65), dict(few=-1), dict(n_items=1, kp=pool(descs=None))):
         assert go(**bad) == _lib.DC_EINVAL, bad
     assert go(n_items=1, parts=1, ws=4096, size=16) == _lib.DC_ESPACE
     assert go(n_items=1, parts=1, ws=None, size=1 << 20) == _lib.DC_ESPACE
