@@ -418,9 +418,10 @@ __device__ __forceinline__ Side make_side(const dc_pool& p, const int32_t* table
   x.f16_bytes = C * geo.head_dim * 2;
   x.row2 = 2 * geo.head_dim;
   x.groups2 = 2 * G;
-  x.at4 = lt * x.token4 + g * (geo.layout == 0 ? C * row : row) + (c0 - g * gs) / 2;
-  x.scale_at = (lt * G + g) * 2;
-  x.f16_at = (lt * geo.head_dim + c0) * 2;
+  const bool in = int(c0) < geo.head_dim;  // (channels past head_dim: any of the page's)
+  x.at4 = lt * x.token4 + (in ? g * (geo.layout == 0 ? C * row : row) + (c0 - g * gs) / 2 : 0);
+  x.scale_at = (lt * G + (in ? g : 0)) * 2;
+  x.f16_at = (lt * geo.head_dim + (in ? c0 : 0)) * 2;
   return x;
 }
 
@@ -437,33 +438,55 @@ __device__ __forceinline__ int unit_kind(const Side& x, const dc_page_desc& d, i
   return !ok ? U_NONE : d.format == DC_FMT_M3_F16 ? U_F16 : !m0 ? U_NONE : b8 ? U_B8 : d.bits == 4 ? U_B4 : U_NONE;
 }
 
-// The unit's bytes: r, and scale and bias (0 where there is none).
-__device__ __forceinline__ void load_unit(const Side& x, const dc_page_desc& d, int kind, uint32_t slot, uint32_t (&r)[8],
-                                          uint32_t& scale, uint32_t& bias) {
-  const uint8_t* blob = x.arena + (uint64_t(d.block) << 8);
-  auto put4 = [&](int i, const uint8_t* p) __attribute__((always_inline)) {
-    const uint4 v = *reinterpret_cast<const uint4*>(p);
-    r[i] = v.x; r[i + 1] = v.y; r[i + 2] = v.z; r[i + 3] = v.w;
-  };
-  if (kind == U_F16) {
-    const uint8_t* p = blob + slot * x.row2 + x.f16_at;
-    put4(0, p);
-    put4(4, p + 16);
-  } else if (kind != U_NONE) {
-    const uint32_t sh = kind == U_B8;
-    const uint8_t* p = blob + ((slot * x.token4) << sh) + (x.at4 << sh);
-    if (kind == U_B8) {
-      put4(0, p);
-    } else {
-      const uint2 v = *reinterpret_cast<const uint2*>(p);
-      r[0] = v.x; r[1] = v.y;
-    }
-    const uint8_t* sp = blob + (x.scales4 << sh) + slot * x.groups2 + x.scale_at;
-    const bool affine = d.format == DC_FMT_M0_AFFINE;
-    scale = *reinterpret_cast<const uint16_t*>(sp);
-    const uint32_t b = *reinterpret_cast<const uint16_t*>(sp + (affine ? x.gap : 0));
-    bias = affine ? b : 0;
+// Loads from a page: the page's and the wavefront's part of the address in
+// scalar registers and the lane's in one vector register where the wavefront
+// shares the page (a buffer load; pointers would take two registers for each
+// load), or by pointer where each lane has its own.  Every load is made
+// whatever the page holds, `ok` false from nowhere (zeros) or from `none`: a
+// register that two branches load would be waited for where they meet.
+template <bool UNI>
+struct PageLoad {
+  const uint8_t* base;
+  const void* none;
+  bool ok;
+  __device__ __forceinline__ uint32_t u16(uint32_t off, uint32_t lane) const {
+    if constexpr (UNI) return uint16_t(__builtin_amdgcn_raw_buffer_load_b16(rsrc(), int(lane), int(ok ? off : 0), 0));
+    return *static_cast<const uint16_t*>(at(off, lane));
   }
+  __device__ __forceinline__ uint2 u64(uint32_t off, uint32_t lane) const {
+    if constexpr (UNI) return __builtin_bit_cast(uint2, __builtin_amdgcn_raw_buffer_load_b64(rsrc(), int(lane), int(ok ? off : 0), 0));
+    return uint2{static_cast<const uint32_t*>(at(off, lane))[0], static_cast<const uint32_t*>(at(off, lane))[1]};
+  }
+  __device__ __forceinline__ uint4 u128(uint32_t off, uint32_t lane) const {
+    if constexpr (UNI) return __builtin_bit_cast(uint4, __builtin_amdgcn_raw_buffer_load_b128(rsrc(), int(lane), int(ok ? off : 0), 0));
+    const uint32_t* p = static_cast<const uint32_t*>(at(off, lane));
+    return uint4{p[0], p[1], p[2], p[3]};
+  }
+
+ private:
+  __device__ __forceinline__ auto rsrc() const {
+    return __builtin_amdgcn_make_buffer_rsrc(const_cast<uint8_t*>(base), 0, ok ? 0x7fffffff : 0, 0x00027000);
+  }
+  __device__ __forceinline__ const void* at(uint32_t off, uint32_t lane) const { return ok ? base + off + lane : none; }
+};
+
+// The unit's bytes: r (a 4-bit unit's are the first two words), and scale and
+// bias (0 where there is none).  A 4-bit unit's 16-byte read ends in the
+// scales at the latest.
+template <bool UNI>
+__device__ __forceinline__ void load_unit(const Side& x, const uint8_t* blob, const void* none, int kind, bool affine, uint32_t slot,
+                                          uint32_t (&r)[8], uint32_t& scale, uint32_t& bias) {
+  const PageLoad<UNI> p{blob, none, kind != U_NONE};
+  const bool f16 = kind == U_F16;
+  const uint32_t sh = kind == U_B8;
+  const uint32_t off = f16 ? slot * x.row2 : (slot * x.token4) << sh, lane = f16 ? x.f16_at : x.at4 << sh;
+  const uint4 u = p.u128(off, lane), v = p.u128(off + (f16 ? 16 : 0), lane);
+  r[0] = u.x; r[1] = u.y; r[2] = u.z; r[3] = u.w;
+  r[4] = v.x; r[5] = v.y; r[6] = v.z; r[7] = v.w;
+  const uint32_t so = f16 ? 0 : (x.scales4 << sh) + slot * x.groups2, sl = f16 ? 0 : x.scale_at;
+  scale = p.u16(so, sl);
+  bias = p.u16(so + (affine ? x.gap : 0), sl);
+  bias = affine ? bias : 0;
 }
 
 __device__ __forceinline__ uint32_t scaled(uint32_t codes, uint32_t zero, h2v s, h2v b) {
@@ -493,6 +516,48 @@ __device__ __forceinline__ void unit_values(int kind, bool affine, const uint32_
   }
 }
 
+// N groups of eight channels of a query row, from channel c0 in steps of `step`.
+template <int N>
+__device__ __forceinline__ void load_rows(const ChunkArgs& a, const uint16_t* p, int c0, int step, bool has_row, int hd,
+                                          uint32_t (&w)[N][4]) {
+  if (a.q_vec) {
+#pragma unroll
+    for (int k = 0; k < N; ++k) {
+      const int ch = c0 + step * k;
+      const uint4 x = *reinterpret_cast<const uint4*>(p + (has_row && ch < hd ? ch : 0));
+      w[k][0] = x.x; w[k][1] = x.y; w[k][2] = x.z; w[k][3] = x.w;
+    }
+  } else {
+#pragma unroll
+    for (int k = 0; k < N; ++k)
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const int ch = (has_row && c0 + step * k < hd ? c0 + step * k : 0) + 2 * i;
+        w[k][i] = p[ch] | uint32_t(p[ch + 1]) << 16;
+      }
+  }
+#pragma unroll
+  for (int k = 0; k < N; ++k)
+#pragma unroll
+    for (int i = 0; i < 4; ++i) w[k][i] = has_row && c0 + step * k < hd ? w[k][i] : 0;
+}
+
+// Them as fp16 matrix operands, in LDS order.
+template <int N>
+__device__ __forceinline__ void to_operands(bool f16, const uint32_t (&w)[N][4], h8v (&q)[N]) {
+  if (f16) {
+#pragma unroll
+    for (int k = 0; k < N; ++k)
+#pragma unroll
+      for (int i = 0; i < 8; ++i) q[k][i] = __builtin_bit_cast(_Float16, uint16_t(w[k][kPerm[i] / 2] >> (16 * (kPerm[i] % 2))));
+  } else {
+#pragma unroll
+    for (int k = 0; k < N; ++k)
+#pragma unroll
+      for (int i = 0; i < 8; ++i) q[k][i] = _Float16(__builtin_bit_cast(float, kPerm[i] % 2 ? w[k][kPerm[i] / 2] & 0xffff0000u : w[k][kPerm[i] / 2] << 16));
+  }
+}
+
 // OR over the wavefront's parts of a token: bit t of the result is token t of
 // the wavefront's N tokens (lane t + N part).
 template <int N>
@@ -509,9 +574,8 @@ __device__ __forceinline__ uint32_t fold_tokens(uint64_t b) {
 // share a tile; a thread turns 16 channels of one token's key and of its value
 // into LDS (unit_values; packed fp16 arithmetic), two tiles in turn: while the
 // matrix instructions take tile i, tile i + 1 is written from registers, the
-// page rows of tile i + 2 are on their way to registers, and the descriptors
-// and page ids of the tiles after it likewise, so that no load is waited for
-// where it was issued.
+// page rows of the next two are on their way to registers, and the descriptors
+// and page ids of the tiles after them likewise.
 // UNI: the NT tokens that a wavefront turns always lie in one page, whose id,
 // descriptor and addresses are then the wavefront's.
 // CS: wavefronts that share 32 rows, each with a part of the output's channels
@@ -557,11 +621,12 @@ __global__ void __launch_bounds__(512, 2) attend_chunk16_kernel(ChunkArgs a) {
   auto page_of = [&](int tile) { return uint32_t((uint64_t(uint32_t(u_first + tile * KT)) * a.page_mul) >> a.page_shift); };
   int32_t kid = -1, vid = -1;
   uint2 kd{}, vd{};  // dc_page_desc
-  uint32_t kr[8], vr[8], k_scale = 0, k_bias = 0, v_scale = 0, v_bias = 0;
-  int k_kind = U_NONE, v_kind = U_NONE;  // of the raw units
-  bool k_affine = false, v_affine = false, counts = false;
-#pragma unroll
-  for (int i = 0; i < 8; ++i) kr[i] = vr[i] = 0;
+  struct Raw {
+    uint32_t kr[8], vr[8], k_scale, k_bias, v_scale, v_bias;
+    int k_kind, v_kind;
+    bool k_affine, v_affine, counts;
+  };
+  Raw even, odds;  // (of even and of odd tiles)
   auto load_ids = [&](int tile) __attribute__((always_inline)) {
     const uint32_t page = page_of(tile);
     const bool in = u_first + tile * KT < it.kv_end && page < uint32_t(a.table_stride);
@@ -576,27 +641,31 @@ __global__ void __launch_bounds__(512, 2) attend_chunk16_kernel(ChunkArgs a) {
     vd = reinterpret_cast<const uint2*>(vs.descs)[in ? vi : 0];
     if (!in) kd.y &= 0xffff0000u;  // (no tokens)
   };
-  auto load_units = [&](int tile) __attribute__((always_inline)) {
+  // The units of a tile, whose descriptors are at hand, and the descriptors and
+  // ids of the next ones: those first, since loads come back in order and
+  // waiting for them would wait for units issued ahead of them too.
+  auto load_units = [&](int tile, Raw& raw) __attribute__((always_inline)) {
     const int u = u_first + tile * KT, slot = u - int(page_of(tile)) * P;
     const auto k = __builtin_bit_cast(dc_page_desc, uint2{uint32_t(uni(kd.x)), uint32_t(uni(kd.y))});
     const auto v = __builtin_bit_cast(dc_page_desc, uint2{uint32_t(uni(vd.x)), uint32_t(uni(vd.y))});
-    k_kind = unit_kind(ks, k, P, slot);
-    v_kind = unit_kind(vs, v, P, slot);
-    k_affine = k.format == DC_FMT_M0_AFFINE;
-    v_affine = v.format == DC_FMT_M0_AFFINE;
+    raw.k_kind = unit_kind(ks, k, P, slot);
+    raw.v_kind = unit_kind(vs, v, P, slot);
+    raw.k_affine = k.format == DC_FMT_M0_AFFINE;
+    raw.v_affine = v.format == DC_FMT_M0_AFFINE;
     // (tokens of the page behind its last and behind kv_end lie in its blob, but do not count)
     const int end = min(min(int(k.tokens), int(v.tokens)), slot + it.kv_end - u);
-    const bool ok = k_kind != U_NONE && v_kind != U_NONE;
-    counts = ok && slot + lt < end;
-    if (ok && has) {
-      load_unit(ks, k, k_kind, slot, kr, k_scale, k_bias);
-      load_unit(vs, v, v_kind, slot, vr, v_scale, v_bias);
-    }
+    const bool ok = raw.k_kind != U_NONE && raw.v_kind != U_NONE;
+    load_descs();
+    load_ids(tile + 2);
+    raw.counts = ok && slot + lt < end;
+    if (!ok) raw.k_kind = raw.v_kind = U_NONE;
+    load_unit<UNI>(ks, ks.arena + (uint64_t(k.block) << 8), a.items, raw.k_kind, raw.k_affine, slot, raw.kr, raw.k_scale, raw.k_bias);
+    load_unit<UNI>(vs, vs.arena + (uint64_t(v.block) << 8), a.items, raw.v_kind, raw.v_affine, slot, raw.vr, raw.v_scale, raw.v_bias);
   };
   const int w_at[2] = {lds_at<CH>(ut, uc / 8), lds_at<CH>(ut, uc / 8 + 1)};  // of the unit's chunks in a tile
-  auto write_tile = [&](int tile) __attribute__((always_inline)) {
+  auto write_tile = [&](int tile, const Raw& raw) __attribute__((always_inline)) {
     const int buf = tile & 1;
-    const bool zero = !(counts && has), border = it.kv_begin + (tile + 1) * KT - 1 > sees_block;  // (border: uniform)
+    const bool zero = !(raw.counts && has), border = it.kv_begin + (tile + 1) * KT - 1 > sees_block;  // (border: uniform)
     uint32_t y[8];
     auto put = [&](uint8_t* to) __attribute__((always_inline)) {
 #pragma unroll
@@ -604,9 +673,9 @@ __global__ void __launch_bounds__(512, 2) attend_chunk16_kernel(ChunkArgs a) {
 #pragma unroll
       for (int k = 0; k < 2; ++k) *reinterpret_cast<uint4*>(to + w_at[k]) = uint4{y[4 * k], y[4 * k + 1], y[4 * k + 2], y[4 * k + 3]};
     };
-    unit_values(k_kind, k_affine, kr, k_scale, k_bias, y);
+    unit_values(raw.k_kind, raw.k_affine, raw.kr, raw.k_scale, raw.k_bias, y);
     put(lds + buf * TILE);
-    unit_values(v_kind, v_affine, vr, v_scale, v_bias, y);
+    unit_values(raw.v_kind, raw.v_affine, raw.vr, raw.v_scale, raw.v_bias, y);
     if (border) {
       uint32_t any = 0;
 #pragma unroll
@@ -619,40 +688,24 @@ __global__ void __launch_bounds__(512, 2) attend_chunk16_kernel(ChunkArgs a) {
       if (lane < NT / 8) poison[buf][pg][tw * (NT / 8) + lane] = uint8_t(bits >> (8 * lane));
     }
     put(lds + (2 + buf) * TILE);
-    const uint32_t bits = fold_tokens<NT>(__ballot(counts));
+    const uint32_t bits = fold_tokens<NT>(__ballot(raw.counts));
     if (pg == 0 && lane < NT / 8) live[buf][tw * (NT / 8) + lane] = uint8_t(bits >> (8 * lane));
   };
   load_ids(0);
   load_descs();
   load_ids(1);
-  load_units(0);
-  load_descs();
-  load_ids(2);
+  load_units(0, even);
+  load_units(1, odds);
 
   // ---- queries: row col, channels 16 k + 8 half .. + 7 in LDS order
   h8v q[QW];
   {
-    const uint16_t* p = reinterpret_cast<const uint16_t*>(a.q) + int64_t(it.q_begin + tok) * a.q_token_stride +
-                        int64_t(head) * a.q_head_stride;
-#pragma unroll
-    for (int k = 0; k < QW; ++k) {
-      const int ch = 16 * k + 8 * half;
-      uint32_t w[4] = {0, 0, 0, 0};
-      if (has_row && ch < hd) {
-        if (a.q_vec) {
-          const uint4 x = *reinterpret_cast<const uint4*>(p + ch);
-          w[0] = x.x; w[1] = x.y; w[2] = x.z; w[3] = x.w;
-        } else {
-#pragma unroll
-          for (int i = 0; i < 4; ++i) w[i] = p[ch + 2 * i] | uint32_t(p[ch + 2 * i + 1]) << 16;
-        }
-      }
-#pragma unroll
-      for (int i = 0; i < 8; ++i) {
-        const uint32_t bits = w[kPerm[i] / 2] >> (16 * (kPerm[i] % 2));
-        q[k][i] = a.dtype == DC_F16 ? __builtin_bit_cast(_Float16, uint16_t(bits)) : _Float16(__builtin_bit_cast(float, bits << 16));
-      }
-    }
+    const int rr = has_row ? row : it.row_begin, rt = rr / a.n_q;  // (rows that do not exist: the first one's, as zeros)
+    const uint16_t* p = reinterpret_cast<const uint16_t*>(a.q) + int64_t(it.q_begin + rt) * a.q_token_stride +
+                        int64_t(it.kv_head * a.n_q + rr - rt * a.n_q) * a.q_head_stride;
+    uint32_t w[QW][4];
+    load_rows<QW>(a, p, 8 * half, 16, has_row, hd, w);
+    to_operands<QW>(a.dtype == DC_F16, w, q);
   }
   const float c = a.scale * kLog2e;
   float m = -INFINITY, l = 0.f;
@@ -662,17 +715,13 @@ __global__ void __launch_bounds__(512, 2) attend_chunk16_kernel(ChunkArgs a) {
 #pragma unroll
     for (int v = 0; v < 16; ++v) o[i][v] = 0.f;
 
-  write_tile(0);
-  load_units(1);
-  load_descs();
-  load_ids(3);
+  write_tile(0, even);
+  load_units(2, even);
   __syncthreads();
-  for (int i = 0; i < tiles; ++i) {
+  auto step = [&](int i, Raw& next) __attribute__((always_inline)) {  // next: tile i + 1's
     if (i + 1 < tiles) {
-      write_tile(i + 1);
-      load_units(i + 2);
-      load_descs();
-      load_ids(i + 4);
+      write_tile(i + 1, next);
+      load_units(i + 3, next);
     }
     const uint8_t* const kt = lds + (i & 1) * TILE;
     const uint8_t* const vt = lds + (2 + (i & 1)) * TILE;
@@ -790,6 +839,10 @@ __global__ void __launch_bounds__(512, 2) attend_chunk16_kernel(ChunkArgs a) {
       }
     }
     __syncthreads();
+  };
+  for (int i = 0; i < tiles; i += 2) {
+    step(i, odds);
+    if (i + 1 < tiles) step(i + 1, even);
   }
   if (!has_row) return;
   l = half_sum(l);
@@ -835,32 +888,6 @@ namespace {
 typedef float f32x4 __attribute__((ext_vector_type(4)));
 constexpr int kFewTile = 32;   // tokens a wavefront takes at a time
 constexpr int kFewWaves = 4;
-
-// Loads from a page: the page's and the wavefront's part of the address in
-// scalar registers and the lane's in one vector register where the wavefront
-// shares the page (a buffer load; pointers would take two registers for each
-// load), or by pointer where each lane has its own.
-template <bool UNI>
-struct PageLoad {
-  const uint8_t* base;
-  __device__ __forceinline__ uint32_t u16(uint32_t off, uint32_t lane) const {
-    if constexpr (UNI) return uint16_t(__builtin_amdgcn_raw_buffer_load_b16(rsrc(), int(lane), int(off), 0));
-    return *reinterpret_cast<const uint16_t*>(base + off + lane);
-  }
-  __device__ __forceinline__ uint32_t u32(uint32_t off, uint32_t lane) const {
-    if constexpr (UNI) return __builtin_amdgcn_raw_buffer_load_b32(rsrc(), int(lane), int(off), 0);
-    return *reinterpret_cast<const uint32_t*>(base + off + lane);
-  }
-  __device__ __forceinline__ uint4 u128(uint32_t off, uint32_t lane) const {
-    if constexpr (UNI) return __builtin_bit_cast(uint4, __builtin_amdgcn_raw_buffer_load_b128(rsrc(), int(lane), int(off), 0));
-    return *reinterpret_cast<const uint4*>(base + off + lane);
-  }
-
- private:
-  __device__ __forceinline__ auto rsrc() const {
-    return __builtin_amdgcn_make_buffer_rsrc(const_cast<uint8_t*>(base), 0, 0x7fffffff, 0x00027000);
-  }
-};
 
 // As lds_at, for tiles whose reads take two chunks of eight tokens at once.
 template <int CH>
@@ -941,33 +968,20 @@ __global__ void __launch_bounds__(64 * kFewWaves, 2) attend_few_kernel(ChunkArgs
   for (int n = 0; n < NB; ++n) {
     const int row = it.row_begin + 16 * n + col;
     const bool has_row = row < it.row_end;
-    const int tok = row / a.n_q, head = it.kv_head * a.n_q + (row - tok * a.n_q);
-    sees[n] = has_row ? it.first + tok : -1;
-    const uint16_t* p = reinterpret_cast<const uint16_t*>(a.q) + int64_t(it.q_begin + tok) * a.q_token_stride +
-                        int64_t(head) * a.q_head_stride;
+    sees[n] = has_row ? it.first + row / a.n_q : -1;
+    const int rr = has_row ? row : it.row_begin, rt = rr / a.n_q;  // (rows that do not exist: the first one's, as zeros)
+    const uint16_t* p = reinterpret_cast<const uint16_t*>(a.q) + int64_t(it.q_begin + rt) * a.q_token_stride +
+                        int64_t(it.kv_head * a.n_q + rr - rt * a.n_q) * a.q_head_stride;
+    uint32_t w[KS][4];
+    h8v x[KS];
+    load_rows<KS>(a, p, 8 * g, 32, has_row, hd, w);
+    to_operands<KS>(a.dtype == DC_F16, w, x);
 #pragma unroll
     for (int k = 0; k < KS; ++k) {
-      const int ch = 32 * k + 8 * g;
-      uint32_t w[4] = {0, 0, 0, 0};
-      if (has_row && ch < hd) {
-        if (a.q_vec) {
-          const uint4 x = *reinterpret_cast<const uint4*>(p + ch);
-          w[0] = x.x; w[1] = x.y; w[2] = x.z; w[3] = x.w;
-        } else {
-#pragma unroll
-          for (int i = 0; i < 4; ++i) w[i] = p[ch + 2 * i] | uint32_t(p[ch + 2 * i + 1]) << 16;
-        }
-      }
-      h8v x;
-#pragma unroll
-      for (int i = 0; i < 8; ++i) {
-        const uint32_t bits = w[kPerm[i] / 2] >> (16 * (kPerm[i] % 2));
-        x[i] = a.dtype == DC_F16 ? __builtin_bit_cast(_Float16, uint16_t(bits)) : _Float16(__builtin_bit_cast(float, bits << 16));
-      }
       if constexpr (!QL)
-        q[n][k] = x;
+        q[n][k] = x[k];
       else if (wave == 0)
-        *reinterpret_cast<h8v*>(ql + lds_at<CH>(16 * n + col, 4 * k + g)) = x;
+        *reinterpret_cast<h8v*>(ql + lds_at<CH>(16 * n + col, 4 * k + g)) = x[k];
     }
   }
   if constexpr (QL) __syncthreads();
@@ -1056,29 +1070,15 @@ __global__ void __launch_bounds__(64 * kFewWaves, 2) attend_few_kernel(ChunkArgs
     }
     return x;
   };
-  // ... and its words
-  uint32_t kr[2][KS][KW], vr[VU][8], k_scale[2][KS], v_scale[VU];  // (scale: fp16 scale, bias above it)
-#pragma unroll
-  for (int b = 0; b < 2; ++b)
-#pragma unroll
-    for (int k = 0; k < KS; ++k) {
-      k_scale[b][k] = 0;
-#pragma unroll
-      for (int w = 0; w < KW; ++w) kr[b][k][w] = 0;
-    }
-#pragma unroll
-  for (int u = 0; u < VU; ++u) {
-    v_scale[u] = 0;
-#pragma unroll
-    for (int w = 0; w < 8; ++w) vr[u][w] = 0;
-  }
+  // ... and its words; scales and biases as they are
+  uint32_t kr[2][KS][KW], vr[VU][8], k_scale[2][KS], k_bias[2][KS], v_scale[VU], v_bias[VU];
   // the lane's offsets in a page, from its tile's first token (from its own where its tokens lie in several pages)
   const uint32_t k4 = kt0 * ks.token4 + 4 * g, k_sc = kt0 * ks.groups2, k16 = kt0 * ks.row2 + 16 * g;
   const uint32_t vc0 = VC * (lane >> 5), v16 = vt0 * vs.row2 + 2 * vc0;
   uint32_t v4[VU], v_sc[VU];
 #pragma unroll
   for (int u = 0; u < VU; ++u) {
-    const uint32_t c = vc0 + 32 * u, gr = c / vgs;
+    const uint32_t c = int(vc0 + 32 * u) < hd ? vc0 + 32 * u : 0, gr = c / vgs;  // (channels past head_dim: the first ones')
     v4[u] = vt0 * vs.token4 + gr * v_plane + (c - gr * vgs) / 2;
     v_sc[u] = vt0 * vs.groups2 + 2 * gr;
   }
@@ -1087,53 +1087,42 @@ __global__ void __launch_bounds__(64 * kFewWaves, 2) attend_few_kernel(ChunkArgs
     for (int b = 0; b < 2; ++b) {
       const Place& x = at[UNI ? 0 : b];
       const uint32_t slot = x.slot + (UNI ? 16 * b : 0);
-      if (x.k_kind == U_F16) {
+      // (fp16 rows are read here where KW is 4, else where they are used)
+      const bool f16 = x.k_kind == U_F16;
+      const PageLoad<UNI> p{x.k, a.items, x.k_kind != U_NONE};
+      const uint32_t sh = x.k_kind == U_B8, lane_at = f16 ? k16 : k4 << sh, lane_s = f16 ? 0 : k_sc;
+      const uint32_t codes = f16 ? slot * ks.row2 : (slot * ks.token4) << sh, scales = f16 ? 0 : (ks.scales4 << sh) + slot * ks.groups2;
+      const uint32_t gap = x.k_affine && !f16 ? ks.gap : 0;
+#pragma unroll
+      for (int k = 0; k < KS; ++k) {
+        const uint32_t c = 32 * k < hd ? 32 * k : 0, gr = c / kgs;  // (channels past head_dim: the first ones')
+        const uint32_t o = codes + (f16 ? 2 * c : (gr * k_plane + (c - gr * kgs) / 2) << sh);
         if constexpr (KW == 4) {
-          const PageLoad<UNI> p{x.k};
-#pragma unroll
-          for (int k = 0; k < KS; ++k)
-            if (32 * k < hd) {
-              const uint4 r = p.u128(slot * ks.row2 + 64 * k, k16);
-              kr[b][k][0] = r.x; kr[b][k][1] = r.y; kr[b][k][2] = r.z; kr[b][k][3] = r.w;
-            }
+          const uint4 r = p.u128(o, lane_at);
+          kr[b][k][0] = r.x; kr[b][k][1] = r.y; kr[b][k][2] = r.z; kr[b][k][3] = r.w;
+        } else {
+          const uint2 r = p.u64(o, lane_at);
+          kr[b][k][0] = r.x; kr[b][k][1] = r.y;
         }
-      } else if (x.k_kind != U_NONE) {
-        const uint32_t sh = x.k_kind == U_B8, off = k4 << sh;
-        const PageLoad<UNI> p{x.k};
-        const uint32_t codes = (slot * ks.token4) << sh, scales = (ks.scales4 << sh) + slot * ks.groups2;
-        const uint32_t gap = x.k_affine ? ks.gap : 0, keep = x.k_affine ? 0xffff0000u : 0u;
-#pragma unroll
-        for (int k = 0; k < KS; ++k)
-          if (32 * k < hd) {
-            const uint32_t gr = 32 * k / kgs, o = (gr * k_plane + (32 * k - gr * kgs) / 2) << sh;
-            // (no else: stores that two branches make to different words would keep the array in memory)
-            kr[b][k][0] = p.u32(codes + o, off);
-            if (sh) kr[b][k][1] = p.u32(codes + o + 4, off);
-            const uint32_t s = p.u16(scales + 2 * gr, k_sc), z = p.u16(scales + 2 * gr + gap, k_sc);
-            k_scale[b][k] = s | ((z << 16) & keep);
-          }
+        k_scale[b][k] = p.u16(scales + (f16 ? 0 : 2 * gr), lane_s);
+        k_bias[b][k] = p.u16(scales + (f16 ? 0 : 2 * gr) + gap, lane_s);
       }
     }
   };
   auto load_values = [&]() __attribute__((always_inline)) {
     const Place x = value_place();
-    if (x.v_kind == U_NONE || x.v_kind == U_F16) return;
-    const uint32_t sh = x.v_kind == U_B8;
-    const PageLoad<UNI> p{x.v};
-    const uint32_t codes = (x.slot * vs.token4) << sh, scales = (vs.scales4 << sh) + x.slot * vs.groups2;
-    const uint32_t gap = x.v_affine ? vs.gap : 0, keep = x.v_affine ? 0xffff0000u : 0u;
+    const bool f16 = x.v_kind == U_F16;  // (read where they are used)
+    const PageLoad<UNI> p{x.v, a.items, x.v_kind != U_NONE && !f16};
+    const uint32_t sh = x.v_kind == U_B8, codes = (x.slot * vs.token4) << sh, scales = (vs.scales4 << sh) + x.slot * vs.groups2;
+    const uint32_t gap = x.v_affine ? vs.gap : 0;
 #pragma unroll
-    for (int u = 0; u < VU; ++u)
-      if (int(vc0 + 32 * u) < hd) {
-        const uint4 r = p.u128(codes, v4[u] << sh);
-        vr[u][0] = r.x; vr[u][1] = r.y; vr[u][2] = r.z; vr[u][3] = r.w;
-        if (sh) {
-          const uint4 y = p.u128(codes + 16, v4[u] << 1);
-          vr[u][4] = y.x; vr[u][5] = y.y; vr[u][6] = y.z; vr[u][7] = y.w;
-        }
-        const uint32_t s = p.u16(scales, v_sc[u]), z = p.u16(scales + gap, v_sc[u]);
-        v_scale[u] = s | ((z << 16) & keep);
-      }
+    for (int u = 0; u < VU; ++u) {
+      const uint4 r = p.u128(codes, v4[u] << sh), t = p.u128(codes + (sh ? 16 : 0), v4[u] << sh);
+      vr[u][0] = r.x; vr[u][1] = r.y; vr[u][2] = r.z; vr[u][3] = r.w;
+      vr[u][4] = t.x; vr[u][5] = t.y; vr[u][6] = t.z; vr[u][7] = t.w;
+      v_scale[u] = p.u16(scales, v_sc[u]);
+      v_bias[u] = p.u16(scales + gap, v_sc[u]);
+    }
   };
 
   const int all = (it.kv_end - it.kv_begin + kFewTile - 1) / kFewTile;
@@ -1171,7 +1160,7 @@ __global__ void __launch_bounds__(64 * kFewWaves, 2) attend_few_kernel(ChunkArgs
       for (int u = 0; u < VU; ++u) {
         uint32_t y[4][4];
         const bool in = int(vc0 + 32 * u) < hd;
-        const h2v s = __builtin_bit_cast(h2v, twice(v_scale[u] & 0xffffu)), b = __builtin_bit_cast(h2v, twice(v_scale[u] >> 16));
+        const h2v s = __builtin_bit_cast(h2v, twice(v_scale[u])), b = __builtin_bit_cast(h2v, x.v_affine ? twice(v_bias[u]) : 0u);
         if (x.v_kind == U_B4) {
 #pragma unroll
           for (int e = 0; e < 4; ++e) eight4(vr[u][e], zero, s, b, y[e]);
@@ -1179,7 +1168,7 @@ __global__ void __launch_bounds__(64 * kFewWaves, 2) attend_few_kernel(ChunkArgs
 #pragma unroll
           for (int e = 0; e < 4; ++e) eight8(vr[u][2 * e], vr[u][2 * e + 1], zero, s, b, y[e]);
         } else if (x.v_kind == U_F16 && in) {
-          const PageLoad<UNI> p{x.v};
+          const PageLoad<UNI> p{x.v, a.items, true};
 #pragma unroll
           for (int e = 0; e < 4; ++e) eight_halves(p.u128(x.slot * vs.row2 + 64 * u + 16 * e, v16), y[e]);
         } else {
@@ -1217,18 +1206,18 @@ __global__ void __launch_bounds__(64 * kFewWaves, 2) attend_few_kernel(ChunkArgs
       if (x.k_kind == U_B4) {
 #pragma unroll
         for (int k = 0; k < KS; ++k)
-          eight4(kr[b][k][0], zero, __builtin_bit_cast(h2v, twice(k_scale[b][k] & 0xffffu)), __builtin_bit_cast(h2v, twice(k_scale[b][k] >> 16)), y[b][k]);
+          eight4(kr[b][k][0], zero, __builtin_bit_cast(h2v, twice(k_scale[b][k])), __builtin_bit_cast(h2v, x.k_affine ? twice(k_bias[b][k]) : 0u), y[b][k]);
       } else if (x.k_kind == U_B8) {
 #pragma unroll
         for (int k = 0; k < KS; ++k)
-          eight8(kr[b][k][0], kr[b][k][1], zero, __builtin_bit_cast(h2v, twice(k_scale[b][k] & 0xffffu)),
-                 __builtin_bit_cast(h2v, twice(k_scale[b][k] >> 16)), y[b][k]);
+          eight8(kr[b][k][0], kr[b][k][1], zero, __builtin_bit_cast(h2v, twice(k_scale[b][k])),
+                 __builtin_bit_cast(h2v, x.k_affine ? twice(k_bias[b][k]) : 0u), y[b][k]);
       } else if (x.k_kind == U_F16) {
         if constexpr (KW == 4) {
 #pragma unroll
           for (int k = 0; k < KS; ++k) eight_halves(uint4{kr[b][k][0], kr[b][k][1], kr[b][k][2], kr[b][k][3]}, y[b][k]);
         } else {
-          const PageLoad<UNI> p{x.k};
+          const PageLoad<UNI> p{x.k, a.items, true};
           const uint32_t rows = (x.slot + (UNI ? 16 * b : 0)) * ks.row2;
 #pragma unroll
           for (int k = 0; k < KS; ++k) eight_halves(p.u128(rows + (32 * k < hd ? 64 * k : 0), k16), y[b][k]);
@@ -1404,29 +1393,93 @@ __global__ void __launch_bounds__(64 * kFewWaves, 2) attend_few_kernel(ChunkArgs
   }
 }
 
-// Joins the partial results of a row tile's token ranges: a wavefront per row,
-// channels over its lanes.
-__global__ void __launch_bounds__(256) merge_chunk_kernel(ChunkArgs a, const dc_chunk_merge* merges) {
+// Joins the partial results of a row tile's token ranges: `lanes` lanes per
+// row, VEC channels a lane and further ones in turn.  Where a range of few rows
+// was cut into many (kMergeMany), the block's lane groups share a row's partial
+// results and join in LDS; otherwise each group has a row of its own.
+constexpr int kMergeBlocks = 32, kMergeMany = 8;
+
+template <int VEC>
+__global__ void __launch_bounds__(256) merge_chunk_kernel(ChunkArgs a, const dc_chunk_merge* merges, int32_t lanes) {
+  __shared__ float joined[256 * VEC];
+  __shared__ float sums[256];
   const dc_chunk_merge mg = merges[blockIdx.x];
   if (!chunk_merge_ok(mg, a)) return;
-  const int lane = threadIdx.x & 63, r = int(blockIdx.y) * 4 + int(threadIdx.x >> 6), row = mg.row_begin + r;
-  if (row >= mg.row_end) return;
+  const int tid = threadIdx.x, groups = 256 / lanes, group = tid / lanes, lane = tid - group * lanes;
+  const bool many = mg.count >= kMergeMany;  // (uniform)
+  const int split = many ? groups : 1, part = many ? group : 0, per_block = many ? 1 : groups;
   const int hd = a.kpool.geometry.head_dim, rows = mg.row_end - mg.row_begin;
-  const int tok = row / a.n_q, head = mg.kv_head * a.n_q + (row - tok * a.n_q);
-  float top = -INFINITY;
-  for (int i = 0; i < mg.count; ++i) top = fmaxf(top, a.part_ml[2 * (int64_t(mg.partial_begin) + int64_t(i) * rows + r)]);
-  const float mu = top == -INFINITY ? 0.f : top;
-  const int64_t off = int64_t(mg.q_begin + tok) * a.o_token_stride + int64_t(head) * a.o_head_stride;
-  for (int ch = lane; ch < hd; ch += 64) {
-    float sum = 0.f, l = 0.f;
-    for (int i = 0; i < mg.count; ++i) {
-      const int64_t at = int64_t(mg.partial_begin) + int64_t(i) * rows + r;
-      const float w = exp2f(a.part_ml[2 * at] - mu);
-      l = fmaf(w, a.part_ml[2 * at + 1], l);
-      sum = fmaf(w, a.part_o[at * hd + ch], sum);
+  for (int r0 = int(blockIdx.y) * per_block; r0 < rows; r0 += int(gridDim.y) * per_block) {  // (uniform)
+    const int r = r0 + (many ? 0 : group), row = mg.row_begin + r;
+    const bool has = r < rows;  // (the others take part in the barriers)
+    const int64_t first = int64_t(mg.partial_begin) + (has ? r : 0);
+    const int tok = row / a.n_q, head = mg.kv_head * a.n_q + (row - tok * a.n_q);
+    const int64_t off = int64_t(mg.q_begin + tok) * a.o_token_stride + int64_t(head) * a.o_head_stride;
+    float top = -INFINITY;
+    for (int i = many ? tid : lane; i < mg.count; i += many ? 256 : lanes) top = fmaxf(top, a.part_ml[2 * (first + int64_t(i) * rows)]);
+    for (int o = 1; o < lanes; o <<= 1) top = fmaxf(top, __shfl_xor(top, o, 64));
+    if (many) {
+      __syncthreads();
+      if (lane == 0) sums[group] = top;
+      __syncthreads();
+      for (int g = 0; g < groups; ++g) top = fmaxf(top, sums[g]);
     }
-    store_value(a.out, a.dtype, off + ch, l == 0.f ? 0.f : sum / l);
+    const float mu = top == -INFINITY ? 0.f : top;
+    for (int c0 = 0; c0 < hd; c0 += VEC * lanes) {
+      const int ch = c0 + VEC * lane;
+      const bool in = ch < hd;
+      float sum[VEC], l = 0.f;
+#pragma unroll
+      for (int k = 0; k < VEC; ++k) sum[k] = 0.f;
+#pragma unroll 8
+      for (int i = part; i < mg.count; i += split) {
+        const int64_t at = first + int64_t(i) * rows;
+        const float2 ml = *reinterpret_cast<const float2*>(a.part_ml + 2 * at);
+        const float w = __builtin_amdgcn_exp2f(ml.x - mu);
+        l = fmaf(w, ml.y, l);
+        const float* po = a.part_o + at * hd + (in ? ch : 0);
+        if constexpr (VEC == 4) {
+          const float4 x = *reinterpret_cast<const float4*>(po);
+          sum[0] = fmaf(w, x.x, sum[0]);
+          sum[1] = fmaf(w, x.y, sum[1]);
+          sum[2] = fmaf(w, x.z, sum[2]);
+          sum[3] = fmaf(w, x.w, sum[3]);
+        } else {
+          sum[0] = fmaf(w, *po, sum[0]);
+        }
+      }
+      if (many) {
+        __syncthreads();
+#pragma unroll
+        for (int k = 0; k < VEC; ++k) joined[VEC * tid + k] = sum[k];
+        sums[tid] = l;
+        __syncthreads();
+        if (part == 0)
+          for (int p = 1; p < split; ++p) {
+            const int t = tid + p * lanes;
+#pragma unroll
+            for (int k = 0; k < VEC; ++k) sum[k] += joined[VEC * t + k];
+            l += sums[t];
+          }
+      }
+      if (!has || !in || part != 0) continue;
+      const float inv = l == 0.f ? 0.f : 1.f / l;
+#pragma unroll
+      for (int k = 0; k < VEC; ++k) store_value(a.out, a.dtype, off + ch + k, sum[k] * inv);
+    }
   }
+}
+
+static int launch_merge_chunk(const ChunkArgs& a, const dc_chunk_merge* merges, int32_t n_merges, hipStream_t stream) {
+  const int hd = a.kpool.geometry.head_dim;
+  const bool vec = hd % 4 == 0;
+  const int lanes = vec && hd <= 64 ? 16 : vec && hd <= 128 ? 32 : 64;
+  const dim3 grid(uint32_t(n_merges), kMergeBlocks);
+  if (vec)
+    hipLaunchKernelGGL((merge_chunk_kernel<4>), grid, dim3(256), 0, stream, a, merges, lanes);
+  else
+    hipLaunchKernelGGL((merge_chunk_kernel<1>), grid, dim3(256), 0, stream, a, merges, lanes);
+  return check_hip(hipGetLastError(), "merge_chunk_kernel launch");
 }
 
 template <typename T, int HDP, int KT>
@@ -1514,7 +1567,6 @@ extern "C" int dc_attend_chunk(dc_pool k_pool, dc_pool v_pool, const int32_t* k_
   const hipStream_t st = hipStream_t(stream);
   a.q_vec = reinterpret_cast<uintptr_t>(q.data) % 16 == 0 && q.token_stride % 8 == 0 && q.head_stride % 8 == 0;
   a.o_vec = reinterpret_cast<uintptr_t>(out.data) % 8 == 0 && out.token_stride % 4 == 0 && out.head_stride % 4 == 0;
-  const int merge_rows = dc::kChunkRows;
   // u / page_capacity = u * page_mul >> page_shift for u < 2^31
   const uint32_t P = uint32_t(k_pool.geometry.page_capacity);
   a.page_shift = 31;
@@ -1542,6 +1594,5 @@ extern "C" int dc_attend_chunk(dc_pool k_pool, dc_pool v_pool, const int32_t* k_
   else
     rc = hd <= 64 ? dc::launch_chunk<_Float16, 64, 128>(a, st) : hd <= 128 ? dc::launch_chunk<_Float16, 128, 64>(a, st) : dc::launch_chunk<_Float16, 256, 32>(a, st);
   if (rc != DC_OK || n_merges == 0) return rc;
-  hipLaunchKernelGGL(dc::merge_chunk_kernel, dim3(n_merges, uint32_t(merge_rows + 3) / 4), dim3(256), 0, st, a, merges);
-  return dc::check_hip(hipGetLastError(), "merge_chunk_kernel launch");
+  return dc::launch_merge_chunk(a, merges, n_merges, st);
 }
