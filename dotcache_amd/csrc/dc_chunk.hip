@@ -449,8 +449,8 @@ struct PageLoad {
   const uint8_t* base;
   const void* none;
   bool ok;
-  __device__ __forceinline__ uint32_t u16(uint32_t off, uint32_t lane) const {
-    if constexpr (UNI) return uint16_t(__builtin_amdgcn_raw_buffer_load_b16(rsrc(), int(lane), int(ok ? off : 0), 0));
+  __device__ __forceinline__ uint16_t u16(uint32_t off, uint32_t lane) const {
+    if constexpr (UNI) return (__builtin_amdgcn_raw_buffer_load_b16(rsrc(), int(lane), int(ok ? off : 0), 0));
     return *static_cast<const uint16_t*>(at(off, lane));
   }
   __device__ __forceinline__ uint2 u64(uint32_t off, uint32_t lane) const {
@@ -470,12 +470,11 @@ struct PageLoad {
   __device__ __forceinline__ const void* at(uint32_t off, uint32_t lane) const { return ok ? base + off + lane : none; }
 };
 
-// The unit's bytes: r (a 4-bit unit's are the first two words), and scale and
-// bias (0 where there is none).  A 4-bit unit's 16-byte read ends in the
+// The unit's bytes: r (a 4-bit unit's are the first two words), scale and bias.  A 4-bit unit's 16-byte read ends in the
 // scales at the latest.
 template <bool UNI>
 __device__ __forceinline__ void load_unit(const Side& x, const uint8_t* blob, const void* none, int kind, bool affine, uint32_t slot,
-                                          uint32_t (&r)[8], uint32_t& scale, uint32_t& bias) {
+                                          uint32_t (&r)[8], uint16_t& scale, uint16_t& bias) {
   const PageLoad<UNI> p{blob, none, kind != U_NONE};
   const bool f16 = kind == U_F16;
   const uint32_t sh = kind == U_B8;
@@ -485,8 +484,7 @@ __device__ __forceinline__ void load_unit(const Side& x, const uint8_t* blob, co
   r[4] = v.x; r[5] = v.y; r[6] = v.z; r[7] = v.w;
   const uint32_t so = f16 ? 0 : (x.scales4 << sh) + slot * x.groups2, sl = f16 ? 0 : x.scale_at;
   scale = p.u16(so, sl);
-  bias = p.u16(so + (affine ? x.gap : 0), sl);
-  bias = affine ? bias : 0;
+  bias = p.u16(so + (affine ? x.gap : 0), sl);  // (the scale again where there is none: nothing here may wait for a load)
 }
 
 __device__ __forceinline__ uint32_t scaled(uint32_t codes, uint32_t zero, h2v s, h2v b) {
@@ -503,7 +501,7 @@ __device__ __forceinline__ void unit_values(int kind, bool affine, const uint32_
       y[i] = __builtin_amdgcn_perm(r[4 * (i / 4) + 2 + (i % 4) / 2], r[4 * (i / 4) + (i % 4) / 2], i & 1 ? 0x07060302u : 0x05040100u);
     return;
   }
-  const h2v s = __builtin_bit_cast(h2v, twice(scale)), b = __builtin_bit_cast(h2v, twice(bias));
+  const h2v s = __builtin_bit_cast(h2v, twice(scale)), b = __builtin_bit_cast(h2v, affine ? twice(bias) : 0u);
   // -(1024 + zero point): 0xe400 is -1024, one unit per code
   const uint32_t zero = twice(affine ? 0xe400u : kind == U_B4 ? 0xe407u : 0xe47fu);
   if (kind == U_B4) {
@@ -619,10 +617,17 @@ __global__ void __launch_bounds__(512, 2) attend_chunk16_kernel(ChunkArgs a) {
   const Side ks = make_side(a.kpool, a.k_table + table, lt, uc), vs = make_side(a.vpool, a.v_table + table, lt, uc);
   auto uni = [](int x) { return UNI ? __builtin_amdgcn_readfirstlane(x) : x; };
   auto page_of = [&](int tile) { return uint32_t((uint64_t(uint32_t(u_first + tile * KT)) * a.page_mul) >> a.page_shift); };
-  int32_t kid = -1, vid = -1;
-  uint2 kd{}, vd{};  // dc_page_desc
+  // (a zero in a vector register: ids and descriptors are then read by vector
+  // loads, which come back in order; a scalar load in flight would make the next
+  // wait for LDS wait for all of LDS and for it)
+  const int v0 = fresh(0);
+  // (loaded values are taken as they are until they are used: an edit would wait for the load)
+  int32_t kid, vid;
+  uint2 kd, vd;  // dc_page_desc
+  bool named = false, listed = false;  // the table names the pages that kid, vid are for; kd, vd are pages of the pools
   struct Raw {
-    uint32_t kr[8], vr[8], k_scale, k_bias, v_scale, v_bias;
+    uint32_t kr[8], vr[8];
+    uint16_t k_scale, k_bias, v_scale, v_bias;
     int k_kind, v_kind;
     bool k_affine, v_affine, counts;
   };
@@ -630,16 +635,16 @@ __global__ void __launch_bounds__(512, 2) attend_chunk16_kernel(ChunkArgs a) {
   auto load_ids = [&](int tile) __attribute__((always_inline)) {
     const uint32_t page = page_of(tile);
     const bool in = u_first + tile * KT < it.kv_end && page < uint32_t(a.table_stride);
-    kid = ks.table[in ? page : 0];
-    vid = vs.table[in ? page : 0];
-    if (!in) kid = -1;
+    kid = ks.table[(in ? int(page) : 0) + v0];
+    vid = vs.table[(in ? int(page) : 0) + v0];
+    named = in;
   };
   auto load_descs = [&]() __attribute__((always_inline)) {
     const int ki = uni(kid), vi = uni(vid);
-    const bool in = uint32_t(ki) < uint32_t(ks.n_descs) && uint32_t(vi) < uint32_t(vs.n_descs);
-    kd = reinterpret_cast<const uint2*>(ks.descs)[in ? ki : 0];
-    vd = reinterpret_cast<const uint2*>(vs.descs)[in ? vi : 0];
-    if (!in) kd.y &= 0xffff0000u;  // (no tokens)
+    const bool in = named && uint32_t(ki) < uint32_t(ks.n_descs) && uint32_t(vi) < uint32_t(vs.n_descs);
+    listed = in;
+    kd = reinterpret_cast<const uint2*>(ks.descs)[(in ? ki : 0) + v0];
+    vd = reinterpret_cast<const uint2*>(vs.descs)[(in ? vi : 0) + v0];
   };
   // The units of a tile, whose descriptors are at hand, and the descriptors and
   // ids of the next ones: those first, since loads come back in order and
@@ -654,7 +659,7 @@ __global__ void __launch_bounds__(512, 2) attend_chunk16_kernel(ChunkArgs a) {
     raw.v_affine = v.format == DC_FMT_M0_AFFINE;
     // (tokens of the page behind its last and behind kv_end lie in its blob, but do not count)
     const int end = min(min(int(k.tokens), int(v.tokens)), slot + it.kv_end - u);
-    const bool ok = raw.k_kind != U_NONE && raw.v_kind != U_NONE;
+    const bool ok = listed && raw.k_kind != U_NONE && raw.v_kind != U_NONE;
     load_descs();
     load_ids(tile + 2);
     raw.counts = ok && slot + lt < end;
@@ -1004,27 +1009,33 @@ __global__ void __launch_bounds__(64 * kFewWaves, 2) attend_few_kernel(ChunkArgs
   auto uni = [](int x) { return UNI ? __builtin_amdgcn_readfirstlane(x) : x; };
   auto token = [&](int tile, int b) { return it.kv_begin + tile * kFewTile + (UNI ? 0 : 16 * b + col); };
   auto page_of = [&](int u) { return uint32_t((uint64_t(uint32_t(u)) * a.page_mul) >> a.page_shift); };
+  // (a zero in a vector register: ids and descriptors are then read by vector
+  // loads, which come back in order; a scalar load in flight would make the next
+  // wait for LDS wait for all of LDS and for it)
+  const int v0 = fresh(0);
+  // (loaded values are taken as they are until they are used: an edit would wait for the load)
   int32_t kid[PB], vid[PB];
   uint2 kd[PB], vd[PB];
+  bool named[PB], listed[PB];  // the table names the pages that kid, vid are for; kd, vd are pages of the pools
   auto load_ids = [&](int tile) __attribute__((always_inline)) {
 #pragma unroll
     for (int b = 0; b < PB; ++b) {
       const int u = token(tile, b);
       const uint32_t page = page_of(u);
       const bool in = u < it.kv_end && page < uint32_t(a.table_stride);
-      kid[b] = ks.table[in ? page : 0];
-      vid[b] = vs.table[in ? page : 0];
-      if (!in) kid[b] = -1;
+      kid[b] = ks.table[(in ? int(page) : 0) + v0];
+      vid[b] = vs.table[(in ? int(page) : 0) + v0];
+      named[b] = in;
     }
   };
   auto load_descs = [&]() __attribute__((always_inline)) {
 #pragma unroll
     for (int b = 0; b < PB; ++b) {
       const int ki = uni(kid[b]), vi = uni(vid[b]);
-      const bool in = uint32_t(ki) < uint32_t(ks.n_descs) && uint32_t(vi) < uint32_t(vs.n_descs);
-      kd[b] = reinterpret_cast<const uint2*>(ks.descs)[in ? ki : 0];
-      vd[b] = reinterpret_cast<const uint2*>(vs.descs)[in ? vi : 0];
-      if (!in) kd[b].y &= 0xffff0000u;  // (no tokens)
+      const bool in = named[b] && uint32_t(ki) < uint32_t(ks.n_descs) && uint32_t(vi) < uint32_t(vs.n_descs);
+      listed[b] = in;
+      kd[b] = reinterpret_cast<const uint2*>(ks.descs)[(in ? ki : 0) + v0];
+      vd[b] = reinterpret_cast<const uint2*>(vs.descs)[(in ? vi : 0) + v0];
     }
   };
   // The raw tile: where it is and what its pages hold (of the lane's tokens 16 b + col, or of all where UNI) ...
@@ -1043,7 +1054,7 @@ __global__ void __launch_bounds__(64 * kFewWaves, 2) attend_few_kernel(ChunkArgs
       x.v_kind = unit_kind(vs, v, P, x.slot);
       // (tokens of the page behind its last and behind kv_end lie in its blob, but do not count)
       x.end = min(min(int(k.tokens), int(v.tokens)) - x.slot, it.kv_end - u);
-      if (x.k_kind == U_NONE || x.v_kind == U_NONE || x.end <= 0) {
+      if (!listed[b] || x.k_kind == U_NONE || x.v_kind == U_NONE || x.end <= 0) {
         x.k_kind = x.v_kind = U_NONE;
         x.end = 0;
       }
@@ -1071,7 +1082,8 @@ __global__ void __launch_bounds__(64 * kFewWaves, 2) attend_few_kernel(ChunkArgs
     return x;
   };
   // ... and its words; scales and biases as they are
-  uint32_t kr[2][KS][KW], vr[VU][8], k_scale[2][KS], k_bias[2][KS], v_scale[VU], v_bias[VU];
+  uint32_t kr[2][KS][KW], vr[VU][8];
+  uint16_t k_scale[2][KS], k_bias[2][KS], v_scale[VU], v_bias[VU];
   // the lane's offsets in a page, from its tile's first token (from its own where its tokens lie in several pages)
   const uint32_t k4 = kt0 * ks.token4 + 4 * g, k_sc = kt0 * ks.groups2, k16 = kt0 * ks.row2 + 16 * g;
   const uint32_t vc0 = VC * (lane >> 5), v16 = vt0 * vs.row2 + 2 * vc0;
@@ -1244,10 +1256,10 @@ __global__ void __launch_bounds__(64 * kFewWaves, 2) attend_few_kernel(ChunkArgs
       }
     }
     locate(i + kFewWaves);
+    load_descs();  // (ahead of the words: loads come back in order)
+    load_ids(i + 3 * kFewWaves);
     load_values();
     load_keys();
-    load_descs();
-    load_ids(i + 3 * kFewWaves);
     // ---- softmax: tokens 16 b + 4 g + v of row col of each block
     h8v p[NB];
 #pragma unroll
