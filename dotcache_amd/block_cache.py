@@ -27,11 +27,13 @@ from dataclasses import dataclass
 
 import numpy as np
 
+from .chunk import attend_cached
 from .config import DotCacheConfig
 from .decode import decode_paged, plan_decode, workspace_bytes
 from .encode import resolve_encode_spec
 from .kv_cache import default_q_head_to_kv_head
 from .page_pool import DevicePagePool, PoolGeometry, page_format_of
+from .rotary import head_norm, index_tensor
 from .types import EncodedPage
 
 
@@ -111,6 +113,7 @@ class DeviceVllmPagedKVCache:
         self._seq_blocks = [[] for _ in range(L)]
         self._seq_len = np.zeros(L, dtype=np.int64)
         self._workspace = None
+        self._chunk_plan = None  # lengths and plan of the last attend_block_tables
 
     # ---- formats and small helpers ------------------------------------------
     def _page_format(self, kind: str, layer_id: int, kv_head_id: int) -> tuple[int, int]:
@@ -124,16 +127,17 @@ class DeviceVllmPagedKVCache:
             raise ValueError(f"layer_id {layer_id} out of range")
         return lid
 
-    def _as_rows(self, x, name: str):
-        """``x [n, H, hd]`` on the device in fp32, fp16 or bf16 (the encoder
+    def _as_rows(self, x, name: str, heads: int | None = None):
+        """``x [n, heads, hd]`` (default: the KV heads) on the device in fp32, fp16 or bf16 (the encoder
         reads each exactly as fp32); other types become fp32."""
         torch = _torch()
         t = x if isinstance(x, torch.Tensor) else torch.from_numpy(np.ascontiguousarray(np.asarray(x, dtype=np.float32)))
         t = t.to(device=self.device)
         if t.dtype not in (torch.float32, torch.float16, torch.bfloat16):
             t = t.float()
-        if t.dim() != 3 or t.shape[1] != self.num_key_value_heads or t.shape[2] != self.config.head_dim:
-            raise ValueError(f"{name} must have shape [tokens, {self.num_key_value_heads}, {self.config.head_dim}]")
+        heads = self.num_key_value_heads if heads is None else heads
+        if t.dim() != 3 or t.shape[1] != heads or t.shape[2] != self.config.head_dim:
+            raise ValueError(f"{name} must have shape [tokens, {heads}, {self.config.head_dim}]")
         return t
 
     def _grow(self, lid: int, block_id: int) -> None:
@@ -215,15 +219,75 @@ class DeviceVllmPagedKVCache:
         fill (a block whose offset 0 is written again starts over).  A block
         whose last slot is written is finalised.  ``token_start`` (optional)
         is the absolute position of row 0, kept for page headers."""
-        torch = _torch()
         lid = self._check_layer(layer_id)
         keys = self._as_rows(key_rows, "key_rows")
         values = self._as_rows(value_rows, "value_rows")
         if keys.shape[0] != values.shape[0]:
             raise ValueError("key_rows and value_rows must hold the same number of tokens")
+        if keys.dtype != values.dtype:
+            keys, values = keys.float(), values.float()
+        hd = self.config.head_dim
+
+        def write(a: int, z: int, run, ids, slot, kept, stores):
+            slots = np.repeat(slot, self.num_key_value_heads)
+            if kept is not None:
+                rows = (kept[:, None] + self.block_size * np.arange(self.num_key_value_heads)) * (kept >= 0)[:, None] - (kept < 0)[:, None]
+                kept = (*stores, rows.ravel())
+            self.k_pool.encode_rows_with(self.v_pool, keys[a:z].reshape(-1, hd), values[a:z].reshape(-1, hd),
+                                         ids[0][run].ravel(), slots, ids[1][run].ravel(), slots, keep=kept)
+
+        self._write_slots(lid, int(keys.shape[0]), slot_mapping, token_start, write)
+
+    def write_slots_rotated(self, layer_id: int, query_rows, key_rows, value_rows, slot_mapping, positions, rotary, *,
+                            q_weight=None, k_weight=None, eps: float = 1e-6, token_start: int | None = None):
+        """:meth:`write_slots` of projections as they are: ``query_rows
+        [n, Hq, hd]`` (or None) and ``key_rows [n, H, hd]`` are normed
+        (``q_weight`` / ``k_weight``, None: not) and rotated to ``positions
+        [n]`` by ``rotary`` (a :class:`~dotcache_amd.rotary.RotaryTable`, or
+        None), keys and values are written, and the queries are returned in
+        their shape and type (fp32 if the three types differ), all in the one
+        launch that writes the slots."""
+        torch = _torch()
+        lid = self._check_layer(layer_id)
+        H, Hq, hd = self.num_key_value_heads, self.num_attention_heads, self.config.head_dim
+        k, v = self._as_rows(key_rows, "key_rows"), self._as_rows(value_rows, "value_rows")
+        q = None if query_rows is None else self._as_rows(query_rows, "query_rows", Hq)
+        n = int(k.shape[0])
+        if any(x is not None and x.shape[0] != n for x in (q, v)):
+            raise ValueError("query_rows, key_rows and value_rows must hold the same number of tokens")
+        if len({x.dtype for x in (q, k, v) if x is not None}) > 1:
+            q, k, v = (x if x is None else x.float() for x in (q, k, v))
+        # (rows of one token's heads contiguous channel by channel, as the launch takes them)
+        q, k, v = (x if x is None or x.stride(2) == 1 else x.contiguous() for x in (q, k, v))
+        pos = None
+        if rotary is not None:
+            if rotary.head_dim != hd or rotary.table.device != k.device:
+                raise ValueError("the rotary table is for another head_dim or device")
+            pos = index_tensor(positions, "positions", n, k.device, rotary.n_positions)
+        head_norm(q_weight, "queries' weight", Hq, hd, float(eps), k.device)
+        head_norm(k_weight, "keys' weight", H, hd, float(eps), k.device)
+        out = None if q is None else torch.empty(q.shape, dtype=q.dtype, device=q.device)
+
+        def write(a: int, z: int, run, ids, slot, kept, stores):
+            index = torch.from_numpy(np.stack([run, slot, slot if kept is None else kept]).astype(np.int32)).to(self.device)
+            tables = torch.from_numpy(np.stack(ids).astype(np.int32)[..., None]).to(self.device)
+            self.k_pool.append_rotary_with(
+                self.v_pool, None if q is None else q[a:z], k[a:z], v[a:z], None if pos is None else pos[a:z], rotary, tables,
+                index[0], index[1], q_weight=q_weight, k_weight=k_weight, eps=eps, out=None if out is None else out[a:z],
+                keep=None if kept is None else (*stores, index[2], self.block_size))
+
+        self._write_slots(lid, n, slot_mapping, token_start, write)
+        return out
+
+    def _write_slots(self, lid: int, n_rows: int, slot_mapping, token_start: int | None, write) -> None:
+        """:meth:`write_slots` around ``write(first row, end row, run, ids,
+        slot, kept, stores)``: each row's run, the runs' page ids (keys,
+        values; ``[runs, H]``, -1: not into a page), each row's slot, and
+        where its first head goes in the fp32 ``stores`` (None: no row does)."""
+        torch = _torch()
         slots = np.asarray(slot_mapping.detach().cpu().numpy() if isinstance(slot_mapping, torch.Tensor) else slot_mapping,
                            dtype=np.int64).reshape(-1)
-        if slots.shape[0] != keys.shape[0]:
+        if slots.shape[0] != n_rows:
             raise ValueError("slot_mapping needs one slot per row")
         if np.any(slots < 0):
             raise ValueError("slots must be non-negative")
@@ -231,8 +295,6 @@ class DeviceVllmPagedKVCache:
         n = slots.shape[0]
         if n == 0:
             return
-        if keys.dtype != values.dtype:
-            keys, values = keys.float(), values.float()
         # runs of consecutive slots of one block
         blocks, offs = slots // P, slots % P
         ends = np.append(np.flatnonzero((np.diff(slots) != 1) | (np.diff(blocks) != 0)) + 1, n).tolist()
@@ -244,7 +306,7 @@ class DeviceVllmPagedKVCache:
             blk, off = int(blocks[i]), int(offs[i])
             self._grow(lid, blk)
             if off == 0 and blk in fills:  # written and reused in one call: the rows so far land first
-                self._write_runs(lid, runs, restart, keys, values, offs, token_start)
+                self._write_runs(lid, runs, restart, write, offs, token_start)
                 runs, fills, restart = [], {}, []
             fill = fills.get(blk, int(self._fill[lid][blk]))
             if off == 0 and fill > 0:
@@ -256,11 +318,11 @@ class DeviceVllmPagedKVCache:
             runs.append((blk, off, i, j))
             fills[blk] = off + j - i
             i = j
-        self._write_runs(lid, runs, restart, keys, values, offs, token_start)
+        self._write_runs(lid, runs, restart, write, offs, token_start)
         if error is not None:
             raise error
 
-    def _write_runs(self, lid: int, runs, restart, keys, values, offs: np.ndarray, token_start: int | None) -> None:
+    def _write_runs(self, lid: int, runs, restart, write, offs: np.ndarray, token_start: int | None) -> None:
         """Rows of checked runs in one launch (two when blocks fill up).  A
         block written whole is encoded straight into its final pages; rows
         of a live block go to its escape pages and, in fp32, to its row
@@ -295,18 +357,15 @@ class DeviceVllmPagedKVCache:
         a, z = int(first[0]), int(end[-1])
         run = np.repeat(np.arange(len(runs)), end - first)
         slot = offs[a:z]
-        heads = np.arange(H)
-        ids = [np.where((full & ~whole)[run][:, None], -1, self._map[kind][lid][blk][run]) for kind in ("K", "V")]
+        ids = [np.where((full & ~whole)[:, None], -1, self._map[kind][lid][blk]) for kind in ("K", "V")]
         rows = self._row_slots[lid]
-        stored = np.asarray([-1 if w else rows[b] for b, w in zip(blk.tolist(), whole.tolist())], dtype=np.int64)[run]
-        keep = np.where(stored[:, None] < 0, -1, (stored[:, None] * 2 * H + heads) * P + slot[:, None])
-        slots = np.repeat(slot, H)
-        flat = self._row_store[lid].view(-1, hd)
-        kept = None
+        kept = stores = None
         if not whole.all():
-            kept = (flat[: flat.shape[0] - H * P], flat[H * P:], keep.ravel())
-        self.k_pool.encode_rows_with(self.v_pool, keys[a:z].reshape(-1, hd), values[a:z].reshape(-1, hd), ids[0].ravel(),
-                                     slots, ids[1].ravel(), slots, keep=kept)
+            stored = np.asarray([-1 if w else rows[b] for b, w in zip(blk.tolist(), whole.tolist())], dtype=np.int64)[run]
+            kept = np.where(stored < 0, -1, stored * (2 * H * P) + slot)
+            flat = self._row_store[lid].view(-1, hd)
+            stores = (flat[: flat.shape[0] - H * P], flat[H * P:])
+        write(a, z, run, ids, slot, kept, stores)
         done = blk[full & ~whole]
         if done.size:
             self._finalise(lid, done)
@@ -332,22 +391,11 @@ class DeviceVllmPagedKVCache:
         self._free_slots[lid].extend(at)
         self._final[lid][blocks] = True
 
-    def decode_block_tables(self, layer_id: int, queries, block_tables, context_lens, q_head_to_kv_head=None, *,
-                            query_scale: float = 1.0):
-        """Attention of ``queries [B, Hq, hd]`` over sequences given as
-        ``block_tables [B, W]`` block ids and ``context_lens [B]``: one
-        decode launch for the batch.  Block b of a sequence holds tokens
-        ``[b * block_size, ...)``; its token count is the block's fill."""
+    def _resolve(self, lid: int, block_tables, context_lens, B: int):
+        """Checked lengths ``[B]``, their block counts, the block tables on the
+        host and their page ids ``[B, H, W]`` (keys, values)."""
         torch = _torch()
-        lid = self._check_layer(layer_id)
-        B, Hq, H, hd, P = None, self.num_attention_heads, self.num_key_value_heads, self.config.head_dim, self.block_size
-        q = queries if isinstance(queries, torch.Tensor) else torch.from_numpy(np.ascontiguousarray(np.asarray(queries, dtype=np.float32)))
-        q = q.to(self.device)
-        if q.dtype not in (torch.float32, torch.float16, torch.bfloat16):
-            q = q.float()
-        B = int(q.shape[0])
-        if q.dim() != 3 or tuple(q.shape[1:]) != (Hq, hd):
-            raise ValueError(f"queries must have shape [batch, {Hq}, {hd}]")
+        P = self.block_size
         lens = np.asarray(context_lens.detach().cpu().numpy() if isinstance(context_lens, torch.Tensor) else context_lens,
                           dtype=np.int64).reshape(-1)
         if lens.shape != (B,) or np.any(lens <= 0):
@@ -372,6 +420,25 @@ class DeviceVllmPagedKVCache:
             raise ValueError(f"sequence {b}: its blocks hold {int(held[b])} tokens, context_lens says {int(lens[b])}")
         # [B, H, W] page ids, keys and values
         kt, vt = (self._map[kind][lid][at].transpose(0, 2, 1) for kind in ("K", "V"))
+        return lens, n_blocks, bt_host, kt, vt
+
+    def decode_block_tables(self, layer_id: int, queries, block_tables, context_lens, q_head_to_kv_head=None, *,
+                            query_scale: float = 1.0):
+        """Attention of ``queries [B, Hq, hd]`` over sequences given as
+        ``block_tables [B, W]`` block ids and ``context_lens [B]``: one
+        decode launch for the batch.  Block b of a sequence holds tokens
+        ``[b * block_size, ...)``; its token count is the block's fill."""
+        torch = _torch()
+        lid = self._check_layer(layer_id)
+        B, Hq, H, hd, P = None, self.num_attention_heads, self.num_key_value_heads, self.config.head_dim, self.block_size
+        q = queries if isinstance(queries, torch.Tensor) else torch.from_numpy(np.ascontiguousarray(np.asarray(queries, dtype=np.float32)))
+        q = q.to(self.device)
+        if q.dtype not in (torch.float32, torch.float16, torch.bfloat16):
+            q = q.float()
+        B = int(q.shape[0])
+        if q.dim() != 3 or tuple(q.shape[1:]) != (Hq, hd):
+            raise ValueError(f"queries must have shape [batch, {Hq}, {hd}]")
+        lens, n_blocks, bt_host, kt, vt = self._resolve(lid, block_tables, context_lens, B)
         k_table, v_table = torch.from_numpy(np.ascontiguousarray(np.stack([kt, vt]))).to(self.device)
         qmap = self.default_q_head_to_kv_head if q_head_to_kv_head is None else np.asarray(q_head_to_kv_head, dtype=np.int64)
         if qmap.shape != (Hq,) or np.any(qmap < 0) or np.any(qmap >= H) or np.any(np.bincount(qmap, minlength=H) != Hq // H):
@@ -397,6 +464,39 @@ class DeviceVllmPagedKVCache:
         res = torch.empty_like(out)
         res[:, order_t] = out
         return res
+
+    def attend_block_tables(self, layer_id: int, queries, new_tokens, block_tables, context_lens, q_head_to_kv_head=None, *,
+                            query_scale: float = 1.0):
+        """Causal attention of chunks: ``queries [sum(new_tokens), Hq, hd]``,
+        one sequence after another, are those of the last ``new_tokens[b]``
+        (0: the sequence waits) of the ``context_lens[b]`` tokens in the
+        blocks of ``block_tables[b]`` (write their slots first).  Prompt
+        chunks, drafted tokens to verify and plain decodes share a call.
+        Returns rows of the queries' shape and type."""
+        torch = _torch()
+        lid = self._check_layer(layer_id)
+        q = self._as_rows(queries, "queries", self.num_attention_heads)
+        new = np.asarray(new_tokens.detach().cpu().numpy() if isinstance(new_tokens, torch.Tensor) else new_tokens,
+                         dtype=np.int64).reshape(-1)
+        lens, _, _, kt, vt = self._resolve(lid, block_tables, context_lens, new.shape[0])
+        if np.any(new < 0) or np.any(new > lens) or int(new.sum()) != q.shape[0]:
+            raise ValueError("new_tokens must lie in [0, context] and add up to the queries' rows")
+        k_table, v_table = torch.from_numpy(np.ascontiguousarray(np.stack([kt, vt]))).to(self.device)
+        q = q if q.stride(2) == 1 else q.contiguous()
+        return attend_cached(self, q, new.astype(np.int32), lens.astype(np.int32), k_table, v_table, q_head_to_kv_head,
+                             self.default_q_head_to_kv_head, query_scale)
+
+    def read_block_tables(self, layer_id: int, block_tables, context_lens, *, dtype=None):
+        """The tokens of sequences as dense rows ``[sum(context_lens), H, hd]``,
+        one sequence after another, keys and values, as their pages hold them
+        (fp32, or ``dtype`` fp16 / bf16)."""
+        torch = _torch()
+        lid = self._check_layer(layer_id)
+        B = np.asarray(block_tables.shape if hasattr(block_tables, "shape") else (len(block_tables),))[0]
+        lens, _, _, kt, vt = self._resolve(lid, block_tables, context_lens, int(B))
+        tables = torch.from_numpy(np.ascontiguousarray(np.stack([kt, vt]))).to(self.device)
+        token = np.arange(int(lens.sum())) - np.repeat(np.cumsum(lens) - lens, lens)
+        return self.k_pool.read_tokens_with(self.v_pool, tables, np.repeat(np.arange(lens.size), lens), token, dtype=dtype)
 
     # ---- the reference's single-sequence interface --------------------------
     def sync_layer_blocks(self, layer_id: int, key_blocks, value_blocks, *, block_ids=None,

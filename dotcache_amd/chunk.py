@@ -175,10 +175,41 @@ def attend_chunk(pool: DevicePagePool, k_table, v_pool: DevicePagePool | None, v
         raise ValueError(f"workspace must be contiguous, {need} bytes at least, on {device}")
     if plan.n_items:
         call_on(device, _lib.lib().dc_attend_chunk, "dc_attend_chunk", pool.c_pool(), vpool.c_pool(), k_table.data_ptr(),
-                v_table.data_ptr(), shape[2], plan.items.data_ptr(), plan.n_items, plan.n_few, plan.few_rows, plan.merges.data_ptr(), plan.n_merges,
-                plan.n_partials, B, plan.kv_heads, plan.n_tokens, q_rows, float(query_scale), out_rows,
+                v_table.data_ptr(), shape[2], plan.items.data_ptr(), plan.n_items, plan.n_few, plan.few_rows,
+                plan.merges.data_ptr(), plan.n_merges, plan.n_partials, B, plan.kv_heads, plan.n_tokens, q_rows, float(query_scale), out_rows,
                 workspace.data_ptr() if need else None, need)
     return out
+
+
+def attend_cached(cache, queries, new: np.ndarray, context: np.ndarray, k_table, v_table, q_head_to_kv_head, default_map,
+                  query_scale: float):
+    """:func:`attend_chunk` of ``queries [tokens, Hq, hd]`` over a cache's pages,
+    its query heads in any order (``q_head_to_kv_head``; None: ``default_map``).
+    ``cache`` keeps the last plan, by its lengths (every layer of a step has the
+    same), and the workspace of its other attention calls."""
+    torch = _torch()
+    H = cache.num_key_value_heads
+    Hq = cache.num_attention_heads
+    qmap = default_map if q_head_to_kv_head is None else np.asarray(q_head_to_kv_head, dtype=np.int64)
+    if qmap.shape != (Hq,) or np.any(qmap < 0) or np.any(qmap >= H) or np.any(np.bincount(qmap, minlength=H) != Hq // H):
+        raise ValueError("q_head_to_kv_head must give every KV head the same number of query heads")
+    lengths = (new.tobytes(), context.tobytes())
+    if cache._chunk_plan is None or cache._chunk_plan[0] != lengths:
+        cache._chunk_plan = (lengths, plan_chunk(cache.k_pool, cache.v_pool, new, context, kv_heads=H, q_per_kv=Hq // H))
+    plan = cache._chunk_plan[1]
+    need = workspace_bytes(plan, cache.config.head_dim)
+    if cache._workspace is None or cache._workspace.numel() < need:
+        cache._workspace = torch.empty(max(need, 16), dtype=torch.uint8, device=cache.device)
+    order = np.argsort(qmap, kind="stable")  # query heads grouped by KV head
+    if np.array_equal(order, np.arange(Hq)):
+        return attend_chunk(cache.k_pool, k_table, cache.v_pool, v_table, queries, plan, query_scale=query_scale,
+                            workspace=cache._workspace)
+    at = torch.from_numpy(order).to(cache.device)
+    out = attend_chunk(cache.k_pool, k_table, cache.v_pool, v_table, queries[:, at], plan, query_scale=query_scale,
+                       workspace=cache._workspace)
+    res = torch.empty_like(out)
+    res[:, at] = out
+    return res
 
 
 def _validate(pool: DevicePagePool, vpool: DevicePagePool, k_table, v_table, plan: ChunkPlan) -> None:

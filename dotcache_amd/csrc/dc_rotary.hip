@@ -35,6 +35,8 @@ struct RotaryJob {
   dc_pool pool;
   float* keep;
   int32_t rotate;
+  // rows out: heads a lane takes; whether the stores bypass the L2
+  int32_t heads, stream;
 };
 
 struct RotaryArgs {
@@ -49,10 +51,12 @@ struct RotaryArgs {
   int32_t keep_head_stride, keep_rows;
 };
 
+typedef uint32_t rot_u4 __attribute__((ext_vector_type(4)));
 typedef __bf16 rot_bf2 __attribute__((ext_vector_type(2)));
 
-// Eight values to row elements off .. off + 7, rounded to nearest even.
-template <bool vec>
+// Eight values to row elements off .. off + 7, rounded to nearest even, past
+// the L2 if stream.
+template <bool vec, bool stream>
 __device__ __forceinline__ void store8(void* p, int32_t dtype, int64_t off, const float (&z)[8]) {
   if (dtype == DC_F32) {
     float* o = reinterpret_cast<float*>(p) + off;
@@ -72,7 +76,11 @@ __device__ __forceinline__ void store8(void* p, int32_t dtype, int64_t off, cons
                            : __builtin_bit_cast(uint32_t, rot_bf2{(__bf16)z[2 * i], (__bf16)z[2 * i + 1]});
   uint16_t* o = reinterpret_cast<uint16_t*>(p) + off;
   if constexpr (vec) {
-    *reinterpret_cast<uint4*>(o) = uint4{w[0], w[1], w[2], w[3]};
+    const rot_u4 x{w[0], w[1], w[2], w[3]};
+    if constexpr (stream)
+      __builtin_nontemporal_store(x, reinterpret_cast<rot_u4*>(o));
+    else
+      *reinterpret_cast<rot_u4*>(o) = x;
   } else {
 #pragma unroll
     for (int i = 0; i < 8; ++i) o[i] = uint16_t(w[i >> 1] >> (16 * (i & 1)));
@@ -102,11 +110,125 @@ __device__ __forceinline__ A row_sum(A v, int lpr, int lane, int q) {
   return s;
 }
 
-// Channels c0 .. c0 + 7 of row (t, h) of J, normed and rotated, computed in A.
-// Lane q of the row's lpr lanes; every lane of the wavefront takes part.  In
-// a half-split rotation the pair's other eight channels are a second load (a
-// hit in the cache: cheaper than eight cross-lane moves).
-template <typename A, int32_t dtype, bool vec>
+// Rows out: a lane takes two chunks of 8 channels, which in a half-split
+// rotation are the two sides of 8 pairs, of `heads` consecutive heads of one
+// token, so that the token's cosines and sines (and weights that heads share)
+// are loaded once for all of them; kHeadsAhead heads' loads are in flight together.
+constexpr int kHeadsAhead = 2;
+
+__host__ __device__ inline int32_t row_lanes(int32_t hd, int32_t split_rd) { return split_rd / 16 + (hd - split_rd + 15) / 16; }
+
+template <int32_t dtype, bool vec, bool vec_out, bool stream>
+__device__ __forceinline__ void rows_out(const RotaryArgs& R, const RotaryJob& J, uint32_t b, int wave, int lane) {
+  const int32_t hd = R.head_dim, rd = J.rotate ? R.rotary.rotary_dim : 0;
+  const bool half = R.rotary.interleaved == 0;
+  const int32_t split = half ? rd : 0;
+  const int lpr = row_lanes(hd, split), rpw = 64 / lpr, q = lane % lpr, rw = lane / lpr;
+  const uint32_t parts = (uint32_t(J.in.n_heads) + J.heads - 1) / J.heads, tile = b / parts;
+  const int32_t h0 = int32_t(b - tile * parts) * J.heads, h1 = min(h0 + J.heads, J.in.n_heads);
+  const int64_t t = (int64_t(tile) * (kRotThreads / 64) + wave) * rpw + rw;
+  const bool in_rows = rw < rpw && t < R.n_tokens;
+  const int64_t tt = in_rows ? t : 0;
+  const bool paired = q < split / 16;
+  const int32_t c0 = paired ? 8 * q : split + 16 * (q - split / 16);
+  const int32_t c1 = paired ? c0 + rd / 2 : c0 + 8;
+  const bool two = c1 < hd;  // (a lane at the end of an odd number of chunks has one)
+  const int32_t cb = two ? c1 : c0;
+  const bool turn0 = c0 < rd, turn1 = two && (half ? turn0 : c1 < rd);
+  const int32_t pos = rd ? R.positions[tt] : 0;
+  const bool known = uint32_t(pos) < uint32_t(rd ? R.rotary.n_positions : 1);
+  float cs[8], sn[8];
+#pragma unroll
+  for (int i = 0; i < 8; ++i) {
+    cs[i] = 1.f;
+    sn[i] = 0.f;
+  }
+  if (rd) {  // (uniform; interleaved: four pairs of each chunk)
+    const float* row = R.rotary.table + int64_t(known ? pos : 0) * rd;
+    const int32_t p0 = half ? (turn0 ? c0 : 0) : (turn0 ? c0 / 2 : 0), p1 = half ? p0 + 4 : (turn1 ? c1 / 2 : 0);
+    const float4 a = *reinterpret_cast<const float4*>(row + p0), e = *reinterpret_cast<const float4*>(row + p1);
+    const float4 f = *reinterpret_cast<const float4*>(row + rd / 2 + p0), g = *reinterpret_cast<const float4*>(row + rd / 2 + p1);
+    if (turn0) {
+      cs[0] = a.x; cs[1] = a.y; cs[2] = a.z; cs[3] = a.w;
+      sn[0] = f.x; sn[1] = f.y; sn[2] = f.z; sn[3] = f.w;
+    }
+    if (turn1) {
+      cs[4] = e.x; cs[5] = e.y; cs[6] = e.z; cs[7] = e.w;
+      sn[4] = g.x; sn[5] = g.y; sn[6] = g.z; sn[7] = g.w;
+    }
+  }
+  const bool norm = J.norm.weight != nullptr;
+  float w0[8], w1[8];
+  if (norm) {
+    load_weight8<vec>(J.norm, h0, c0, w0);
+    load_weight8<vec>(J.norm, h0, cb, w1);
+  }
+  const float inv = 1.f / float(hd);
+  for (int32_t h = h0; h < h1; h += kHeadsAhead) {
+    float x[kHeadsAhead][8], y[kHeadsAhead][8];
+#pragma unroll
+    for (int k = 0; k < kHeadsAhead; ++k) {
+      const int64_t base = tt * J.in.token_stride + int64_t(min(h + k, h1 - 1)) * J.in.head_stride;
+      load8<dtype, vec>(J.in.data, base + c0, x[k]);
+      load8<dtype, vec>(J.in.data, base + cb, y[k]);
+    }
+#pragma unroll
+    for (int k = 0; k < kHeadsAhead; ++k) {
+      if (h + k >= h1) break;  // (uniform)
+      if (norm) {
+        if (J.norm.head_stride != 0 && h + k > h0) {
+          load_weight8<vec>(J.norm, h + k, c0, w0);
+          load_weight8<vec>(J.norm, h + k, cb, w1);
+        }
+        float ss = 0.f, s1 = 0.f;
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+          ss = __builtin_fmaf(x[k][i], x[k][i], ss);
+          s1 = __builtin_fmaf(y[k][i], y[k][i], s1);
+        }
+        ss = row_sum<float>(two ? ss + s1 : ss, lpr, lane, q);
+        const float r = 1.f / sqrtf(__builtin_fmaf(ss, inv, J.norm.eps));
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+          x[k][i] *= r * w0[i];
+          y[k][i] *= r * w1[i];
+        }
+      }
+      if (half) {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+          const float u = x[k][i], v = y[k][i];
+          x[k][i] = paired ? __builtin_fmaf(u, cs[i], -v * sn[i]) : u;
+          y[k][i] = paired ? __builtin_fmaf(v, cs[i], u * sn[i]) : v;
+        }
+      } else {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const float u = x[k][2 * i], v = x[k][2 * i + 1], u1 = y[k][2 * i], v1 = y[k][2 * i + 1];
+          x[k][2 * i] = turn0 ? __builtin_fmaf(u, cs[i], -v * sn[i]) : u;
+          x[k][2 * i + 1] = turn0 ? __builtin_fmaf(v, cs[i], u * sn[i]) : v;
+          y[k][2 * i] = turn1 ? __builtin_fmaf(u1, cs[i + 4], -v1 * sn[i + 4]) : u1;
+          y[k][2 * i + 1] = turn1 ? __builtin_fmaf(v1, cs[i + 4], u1 * sn[i + 4]) : v1;
+        }
+      }
+      if (!known) {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) x[k][i] = y[k][i] = __builtin_nanf("");
+      }
+      if (in_rows) {
+        const int64_t o = t * J.out.token_stride + int64_t(h + k) * J.out.head_stride;
+        store8<vec_out, stream>(J.out.data, J.out.dtype, o + c0, x[k]);
+        if (two) store8<vec_out, stream>(J.out.data, J.out.dtype, o + c1, y[k]);
+      }
+    }
+  }
+}
+
+// Rows into pages: channels c0 .. c0 + 7 of row (t, h) of J, normed and
+// rotated in fp64.  Lane q of the row's lpr lanes; every lane of the wavefront
+// takes part.  In a half-split rotation the pair's other eight channels are a
+// second load (a hit in the cache: cheaper than eight cross-lane moves).
+template <int32_t dtype, bool vec>
 __device__ __forceinline__ void rotated8(const RotaryArgs& R, const RotaryJob& J, int64_t t, int32_t h, int lpr, int lane,
                                          int q, int32_t c0, float (&z)[8]) {
   const int64_t base = t * J.in.token_stride + h * J.in.head_stride;
@@ -142,39 +264,39 @@ __device__ __forceinline__ void rotated8(const RotaryArgs& R, const RotaryJob& J
       sn[0] = b.x; sn[1] = b.y; sn[2] = b.z; sn[3] = b.w;
     }
   }
-  A y[8], yp[8];
+  double y[8], yp[8];
 #pragma unroll
   for (int i = 0; i < 8; ++i) {
-    y[i] = A(x[i]);
-    yp[i] = half && rd ? A(xp[i]) : A(0);
+    y[i] = x[i];
+    yp[i] = half && rd ? double(xp[i]) : 0.0;
   }
   if (J.norm.weight != nullptr) {  // (uniform)
-    A ss = 0;
+    double ss = 0;
 #pragma unroll
     for (int i = 0; i < 8; ++i) ss = fma(y[i], y[i], ss);
-    ss = row_sum<A>(has ? ss : A(0), lpr, lane, q);
-    const A r = A(1) / sqrt(ss / A(hd) + A(J.norm.eps));
+    ss = row_sum<double>(has ? ss : 0.0, lpr, lane, q);
+    const double r = 1.0 / sqrt(ss / hd + double(J.norm.eps));
     float w[8];
     load_weight8<vec>(J.norm, h, c, w);
 #pragma unroll
-    for (int i = 0; i < 8; ++i) y[i] = y[i] * (r * A(w[i]));
+    for (int i = 0; i < 8; ++i) y[i] = y[i] * (r * double(w[i]));
     if (half && rd) {
       load_weight8<vec>(J.norm, h, pc, w);
 #pragma unroll
-      for (int i = 0; i < 8; ++i) yp[i] = yp[i] * (r * A(w[i]));
+      for (int i = 0; i < 8; ++i) yp[i] = yp[i] * (r * double(w[i]));
     }
   }
   if (rd) {
     if (half) {
 #pragma unroll
       for (int i = 0; i < 8; ++i) {
-        const A v = fma(y[i], A(cs[i]), (second ? yp[i] : -yp[i]) * A(sn[i]));
+        const double v = fma(y[i], double(cs[i]), (second ? yp[i] : -yp[i]) * double(sn[i]));
         y[i] = turns ? v : y[i];
       }
     } else {
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
-        const A a = y[2 * i], b = y[2 * i + 1], co = A(cs[i]), si = A(sn[i]);
+        const double a = y[2 * i], b = y[2 * i + 1], co = cs[i], si = sn[i];
         y[2 * i] = turns ? fma(a, co, -b * si) : a;
         y[2 * i + 1] = turns ? fma(b, co, a * si) : b;
       }
@@ -205,8 +327,7 @@ __device__ __forceinline__ int32_t keep_at(const RotaryArgs& R, const RotaryJob&
 }
 
 // Blocks [0, b1) take rows of j0, [b1, b2) rows of j1 and the rest rows of j2.
-// A block that writes rows takes consecutive (token, head) rows, whose heads
-// share a table row.  A block that writes pages takes consecutive tokens of
+// A block that writes pages takes consecutive tokens of
 // one head: their codes are neighbours in the page, and lines written whole.
 template <int32_t dtype, bool vec, bool vec_out>
 __global__ void __launch_bounds__(kRotThreads) rotary_rows8_kernel(RotaryArgs R, RotaryJob j0, RotaryJob j1, RotaryJob j2,
@@ -216,16 +337,11 @@ __global__ void __launch_bounds__(kRotThreads) rotary_rows8_kernel(RotaryArgs R,
   const RotaryJob J = block < b1 ? j0 : block < b2 ? j1 : j2;
   const uint32_t b = block < b1 ? block : block < b2 ? block - b1 : block - b2;
   const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
-  float z[8];
   if (J.out.data != nullptr) {  // (uniform)
-    const int lpr = R.head_dim / 8, rpw = 64 / lpr, q = lane % lpr, rw = lane / lpr;
-    const int64_t r = (int64_t(b) * (kRotThreads / 64) + wave) * rpw + rw;
-    const bool in_rows = rw < rpw && r < R.n_tokens * J.in.n_heads;
-    const int64_t rr = in_rows ? r : 0;
-    const int64_t t = int64_t(uint64_t(rr) / uint32_t(J.in.n_heads));
-    const int32_t h = int32_t(rr - t * J.in.n_heads);
-    rotated8<float, dtype, vec>(R, J, t, h, lpr, lane, q, 8 * q, z);
-    if (in_rows) store8<vec_out>(J.out.data, J.out.dtype, t * J.out.token_stride + h * J.out.head_stride + 8 * q, z);
+    if (vec_out && J.stream)
+      rows_out<dtype, vec, vec_out, vec_out>(R, J, b, wave, lane);
+    else
+      rows_out<dtype, vec, vec_out, false>(R, J, b, wave, lane);
     return;
   }
   const dc_page_geometry geo = J.pool.geometry;
@@ -239,7 +355,8 @@ __global__ void __launch_bounds__(kRotThreads) rotary_rows8_kernel(RotaryArgs R,
   int32_t page, slot;
   token_dest(R, J, tt, h, &page, &slot);
   const int32_t kr = keep_at(R, J, tt, h);
-  rotated8<double, dtype, vec>(R, J, tt, h, lpr, lane, q, c0, z);
+  float z[8];
+  rotated8<dtype, vec>(R, J, tt, h, lpr, lane, q, c0, z);
   if (in_rows && kr >= 0 && c0 < geo.head_dim) {
     float4* o = reinterpret_cast<float4*>(J.keep + int64_t(kr) * geo.head_dim + c0);
     o[0] = float4{z[0], z[1], z[2], z[3]};
@@ -356,7 +473,16 @@ static int check_rotary(const RotaryArgs& R, const char* who) {
   return DC_OK;
 }
 
-static int launch_rotary(const RotaryArgs& R, const RotaryJob* jobs, int n_jobs, hipStream_t stream) {
+// A lane takes several heads of a token as long as that leaves kRowBlocks
+// blocks, and rows that the L2 would not hold bypass it.  16384 tokens of 28 + 4
+// heads of 128 channels, bf16 (277 MB): 46 us (6.0 TB/s); with at most 8 heads a
+// lane, four of them in flight, 53 us; without the bypass 59; with 2048 / 4096
+// blocks asked for 61 / 67 (all with four in flight).
+constexpr int64_t kRowBlocks = 1024;
+constexpr int32_t kMaxHeads = 16;
+constexpr int64_t kStreamBytes = int64_t(32) << 20;  // the L2 of all dies
+
+static int launch_rotary(const RotaryArgs& R, RotaryJob* jobs, int n_jobs, hipStream_t stream) {
   // the 8-channel kernel where every row and pair fits it
   const int32_t hd = R.head_dim, rd = R.rotary.rotary_dim;
   bool fast = hd % 8 == 0 && hd <= 512 && rd % (R.rotary.interleaved ? 8 : 16) == 0;
@@ -377,13 +503,19 @@ static int launch_rotary(const RotaryArgs& R, const RotaryJob* jobs, int n_jobs,
   for (int i = 0; i < 3; ++i) {
     int64_t blocks = 0;
     if (i < n_jobs) {
-      const RotaryJob& j = jobs[i];
+      RotaryJob& j = jobs[i];
       const int64_t rows = R.n_tokens * j.in.n_heads;
       if (!fast) {
         blocks = rows;
       } else if (j.out.data) {
-        const int64_t per = kRotThreads / 64 * (64 / (hd / 8));
-        blocks = (rows + per - 1) / per;
+        // as many heads a lane as leave kRowBlocks blocks
+        const int64_t per = kRotThreads / 64 * (64 / row_lanes(hd, R.rotary.interleaved || !j.rotate ? 0 : rd));
+        const int64_t tiles = (R.n_tokens + per - 1) / per;
+        auto parts = [&](int32_t heads) { return int64_t((j.in.n_heads + heads - 1) / heads); };
+        j.stream = rows * hd * esize(j.out.dtype) > kStreamBytes;
+        j.heads = 1;
+        while (j.heads < kMaxHeads && j.heads < j.in.n_heads && tiles * parts(2 * j.heads) >= kRowBlocks) j.heads *= 2;
+        blocks = tiles * parts(j.heads);
       } else {
         const int64_t per = kRotThreads / 64 * (64 / (num_groups(j.pool.geometry) * j.pool.geometry.group_size / 8));
         blocks = (R.n_tokens + per - 1) / per * j.in.n_heads;

@@ -29,15 +29,23 @@ policy become M3 (the recent window), and the header fields
 record the choice.  Page statistics (``observe_page``) are computed on the
 device, only when a candidate needs them.  Several sequences
 (``batch_size``) share the pools and decode in one launch per layer.
+
+A model's projections can be handed over as they are: ``append_rotated``
+norms and rotates a chunk's queries and keys and appends its keys and values in
+one launch, ``attend_chunk`` attends the chunk's queries causally (a prompt's
+chunk, drafted tokens to verify), and ``read_layer`` gives the cached tokens
+back as dense rows.
 """
 from __future__ import annotations
 
 import numpy as np
 
+from .chunk import attend_cached
 from .config import DotCacheConfig, observe_page
 from .decode import decode_paged, plan_decode, workspace_bytes
 from .encode import make_header, resolve_encode_spec
 from .page_pool import DevicePagePool, PoolGeometry, page_format_of
+from .rotary import head_norm, index_tensor
 
 
 def _torch():
@@ -105,6 +113,7 @@ class DevicePagedKVCache:
         self._host_tables = [None] * L  # the same tables on the host
         self._spec_memo: dict = {}
         self._workspace = None
+        self._chunk_plan = None  # lengths and plan of the last attend_chunk
 
     # ---- formats -----------------------------------------------------------
     def _page_format(self, kind: str, layer_id: int, kv_head_id: int) -> tuple[int, int]:
@@ -258,40 +267,14 @@ class DevicePagedKVCache:
         if np.any(self._seq_len[lid] != int(token_index)):
             raise ValueError(f"layer {lid} expected token_index {int(self._seq_len[lid, 0])}, received {token_index}")
         keys, values = self._one_dtype(keys, values)
-        B, H, P, hd = self.batch_size, self.num_key_value_heads, self.config.tokens_per_page, self.config.head_dim
-        n = int(keys.shape[2])
-        done = 0
-        while done < n:
-            fill = int(self._seq_len[lid, 0] - self._tail_start[lid, 0])
-            take = min(P - fill, n - done)
-            tails = [self._tail_ids(kind, lid) for kind in ("K", "V")]
-            for kind, tail in zip(("K", "V"), tails):
-                self._pool(kind).set_tokens(tail, fill + take)
-            # rows into the tail pages (exact) and the fp32 tail
-            self.k_pool.encode_streams_with(self.v_pool, keys[:, :, done: done + take].reshape(B * H, take, hd),
-                                            values[:, :, done: done + take].reshape(B * H, take, hd),
-                                            self._upload_tables(tails[0][:, None], tails[1][:, None]), first_slot=fill,
-                                            keep=self._tails(lid))
-            done += take
-            self._seq_len[lid, :] += take
-            if fill + take == P:  # every stream's tail is full: encode it into a page
-                # the page's context is the whole step's (reference
-                # model_kv_cache.py:3887-3892 passes token_index + n)
-                starts = np.repeat(self._tail_start[lid], H)[:, None]
-                ids = []
-                for kind in ("K", "V"):
-                    rows = lambda s, i, kind=kind: self._tail_rows[kind][lid, s // H, s % H]  # noqa: E731
-                    ids.append(self._new_pages(kind, lid, rows, starts, np.full((B * H, 1), int(token_index) + n)))
-                    self._pool(kind).set_tokens(self._tail_page[kind][lid].reshape(-1), 0)
-                self.k_pool.encode_streams_with(self.v_pool, *(t.view(B * H, P, hd) for t in self._tails(lid)),
-                                                self._upload_tables(*ids))
-                self._tail_start[lid, :] = self._seq_len[lid, :]
-                self._tables[lid] = None
-            elif fill == 0:
-                self._tables[lid] = None  # the tail joins the tables
-            elif self._tables[lid] is not None:  # the same pages, a longer tail
-                k_table, v_table, counts, _ = self._tables[lid]
-                self._tables[lid] = (k_table, v_table, counts, np.full(B, fill + take, dtype=np.int32))
+        B, H, hd = self.batch_size, self.num_key_value_heads, self.config.head_dim
+
+        def write(first: int, take: int, tables, slot: int, keep: bool):
+            self.k_pool.encode_streams_with(self.v_pool, keys[:, :, first: first + take].reshape(B * H, take, hd),
+                                            values[:, :, first: first + take].reshape(B * H, take, hd),
+                                            tables.view(2, B * H, -1), first_slot=slot, keep=self._tails(lid))
+
+        self._append(lid, int(keys.shape[2]), int(token_index), write, direct=False)
 
     def decode_layer(self, layer_id: int, query_step, q_head_to_kv_head=None, *, query_scale: float = 1.0):
         """Attention of ``query_step [B, Hq, hd]`` over layer ``layer_id``'s
@@ -340,6 +323,168 @@ class DevicePagedKVCache:
         res = torch.empty_like(out)
         res[:, torch.from_numpy(order).to(self.device)] = out
         return res
+
+    # ---- chunks of tokens ------------------------------------------------------
+    def _token_major(self, x, heads: int, tokens: int | None, name: str):
+        """``x [B, heads, n, hd]`` (``[heads, n, hd]`` with batch 1) on the
+        device as ``[B, n, heads, hd]``, in fp32, fp16 or bf16."""
+        torch = _torch()
+        t = x if isinstance(x, torch.Tensor) else torch.from_numpy(np.ascontiguousarray(np.asarray(x, dtype=np.float32)))
+        t = t.to(device=self.device)
+        if t.dtype not in (torch.float32, torch.float16, torch.bfloat16):
+            t = t.float()
+        if t.dim() == 3 and self.batch_size == 1:
+            t = t.unsqueeze(0)
+        B, hd = self.batch_size, self.config.head_dim
+        if t.dim() != 4 or (t.shape[0], t.shape[1], t.shape[3]) != (B, heads, hd):
+            raise ValueError(f"{name} must have shape [{B}, {heads}, tokens, {hd}]" + (" or [heads, tokens, head_dim]" if B == 1 else ""))
+        if tokens is not None and t.shape[2] != tokens:
+            raise ValueError(f"{name} must hold {tokens} tokens")
+        return (t if t.stride(3) == 1 else t.contiguous()).transpose(1, 2)
+
+    def append_rotated(self, layer_id: int, query_step, key_step, value_step, token_index: int, rotary, *, positions=None,
+                       q_weight=None, k_weight=None, eps: float = 1e-6):
+        """:meth:`append_step` of projections as they are: ``query_step
+        [B, Hq, n, hd]`` (or None) and ``key_step [B, H, n, hd]`` are normed
+        (``q_weight`` / ``k_weight``, None: not) and rotated to ``positions``
+        (``[n]`` or ``[B, n]``; default ``token_index ..``) by ``rotary`` (a
+        :class:`~dotcache_amd.rotary.RotaryTable`, or None), keys and
+        ``value_step`` are appended, and the queries are returned in their
+        shape and type (fp32 if the three types differ).  One launch per
+        stretch of pages: the one that fills the tail, whole pages straight
+        into their formats, the new tail."""
+        torch = _torch()
+        lid = self._check_layer(layer_id)
+        B, H, P, hd = self.batch_size, self.num_key_value_heads, self.config.tokens_per_page, self.config.head_dim
+        k = self._token_major(key_step, H, None, "key_step")
+        n = int(k.shape[1])
+        v = self._token_major(value_step, H, n, "value_step")
+        q = None if query_step is None else self._token_major(query_step, self.num_attention_heads, n, "query_step")
+        if len({x.dtype for x in (q, k, v) if x is not None}) > 1:
+            q, k, v = (x if x is None else x.float() for x in (q, k, v))
+        token_index = int(token_index)
+        if np.any(self._seq_len[lid] != token_index):
+            raise ValueError(f"layer {lid} expected token_index {int(self._seq_len[lid, 0])}, received {token_index}")
+        # what the launches below would refuse, before anything is appended
+        pos = None
+        if rotary is not None:
+            if rotary.head_dim != hd or rotary.table.device != k.device:
+                raise ValueError("the rotary table is for another head_dim or device")
+            pos = np.arange(token_index, token_index + n) if positions is None else positions
+            pos = pos if isinstance(pos, torch.Tensor) else np.asarray(pos)
+            if tuple(pos.shape) not in ((n,), (B, n)):
+                raise ValueError(f"positions must have shape [{n}] or [{B}, {n}]")
+            flat = pos.expand(B, n).reshape(-1) if isinstance(pos, torch.Tensor) else np.broadcast_to(pos, (B, n)).reshape(-1)
+            pos = index_tensor(flat, "positions", B * n, k.device, rotary.n_positions).view(B, n)
+        head_norm(q_weight, "queries' weight", self.num_attention_heads, hd, float(eps), k.device)
+        head_norm(k_weight, "keys' weight", H, hd, float(eps), k.device)
+        out = None if q is None else torch.empty((B, n, self.num_attention_heads, hd), dtype=q.dtype, device=q.device)
+
+        def write(first: int, take: int, tables, slot: int, keep: bool):
+            """Tokens [first, first + take) of the step to tables ``[2, B, H,
+            pages]`` from their slot ``slot`` on, and (keep) to the fp32 tail."""
+            b, t = np.repeat(np.arange(B), take), np.tile(np.arange(slot, slot + take), B)
+            row, token, kept = torch.from_numpy(np.stack([b, t, b * (H * P) + t]).astype(np.int32)).to(self.device)
+            part = [None if x is None else x[:, first: first + take].reshape(B * take, -1, hd) for x in (q, k, v, out)]
+            if out is not None and B > 1 and take < n:  # (a slice of a batch is not rows of one stride)
+                part[3] = torch.empty_like(part[0])
+            self.k_pool.append_rotary_with(
+                self.v_pool, *part[:3], None if pos is None else pos[:, first: first + take].reshape(-1), rotary, tables, row,
+                token, q_weight=q_weight, k_weight=k_weight, eps=eps, out=part[3],
+                keep=(*self._tails(lid), kept, P) if keep else None)
+            if out is not None and B > 1 and take < n:
+                out[:, first: first + take] = part[3].view(B, take, -1, hd)
+
+        self._append(lid, n, token_index, write,
+                     direct=not any(self.config.chooses_page_modes(kind) for kind in ("K", "V")))
+        return None if out is None else out.transpose(1, 2)
+
+    def _append(self, lid: int, n: int, token_index: int, write, direct: bool) -> None:
+        """The lifecycle of :meth:`append_step` around ``write(first, take,
+        tables, slot, keep)``.  direct: whole pages of the step that the tail
+        holds nothing of are written as they are (their modes do not depend
+        on their rows)."""
+        B, H, P, hd = self.batch_size, self.num_key_value_heads, self.config.tokens_per_page, self.config.head_dim
+        done = 0
+        while done < n:
+            fill = int(self._seq_len[lid, 0] - self._tail_start[lid, 0])
+            pages = (n - done) // P if direct and fill == 0 else 0
+            if pages:
+                starts = np.repeat(self._tail_start[lid], H)[:, None] + P * np.arange(pages)
+                ids = [self._new_pages(kind, lid, None, starts, np.full(starts.shape, token_index + n)) for kind in ("K", "V")]
+                write(done, pages * P, self._upload_tables(*ids).view(2, B, H, pages), 0, False)
+                done += pages * P
+                self._seq_len[lid, :] += pages * P
+                self._tail_start[lid, :] = self._seq_len[lid, :]
+                self._tables[lid] = None
+                continue
+            take = min(P - fill, n - done)
+            tails = [self._tail_ids(kind, lid) for kind in ("K", "V")]
+            for kind, tail in zip(("K", "V"), tails):
+                self._pool(kind).set_tokens(tail, fill + take)
+            # rows into the tail pages (exact) and the fp32 tail
+            write(done, take, self._upload_tables(tails[0][:, None], tails[1][:, None]).view(2, B, H, 1), fill, True)
+            done += take
+            self._seq_len[lid, :] += take
+            if fill + take == P:  # every stream's tail is full: encode it into a page
+                # the page's context is the whole step's (reference
+                # model_kv_cache.py:3887-3892 passes token_index + n)
+                starts = np.repeat(self._tail_start[lid], H)[:, None]
+                ids = []
+                for kind in ("K", "V"):
+                    rows = lambda s, i, kind=kind: self._tail_rows[kind][lid, s // H, s % H]  # noqa: E731
+                    ids.append(self._new_pages(kind, lid, rows, starts, np.full((B * H, 1), token_index + n)))
+                    self._pool(kind).set_tokens(self._tail_page[kind][lid].reshape(-1), 0)
+                self.k_pool.encode_streams_with(self.v_pool, *(t.view(B * H, P, hd) for t in self._tails(lid)),
+                                                self._upload_tables(*ids))
+                self._tail_start[lid, :] = self._seq_len[lid, :]
+                self._tables[lid] = None
+            elif fill == 0:
+                self._tables[lid] = None  # the tail joins the tables
+            elif self._tables[lid] is not None:  # the same pages, a longer tail
+                k_table, v_table, counts, _ = self._tables[lid]
+                self._tables[lid] = (k_table, v_table, counts, np.full(B, fill + take, dtype=np.int32))
+
+    def attend_chunk(self, layer_id: int, query_chunk, q_head_to_kv_head=None, *, query_scale: float = 1.0):
+        """Causal attention of ``query_chunk [B, Hq, n, hd]``, the queries of
+        each sequence's last n cached tokens (append them first): token i
+        attends itself and all before it.  Heads map as in
+        :meth:`decode_layer`.  Returns ``[B, Hq, n, hd]`` in the queries'
+        type on the device."""
+        lid = self._check_layer(layer_id)
+        q = self._token_major(query_chunk, self.num_attention_heads, None, "query_chunk")
+        B, n, Hq, hd = q.shape
+        held = self._held(lid)
+        if np.any(held < n):
+            raise ValueError(f"layer {lid} holds {int(held.min())} tokens, fewer than the chunk's {n}")
+        if n == 0:
+            return q.transpose(1, 2).clone()
+        k_table, v_table, _, _ = self._layer_tables(lid)
+        out = attend_cached(self, q.reshape(B * n, Hq, hd), np.full(B, n, dtype=np.int32), held.astype(np.int32), k_table,
+                            v_table, q_head_to_kv_head, self.q_head_to_kv_head, query_scale)
+        return out.view(B, n, Hq, hd).transpose(1, 2)
+
+    def _held(self, lid: int) -> np.ndarray:
+        """Tokens in each sequence's pages and tail (a prefill may have stored
+        only the last of its context)."""
+        P = self.config.tokens_per_page
+        pages = np.array([len(self._pages["K"][lid][b][0]) for b in range(self.batch_size)])
+        return P * pages + (self._seq_len[lid] - self._tail_start[lid])
+
+    def read_layer(self, layer_id: int, *, dtype=None):
+        """The cached tokens of a layer as dense rows ``[B, H, T, hd]``, keys
+        and values, as their pages hold them (fp32, or ``dtype`` fp16 / bf16)."""
+        torch = _torch()
+        lid = self._check_layer(layer_id)
+        B, H, hd = self.batch_size, self.num_key_value_heads, self.config.head_dim
+        T = int(self._held(lid)[0])
+        if T == 0:
+            x = torch.empty((2, B, H, 0, hd), dtype=dtype or torch.float32, device=self.device)
+            return x[0], x[1]
+        k_table, v_table, _, _ = self._layer_tables(lid)
+        row, token = np.repeat(np.arange(B), T), np.tile(np.arange(T), B)
+        rows = self.k_pool.read_tokens_with(self.v_pool, torch.stack([k_table, v_table]), row, token, dtype=dtype)
+        return tuple(x.view(B, T, H, hd).transpose(1, 2) for x in rows)
 
     # ---- bookkeeping -------------------------------------------------------
     def _layer_tables(self, lid: int):

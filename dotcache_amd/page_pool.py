@@ -91,15 +91,17 @@ def current_stream_ptr() -> int:
 def call_on(device, fn, what: str, *args) -> None:
     """``fn(*args, stream)`` on the current stream of the tensors' device
     (which need not be the current device), its status checked."""
-    cuda = _torch().cuda
     if device.type != "cuda":
         raise ValueError(f"{what}: tensors must be on a GPU")
+    torch = _torch()
+    cuda = torch.cuda
     if device.index == cuda.current_device():
-        st = fn(*args, current_stream_ptr())
+        st = fn(*args, torch._C._cuda_getCurrentRawStream(device.index))
     else:
         with cuda.device(device):
-            st = fn(*args, current_stream_ptr())
-    _lib.check(st, what)
+            st = fn(*args, torch._C._cuda_getCurrentRawStream(device.index))
+    if st:
+        _lib.check(st, what)
 
 
 @dataclass(frozen=True)
@@ -625,21 +627,20 @@ class DevicePagePool:
 
         torch = _torch()
         g, vg = self.geometry, v_pool.geometry
-        if (vg.head_dim, vg.page_capacity) != (g.head_dim, g.page_capacity):
+        if vg is not g and (vg.head_dim, vg.page_capacity) != (g.head_dim, g.page_capacity):
             raise ValueError("key and value pools must share head_dim and page_capacity")
-        device = self.arena.device
+        device, shape = self.arena.device, tables.shape
         if v_pool.arena.device != device or tables.device != device:
             raise ValueError(f"pools and tables must be on {device}")
-        if tables.dtype != torch.int32 or tables.dim() != 4 or tables.shape[0] != 2 or not tables.is_contiguous():
+        if tables.dtype is not torch.int32 or len(shape) != 4 or shape[0] != 2 or not tables.is_contiguous():
             raise ValueError("tables must be contiguous int32 [2, rows, heads, pages]")
-        _, R, H, W = tables.shape
+        _, R, H, W = shape
         if R == 0 or H == 0 or W == 0:
             raise ValueError("tables must name at least one page")
-        row = index_tensor(row, "row", len(row), device)
-        token = index_tensor(token, "token", int(row.shape[0]), device)
+        T = len(row)
+        row, token = index_tensor(row, "row", T, device), index_tensor(token, "token", T, device)
         at = tables.data_ptr()
-        dest = _lib.TokenDest(at, at + 4 * R * H * W, row.data_ptr(), token.data_ptr(), R, W, g.page_capacity)
-        return dest, (row, token)
+        return _lib.TokenDest(at, at + 4 * R * H * W, row.data_ptr(), token.data_ptr(), R, W, g.page_capacity), (row, token)
 
     def append_rotary_with(self, v_pool: "DevicePagePool", queries, keys, values, positions, rotary, tables, row, token, *,
                            q_weight=None, k_weight=None, eps: float = 1e-6, keep=None, out=None):
@@ -663,22 +664,23 @@ class DevicePagePool:
         at row ``row[t] + h * head_stride`` (``row[t]`` < 0: not; no row
         twice) of two fp32 buffers ``[m, hd]``.  Pages' token counts are not changed.  ``out``
         takes the queries (their dtype or fp32; may be ``queries`` itself)."""
-        from .rotary import _NO_NORM, _NO_ROWS, head_norm, index_tensor, token_rows
+        from .rotary import _ABSENT, _NO_ROTARY, head_norm, index_tensor, token_rows
 
         torch = _torch()
         hd, device = self.geometry.head_dim, self.arena.device
         dest, held = self._token_dest(v_pool, tables, row, token)
-        T, H = int(held[0].shape[0]), int(tables.shape[2])
+        T, H = held[0].shape[0], tables.shape[2]
+        eps = float(eps)
         for x, name in ((keys, "keys"), (values, "values")):
-            if x.dim() != 3 or x.shape[0] != T or x.shape[1] != H or x.dtype != keys.dtype:
+            if x.shape[:2] != (T, H) or x.dtype != keys.dtype:
                 raise ValueError(f"{name} must have shape [{T}, {H}, {hd}] and the keys' dtype")
         if rotary is not None:
             if rotary.head_dim != hd or rotary.table.device != device:
                 raise ValueError("the rotary table is for another head_dim or device")
             positions = index_tensor(positions, "positions", T, device, rotary.n_positions)
-        q_args = (_NO_ROWS, _NO_NORM, _NO_ROWS)
+        q_args = _ABSENT
         if queries is not None:
-            if queries.dim() != 3 or queries.shape[0] != T or queries.dtype != keys.dtype:
+            if queries.shape[0] != T or queries.dim() != 3 or queries.dtype != keys.dtype:
                 raise ValueError("queries must have the keys' tokens and dtype")
             if out is None:
                 out = torch.empty(queries.shape, dtype=queries.dtype, device=device)
@@ -696,9 +698,8 @@ class DevicePagePool:
             keep_row = index_tensor(keep[2], "kept rows' index", T, device)
             held += (keep_row,)
             keep_args = (keep[0].data_ptr(), keep[1].data_ptr(), keep_row.data_ptr(), int(keep[3]), int(keep[0].shape[0]))
-        args = (positions.data_ptr() if rotary is not None else None,
-                rotary.c() if rotary is not None else _lib.Rotary(), *q_args, token_rows(keys, "keys", hd, device),
-                head_norm(k_weight, "keys' weight", H, hd, eps, device), token_rows(values, "values", hd, device), dest,
+        args = (positions.data_ptr() if rotary is not None else None, rotary._c if rotary is not None else _NO_ROTARY, *q_args,
+                token_rows(keys, "keys", hd, device), head_norm(k_weight, "keys' weight", H, hd, eps, device), token_rows(values, "values", hd, device), dest,
                 self.c_pool(), v_pool.c_pool(), *keep_args)
         if T:
             call_on(device, _lib.lib().dc_append_rotary, "dc_append_rotary", T, *args)

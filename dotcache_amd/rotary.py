@@ -17,8 +17,6 @@ into pages), rounded once to the output's type.
 """
 from __future__ import annotations
 
-import ctypes as C
-
 import numpy as np
 
 from . import _lib
@@ -26,6 +24,8 @@ from .page_pool import call_on, dtype_code
 
 _NO_ROWS = _lib.TokenRows()
 _NO_NORM = _lib.Norm()
+_NO_ROTARY = _lib.Rotary()
+_ABSENT = (_NO_ROWS, _NO_NORM, _NO_ROWS)
 
 
 def _torch():
@@ -71,26 +71,28 @@ class RotaryTable:
 
 def token_rows(x, name: str, head_dim: int, device) -> _lib.TokenRows:
     """``dc_token_rows`` of a tensor ``[tokens, heads, head_dim]``."""
-    if x.dim() != 3 or x.shape[2] != head_dim or (x.stride(2) != 1 and head_dim > 1):
+    shape, stride = x.shape, x.stride()
+    if len(shape) != 3 or shape[2] != head_dim or (stride[2] != 1 and head_dim > 1):
         raise ValueError(f"{name} must have shape [tokens, heads, {head_dim}] with contiguous channels")
     if x.device != device:
         raise ValueError(f"{name} must be on {device}")
-    if x.shape[1] == 0:
+    if shape[1] == 0:
         raise ValueError(f"{name} must have at least one head")
-    return _lib.TokenRows(x.data_ptr(), x.stride(0), x.stride(1), x.shape[1], dtype_code(x))
+    return _lib.TokenRows(x.data_ptr(), stride[0], stride[1], shape[1], dtype_code(x))
 
 
 def head_norm(weight, name: str, heads: int, head_dim: int, eps: float, device) -> _lib.Norm:
     """``dc_norm`` of a weight ``[head_dim]`` or ``[heads, head_dim]`` (None: no norm)."""
     if weight is None:
         return _NO_NORM
-    if tuple(weight.shape) not in ((head_dim,), (heads, head_dim)) or not weight.is_contiguous():
+    shape = weight.shape
+    if (shape != (head_dim,) and shape != (heads, head_dim)) or not weight.is_contiguous():
         raise ValueError(f"{name} must be contiguous, [{head_dim}] or [{heads}, {head_dim}]")
     if weight.device != device:
         raise ValueError(f"{name} must be on {device}")
-    if not float(eps) >= 0.0:
+    if not eps >= 0.0:
         raise ValueError("eps must be non-negative")
-    return _lib.Norm(weight.data_ptr(), dtype_code(weight), head_dim if weight.dim() == 2 else 0, float(eps))
+    return _lib.Norm(weight.data_ptr(), dtype_code(weight), head_dim if len(shape) == 2 else 0, eps)
 
 
 def index_tensor(x, name: str, tokens: int, device, limit: int | None = None):
@@ -98,6 +100,9 @@ def index_tensor(x, name: str, tokens: int, device, limit: int | None = None):
     Host values (a list or numpy array) are checked against ``[0, limit)``;
     device values are guarded by the kernels."""
     torch = _torch()
+    if type(x) is torch.Tensor and x.dtype is torch.int32 and x.shape == (tokens,) and x.device == device and x.is_contiguous() \
+            and device.type != "cpu":
+        return x
     if not isinstance(x, torch.Tensor) or x.device.type == "cpu":
         host = np.asarray(x)
         if host.size and not np.issubdtype(host.dtype, np.integer):
@@ -133,35 +138,40 @@ def norm_rotate(queries, keys, positions, rotary: RotaryTable | None, *, q_weigh
     the table gives NaN rows; a host one raises ValueError.
     """
     torch = _torch()
-    given = [x for x in (queries, keys) if x is not None]
-    if not given:
+    first = queries if queries is not None else keys
+    if first is None:
         raise ValueError("norm_rotate needs queries or keys")
-    first = given[0]
-    T, hd, device = int(first.shape[0]), int(first.shape[-1]), first.device
+    if first.dim() != 3:
+        raise ValueError("queries and keys must have shape [tokens, heads, head_dim]")
+    T, _, hd = first.shape
+    device, dtype = first.device, first.dtype
+    at, table = None, _NO_ROTARY
     if rotary is not None:
         if rotary.head_dim != hd:
             raise ValueError("the rotary table is for another head_dim")
         if rotary.table.device != device:
             raise ValueError(f"the rotary table must be on {device}")
         positions = index_tensor(positions, "positions", T, device, rotary.n_positions)
-    if out is None:
-        out = tuple(None if x is None else torch.empty(x.shape, dtype=x.dtype, device=device) for x in (queries, keys))
-    args = []
-    for x, y, w, name in ((queries, out[0], q_weight, "queries"), (keys, out[1], k_weight, "keys")):
+        at, table = positions.data_ptr(), rotary._c
+    eps = float(eps)
+    made, args = [], []
+    for i, (x, w, name) in enumerate(((queries, q_weight, "queries"), (keys, k_weight, "keys"))):
+        y = None if out is None else out[i]
         if x is None:
-            args += [_NO_ROWS, _NO_NORM, _NO_ROWS]
-            continue
-        if x.shape[0] != T or x.dtype != first.dtype:
-            raise ValueError("queries and keys must have the same tokens and dtype")
-        if y is None or y.shape != x.shape or y.dtype not in (x.dtype, torch.float32):
-            raise ValueError(f"out must hold {name} of their shape, in their dtype or fp32")
-        args += [token_rows(x, name, hd, device), head_norm(w, name + "' weight", x.shape[1], hd, eps, device),
-                 token_rows(y, name + " out", hd, device)]
+            args += _ABSENT
+        else:
+            if x.shape[0] != T or x.dtype != dtype:
+                raise ValueError("queries and keys must have the same tokens and dtype")
+            if out is None:
+                y = torch.empty(x.shape, dtype=dtype, device=device)
+            elif y is None or y.shape != x.shape or (y.dtype != dtype and y.dtype != torch.float32):
+                raise ValueError(f"out must hold {name} of their shape, in their dtype or fp32")
+            args += (token_rows(x, name, hd, device), head_norm(w, name + "' weight", x.shape[1], hd, eps, device),
+                     token_rows(y, name + " out", hd, device))
+        made.append(y)
     if T:
-        call_on(device, _lib.lib().dc_norm_rotate, "dc_norm_rotate", T, hd,
-                C.c_void_p(positions.data_ptr() if rotary is not None else 0),
-                rotary.c() if rotary is not None else _lib.Rotary(), *args)
-    return tuple(out)
+        call_on(device, _lib.lib().dc_norm_rotate, "dc_norm_rotate", T, hd, at, table, *args)
+    return tuple(made)
 
 
 __all__ = ["RotaryTable", "norm_rotate"]
