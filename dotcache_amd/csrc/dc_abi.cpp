@@ -3,6 +3,9 @@
 #include <algorithm>
 #include <cmath>
 #include <cstdint>
+#include <functional>
+#include <queue>
+#include <utility>
 #include <vector>
 #include <cstdarg>
 #include <cstdio>
@@ -288,54 +291,129 @@ int dc_plan_chunk(const int32_t* new_tokens, const int32_t* context, int32_t n_s
       auto takes = [&](int32_t b) {
         return new_tokens[b] > 0 && (int64_t(new_tokens[b]) * n_q <= dc::few_row_limit(head_dim)) == few;
       };
-      auto steps = [&](int32_t b, int64_t row_end) {
-        return (int64_t(context[b]) - new_tokens[b] + (row_end - 1) / n_q + 1 + step - 1) / step;
+      // Row tiles and the steps of their token ranges, streams in order.
+      struct Tile {
+        dc_chunk_item item;
+        int64_t begin, len;
       };
-      int64_t total = 0;  // steps of every row tile's token range
-      for (int32_t b = 0; b < n_seqs; ++b) {
-        if (!takes(b)) continue;
-        const int64_t rows = int64_t(new_tokens[b]) * n_q;
-        if (few) *few_rows = std::max<int32_t>(*few_rows, int32_t(rows));
-        for (int64_t r = 0; r < rows; r += dc::kChunkRows) total += steps(b, std::min<int64_t>(r + dc::kChunkRows, rows)) * n_kv_heads;
-      }
-      // (two blocks of the few-row kernel share a compute unit)
-      const int64_t target = few ? 2 * int64_t(target_items) - 1 : target_items;
-      const int64_t per = std::max<int64_t>((total + target - 1) / target, (min_tokens + step - 1) / step);
-      std::vector<dc_chunk_item> all;
+      std::vector<Tile> tiles;
+      int64_t total = 0;
       int32_t q_begin = 0;
       for (int32_t b = 0; b < n_seqs; q_begin += new_tokens[b], ++b) {
         if (!takes(b)) continue;
         const int32_t rows = new_tokens[b] * n_q, first = context[b] - new_tokens[b];
+        if (few) *few_rows = std::max(*few_rows, rows);
         for (int32_t h = 0; h < n_kv_heads; ++h)
           for (int32_t r = 0; r < rows; r += dc::kChunkRows) {
-            const int32_t r1 = std::min(r + dc::kChunkRows, rows);
-            const int64_t len = steps(b, r1), n = (len + per - 1) / per;
-            if (n > 1 && parts + n * (r1 - r) > INT32_MAX) return dc::fail(DC_EINVAL, "dc_plan_chunk: too many partial results");
-            const int32_t end = first + (r1 - 1) / n_q + 1;
-            if (n > 1) joins.push_back({h, q_begin, r, r1, int32_t(parts), int32_t(n)});
-            for (int64_t i = 0; i < n; ++i)
-              all.push_back({b, h, q_begin, r, r1, first, int32_t(len * i / n * step),
-                             int32_t(std::min<int64_t>(len * (i + 1) / n * step, end)), n > 1 ? int32_t(parts + i * (r1 - r)) : -1});
-            if (n > 1) parts += n * (r1 - r);
+            const int32_t r1 = std::min(r + dc::kChunkRows, rows), end = first + (r1 - 1) / n_q + 1;
+            const int64_t len = (int64_t(end) + step - 1) / step;
+            tiles.push_back({{b, h, q_begin, r, r1, first, 0, end, -1}, total, len});
+            total += len;
           }
       }
-      // A die takes a run of items of equal total length, streams kept together,
-      // the longest first; block i runs on die i % kChunkXcds.
-      auto length = [](const dc_chunk_item& x) { return int64_t(x.kv_end - x.kv_begin); };
-      int64_t sum = 0, seen = 0;
-      for (const auto& x : all) sum += length(x);
-      std::vector<std::vector<dc_chunk_item>> die(dc::kChunkXcds);
-      for (const auto& x : all) {
-        die[std::min<int64_t>((seen + length(x) / 2) * dc::kChunkXcds / std::max<int64_t>(sum, 1), dc::kChunkXcds - 1)].push_back(x);
-        seen += length(x);
+      if (tiles.empty()) continue;
+      // Blocks that run at once: two of the few-row kernel share a compute
+      // unit; tiles of more than 128 channels are two blocks each.
+      const int64_t least = (min_tokens + step - 1) / step, dies = dc::kChunkXcds;
+      const int64_t wide = few ? 2 * int64_t(target_items) - 1 : head_dim > 128 ? (int64_t(target_items) + 1) / 2 : target_items;
+      const int64_t slots = std::max<int64_t>(std::min(wide, total / least), 1);
+      struct Piece {
+        int64_t tile, begin, end, slot;  // steps of the tile
+      };
+      // Two ways to split the tiles.  Even: every tile into equal parts of at
+      // most `per` steps.  Packed: the tiles laid end to end are cut where a
+      // slot has its share, so that a slot's parts add up to it; a part is
+      // never shorter than `least`.
+      auto split = [&](int64_t per) {  // 0: packed
+        std::vector<Piece> out;
+        for (size_t t = 0; t < tiles.size(); ++t) {
+          const int64_t x0 = tiles[t].begin, len = tiles[t].len;
+          std::vector<int64_t> cut{0};
+          if (per > 0) {
+            const int64_t n = (len + per - 1) / per;
+            for (int64_t i = 1; i < n; ++i) cut.push_back(len * i / n);
+          } else {
+            for (int64_t k = x0 * slots / total; k * total / slots < x0 + len; ++k) {
+              const int64_t at = k * total / slots - x0;
+              if (at - cut.back() >= least && len - at >= least) cut.push_back(at);
+            }
+          }
+          cut.push_back(len);
+          for (size_t i = 0; i + 1 < cut.size(); ++i)
+            out.push_back({int64_t(t), cut[i], cut[i + 1], std::min((2 * x0 + cut[i] + cut[i + 1]) * slots / (2 * total), slots - 1)});
+        }
+        return out;
+      };
+      // A die takes a run of slots, the longest of its parts first; block i
+      // runs on die i % dies.  Time of a split, in steps: each part goes to the
+      // slot that is free first, and costs kPart more than its length.
+      constexpr int64_t kPart = 2;
+      auto by_die = [&](const std::vector<Piece>& parts) {
+        std::vector<std::vector<Piece>> die(dies);
+        for (const auto& x : parts) die[x.slot * dies / slots].push_back(x);
+        for (auto& d : die)
+          std::stable_sort(d.begin(), d.end(), [](const Piece& x, const Piece& y) { return x.end - x.begin > y.end - y.begin; });
+        return die;
+      };
+      auto time_of = [&](const std::vector<std::vector<Piece>>& die) {
+        int64_t worst = 0;
+        for (const auto& d : die) {
+          std::priority_queue<int64_t, std::vector<int64_t>, std::greater<int64_t>> free;
+          for (int64_t i = 0; i < (wide + dies - 1) / dies; ++i) free.push(0);
+          for (const auto& x : d) {
+            const int64_t done = free.top() + x.end - x.begin + kPart;
+            free.pop();
+            free.push(done);
+            worst = std::max(worst, done);
+          }
+        }
+        return worst;
+      };
+      const int64_t per = std::max((total + wide - 1) / wide, least);
+      std::vector<std::vector<Piece>> die;
+      int64_t best = INT64_MAX;
+      const int64_t more = (per + 9) / 10;
+      for (const int64_t how : {per, per + more, per + 2 * more, per + 3 * more, int64_t(0)}) {
+        auto d = by_die(split(how));
+        const int64_t t = time_of(d);
+        if (t < best) {
+          best = t;
+          die = std::move(d);
+        }
       }
+      // partial results of a split tile, one part after another
+      std::vector<std::vector<std::pair<int64_t, int64_t>>> of(tiles.size());  // per tile: begin, first partial row
       size_t most = 0;
-      for (auto& d : die) {
-        std::stable_sort(d.begin(), d.end(), [&](const dc_chunk_item& x, const dc_chunk_item& y) { return length(x) > length(y); });
+      for (const auto& d : die) {
         most = std::max(most, d.size());
+        for (const auto& x : d) of[x.tile].push_back({x.begin, -1});
+      }
+      for (size_t t = 0; t < tiles.size(); ++t) {
+        if (of[t].size() < 2) continue;
+        const dc_chunk_item& x = tiles[t].item;
+        const int64_t rows = x.row_end - x.row_begin, n = int64_t(of[t].size());
+        if (parts + n * rows > INT32_MAX) return dc::fail(DC_EINVAL, "dc_plan_chunk: too many partial results");
+        std::sort(of[t].begin(), of[t].end());
+        joins.push_back({x.kv_head, x.q_begin, x.row_begin, x.row_end, int32_t(parts), int32_t(n)});
+        for (auto& p : of[t]) {
+          p.second = parts;
+          parts += rows;
+        }
       }
       for (size_t i = 0; i < most; ++i)
-        for (auto& d : die) order.push_back(i < d.size() ? d[i] : dc_chunk_item{-1, 0, 0, 0, 0, 0, 0, 0, -1});
+        for (const auto& d : die) {
+          if (i >= d.size()) {
+            order.push_back({-1, 0, 0, 0, 0, 0, 0, 0, -1});
+            continue;
+          }
+          const Tile& t = tiles[d[i].tile];
+          dc_chunk_item x = t.item;
+          x.kv_begin = int32_t(d[i].begin * step);
+          x.kv_end = int32_t(std::min<int64_t>(d[i].end * step, x.kv_end));
+          const auto& p = of[d[i].tile];
+          x.partial = int32_t(std::lower_bound(p.begin(), p.end(), std::make_pair(d[i].begin, int64_t(-1)))->second);
+          order.push_back(x);
+        }
       while (!order.empty() && order.back().seq < 0) order.pop_back();
       if (order.size() > INT32_MAX) return dc::fail(DC_EINVAL, "dc_plan_chunk: too many items");
       if (few) *n_few = int32_t(order.size());

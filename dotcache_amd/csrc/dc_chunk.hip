@@ -17,6 +17,8 @@
 //                 which S^T left them, and V's operand is read in that order.
 // The running maximum moves only when a tile's exceeds it by 2^kLazy, so that
 // rescaling the output is rare; sums and the output are fp32.
+#include <atomic>
+
 #include "dc_chunk.h"
 #include "dc_unpack.h"
 
@@ -110,9 +112,21 @@ __device__ __forceinline__ bool page_holds(const dc_pool& pool, const dc_page_de
          (int64_t(d.block) << 8) + blob_layout(d.format, d.bits, pool.geometry).total <= pool.arena_bytes;
 }
 
-// Narrows an item to this block's `rows` rows (blockIdx.y); false: none left.
-__device__ __forceinline__ bool block_rows(dc_chunk_item& it, int rows, int n_q) {
-  const int skip = rows * int(blockIdx.y);
+// This block's item where each takes `parts` blocks, which run on one die (they
+// read the same pages), and which of them the block is.
+__device__ __forceinline__ dc_chunk_item block_item(const ChunkArgs& a, int parts, int* part) {
+  const uint32_t turn = blockIdx.x / kChunkXcds, i = turn / parts * kChunkXcds + blockIdx.x % kChunkXcds;
+  *part = int(turn % parts);
+  return i < uint32_t(a.n_items) ? a.items[i] : dc_chunk_item{-1};
+}
+
+inline dim3 item_grid(int32_t n_items, int parts) {
+  return dim3(parts == 1 ? uint32_t(n_items) : (uint32_t(n_items) + kChunkXcds - 1) / kChunkXcds * kChunkXcds * parts);
+}
+
+// Narrows an item to its part of `rows` rows; false: none left.
+__device__ __forceinline__ bool block_rows(dc_chunk_item& it, int part, int rows, int n_q) {
+  const int skip = rows * part;
   if (it.row_begin + skip >= it.row_end) return false;
   it.row_begin += skip;
   if (it.partial >= 0) it.partial += skip;
@@ -138,9 +152,9 @@ __global__ void __launch_bounds__(256, sizeof(T) == 4 && HDP == 256 ? 1 : 2) att
   __shared__ uint32_t poison[TB];  // it has a value that is not finite (in a tile that some row does not see whole)
   __shared__ float odd[HDP];       // such a token's values
 
-  dc_chunk_item it = a.items[blockIdx.x];
-  if (!chunk_item_ok(it, a)) return;
-  if (!block_rows(it, 128, a.n_q)) return;
+  int of_item;
+  dc_chunk_item it = block_item(a, kChunkRows / 128, &of_item);
+  if (!chunk_item_ok(it, a) || !block_rows(it, of_item, 128, a.n_q)) return;
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int col = lane & 31, half = lane >> 5;
   const int hd = a.kpool.geometry.head_dim, P = a.kpool.geometry.page_capacity;
@@ -588,11 +602,9 @@ __global__ void __launch_bounds__(512, 2) attend_chunk16_kernel(ChunkArgs a) {
   __shared__ __attribute__((aligned(4))) uint8_t live[2][KT / 8], poison[2][PG][KT / 8];  // one bit per token, as in attend_chunk_kernel
   __shared__ float odd[HDP];
 
-  dc_chunk_item it = a.items[blockIdx.x];
-  if (!chunk_item_ok(it, a)) return;
-  if constexpr (CS > 1) {
-    if (!block_rows(it, 256 / CS, a.n_q)) return;
-  }
+  int of_item;
+  dc_chunk_item it = block_item(a, CS, &of_item);
+  if (!chunk_item_ok(it, a) || !block_rows(it, of_item, 256 / CS, a.n_q)) return;
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int col = lane & 31, half = lane >> 5;
   const int hd = a.kpool.geometry.head_dim, P = a.kpool.geometry.page_capacity;
@@ -1406,15 +1418,17 @@ __global__ void __launch_bounds__(64 * kFewWaves, 2) attend_few_kernel(ChunkArgs
 }
 
 // Joins the partial results of a row tile's token ranges: `lanes` lanes per
-// row, VEC channels a lane and further ones in turn.  Where a range of few rows
-// was cut into many (kMergeMany), the block's lane groups share a row's partial
-// results and join in LDS; otherwise each group has a row of its own.
-constexpr int kMergeBlocks = 32, kMergeMany = 8;
+// row, VEC channels a lane and further ones in turn, kMergeBatch ranges' results
+// in flight at once (their weights follow from running maxima, so that nothing
+// is read twice).  Where a range of few rows was cut into many (kMergeMany), the
+// block's lane groups share a row's partial results and join in LDS; otherwise
+// each group has a row of its own.
+constexpr int kMergeBlocks = 64, kMergeMany = 8, kMergeBatch = 4;
 
 template <int VEC>
 __global__ void __launch_bounds__(256) merge_chunk_kernel(ChunkArgs a, const dc_chunk_merge* merges, int32_t lanes) {
   __shared__ float joined[256 * VEC];
-  __shared__ float sums[256];
+  __shared__ float sums[256], tops[256];
   const dc_chunk_merge mg = merges[blockIdx.x];
   if (!chunk_merge_ok(mg, a)) return;
   const int tid = threadIdx.x, groups = 256 / lanes, group = tid / lanes, lane = tid - group * lanes;
@@ -1427,37 +1441,46 @@ __global__ void __launch_bounds__(256) merge_chunk_kernel(ChunkArgs a, const dc_
     const int64_t first = int64_t(mg.partial_begin) + (has ? r : 0);
     const int tok = row / a.n_q, head = mg.kv_head * a.n_q + (row - tok * a.n_q);
     const int64_t off = int64_t(mg.q_begin + tok) * a.o_token_stride + int64_t(head) * a.o_head_stride;
-    float top = -INFINITY;
-    for (int i = many ? tid : lane; i < mg.count; i += many ? 256 : lanes) top = fmaxf(top, a.part_ml[2 * (first + int64_t(i) * rows)]);
-    for (int o = 1; o < lanes; o <<= 1) top = fmaxf(top, __shfl_xor(top, o, 64));
-    if (many) {
-      __syncthreads();
-      if (lane == 0) sums[group] = top;
-      __syncthreads();
-      for (int g = 0; g < groups; ++g) top = fmaxf(top, sums[g]);
-    }
-    const float mu = top == -INFINITY ? 0.f : top;
     for (int c0 = 0; c0 < hd; c0 += VEC * lanes) {
       const int ch = c0 + VEC * lane;
       const bool in = ch < hd;
-      float sum[VEC], l = 0.f;
+      float sum[VEC], l = 0.f, top = -INFINITY;
 #pragma unroll
       for (int k = 0; k < VEC; ++k) sum[k] = 0.f;
-#pragma unroll 8
-      for (int i = part; i < mg.count; i += split) {
-        const int64_t at = first + int64_t(i) * rows;
-        const float2 ml = *reinterpret_cast<const float2*>(a.part_ml + 2 * at);
-        const float w = __builtin_amdgcn_exp2f(ml.x - mu);
-        l = fmaf(w, ml.y, l);
-        const float* po = a.part_o + at * hd + (in ? ch : 0);
-        if constexpr (VEC == 4) {
-          const float4 x = *reinterpret_cast<const float4*>(po);
-          sum[0] = fmaf(w, x.x, sum[0]);
-          sum[1] = fmaf(w, x.y, sum[1]);
-          sum[2] = fmaf(w, x.z, sum[2]);
-          sum[3] = fmaf(w, x.w, sum[3]);
-        } else {
-          sum[0] = fmaf(w, *po, sum[0]);
+      for (int i0 = part; i0 < mg.count; i0 += split * kMergeBatch) {
+        float2 ml[kMergeBatch];
+        float x[kMergeBatch][VEC];
+#pragma unroll
+        for (int j = 0; j < kMergeBatch; ++j) {
+          const int i = i0 + j * split;
+          const int64_t at = first + int64_t(i < mg.count ? i : i0) * rows;
+          ml[j] = *reinterpret_cast<const float2*>(a.part_ml + 2 * at);
+          const float* po = a.part_o + at * hd + (in ? ch : 0);
+          if constexpr (VEC == 4) {
+            const float4 v = *reinterpret_cast<const float4*>(po);
+            x[j][0] = v.x; x[j][1] = v.y; x[j][2] = v.z; x[j][3] = v.w;
+          } else {
+            x[j][0] = *po;
+          }
+        }
+        float high = top;
+#pragma unroll
+        for (int j = 0; j < kMergeBatch; ++j) high = fmaxf(high, ml[j].x);  // (a repeated result changes no maximum)
+        const float mu = high == -INFINITY ? 0.f : high;
+        if (high > top) {
+          const float f = __builtin_amdgcn_exp2f(top - mu);
+          l = top == -INFINITY ? 0.f : l * f;
+#pragma unroll
+          for (int k = 0; k < VEC; ++k) sum[k] = top == -INFINITY ? sum[k] : sum[k] * f;
+          top = high;
+        }
+#pragma unroll
+        for (int j = 0; j < kMergeBatch; ++j) {
+          if (j > 0 && i0 + j * split >= mg.count) break;
+          const float w = __builtin_amdgcn_exp2f(ml[j].x - mu);
+          l = fmaf(w, ml[j].y, l);
+#pragma unroll
+          for (int k = 0; k < VEC; ++k) sum[k] = fmaf(w, x[j][k], sum[k]);
         }
       }
       if (many) {
@@ -1465,14 +1488,23 @@ __global__ void __launch_bounds__(256) merge_chunk_kernel(ChunkArgs a, const dc_
 #pragma unroll
         for (int k = 0; k < VEC; ++k) joined[VEC * tid + k] = sum[k];
         sums[tid] = l;
+        tops[tid] = top;
         __syncthreads();
-        if (part == 0)
+        if (part == 0) {
+          float high = top;
+          for (int p = 1; p < split; ++p) high = fmaxf(high, tops[tid + p * lanes]);
+          const float mu = high == -INFINITY ? 0.f : high, f = __builtin_amdgcn_exp2f(top - mu);
+          l *= f;
+#pragma unroll
+          for (int k = 0; k < VEC; ++k) sum[k] *= f;
           for (int p = 1; p < split; ++p) {
             const int t = tid + p * lanes;
+            const float w = __builtin_amdgcn_exp2f(tops[t] - mu);
 #pragma unroll
-            for (int k = 0; k < VEC; ++k) sum[k] += joined[VEC * t + k];
-            l += sums[t];
+            for (int k = 0; k < VEC; ++k) sum[k] = fmaf(w, joined[VEC * t + k], sum[k]);
+            l = fmaf(w, sums[t], l);
           }
+        }
       }
       if (!has || !in || part != 0) continue;
       const float inv = l == 0.f ? 0.f : 1.f / l;
@@ -1494,23 +1526,35 @@ static int launch_merge_chunk(const ChunkArgs& a, const dc_chunk_merge* merges, 
   return check_hip(hipGetLastError(), "merge_chunk_kernel launch");
 }
 
+// A kernel's dynamic LDS limit, raised once on every device that launches it.
+struct LdsLimit {
+  std::atomic<uint64_t> raised{0};
+  int raise(const void* kernel, int bytes, const char* what) {
+    int device = 0;
+    if (int rc = check_hip(hipGetDevice(&device), what)) return rc;
+    const uint64_t bit = uint64_t(1) << (device & 63);
+    if (device < 64 && (raised.load(std::memory_order_acquire) & bit)) return DC_OK;
+    if (int rc = check_hip(hipFuncSetAttribute(kernel, hipFuncAttributeMaxDynamicSharedMemorySize, bytes), what)) return rc;
+    raised.fetch_or(device < 64 ? bit : 0, std::memory_order_release);
+    return DC_OK;
+  }
+};
+
 template <typename T, int HDP, int KT>
 static int launch_chunk(const ChunkArgs& a, hipStream_t stream) {
   constexpr int bytes = 2 * KT * HDP * int(sizeof(T)) + 16;
-  static const hipError_t set = hipFuncSetAttribute(reinterpret_cast<const void*>(&attend_chunk_kernel<T, HDP, KT>),
-                                                    hipFuncAttributeMaxDynamicSharedMemorySize, bytes);
-  if (int rc = check_hip(set, "attend_chunk_kernel LDS")) return rc;
-  hipLaunchKernelGGL((attend_chunk_kernel<T, HDP, KT>), dim3(a.n_items, kChunkRows / 128), dim3(256), bytes, stream, a);
+  static LdsLimit limit;
+  if (int rc = limit.raise(reinterpret_cast<const void*>(&attend_chunk_kernel<T, HDP, KT>), bytes, "attend_chunk_kernel LDS")) return rc;
+  hipLaunchKernelGGL((attend_chunk_kernel<T, HDP, KT>), item_grid(a.n_items, kChunkRows / 128), dim3(256), bytes, stream, a);
   return check_hip(hipGetLastError(), "attend_chunk_kernel launch");
 }
 
 template <int HDP, int KT, bool UNI, int CS>
 static int launch_chunk16_as(const ChunkArgs& a, hipStream_t stream) {
   constexpr int bytes = 4 * KT * HDP * 2;
-  static const hipError_t set = hipFuncSetAttribute(reinterpret_cast<const void*>(&attend_chunk16_kernel<HDP, KT, UNI, CS>),
-                                                    hipFuncAttributeMaxDynamicSharedMemorySize, bytes);
-  if (int rc = check_hip(set, "attend_chunk16_kernel LDS")) return rc;
-  hipLaunchKernelGGL((attend_chunk16_kernel<HDP, KT, UNI, CS>), dim3(a.n_items, CS), dim3(512), bytes, stream, a);
+  static LdsLimit limit;
+  if (int rc = limit.raise(reinterpret_cast<const void*>(&attend_chunk16_kernel<HDP, KT, UNI, CS>), bytes, "attend_chunk16_kernel LDS")) return rc;
+  hipLaunchKernelGGL((attend_chunk16_kernel<HDP, KT, UNI, CS>), item_grid(a.n_items, CS), dim3(512), bytes, stream, a);
   return check_hip(hipGetLastError(), "attend_chunk16_kernel launch");
 }
 
@@ -1523,9 +1567,8 @@ static int launch_chunk16(const ChunkArgs& a, hipStream_t stream) {
 template <int HDP, int NB, int KW, bool UNI>
 static int launch_few_as(const ChunkArgs& a, hipStream_t stream) {
   constexpr int tiles = kFewWaves * kFewTile * HDP * 2 + (NB * HDP >= 256 ? 16 * NB * HDP * 2 : 0), joined = 16 * NB * (HDP + 4) * 4, bytes = tiles > joined ? tiles : joined;
-  static const hipError_t set = hipFuncSetAttribute(reinterpret_cast<const void*>(&attend_few_kernel<HDP, NB, KW, UNI>),
-                                                    hipFuncAttributeMaxDynamicSharedMemorySize, bytes);
-  if (int rc = check_hip(set, "attend_few_kernel LDS")) return rc;
+  static LdsLimit limit;
+  if (int rc = limit.raise(reinterpret_cast<const void*>(&attend_few_kernel<HDP, NB, KW, UNI>), bytes, "attend_few_kernel LDS")) return rc;
   hipLaunchKernelGGL((attend_few_kernel<HDP, NB, KW, UNI>), dim3(a.n_items), dim3(64 * kFewWaves), bytes, stream, a);
   return check_hip(hipGetLastError(), "attend_few_kernel launch");
 }
