@@ -29,7 +29,7 @@ from .rotary import token_rows
 MAX_HEAD_DIM = 256
 # A token range that a tile of query rows is split into holds at least this
 # many tokens.
-MIN_SPLIT_TOKENS = 256
+MIN_SPLIT_TOKENS = 128
 
 
 def _torch():

@@ -172,20 +172,31 @@ __global__ void __launch_bounds__(256, sizeof(T) == 4 && HDP == 256 ? 1 : 2) att
   typedef std::conditional_t<F32, float4, h8v> QV;
   QV q[QW];
   {
-    const int64_t off = int64_t(it.q_begin + tok) * a.q_token_stride + int64_t(head) * a.q_head_stride;
+    // (channels past head_dim and rows that do not exist: an element that does, then zero; no branch between the loads)
+    constexpr int W = F32 ? 4 : 8;
+    typedef std::conditional_t<F32, float, uint16_t> QT;  // (16-bit: bits of either type)
+    const int rr = has_row ? row : it.row_begin, rt = rr / a.n_q;
+    const QT* const p = reinterpret_cast<const QT*>(a.q) + int64_t(it.q_begin + rt) * a.q_token_stride +
+                        int64_t(it.kv_head * a.n_q + rr - rt * a.n_q) * a.q_head_stride;
+    QT w[QW][W];
 #pragma unroll
-    for (int i = 0; i < QW; ++i) {
-      constexpr int W = F32 ? 4 : 8;
-      const int c = 2 * W * i + W * half;
+    for (int i = 0; i < QW; ++i)
 #pragma unroll
       for (int k = 0; k < W; ++k) {
-        const float x = has_row && c + k < hd ? load_value(a.q, a.dtype, off + c + k) : 0.f;
-        if constexpr (F32)
-          (&q[i].x)[k] = x;
-        else
-          q[i][k] = _Float16(x);
+        const int ch = 2 * W * i + W * half + k;
+        w[i][k] = p[ch < hd ? ch : 0];
       }
-    }
+    const bool f16 = a.dtype == DC_F16;
+#pragma unroll
+    for (int i = 0; i < QW; ++i)
+#pragma unroll
+      for (int k = 0; k < W; ++k) {
+        const bool in = has_row && 2 * W * i + W * half + k < hd;
+        if constexpr (F32)
+          (&q[i].x)[k] = in ? w[i][k] : 0.f;
+        else
+          q[i][k] = !in ? _Float16(0) : f16 ? __builtin_bit_cast(_Float16, w[i][k]) : _Float16(__uint_as_float(uint32_t(w[i][k]) << 16));
+      }
   }
   const float c = a.scale * kLog2e;
   float m = -INFINITY, l = 0.f;  // maximum (of scaled log2 logits), sum of this half's weights
@@ -277,6 +288,7 @@ __global__ void __launch_bounds__(256, sizeof(T) == 4 && HDP == 256 ? 1 : 2) att
 
     // S^T: block tb's token 8 (v / 4) + 4 half + v % 4 against this lane's row
     f32x16 s[TB];
+    const int k_at = fresh(lds_at<CH>(col, half));
 #pragma unroll
     for (int tb = 0; tb < TB; ++tb) {
 #pragma unroll
@@ -284,11 +296,11 @@ __global__ void __launch_bounds__(256, sizeof(T) == 4 && HDP == 256 ? 1 : 2) att
 #pragma unroll
       for (int i = 0; i < QW; ++i) {
         if constexpr (F32) {
-          const float4 x = *reinterpret_cast<const float4*>(kt + lds_at<CH>(32 * tb + col, 2 * i + half));
+          const float4 x = *reinterpret_cast<const float4*>(kt + (k_at ^ (32 * i)) + 32 * tb * CH * 16);
 #pragma unroll
           for (int k = 0; k < 4; ++k) s[tb] = __builtin_amdgcn_mfma_f32_32x32x2f32((&x.x)[k], (&q[i].x)[k], s[tb], 0, 0, 0);
         } else {
-          const h8v x = *reinterpret_cast<const h8v*>(kt + lds_at<CH>(32 * tb + col, 2 * i + half));
+          const h8v x = *reinterpret_cast<const h8v*>(kt + (k_at ^ (32 * i)) + 32 * tb * CH * 16);
           s[tb] = __builtin_amdgcn_mfma_f32_32x32x16_f16(x, q[i], s[tb], 0, 0, 0);
         }
       }
@@ -311,7 +323,7 @@ __global__ void __launch_bounds__(256, sizeof(T) == 4 && HDP == 256 ? 1 : 2) att
     top = half_max(top) * c;
     if (__any(top > m + kLazy || (m == -INFINITY && top > m))) {
       const float mn = fmaxf(m, top);
-      const float f = mn == -INFINITY ? 1.f : exp2f(m - mn);
+      const float f = m == -INFINITY ? 1.f : exp2f(m - mn);
       m = mn;
       l *= f;
 #pragma unroll
@@ -328,15 +340,18 @@ __global__ void __launch_bounds__(256, sizeof(T) == 4 && HDP == 256 ? 1 : 2) att
         l += s[tb][v];
       }
     // O^T: channel block i's channel 8 (v / 4) + 4 half + v % 4 of this lane's row
+    // (F32: the value of token 32 tb + 8 (v / 4) + 4 half + v % 4, channel 32 i + col)
+    const int v_at = fresh(4 * half * CH * 16 + ((col / 4) ^ half) * 16 + 4 * (col % 4));
 #pragma unroll
     for (int tb = 0; tb < TB; ++tb) {
       if constexpr (F32) {
+        static_assert(!F32 || CH >= 16, "the exchange of chunks that v_at joins in");
 #pragma unroll
         for (int i = 0; i < CB; ++i)
 #pragma unroll
           for (int v = 0; v < 16; ++v) {
-            const int t = 32 * tb + 8 * (v / 4) + 4 * half + v % 4, ch = 32 * i + col;
-            const float x = *reinterpret_cast<const float*>(vt + lds_at<CH>(t, ch / 4) + 4 * (ch % 4));
+            const int exchanged = (8 * i) ^ ((v % 4) << 2 | (2 * (v / 4) & 3)), first = (32 * tb + 8 * (v / 4) + v % 4) * CH * 16;
+            const float x = *reinterpret_cast<const float*>(vt + (v_at ^ (16 * exchanged)) + first);
             o[i] = __builtin_amdgcn_mfma_f32_32x32x2f32(x, s[tb][v], o[i], 0, 0, 0);
           }
       } else {
@@ -808,7 +823,7 @@ __global__ void __launch_bounds__(512, 2) attend_chunk16_kernel(ChunkArgs a) {
       top = half_max(top) * c;
       if (__any(top > m + kLazy || (m == -INFINITY && top > m))) {
         const float mn = fmaxf(m, top);
-        const float f = mn == -INFINITY ? 1.f : __builtin_amdgcn_exp2f(m - mn);
+        const float f = m == -INFINITY ? 1.f : __builtin_amdgcn_exp2f(m - mn);
         m = mn;
         l *= f;
 #pragma unroll
@@ -1290,7 +1305,7 @@ __global__ void __launch_bounds__(64 * kFewWaves, 2) attend_few_kernel(ChunkArgs
       top = quarter_max(top) * c;
       if (__any(top > m[n] + kLazy || (m[n] == -INFINITY && top > m[n]))) {
         const float mn = fmaxf(m[n], top);
-        const float f = mn == -INFINITY ? 1.f : __builtin_amdgcn_exp2f(m[n] - mn);
+        const float f = m[n] == -INFINITY ? 1.f : __builtin_amdgcn_exp2f(m[n] - mn);
         m[n] = mn;
         l[n] *= f;
 #pragma unroll
