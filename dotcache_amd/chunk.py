@@ -138,7 +138,9 @@ def attend_chunk(pool: DevicePagePool, k_table, v_pool: DevicePagePool | None, v
     are fp16 matrix operands (values past +-65504 overflow, as in fp16 pages)
     and all sums fp32; with fp32 queries everything is fp32.  ``workspace``:
     uint8, :func:`workspace_bytes` at least, not shared by calls that may
-    overlap (default: one of its own).  ``validate`` reads the tables back and
+    overlap (default: one of its own).  The kernel follows from the formats that
+    the pools have held: a captured call is captured anew once a pool takes
+    pages of a format that it had not.  ``validate`` reads the tables back and
     checks them against the pools (the kernel itself leaves out, and never
     reads, what a table does not name)."""
     torch = _torch()

@@ -277,6 +277,8 @@ int dc_plan_chunk(const int32_t* new_tokens, const int32_t* context, int32_t n_s
     for (int32_t b = 0; b < n_seqs; ++b) {
       if (new_tokens[b] < 0 || context[b] < new_tokens[b])
         return dc::fail(DC_EINVAL, "dc_plan_chunk: sequence %d has %d new tokens in a context of %d", b, new_tokens[b], context[b]);
+      // (the kernels look a few tiles past a range's end)
+      if (context[b] > INT32_MAX - 65536) return dc::fail(DC_EINVAL, "dc_plan_chunk: sequence %d has too long a context", b);
       if (int64_t(new_tokens[b]) * n_q > INT32_MAX - dc::kChunkRows) return dc::fail(DC_EINVAL, "dc_plan_chunk: sequence %d has too many new tokens", b);
       q_tokens += new_tokens[b];
     }

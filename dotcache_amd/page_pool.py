@@ -708,7 +708,8 @@ class DevicePagePool:
     def read_tokens_with(self, v_pool: "DevicePagePool", tables, row, token, *, dtype=None, out=None):
         """Keys and values of tokens as dense rows ``[T, heads, hd]`` each, the
         values their pages stand for (``dc_read_tokens``), for tokens named as
-        in :meth:`append_rotary_with`; a token without a page gives zeros.
+        in :meth:`append_rotary_with`; a token without a page gives zeros, a slot
+        that was not written what its page holds there.
         ``dtype``: fp32 (default), fp16 or bf16; ``out = (keys, values)``
         takes them instead.  The pages of one prefix handed to another
         engine, or to attention over dense rows, need no host round trip."""

@@ -131,3 +131,28 @@ def test_c_entry_refusals():
         assert go(**bad) == _lib.DC_EINVAL, bad
     assert go(n_items=1, parts=1, ws=4096, size=16) == _lib.DC_ESPACE
     assert go(n_items=1, parts=1, ws=None, size=1 << 20) == _lib.DC_ESPACE
+
+
+def test_long_contexts_are_refused():
+    with pytest.raises(ValueError, match="too long a context"):
+        _plan([1], [2 ** 31 - 65536])
+    assert _plan([1], [2 ** 31 - 65537], target_items=4).n_items > 0
+
+
+@pytest.mark.parametrize("new,ctx,H,n_q", [([2048, 2048], [16384, 16384], 4, 7), ([5, 5, 5, 5], [131000, 60000, 3000, 900], 4, 7),
+                                           ([700, 1, 333, 64, 512], [8192, 5000, 900, 4097, 700], 4, 4)])
+def test_work_is_spread_over_the_card(new, ctx, H, n_q):
+    """Blocks start in order, each on the first free slot of its die: the last is
+    done within a quarter of an even share, or within the longest part."""
+    plan = _plan(new, ctx, H, n_q, target_items=256)
+    for part, slots in ((plan.host_items[: plan.n_few], 512), (plan.host_items[plan.n_few:], 256)):
+        length = np.where(part[:, 0] >= 0, part[:, 7] - part[:, 6], 0)
+        if not length.any():
+            continue
+        done = 0
+        for die in range(8):
+            free = np.zeros(slots // 8, dtype=np.int64)
+            for n in length[die::8]:
+                free[np.argmin(free)] += n
+            done = max(done, int(free.max()))
+        assert done <= max(1.25 * length.sum() / slots, length.max())

@@ -363,3 +363,29 @@ def test_long_offsets():
     batch.read()
     assert all(np.array_equal(a, b) for a, b in zip(batch.rows, want_rows))
     _check(batch, [33], 2, "f16", rng)
+
+
+@pytest.mark.parametrize("dtype", ["f32", "f16"])
+@pytest.mark.parametrize("n", [5, 50])
+@pytest.mark.parametrize("value", ["m3", "m3_f32"])
+def test_an_infinity_where_a_range_begins(value, n, dtype):
+    """A range's first tile has no maximum to rescale from: an infinity there
+    stays one for the rows that see it, with few rows and many."""
+    import torch
+
+    rng = np.random.default_rng(n)
+    hd, ctx = 64, 300
+    print(f"chunk infinity {value} {n} {dtype}", flush=True)
+    batch = _Batch(rng, [ctx], 1, hd, 32, "m3", value, tail=False)
+    bad = torch.from_numpy(rng.normal(size=(1, hd)).astype(np.float32)).cuda()
+    bad[0, 7] = float("inf")
+    u = ctx - n + 2 if n < 44 else 258  # in the last range of 128, seen by some of the rows
+    batch.pools[1].encode_rows(bad, [int(batch.host[1][0, 0, u // 32])], [u % 32])
+    batch.read()
+    q = torch.from_numpy((0.5 * rng.normal(size=(n, 2, hd))).astype(np.float32)).to(_dt(dtype)).cuda()
+    plan = batch.plan([n], 2, dtype=q.dtype, target_items=64)
+    assert plan.n_partials > 0
+    got = batch.attend(q, plan, 0.125).double().cpu().numpy()
+    first = u - (ctx - n)  # the first row that sees it
+    assert np.isposinf(got[first:, :, 7]).all() and np.isfinite(got[:first]).all()
+    assert np.isfinite(np.delete(got, 7, axis=2)).all()

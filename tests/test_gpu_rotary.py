@@ -312,3 +312,39 @@ def test_append_in_a_graph_and_on_another_stream():
     side.synchronize()
     for a, b in zip(got, want):
         assert torch.equal(a, b)
+
+
+@pytest.mark.parametrize("dtype", ["f32", "f16", "bf16"])
+@pytest.mark.parametrize("hd", [128, 96])
+def test_large_calls_are_small_calls_side_by_side(hd, dtype):
+    """Calls whose rows the caches would not hold store past them, and lanes take
+    several heads: the same bits as the same rows in small calls."""
+    import torch
+
+    from dotcache_amd.page_pool import DevicePagePool, PoolGeometry
+    from dotcache_amd.rotary import RotaryTable, norm_rotate
+
+    dt = {"f32": torch.float32, "f16": torch.float16, "bf16": torch.bfloat16}[dtype]
+    T, heads, small = 24001, 7, 900
+    torch.manual_seed(hd)
+    x = torch.randn(T, heads, hd, device="cuda").to(dt)
+    w = torch.rand(hd, device="cuda") + 0.5
+    rotary = RotaryTable(hd, 4096, rotary_dim=hd // 3 // 32 * 32 + 32)
+    pos = torch.randint(0, 4096, (T,), dtype=torch.int32, device="cuda")
+    y, _ = norm_rotate(x, None, pos, rotary, q_weight=w)
+    for a in range(0, T, small):
+        z, _ = norm_rotate(x[a: a + small], None, pos[a: a + small], rotary, q_weight=w)
+        assert torch.equal(z, y[a: a + small])
+    pools = [DevicePagePool(PoolGeometry(hd, 32, 64), reserve_bytes=1 << 20, reserve_pages=64) for _ in range(2)]
+    tables = []
+    for p, form in zip(pools, (_form("a4"), _form("s3"))):
+        ids = p.allocate(*form, 2 * 5 * 3, tokens=64)
+        p.encode_rows(torch.randn(30 * 64, hd, device="cuda"), np.repeat(ids, 64), np.tile(np.arange(64), 30))
+        tables.append(torch.from_numpy(np.asarray(ids, dtype=np.int32).reshape(2, 5, 3)).cuda())
+    tables = torch.stack(tables).contiguous()
+    row = torch.randint(-1, 3, (T,), dtype=torch.int32, device="cuda")  # (some tokens without a page)
+    token = torch.randint(0, 3 * 64, (T,), dtype=torch.int32, device="cuda")
+    k, v = pools[0].read_tokens_with(pools[1], tables, row, token, dtype=dt)
+    for a in range(0, T, small):
+        kk, vv = pools[0].read_tokens_with(pools[1], tables, row[a: a + small], token[a: a + small], dtype=dt)
+        assert torch.equal(kk, k[a: a + small]) and torch.equal(vv, v[a: a + small])
