@@ -65,9 +65,6 @@ class RotaryTable:
         self.table = torch.cat([angle.cos() * float(amplitude), angle.sin() * float(amplitude)], dim=-1).float()
         self._c = _lib.Rotary(self.table.data_ptr(), self.n_positions, rd, int(self.interleaved))
 
-    def c(self) -> _lib.Rotary:
-        return self._c
-
 
 def token_rows(x, name: str, head_dim: int, device) -> _lib.TokenRows:
     """``dc_token_rows`` of a tensor ``[tokens, heads, head_dim]``."""

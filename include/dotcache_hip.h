@@ -578,9 +578,10 @@ typedef struct dc_chunk_merge {
  * none for a sequence that waits) of a context of context[b] tokens with them,
  * packed one sequence after another in the queries.  Sequences of few rows
  * (new_tokens * n_q) come first, *n_few items of at most *few_rows rows, the
- * others in row tiles of 256.  Each is cut into token ranges until about
- * target_items items of near-equal length exist (at least min_tokens tokens
- * each), ordered so that items of one stream run on one die, the longest
+ * others in row tiles of 256.  Their token ranges are cut (to at least min_tokens
+ * tokens) for a card that runs target_items blocks at once (twice as many of few
+ * rows): evenly, or where a block's even share of the work ends, whichever is
+ * done first by a greedy model.  Items of one stream run on one die, the longest
  * first.  DC_ESPACE if the output arrays are too small (counts are still
  * written).  No reference counterpart: the reference decodes one token
  * (dotcache/integrations/llama.py:424-425). */
@@ -610,8 +611,8 @@ int64_t dc_chunk_workspace_bytes(int32_t n_partials, int32_t head_dim);
  * dotcache/attention_runtime.py:179-315. */
 int dc_attend_chunk(dc_pool k_pool, dc_pool v_pool, const int32_t* k_table, const int32_t* v_table, int32_t table_stride,
                     const dc_chunk_item* items, int32_t n_items, int32_t n_few, int32_t few_rows,
-                    const dc_chunk_merge* merges, int32_t n_merges, int32_t n_partials, int32_t n_seqs, int32_t n_kv_heads, int64_t n_tokens, dc_token_rows q,
-                    float query_scale, dc_token_rows out, void* workspace, int64_t workspace_bytes, dc_stream_t stream);
+                    const dc_chunk_merge* merges, int32_t n_merges, int32_t n_partials, int32_t n_seqs,
+                    int32_t n_kv_heads, int64_t n_tokens, dc_token_rows q, float query_scale, dc_token_rows out, void* workspace, int64_t workspace_bytes, dc_stream_t stream);
 
 /* Process-wide decode kernel choice: 0 (default) runs the MFMA kernel when
  * every page format (M3 fp16 keys and values, M0 4- or 8-bit keys of group

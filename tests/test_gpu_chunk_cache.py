@@ -66,7 +66,7 @@ def _dt(name):
 
 @pytest.mark.parametrize("batch,hd,P,dtype,mode,gain", [
     (1, 64, 16, "bf16", "M0", True), (2, 128, 32, "f16", "M0", True), (3, 96, 16, "f32", "M0", False),
-    (2, 64, 16, "bf16", "M3", True)])
+    (2, 64, 16, "bf16", "M3", True), (1, 64, 16, "f32", "strict", True)])
 def test_a_layer_of_the_paged_cache(batch, hd, P, dtype, mode, gain):
     import torch
 
@@ -76,7 +76,8 @@ def test_a_layer_of_the_paged_cache(batch, hd, P, dtype, mode, gain):
     H, Hq, eps, scale = 2, 6, 1e-6, 1.0 / np.sqrt(hd)
     print(f"paged layer batch {batch} hd {hd} {dtype} {mode}", flush=True)
     rng = np.random.default_rng(hd + batch)
-    cfg = DotCacheConfig(head_dim=hd, group_size=32, tokens_per_page=P, bits_k=4, bits_v=4, default_mode_k=mode, default_mode_v="M0")
+    how = dict(key_policy_tier="strict") if mode == "strict" else dict(default_mode_k=mode)  # (strict: by the page's age and rows)
+    cfg = DotCacheConfig(head_dim=hd, group_size=32, tokens_per_page=P, bits_k=4, bits_v=4, default_mode_v="M0", **how)
     cache = DevicePagedKVCache(cfg, num_hidden_layers=2, num_attention_heads=Hq, num_key_value_heads=H, batch_size=batch)
     plain = DevicePagedKVCache(cfg, num_hidden_layers=2, num_attention_heads=Hq, num_key_value_heads=H, batch_size=batch)
     rotary = RotaryTable(hd, 256)

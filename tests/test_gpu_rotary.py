@@ -50,7 +50,8 @@ def _close(got, want, size, dtype, hd):
 # pairs that start inside a lane's 8 channels; head_dims that are no multiple of 8;
 # rows longer than a wavefront's lanes
 _SHAPES = [(128, 128, False), (64, 64, True), (256, 64, False), (96, 48, False), (96, 40, True), (80, 20, False),
-           (40, 36, True), (30, 30, False), (7, 2, True), (576, 64, False), (128, 0, False)]
+           (40, 36, True), (30, 30, False), (7, 2, True), (576, 64, False), (128, 0, False),
+           (72, 32, False), (88, 24, True), (24, 8, True), (512, 512, False)]  # (lanes with one chunk of eight; 32 lanes a row)
 
 
 @pytest.mark.parametrize("hd,rd,interleaved", _SHAPES)
