@@ -619,7 +619,9 @@ __device__ __forceinline__ uint32_t fold_tokens(uint64_t b) {
 // descriptor and addresses are then the wavefront's.
 // CS: wavefronts that share 32 rows, each with a part of the output's channels
 // (head_dim 256, whose queries and output of 32 rows fill the registers).
-template <int HDP, int KT, bool UNI, int CS>
+// WHOLE: head_dim is HDP, so that no channel is left out and no mask kept for it
+// (12 sequences at head_dim 256 608 -> 597 us, five rows of four long sequences 98 -> 95).
+template <int HDP, int KT, bool UNI, int CS, bool WHOLE>
 __global__ void __launch_bounds__(512, 2) attend_chunk16_kernel(ChunkArgs a) {
   constexpr int CH = HDP / 8, TB = KT / 32, CB = HDP / 32 / CS, TILE = KT * HDP * 2, QW = HDP / 16;
   constexpr int NT = KT < 64 ? 8 : KT / 8;  // tokens a wavefront turns
@@ -634,7 +636,7 @@ __global__ void __launch_bounds__(512, 2) attend_chunk16_kernel(ChunkArgs a) {
   if (!chunk_item_ok(it, a) || !block_rows(it, of_item, 256 / CS, a.n_q)) return;
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int col = lane & 31, half = lane >> 5;
-  const int hd = a.kpool.geometry.head_dim, P = a.kpool.geometry.page_capacity;
+  const int hd = WHOLE ? HDP : a.kpool.geometry.head_dim, P = a.kpool.geometry.page_capacity;
 
   const int rows_at = 32 * (wave % (8 / CS)), cb0 = CS > 1 ? CB * (wave / (8 / CS)) : 0;  // (cb0: first channel block)
   const int row = it.row_begin + rows_at + col;
@@ -987,7 +989,7 @@ __device__ __forceinline__ uint32_t zero_of(int kind, bool affine) {
 // values' operand is read.
 // KW: words of a key operand that are read ahead (4: also fp16 rows; 2: codes
 // only, and fp16 rows when they are needed).  UNI: a tile's tokens lie in one page.
-template <int HDP, int NB, int KW, bool UNI>
+template <int HDP, int NB, int KW, bool UNI, bool WHOLE>
 __global__ void __launch_bounds__(64 * kFewWaves, 2) attend_few_kernel(ChunkArgs a) {
   constexpr int CH = HDP / 8, KS = HDP / 32, CB = HDP / 16, TILE = kFewTile * HDP * 2;
   constexpr int VC = HDP / 2, VU = VC / 32;  // a lane's value channels, in units of 32
@@ -1002,7 +1004,7 @@ __global__ void __launch_bounds__(64 * kFewWaves, 2) attend_few_kernel(ChunkArgs
   if (!chunk_item_ok(it, a) || it.row_end - it.row_begin > 16 * NB) return;
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int col = lane & 15, g = lane >> 4;
-  const int hd = a.kpool.geometry.head_dim, P = a.kpool.geometry.page_capacity;
+  const int hd = WHOLE ? HDP : a.kpool.geometry.head_dim, P = a.kpool.geometry.page_capacity;
   const int rows = it.row_end - it.row_begin;
 
   int sees[NB];
@@ -1576,34 +1578,36 @@ static int launch_chunk(const ChunkArgs& a, hipStream_t stream) {
   return check_hip(hipGetLastError(), "attend_chunk_kernel launch");
 }
 
-template <int HDP, int KT, bool UNI, int CS>
+template <int HDP, int KT, bool UNI, int CS, bool WHOLE>
 static int launch_chunk16_as(const ChunkArgs& a, hipStream_t stream) {
   constexpr int bytes = 4 * KT * HDP * 2;
   static LdsLimit limit;
-  if (int rc = limit.raise(reinterpret_cast<const void*>(&attend_chunk16_kernel<HDP, KT, UNI, CS>), bytes, "attend_chunk16_kernel LDS")) return rc;
-  hipLaunchKernelGGL((attend_chunk16_kernel<HDP, KT, UNI, CS>), item_grid(a.n_items, CS), dim3(512), bytes, stream, a);
+  if (int rc = limit.raise(reinterpret_cast<const void*>(&attend_chunk16_kernel<HDP, KT, UNI, CS, WHOLE>), bytes, "attend_chunk16_kernel LDS")) return rc;
+  hipLaunchKernelGGL((attend_chunk16_kernel<HDP, KT, UNI, CS, WHOLE>), item_grid(a.n_items, CS), dim3(512), bytes, stream, a);
   return check_hip(hipGetLastError(), "attend_chunk16_kernel launch");
 }
 
 template <int HDP, int KT, int CS>
 static int launch_chunk16(const ChunkArgs& a, hipStream_t stream) {
-  return a.kpool.geometry.page_capacity % (KT < 64 ? 8 : KT / 8) == 0 ? launch_chunk16_as<HDP, KT, true, CS>(a, stream)
-                                                        : launch_chunk16_as<HDP, KT, false, CS>(a, stream);
+  if (a.kpool.geometry.page_capacity % (KT < 64 ? 8 : KT / 8) != 0) return launch_chunk16_as<HDP, KT, false, CS, false>(a, stream);
+  return a.kpool.geometry.head_dim == HDP ? launch_chunk16_as<HDP, KT, true, CS, true>(a, stream)
+                                          : launch_chunk16_as<HDP, KT, true, CS, false>(a, stream);
 }
 
-template <int HDP, int NB, int KW, bool UNI>
+template <int HDP, int NB, int KW, bool UNI, bool WHOLE>
 static int launch_few_as(const ChunkArgs& a, hipStream_t stream) {
   constexpr int tiles = kFewWaves * kFewTile * HDP * 2 + (NB * HDP >= 256 ? 16 * NB * HDP * 2 : 0), joined = 16 * NB * (HDP + 4) * 4, bytes = tiles > joined ? tiles : joined;
   static LdsLimit limit;
-  if (int rc = limit.raise(reinterpret_cast<const void*>(&attend_few_kernel<HDP, NB, KW, UNI>), bytes, "attend_few_kernel LDS")) return rc;
-  hipLaunchKernelGGL((attend_few_kernel<HDP, NB, KW, UNI>), dim3(a.n_items), dim3(64 * kFewWaves), bytes, stream, a);
+  if (int rc = limit.raise(reinterpret_cast<const void*>(&attend_few_kernel<HDP, NB, KW, UNI, WHOLE>), bytes, "attend_few_kernel LDS")) return rc;
+  hipLaunchKernelGGL((attend_few_kernel<HDP, NB, KW, UNI, WHOLE>), dim3(a.n_items), dim3(64 * kFewWaves), bytes, stream, a);
   return check_hip(hipGetLastError(), "attend_few_kernel launch");
 }
 
 template <int HDP, int NB, int KW>
 static int launch_few(const ChunkArgs& a, hipStream_t stream) {
-  return a.kpool.geometry.page_capacity % kFewTile == 0 ? launch_few_as<HDP, NB, KW, true>(a, stream)
-                                                        : launch_few_as<HDP, NB, KW, false>(a, stream);
+  if (a.kpool.geometry.page_capacity % kFewTile != 0) return launch_few_as<HDP, NB, KW, false, false>(a, stream);
+  return a.kpool.geometry.head_dim == HDP ? launch_few_as<HDP, NB, KW, true, true>(a, stream)
+                                          : launch_few_as<HDP, NB, KW, true, false>(a, stream);
 }
 
 // Whether a thread's 32 channels share a scale and lie at 16-byte multiples,
