@@ -136,7 +136,8 @@ def attend_chunk(pool: DevicePagePool, k_table, v_pool: DevicePagePool | None, v
 
     With 16-bit queries, the queries, the pages' values and the softmax weights
     are fp16 matrix operands (values past +-65504 overflow, as in fp16 pages)
-    and all sums fp32; with fp32 queries everything is fp32.  ``workspace``:
+    and all sums fp32; with fp32 queries everything is fp32.  ``query_scale`` may
+    have either sign, or be 0.  ``workspace``:
     uint8, :func:`workspace_bytes` at least, not shared by calls that may
     overlap (default: one of its own).  The kernel follows from the formats that
     the pools have held: a captured call is captured anew once a pool takes

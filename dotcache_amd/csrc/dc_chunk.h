@@ -25,7 +25,8 @@ struct ChunkArgs {
   const void* q;
   int64_t q_token_stride, q_head_stride;
   int32_t dtype;
-  float scale;
+  float scale;  // positive ...
+  float sign;   // ... and what the queries are multiplied by: 1, -1, or 0 (scale 1)
   void* out;
   int64_t o_token_stride, o_head_stride;
   float* part_o;   // [n_partials][head_dim]

@@ -16,7 +16,10 @@
 //                 instruction's k index runs over the tokens in the order in
 //                 which S^T left them, and V's operand is read in that order.
 // The running maximum moves only when a tile's exceeds it by 2^kLazy, so that
-// rescaling the output is rare; sums and the output are fp32.
+// rescaling the output is rare; sums and the output are fp32.  The maximum is
+// taken of unscaled logits, and a masked one is an infinity before it is
+// scaled, which needs a positive scale: the queries carry the scale's sign
+// (exactly; with a scale of 0 they are zeros, and the scale 1).
 //
 // Three kernels, by what the pools hold and by rows: attend_chunk16_kernel
 // (16-bit queries, pages of 32-channel units: 2 x 2048 rows of 7 heads a KV head
@@ -204,9 +207,11 @@ __global__ void __launch_bounds__(256, sizeof(T) == 4 && HDP == 256 ? 1 : 2) att
       for (int k = 0; k < W; ++k) {
         const bool in = has_row && 2 * W * i + W * half + k < hd;
         if constexpr (F32)
-          (&q[i].x)[k] = in ? w[i][k] : 0.f;
+          (&q[i].x)[k] = in ? w[i][k] * a.sign : 0.f;
         else
-          q[i][k] = !in ? _Float16(0) : f16 ? __builtin_bit_cast(_Float16, w[i][k]) : _Float16(__uint_as_float(uint32_t(w[i][k]) << 16));
+          q[i][k] = !in   ? _Float16(0)
+                    : f16 ? __builtin_bit_cast(_Float16, w[i][k]) * _Float16(a.sign)
+                          : _Float16(__uint_as_float(uint32_t(w[i][k]) << 16) * a.sign);
       }
   }
   const float c = a.scale * kLog2e;
@@ -581,19 +586,19 @@ __device__ __forceinline__ void load_rows(const ChunkArgs& a, const uint16_t* p,
     for (int i = 0; i < 4; ++i) w[k][i] = has_row && c0 + step * k < hd ? w[k][i] : 0;
 }
 
-// Them as fp16 matrix operands, in LDS order.
+// Them, times `sign`, as fp16 matrix operands, in LDS order.
 template <int N>
-__device__ __forceinline__ void to_operands(bool f16, const uint32_t (&w)[N][4], h8v (&q)[N]) {
+__device__ __forceinline__ void to_operands(bool f16, float sign, const uint32_t (&w)[N][4], h8v (&q)[N]) {
   if (f16) {
 #pragma unroll
     for (int k = 0; k < N; ++k)
 #pragma unroll
-      for (int i = 0; i < 8; ++i) q[k][i] = __builtin_bit_cast(_Float16, uint16_t(w[k][kPerm[i] / 2] >> (16 * (kPerm[i] % 2))));
+      for (int i = 0; i < 8; ++i) q[k][i] = __builtin_bit_cast(_Float16, uint16_t(w[k][kPerm[i] / 2] >> (16 * (kPerm[i] % 2)))) * _Float16(sign);
   } else {
 #pragma unroll
     for (int k = 0; k < N; ++k)
 #pragma unroll
-      for (int i = 0; i < 8; ++i) q[k][i] = _Float16(__builtin_bit_cast(float, kPerm[i] % 2 ? w[k][kPerm[i] / 2] & 0xffff0000u : w[k][kPerm[i] / 2] << 16));
+      for (int i = 0; i < 8; ++i) q[k][i] = _Float16(__builtin_bit_cast(float, kPerm[i] % 2 ? w[k][kPerm[i] / 2] & 0xffff0000u : w[k][kPerm[i] / 2] << 16) * sign);
   }
 }
 
@@ -751,7 +756,7 @@ __global__ void __launch_bounds__(512, 2) attend_chunk16_kernel(ChunkArgs a) {
                         int64_t(it.kv_head * a.n_q + rr - rt * a.n_q) * a.q_head_stride;
     uint32_t w[QW][4];
     load_rows<QW>(a, p, 8 * half, 16, has_row, hd, w);
-    to_operands<QW>(a.dtype == DC_F16, w, q);
+    to_operands<QW>(a.dtype == DC_F16, a.sign, w, q);
   }
   const float c = a.scale * kLog2e;
   float m = -INFINITY, l = 0.f;
@@ -1021,7 +1026,7 @@ __global__ void __launch_bounds__(64 * kFewWaves, 2) attend_few_kernel(ChunkArgs
     uint32_t w[KS][4];
     h8v x[KS];
     load_rows<KS>(a, p, 8 * g, 32, has_row, hd, w);
-    to_operands<KS>(a.dtype == DC_F16, w, x);
+    to_operands<KS>(a.dtype == DC_F16, a.sign, w, x);
 #pragma unroll
     for (int k = 0; k < KS; ++k) {
       if constexpr (!QL)
@@ -1648,7 +1653,8 @@ extern "C" int dc_attend_chunk(dc_pool k_pool, dc_pool v_pool, const int32_t* k_
   if (workspace_bytes < dc_chunk_workspace_bytes(n_partials, hd) || (n_partials && !workspace))
     return dc::fail(DC_ESPACE, "%s: workspace too small", who);
   dc::ChunkArgs a{k_pool, v_pool, k_table, v_table, table_stride, items, n_items, n_seqs, n_kv_heads, q.n_heads / n_kv_heads,
-                  n_tokens, n_partials, q.data, q.token_stride, q.head_stride, q.dtype, query_scale, out.data, out.token_stride,
+                  n_tokens, n_partials, q.data, q.token_stride, q.head_stride, q.dtype,
+                  query_scale == 0.f ? 1.f : fabsf(query_scale), query_scale > 0.f ? 1.f : query_scale < 0.f ? -1.f : 0.f, out.data, out.token_stride,
                   out.head_stride, static_cast<float*>(workspace), static_cast<float*>(workspace) + int64_t(n_partials) * hd};
   const hipStream_t st = hipStream_t(stream);
   a.q_vec = reinterpret_cast<uintptr_t>(q.data) % 16 == 0 && q.token_stride % 8 == 0 && q.head_stride % 8 == 0;

@@ -605,8 +605,9 @@ int64_t dc_chunk_workspace_bytes(int32_t n_partials, int32_t head_dim);
  * With 16-bit queries the matrix operands are fp16: queries, the pages' values
  * and the softmax weights are each rounded to it once (values beyond +-65504
  * overflow, as in fp16 pages), products and sums are fp32.  With DC_F32
- * everything is fp32.  A token whose page the table does not name or that its
- * page does not hold is left out; a row that sees no token gives zeros.
+ * everything is fp32.  query_scale may have either sign, or be 0.  A token whose
+ * page the table does not name or that its page does not hold is left out; a row
+ * that sees no token gives zeros.
  * head_dim <= 256.  Replaces, token by token, reference
  * dotcache/attention_runtime.py:179-315. */
 int dc_attend_chunk(dc_pool k_pool, dc_pool v_pool, const int32_t* k_table, const int32_t* v_table, int32_t table_stride,
