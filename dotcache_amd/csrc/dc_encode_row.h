@@ -315,7 +315,9 @@ __device__ __forceinline__ void encode_row(const dc_pool& pool, const float (&x)
   // 8 bits li of its group's words and may share words with the next lane;
   // OR them into the wavefront's LDS words, then store whole words
   const bool narrow = m0 && bits < 4;
-  const int wpr = G * L.words;  // words of one row (the same for every narrow row of this job)
+  // (a wavefront's rows may lie in pages of either width: each has room for 3-bit
+  // codes, which fits_rows8 checks)
+  const int wpr = G * words_per_group(gs, 3);
   for (int i = lane; i < kPackWords; i += 64) pack[wave][i] = 0u;
   __syncthreads();
   if (narrow) {
