@@ -33,7 +33,7 @@ from .decode import decode_paged, plan_decode, workspace_bytes
 from .encode import resolve_encode_spec
 from .kv_cache import default_q_head_to_kv_head
 from .page_pool import DevicePagePool, PoolGeometry, page_format_of
-from .rotary import head_norm, index_tensor
+from .rotary import cached_positions, head_norm
 from .types import EncodedPage
 
 
@@ -243,8 +243,9 @@ class DeviceVllmPagedKVCache:
         """:meth:`write_slots` of projections as they are: ``query_rows
         [n, Hq, hd]`` (or None) and ``key_rows [n, H, hd]`` are normed
         (``q_weight`` / ``k_weight``, None: not) and rotated to ``positions
-        [n]`` by ``rotary`` (a :class:`~dotcache_amd.rotary.RotaryTable`, or
-        None), keys and values are written, and the queries are returned in
+        [n]`` (on the device they are read back, to be checked) by ``rotary``
+        (a :class:`~dotcache_amd.rotary.RotaryTable`, or None), keys and values
+        are written, and the queries are returned in
         their shape and type (fp32 if the three types differ), all in the one
         launch that writes the slots."""
         torch = _torch()
@@ -263,7 +264,7 @@ class DeviceVllmPagedKVCache:
         if rotary is not None:
             if rotary.head_dim != hd or rotary.table.device != k.device:
                 raise ValueError("the rotary table is for another head_dim or device")
-            pos = index_tensor(positions, "positions", n, k.device, rotary.n_positions)
+            pos = cached_positions(positions, n, k.device, rotary)
         head_norm(q_weight, "queries' weight", Hq, hd, float(eps), k.device)
         head_norm(k_weight, "keys' weight", H, hd, float(eps), k.device)
         out = None if q is None else torch.empty(q.shape, dtype=q.dtype, device=q.device)

@@ -45,7 +45,7 @@ from .config import DotCacheConfig, observe_page
 from .decode import decode_paged, plan_decode, workspace_bytes
 from .encode import make_header, resolve_encode_spec
 from .page_pool import DevicePagePool, PoolGeometry, page_format_of
-from .rotary import head_norm, index_tensor
+from .rotary import cached_positions, head_norm
 
 
 def _torch():
@@ -347,7 +347,8 @@ class DevicePagedKVCache:
         """:meth:`append_step` of projections as they are: ``query_step
         [B, Hq, n, hd]`` (or None) and ``key_step [B, H, n, hd]`` are normed
         (``q_weight`` / ``k_weight``, None: not) and rotated to ``positions``
-        (``[n]`` or ``[B, n]``; default ``token_index ..``) by ``rotary`` (a
+        (``[n]`` or ``[B, n]``; default ``token_index ..``; on the device
+        they are read back, to be checked) by ``rotary`` (a
         :class:`~dotcache_amd.rotary.RotaryTable`, or None), keys and
         ``value_step`` are appended, and the queries are returned in their
         shape and type (fp32 if the three types differ).  One launch per
@@ -375,7 +376,7 @@ class DevicePagedKVCache:
             if tuple(pos.shape) not in ((n,), (B, n)):
                 raise ValueError(f"positions must have shape [{n}] or [{B}, {n}]")
             flat = pos.expand(B, n).reshape(-1) if isinstance(pos, torch.Tensor) else np.broadcast_to(pos, (B, n)).reshape(-1)
-            pos = index_tensor(flat, "positions", B * n, k.device, rotary.n_positions).view(B, n)
+            pos = cached_positions(flat, B * n, k.device, rotary).view(B, n)
         head_norm(q_weight, "queries' weight", self.num_attention_heads, hd, float(eps), k.device)
         head_norm(k_weight, "keys' weight", H, hd, float(eps), k.device)
         out = None if q is None else torch.empty((B, n, self.num_attention_heads, hd), dtype=q.dtype, device=q.device)

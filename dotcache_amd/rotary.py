@@ -121,6 +121,19 @@ def index_tensor(x, name: str, tokens: int, device, limit: int | None = None):
     return x if x.is_contiguous() else x.contiguous()
 
 
+def cached_positions(x, tokens: int, device, rotary: RotaryTable):
+    """:func:`index_tensor` of positions of tokens that a cache counts as its
+    own.  Device values are read back and checked like host values: the launch
+    would leave a token outside the table out of its pages, which then show
+    what they held before."""
+    at = index_tensor(x, "positions", tokens, device, rotary.n_positions)
+    if tokens and _torch().is_tensor(x) and x.device.type != "cpu":
+        host = at.cpu().numpy()
+        if host.min() < 0 or host.max() >= rotary.n_positions:
+            raise ValueError(f"positions must lie in [0, {rotary.n_positions})")
+    return at
+
+
 def norm_rotate(queries, keys, positions, rotary: RotaryTable | None, *, q_weight=None, k_weight=None,
                 eps: float = 1e-6, out=None):
     """``queries [T, Hq, hd]`` and ``keys [T, H, hd]`` (either may be None)
