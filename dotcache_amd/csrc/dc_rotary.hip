@@ -306,13 +306,17 @@ __device__ __forceinline__ void rotated8(const RotaryArgs& R, const RotaryJob& J
   for (int i = 0; i < 8; ++i) z[i] = !has ? 0.f : known ? float(y[i]) : __builtin_nanf("");
 }
 
+// Whether token t has a row of cosines and sines (or needs none).
+__device__ __forceinline__ bool has_position(const RotaryArgs& R, int64_t t) {
+  return R.rotary.rotary_dim == 0 || uint32_t(R.positions[t]) < uint32_t(R.rotary.n_positions);
+}
+
 // Page id and slot of token t, head h; -1 where it is not written.
 __device__ __forceinline__ void token_dest(const RotaryArgs& R, const RotaryJob& J, int64_t t, int32_t h, int32_t* page,
                                            int32_t* slot) {
   const int32_t row = R.row[t], tok = R.token[t];
   const uint32_t p = uint32_t(tok) / uint32_t(R.page_tokens);
-  bool ok = uint32_t(row) < uint32_t(R.dest_rows) && tok >= 0 && p < uint32_t(R.dest_pages);
-  if (R.rotary.rotary_dim) ok = ok && uint32_t(R.positions[t]) < uint32_t(R.rotary.n_positions);
+  const bool ok = uint32_t(row) < uint32_t(R.dest_rows) && tok >= 0 && p < uint32_t(R.dest_pages) && has_position(R, t);
   *slot = tok - int32_t(p * R.page_tokens);
   *page = -1;
   if (ok) *page = J.pages[(int64_t(row) * J.in.n_heads + h) * R.dest_pages + p];
@@ -323,7 +327,7 @@ __device__ __forceinline__ int32_t keep_at(const RotaryArgs& R, const RotaryJob&
   if (J.keep == nullptr) return -1;
   const int32_t k = R.keep_row[t];
   const int64_t at = k + int64_t(h) * R.keep_head_stride;
-  return k >= 0 && at < R.keep_rows ? int32_t(at) : -1;
+  return k >= 0 && at < R.keep_rows && has_position(R, t) ? int32_t(at) : -1;
 }
 
 // Blocks [0, b1) take rows of j0, [b1, b2) rows of j1 and the rest rows of j2.

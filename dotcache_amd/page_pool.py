@@ -656,13 +656,15 @@ class DevicePagePool:
         int32 or int64 per token): a row is a sequence of a page table, or a
         block of a block cache.  No two tokens of a call may share a slot.  A
         token < 0 (padding), an index outside the table or a page id that the
-        pool does not hold is not written; its query row is still made.
+        pool does not hold is not written, nor is one whose device position
+        lies outside the rotation's table; its query row is still made.
         ``positions``, ``rotary``, ``q_weight``, ``k_weight`` and ``eps`` as in
         :func:`~dotcache_amd.rotary.norm_rotate`.
 
         ``keep = (k_rows, v_rows, row, head_stride)`` also stores the fp32 rows
-        at row ``row[t] + h * head_stride`` (``row[t]`` < 0: not; no row
-        twice) of two fp32 buffers ``[m, hd]``.  Pages' token counts are not changed.  ``out``
+        at row ``row[t] + h * head_stride`` (``row[t]`` < 0, or a device
+        position outside the table: not; no row twice) of two fp32 buffers
+        ``[m, hd]``.  Pages' token counts are not changed.  ``out``
         takes the queries (their dtype or fp32; may be ``queries`` itself)."""
         from .rotary import _ABSENT, _NO_ROTARY, head_norm, index_tensor, token_rows
 

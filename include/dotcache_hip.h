@@ -282,7 +282,8 @@ int dc_norm_rotate(int64_t n_tokens, int32_t head_dim, const int32_t* positions,
  * order of a norm's sum.  A token without a page, or whose position is outside
  * the table, is not written.  k_keep / v_keep (NULL: none): the fp32 rows are
  * also stored at row keep_row[t] + h * keep_head_stride of buffers of
- * keep_rows rows (keep_row[t] < 0: not).  Does not change desc.tokens.
+ * keep_rows rows (keep_row[t] < 0, or a position outside the table: not).  Does
+ * not change desc.tokens.
  * Replaces the rotation ahead of reference dotcache/model_kv_cache.py:3830-3902
  * (append_step) and that append. */
 int dc_append_rotary(int64_t n_tokens, const int32_t* positions, dc_rotary rotary, dc_token_rows q, dc_norm q_norm,
