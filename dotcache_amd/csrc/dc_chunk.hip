@@ -29,8 +29,11 @@
 // heads of four sequences to 131072 tokens, 126 MB, 99 us, where the copy
 // rate would take 27; when it was made 170 us, the 256-row kernel 320) and
 // attend_chunk_kernel (the rest: 3 x 61 rows of 1001 tokens in fp32 82 us).
-// 16-bit queries' operands are fp16, each rounded once (2^-11 relative): the
-// matrix unit takes them at eight times the fp32 rate.
+// 16-bit queries' operands are fp16, which the matrix unit takes at eight times
+// the fp32 rate: a query, a page's value and a weight are each rounded to it
+// once, by 2^-11 relative, or below 2^-14 (a weight: below 2^-21 of the row's
+// largest) by 2^-25 (2^-32 of the largest).  All of a row's ranges lift their
+// weights alike (kLift), so that joins and the final division cancel it.
 #include <atomic>
 
 #include "dc_chunk.h"
@@ -46,7 +49,11 @@ typedef short s4v __attribute__((ext_vector_type(4)));
 typedef __bf16 b2v __attribute__((ext_vector_type(2)));
 typedef float f32x16 __attribute__((ext_vector_type(16)));
 
-constexpr float kLazy = 8.f;  // log2 of how far a weight may pass 1 before the maximum moves
+constexpr float kLazy = 8.f;  // log2 of how far a weight may pass the maximum's before the maximum moves
+// log2 of the weight that a row's maximum has as an fp16 operand.  The steps of
+// small weights, 2^-24 of 2^7, are then 2^-31 of the maximum's; the largest
+// weight, 2^(kLift + kLazy), is half of what fp16 holds.
+constexpr float kLift = 7.f;
 
 // Byte offset of 16-byte chunk ch of token t's row in an LDS tile whose rows
 // have CH chunks.  Chunks are exchanged within a row so that reads of one
@@ -348,7 +355,7 @@ __global__ void __launch_bounds__(256, sizeof(T) == 4 && HDP == 256 ? 1 : 2) att
 #pragma unroll
         for (int v = 0; v < 16; ++v) o[i][v] *= f;
     }
-    const float mu = m == -INFINITY ? 0.f : m;
+    const float mu = (m == -INFINITY ? 0.f : m) - (F32 ? 0.f : kLift);
 #pragma unroll
     for (int tb = 0; tb < TB; ++tb)
 #pragma unroll
@@ -850,7 +857,7 @@ __global__ void __launch_bounds__(512, 2) attend_chunk16_kernel(ChunkArgs a) {
 #pragma unroll
           for (int v = 0; v < 16; ++v) o[j][v] *= f;
       }
-      const float mu = m == -INFINITY ? 0.f : m;
+      const float mu = (m == -INFINITY ? 0.f : m) - kLift;
 #pragma unroll
       for (int tb = 0; tb < TB; ++tb)
 #pragma unroll
@@ -1330,7 +1337,7 @@ __global__ void __launch_bounds__(64 * kFewWaves, 2) attend_few_kernel(ChunkArgs
 #pragma unroll
         for (int j = 0; j < CB; ++j) o[n][j] *= f;
       }
-      const float mu = m[n] == -INFINITY ? 0.f : m[n];
+      const float mu = (m[n] == -INFINITY ? 0.f : m[n]) - kLift;
 #pragma unroll
       for (int v = 0; v < 8; v += 2) {
         const h2v e = {(_Float16)__builtin_amdgcn_exp2f(fmaf(s[n][v / 4][v % 4], c, -mu)),
