@@ -392,9 +392,11 @@ class DeviceVllmPagedKVCache:
         self._free_slots[lid].extend(at)
         self._final[lid][blocks] = True
 
-    def _resolve(self, lid: int, block_tables, context_lens, B: int):
+    def _resolve(self, lid: int, block_tables, context_lens, B: int, *, by_position: bool = False):
         """Checked lengths ``[B]``, their block counts, the block tables on the
-        host and their page ids ``[B, H, W]`` (keys, values)."""
+        host and their page ids ``[B, H, W]`` (keys, values).  ``by_position``:
+        the call finds token t in slot ``t % block_size`` of its block ``t //
+        block_size``, so all blocks of a sequence but the last must be full."""
         torch = _torch()
         P = self.block_size
         lens = np.asarray(context_lens.detach().cpu().numpy() if isinstance(context_lens, torch.Tensor) else context_lens,
@@ -419,6 +421,10 @@ class DeviceVllmPagedKVCache:
             if unknown[b]:
                 raise ValueError(f"sequence {b} names a block with no pages in layer {lid}")
             raise ValueError(f"sequence {b}: its blocks hold {int(held[b])} tokens, context_lens says {int(lens[b])}")
+        if by_position:
+            short = (np.arange(bt_host.shape[1])[None, :] < n_blocks[:, None] - 1) & (self._fill[lid][at] != P)
+            if short.any():
+                raise ValueError(f"sequence {int(np.flatnonzero(short.any(axis=1))[0])}: a block before its last is not full")
         # [B, H, W] page ids, keys and values
         kt, vt = (self._map[kind][lid][at].transpose(0, 2, 1) for kind in ("K", "V"))
         return lens, n_blocks, bt_host, kt, vt
@@ -471,7 +477,8 @@ class DeviceVllmPagedKVCache:
         """Causal attention of chunks: ``queries [sum(new_tokens), Hq, hd]``,
         one sequence after another, are those of the last ``new_tokens[b]``
         (0: the sequence waits) of the ``context_lens[b]`` tokens in the
-        blocks of ``block_tables[b]`` (write their slots first).  Prompt
+        blocks of ``block_tables[b]`` (write their slots first; all but the
+        last full).  Prompt
         chunks, drafted tokens to verify and plain decodes share a call.
         Returns rows of the queries' shape and type."""
         torch = _torch()
@@ -479,7 +486,7 @@ class DeviceVllmPagedKVCache:
         q = self._as_rows(queries, "queries", self.num_attention_heads)
         new = np.asarray(new_tokens.detach().cpu().numpy() if isinstance(new_tokens, torch.Tensor) else new_tokens,
                          dtype=np.int64).reshape(-1)
-        lens, _, _, kt, vt = self._resolve(lid, block_tables, context_lens, new.shape[0])
+        lens, _, _, kt, vt = self._resolve(lid, block_tables, context_lens, new.shape[0], by_position=True)
         if np.any(new < 0) or np.any(new > lens) or int(new.sum()) != q.shape[0]:
             raise ValueError("new_tokens must lie in [0, context] and add up to the queries' rows")
         k_table, v_table = torch.from_numpy(np.ascontiguousarray(np.stack([kt, vt]))).to(self.device)
@@ -490,11 +497,11 @@ class DeviceVllmPagedKVCache:
     def read_block_tables(self, layer_id: int, block_tables, context_lens, *, dtype=None):
         """The tokens of sequences as dense rows ``[sum(context_lens), H, hd]``,
         one sequence after another, keys and values, as their pages hold them
-        (fp32, or ``dtype`` fp16 / bf16)."""
+        (all blocks of a sequence but the last full; fp32, or ``dtype`` fp16 / bf16)."""
         torch = _torch()
         lid = self._check_layer(layer_id)
         B = np.asarray(block_tables.shape if hasattr(block_tables, "shape") else (len(block_tables),))[0]
-        lens, _, _, kt, vt = self._resolve(lid, block_tables, context_lens, int(B))
+        lens, _, _, kt, vt = self._resolve(lid, block_tables, context_lens, int(B), by_position=True)
         tables = torch.from_numpy(np.ascontiguousarray(np.stack([kt, vt]))).to(self.device)
         token = np.arange(int(lens.sum())) - np.repeat(np.cumsum(lens) - lens, lens)
         return self.k_pool.read_tokens_with(self.v_pool, tables, np.repeat(np.arange(lens.size), lens), token, dtype=dtype)
