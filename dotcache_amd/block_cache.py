@@ -113,7 +113,7 @@ class DeviceVllmPagedKVCache:
         self._seq_blocks = [[] for _ in range(L)]
         self._seq_len = np.zeros(L, dtype=np.int64)
         self._workspace = None
-        self._chunk_plan = None  # lengths and plan of the last attend_block_tables
+        self._chunk_plan = None  # lengths and stream of the last attend_block_tables, and its plan
 
     # ---- formats and small helpers ------------------------------------------
     def _page_format(self, kind: str, layer_id: int, kv_head_id: int) -> tuple[int, int]:
@@ -478,9 +478,9 @@ class DeviceVllmPagedKVCache:
         one sequence after another, are those of the last ``new_tokens[b]``
         (0: the sequence waits) of the ``context_lens[b]`` tokens in the
         blocks of ``block_tables[b]`` (write their slots first; all but the
-        last full).  Prompt
-        chunks, drafted tokens to verify and plain decodes share a call.
-        Returns rows of the queries' shape and type."""
+        last full).  Prompt chunks, drafted tokens to verify and plain decodes
+        share a call.  Returns rows of the queries' shape and type.  Not to be
+        captured into a graph."""
         torch = _torch()
         lid = self._check_layer(layer_id)
         q = self._as_rows(queries, "queries", self.num_attention_heads)

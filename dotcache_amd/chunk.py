@@ -189,27 +189,26 @@ def attend_cached(cache, queries, new: np.ndarray, context: np.ndarray, k_table,
     """:func:`attend_chunk` of ``queries [tokens, Hq, hd]`` over a cache's pages,
     its query heads in any order (``q_head_to_kv_head``; None: ``default_map``).
     ``cache`` keeps the last plan, by its lengths (every layer of a step has the
-    same), and the workspace of its other attention calls."""
+    same) and the stream it was made on, whose order its memory's reuse follows;
+    each call has a workspace of its own.  A captured call would read the plan
+    after the cache has dropped it, so it is refused."""
     torch = _torch()
+    if queries.is_cuda and torch.cuda.is_current_stream_capturing():
+        raise RuntimeError("a cache's chunk attention cannot be captured: capture attend_chunk with a plan of your own")
     H = cache.num_key_value_heads
     Hq = cache.num_attention_heads
     qmap = default_map if q_head_to_kv_head is None else np.asarray(q_head_to_kv_head, dtype=np.int64)
     if qmap.shape != (Hq,) or np.any(qmap < 0) or np.any(qmap >= H) or np.any(np.bincount(qmap, minlength=H) != Hq // H):
         raise ValueError("q_head_to_kv_head must give every KV head the same number of query heads")
-    lengths = (new.tobytes(), context.tobytes())
-    if cache._chunk_plan is None or cache._chunk_plan[0] != lengths:
-        cache._chunk_plan = (lengths, plan_chunk(cache.k_pool, cache.v_pool, new, context, kv_heads=H, q_per_kv=Hq // H))
+    key = (new.tobytes(), context.tobytes(), torch.cuda.current_stream(queries.device).cuda_stream if queries.is_cuda else 0)
+    if cache._chunk_plan is None or cache._chunk_plan[0] != key:
+        cache._chunk_plan = (key, plan_chunk(cache.k_pool, cache.v_pool, new, context, kv_heads=H, q_per_kv=Hq // H))
     plan = cache._chunk_plan[1]
-    need = workspace_bytes(plan, cache.config.head_dim)
-    if cache._workspace is None or cache._workspace.numel() < need:
-        cache._workspace = torch.empty(max(need, 16), dtype=torch.uint8, device=cache.device)
     order = np.argsort(qmap, kind="stable")  # query heads grouped by KV head
     if np.array_equal(order, np.arange(Hq)):
-        return attend_chunk(cache.k_pool, k_table, cache.v_pool, v_table, queries, plan, query_scale=query_scale,
-                            workspace=cache._workspace)
+        return attend_chunk(cache.k_pool, k_table, cache.v_pool, v_table, queries, plan, query_scale=query_scale)
     at = torch.from_numpy(order).to(cache.device)
-    out = attend_chunk(cache.k_pool, k_table, cache.v_pool, v_table, queries[:, at], plan, query_scale=query_scale,
-                       workspace=cache._workspace)
+    out = attend_chunk(cache.k_pool, k_table, cache.v_pool, v_table, queries[:, at], plan, query_scale=query_scale)
     res = torch.empty_like(out)
     res[:, at] = out
     return res

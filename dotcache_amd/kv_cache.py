@@ -113,7 +113,7 @@ class DevicePagedKVCache:
         self._host_tables = [None] * L  # the same tables on the host
         self._spec_memo: dict = {}
         self._workspace = None
-        self._chunk_plan = None  # lengths and plan of the last attend_chunk
+        self._chunk_plan = None  # lengths and stream of the last attend_chunk, and its plan
 
     # ---- formats -----------------------------------------------------------
     def _page_format(self, kind: str, layer_id: int, kv_head_id: int) -> tuple[int, int]:
@@ -451,7 +451,7 @@ class DevicePagedKVCache:
         each sequence's last n cached tokens (append them first): token i
         attends itself and all before it.  Heads map as in
         :meth:`decode_layer`.  Returns ``[B, Hq, n, hd]`` in the queries'
-        type on the device."""
+        type on the device.  Not to be captured into a graph."""
         lid = self._check_layer(layer_id)
         q = self._token_major(query_chunk, self.num_attention_heads, None, "query_chunk")
         B, n, Hq, hd = q.shape
