@@ -138,8 +138,8 @@ def attend_chunk(pool: DevicePagePool, k_table, v_pool: DevicePagePool | None, v
     are fp16 matrix operands (values past +-65504 overflow, as in fp16 pages)
     and all sums fp32; with fp32 queries everything is fp32.  ``query_scale`` may
     have either sign, or be 0.  ``workspace``:
-    uint8, :func:`workspace_bytes` at least, not shared by calls that may
-    overlap (default: one of its own).  The kernel follows from the formats that
+    uint8, :func:`workspace_bytes` at least, 16-byte aligned, not shared by calls
+    that may overlap (default: one of its own).  The kernel follows from the formats that
     the pools have held: a captured call is captured anew once a pool takes
     pages of a format that it had not.  ``validate`` reads the tables back and
     checks them against the pools (the kernel itself leaves out, and never
@@ -176,6 +176,8 @@ def attend_chunk(pool: DevicePagePool, k_table, v_pool: DevicePagePool | None, v
         workspace = torch.empty(need, dtype=torch.uint8, device=device)
     elif workspace.numel() * workspace.element_size() < need or not workspace.is_contiguous() or workspace.device != device:
         raise ValueError(f"workspace must be contiguous, {need} bytes at least, on {device}")
+    elif workspace.data_ptr() % 16:
+        raise ValueError("workspace must be 16-byte aligned")
     if plan.n_items:
         call_on(device, _lib.lib().dc_attend_chunk, "dc_attend_chunk", pool.c_pool(), vpool.c_pool(), k_table.data_ptr(),
                 v_table.data_ptr(), shape[2], plan.items.data_ptr(), plan.n_items, plan.n_few, plan.few_rows,

@@ -1495,7 +1495,7 @@ __global__ void __launch_bounds__(256) merge_chunk_kernel(ChunkArgs a, const dc_
         for (int j = 0; j < kMergeBatch; ++j) {
           const int i = i0 + j * split;
           const int64_t at = first + int64_t(i < mg.count ? i : i0) * rows;
-          ml[j] = *reinterpret_cast<const float2*>(a.part_ml + 2 * at);
+          ml[j] = float2{a.part_ml[2 * at], a.part_ml[2 * at + 1]};  // (an odd head_dim: at any 4 bytes)
           const float* po = a.part_o + at * hd + (in ? ch : 0);
           if constexpr (VEC == 4) {
             const float4 v = *reinterpret_cast<const float4*>(po);
@@ -1659,6 +1659,7 @@ extern "C" int dc_attend_chunk(dc_pool k_pool, dc_pool v_pool, const int32_t* k_
     return dc::fail(DC_EINVAL, "%s: the output needs the queries' dtype and heads, a multiple of the KV heads", who);
   if (workspace_bytes < dc_chunk_workspace_bytes(n_partials, hd) || (n_partials && !workspace))
     return dc::fail(DC_ESPACE, "%s: workspace too small", who);
+  if (reinterpret_cast<uintptr_t>(workspace) % 16 != 0) return dc::fail(DC_EINVAL, "%s: workspace must be 16-byte aligned", who);
   dc::ChunkArgs a{k_pool, v_pool, k_table, v_table, table_stride, items, n_items, n_seqs, n_kv_heads, q.n_heads / n_kv_heads,
                   n_tokens, n_partials, q.data, q.token_stride, q.head_stride, q.dtype,
                   query_scale == 0.f ? 1.f : fabsf(query_scale), query_scale > 0.f ? 1.f : query_scale < 0.f ? -1.f : 0.f, out.data, out.token_stride,

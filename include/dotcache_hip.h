@@ -602,7 +602,7 @@ int64_t dc_chunk_workspace_bytes(int32_t n_partials, int32_t head_dim);
  *   tables : device int32 [n_seqs][n_kv_heads][table_stride]; token u of a
  *            sequence is slot u % page_capacity of its page u / page_capacity
  *            (every page but a sequence's last is full)
- *   workspace : at least dc_chunk_workspace_bytes(n_partials, head_dim)
+ *   workspace : at least dc_chunk_workspace_bytes(n_partials, head_dim), 16-byte aligned
  * With 16-bit queries the matrix operands are fp16: queries, the pages' values
  * and the softmax weights are each rounded to it once (values beyond +-65504
  * overflow, as in fp16 pages), products and sums are fp32.  With DC_F32
