@@ -72,8 +72,8 @@ def _lengths(x, name: str) -> np.ndarray:
 def plan_chunk(pool: DevicePagePool, v_pool: DevicePagePool | None, new, context, *, kv_heads: int, q_per_kv: int,
                dtype=None, target_items: int | None = None) -> ChunkPlan:
     """The plan for ``new[b]`` new tokens (0: a sequence that waits) of
-    ``context[b]`` tokens in all, on the pools' device.  ``dtype``: the
-    queries' type (default bf16)."""
+    ``context[b]`` tokens in all, on the pools' device.  ``dtype``, the
+    queries' type, is checked if given; a plan serves any of them."""
     torch = _torch()
     vpool = pool if v_pool is None else v_pool
     _check_pools(pool, vpool)
@@ -82,6 +82,8 @@ def plan_chunk(pool: DevicePagePool, v_pool: DevicePagePool | None, new, context
         raise ValueError("new and context must hold one length per sequence")
     if np.any(n > ctx):
         raise ValueError("a sequence's context includes its new tokens")
+    if dtype is not None and dtype not in (torch.float32, torch.float16, torch.bfloat16):
+        raise ValueError(f"unsupported query dtype {dtype}")
     if int(kv_heads) <= 0 or int(q_per_kv) <= 0:
         raise ValueError("kv_heads and q_per_kv must be positive")
     target = default_target_items() // 4 if target_items is None else int(target_items)

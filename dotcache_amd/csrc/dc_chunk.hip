@@ -1623,7 +1623,7 @@ static int launch_few(const ChunkArgs& a, hipStream_t stream) {
 }
 
 // Whether a thread's 32 channels share a scale and lie at 16-byte multiples,
-// with offsets in a blob that fit 32 bits, in the formats that load_raw takes.
+// with offsets in a blob that fit 32 bits, in the formats that load_unit takes.
 static bool units32(const dc_pool& p) {
   const dc_page_geometry& g = p.geometry;
   uint64_t takes = uint64_t(1) << (DC_FMT_M3_F16 * 9);

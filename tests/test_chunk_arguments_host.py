@@ -31,3 +31,16 @@ def test_a_workspace_off_16_bytes():
     for off, match in ((0, "on a GPU"), (1, "16-byte"), (8, "16-byte")):
         with pytest.raises(ValueError, match=match):
             attend_chunk(pools[0], table, pools[1], table, torch.zeros(1, 1, 64), split, workspace=space[start + off:])
+
+
+def test_a_plan_serves_every_query_type():
+    """``dtype`` is checked; the plan does not depend on it."""
+    import numpy as np
+
+    plans = [plan_chunk(*_pools(), [5, 90], [700, 300], kv_heads=2, q_per_kv=3, target_items=16, dtype=dt)
+             for dt in (None, torch.float32, torch.float16, torch.bfloat16)]
+    for p in plans[1:]:
+        assert np.array_equal(p.host_items, plans[0].host_items) and np.array_equal(p.host_merges, plans[0].host_merges)
+    for dt in (torch.float64, torch.int8, "bf16"):
+        with pytest.raises(ValueError, match="dtype"):
+            plan_chunk(*_pools(), [5], [700], kv_heads=2, q_per_kv=3, dtype=dt)
