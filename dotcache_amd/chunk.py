@@ -137,15 +137,21 @@ def attend_chunk(pool: DevicePagePool, k_table, v_pool: DevicePagePool | None, v
     tokens are left as they are).
 
     With 16-bit queries, the queries, the pages' values and the softmax weights
-    are fp16 matrix operands (values past +-65504 overflow, as in fp16 pages)
-    and all sums fp32; with fp32 queries everything is fp32.  ``query_scale`` may
-    have either sign, or be 0.  ``workspace``:
-    uint8, :func:`workspace_bytes` at least, 16-byte aligned, not shared by calls
-    that may overlap (default: one of its own).  The kernel follows from the formats that
-    the pools have held: a captured call is captured anew once a pool takes
-    pages of a format that it had not.  ``validate`` reads the tables back and
-    checks them against the pools (the kernel itself leaves out, and never
-    reads, what a table does not name)."""
+    are fp16 matrix operands, each rounded once, and all sums fp32: an output is
+    off by about 2^-11 of its terms, beside its own rounding.  Values past
+    +-65504 overflow, as in fp16 pages; bf16 queries below 2^-14 lose bits, below
+    2^-25 they are zeros.  With fp32 queries everything is fp32.  ``query_scale``
+    may have either sign, or be 0.  ``workspace``: uint8, :func:`workspace_bytes`
+    at least, 16-byte aligned, not shared by calls that may overlap (default: one
+    of its own).  ``validate`` reads the tables back and checks them against the
+    pools (the kernel itself leaves out, and never reads, what a table does not
+    name).
+
+    The kernel follows from the formats that the pools have ever held.  Once a
+    pool has taken a 2- or 3-bit, int8 or fp32 page (a cache's tail, by
+    ``escape_dtype``), 16-bit queries take the general kernel, two to six times
+    as long; and a captured call is captured anew once a pool takes pages of a
+    format that it had not."""
     torch = _torch()
     vpool = pool if v_pool is None else v_pool
     _check_pools(pool, vpool)

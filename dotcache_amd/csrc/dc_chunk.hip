@@ -23,12 +23,14 @@
 //
 // Three kernels, by what the pools hold and by rows: attend_chunk16_kernel
 // (16-bit queries, pages of 32-channel units: 2 x 2048 rows of 7 heads a KV head
-// over 16384 tokens, fp16 keys and 4-bit values, 1.30 ms, 693 TFLOP/s of an
-// fp16 library product's 1178; 1.04 ms of it without its page loads),
+// over 16384 tokens, fp16 keys and 4-bit values, 1.31 ms with the join, 690
+// TFLOP/s of an fp16 library product's 1178; 1.04 ms without the page loads),
 // attend_few_kernel (the same pages, few rows against a long range: 5 rows of 7
-// heads of four sequences to 131072 tokens, 126 MB, 99 us, where the copy
-// rate would take 27; when it was made 170 us, the 256-row kernel 320) and
-// attend_chunk_kernel (the rest: 3 x 61 rows of 1001 tokens in fp32 82 us).
+// heads of four sequences to 131072 tokens, 126 MB, 101 us with the join, where
+// the copy rate would take 27; when it was made 170 us, the 256-row kernel 320) and
+// attend_chunk_kernel (the rest: 3 x 61 rows of 1001 tokens in fp32 83 us and 7
+// for the join; the two calls above, made with 16-bit queries on pools that have
+// held a 2-bit page, 4.3 ms and 0.61).
 // 16-bit queries' operands are fp16, which the matrix unit takes at eight times
 // the fp32 rate: a query, a page's value and a weight are each rounded to it
 // once, by 2^-11 relative, or below 2^-14 (a weight: below 2^-21 of the row's

@@ -8,7 +8,8 @@
 // lines.  Four lanes of a row turn their 16-byte units about, so that each
 // store of theirs covers 64 bytes in a row, and stores of more than the L2
 // holds bypass it (kStreamBytes): 8 x 16384 tokens of 4 heads of 128 channels
-// from 4-bit pages as bf16 (352 MB in all) take 67 us (5.3 TB/s); 119 us with
+// from 4-bit pages as bf16 (352 MB in all) take 65 to 74 us (5 TB/s) where the last
+// cache still holds the pages, 97 (3.6) where it does not.  The former: 119 us with
 // the units turned alone, 130 us with the bypass alone, 118 us with neither
 // (a bypassing store of half a line is written as it is).  Four tokens a lane
 // with their loads in flight together were 76 us.  Geometries without such

@@ -479,8 +479,9 @@ static int check_rotary(const RotaryArgs& R, const char* who) {
 
 // A lane takes several heads of a token as long as that leaves kRowBlocks
 // blocks, and rows that the L2 would not hold bypass it.  16384 tokens of 28 + 4
-// heads of 128 channels, bf16 (277 MB): 46 us (6.0 TB/s); with at most 8 heads a
-// lane, four of them in flight, 53 us; without the bypass 59; with 2048 / 4096
+// heads of 128 channels, bf16 (277 MB): 46 us (6.0 TB/s) on rows that the last
+// cache still holds in part, 60 (4.6) on others.  The former with at most 8 heads
+// a lane, four of them in flight, 53 us; without the bypass 59; with 2048 / 4096
 // blocks asked for 61 / 67 (all with four in flight).
 constexpr int64_t kRowBlocks = 1024;
 constexpr int32_t kMaxHeads = 16;

@@ -605,7 +605,9 @@ int64_t dc_chunk_workspace_bytes(int32_t n_partials, int32_t head_dim);
  *   workspace : at least dc_chunk_workspace_bytes(n_partials, head_dim), 16-byte aligned
  * With 16-bit queries the matrix operands are fp16: queries, the pages' values
  * and the softmax weights are each rounded to it once (values beyond +-65504
- * overflow, as in fp16 pages), products and sums are fp32.  With DC_F32
+ * overflow, as in fp16 pages; bf16 queries below 2^-14 lose bits, below 2^-25
+ * they are zeros; weights below 2^-21 and 2^-32 of a row's largest likewise),
+ * products and sums are fp32.  With DC_F32
  * everything is fp32.  query_scale may have either sign, or be 0.  A token whose
  * page the table does not name or that its page does not hold is left out; a row
  * that sees no token gives zeros.
