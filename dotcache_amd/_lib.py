@@ -72,6 +72,10 @@ class TokenDest(C.Structure):
                 ("n_rows", C.c_int32), ("n_pages", C.c_int32), ("page_tokens", C.c_int32)]
 
 
+class ScoreRule(C.Structure):
+    _fields_ = [("cap", C.c_float), ("slopes", C.c_void_p), ("ranges", C.c_void_p), ("gaps", C.c_void_p)]
+
+
 CHUNK_ITEM_FIELDS = ("seq", "kv_head", "q_begin", "row_begin", "row_end", "first", "kv_begin", "kv_end", "partial")
 CHUNK_MERGE_FIELDS = ("kv_head", "q_begin", "row_begin", "row_end", "partial_begin", "count")
 
@@ -106,6 +110,13 @@ SIGNATURES = {
     "dc_attend_chunk": (C.c_int, [Pool, Pool, C.c_void_p, C.c_void_p, C.c_int32, C.c_void_p, C.c_int32, C.c_int32,
                                   C.c_int32, C.c_void_p, C.c_int32, C.c_int32, C.c_int32, C.c_int32, C.c_int64, TokenRows, C.c_float, TokenRows,
                                   C.c_void_p, C.c_int64, C.c_void_p]),
+    "dc_plan_chunk_ranges": (C.c_int, [C.c_void_p, C.c_void_p, C.c_void_p, C.c_int32, C.c_int32, C.c_int32, C.c_int32,
+                                       C.c_int32, C.c_int32, C.c_void_p, C.c_void_p, C.c_int32, C.POINTER(C.c_int32),
+                                       C.POINTER(C.c_int32), C.POINTER(C.c_int32), C.c_void_p, C.c_int32,
+                                       C.POINTER(C.c_int32), C.POINTER(C.c_int32)]),
+    "dc_attend_chunk_rule": (C.c_int, [Pool, Pool, C.c_void_p, C.c_void_p, C.c_int32, C.c_void_p, C.c_int32, C.c_int32,
+                                       C.c_int32, C.c_void_p, C.c_int32, C.c_int32, C.c_int32, C.c_int32, C.c_int64,
+                                       TokenRows, C.c_float, ScoreRule, TokenRows, C.c_void_p, C.c_int64, C.c_void_p]),
     "dc_set_encode_path": (C.c_int, [C.c_int32]),
     "dc_score_pages": (C.c_int, [Pool, C.c_void_p, C.c_void_p, C.c_int32, C.c_void_p, C.c_int32, C.c_void_p, C.c_int64, C.c_void_p]),
     "dc_mix_pages": (C.c_int, [Pool, C.c_void_p, C.c_void_p, C.c_int32, C.c_void_p, C.c_int32, C.c_int64, C.c_void_p, C.c_int32, C.c_void_p]),

@@ -113,7 +113,7 @@ class DeviceVllmPagedKVCache:
         self._seq_blocks = [[] for _ in range(L)]
         self._seq_len = np.zeros(L, dtype=np.int64)
         self._workspace = None
-        self._chunk_plan = None  # lengths and stream of the last attend_block_tables, and its plan
+        self._chunk_plan = None  # lengths and stream of the last attend_block_tables, and its plans by mask
 
     # ---- formats and small helpers ------------------------------------------
     def _page_format(self, kind: str, layer_id: int, kv_head_id: int) -> tuple[int, int]:
@@ -473,8 +473,10 @@ class DeviceVllmPagedKVCache:
         return res
 
     def attend_block_tables(self, layer_id: int, queries, new_tokens, block_tables, context_lens, q_head_to_kv_head=None, *,
-                            query_scale: float = 1.0):
-        """Causal attention of chunks: ``queries [sum(new_tokens), Hq, hd]``,
+                            query_scale: float = 1.0, mask=None, cap: float | None = None, slopes=None):
+        """Attention of chunks, causal or by ``mask``
+        (:class:`~dotcache_amd.chunk.ChunkMask`), scores shaped by ``cap`` and
+        ``slopes [Hq]`` as in :func:`~dotcache_amd.chunk.attend_chunk`: ``queries [sum(new_tokens), Hq, hd]``,
         one sequence after another, are those of the last ``new_tokens[b]``
         (0: the sequence waits) of the ``context_lens[b]`` tokens in the
         blocks of ``block_tables[b]`` (write their slots first; all but the
@@ -492,7 +494,7 @@ class DeviceVllmPagedKVCache:
         k_table, v_table = torch.from_numpy(np.ascontiguousarray(np.stack([kt, vt]))).to(self.device)
         q = q if q.stride(2) == 1 else q.contiguous()
         return attend_cached(self, q, new.astype(np.int32), lens.astype(np.int32), k_table, v_table, q_head_to_kv_head,
-                             self.default_q_head_to_kv_head, query_scale)
+                             self.default_q_head_to_kv_head, query_scale, mask, cap, slopes)
 
     def read_block_tables(self, layer_id: int, block_tables, context_lens, *, dtype=None):
         """The tokens of sequences as dense rows ``[sum(context_lens), H, hd]``,

@@ -264,26 +264,33 @@ int64_t dc_chunk_workspace_bytes(int32_t n_partials, int32_t head_dim) {
   return int64_t(n_partials) * (head_dim + 2) * 4;
 }
 
-int dc_plan_chunk(const int32_t* new_tokens, const int32_t* context, int32_t n_seqs, int32_t n_kv_heads, int32_t n_q,
-                  int32_t head_dim, int32_t target_items, int32_t min_tokens, dc_chunk_item* items, int32_t max_items,
-                  int32_t* n_items, int32_t* n_few, int32_t* few_rows, dc_chunk_merge* merges, int32_t max_merges,
-                  int32_t* n_merges, int32_t* n_partials) {
+// ranges, gaps null: causal.
+static int plan_chunk(const char* who, const int32_t* new_tokens, const int32_t* context, const int32_t* ranges, int32_t n_seqs,
+                      int32_t n_kv_heads, int32_t n_q, int32_t head_dim, int32_t target_items, int32_t min_tokens,
+                      dc_chunk_item* items, int32_t* gaps, int32_t max_items, int32_t* n_items, int32_t* n_few, int32_t* few_rows,
+                      dc_chunk_merge* merges, int32_t max_merges, int32_t* n_merges, int32_t* n_partials) {
   if (!new_tokens || !context || n_seqs <= 0 || n_kv_heads <= 0 || n_q <= 0 || head_dim <= 0 || target_items <= 0 || min_tokens <= 0 ||
       !n_items || !n_few || !few_rows || !n_merges || !n_partials)
-    return dc::fail(DC_EINVAL, "dc_plan_chunk: bad arguments");
+    return dc::fail(DC_EINVAL, "%s: bad arguments", who);
   try {
     const int64_t step = dc::kChunkStep;
     int64_t q_tokens = 0;
     for (int32_t b = 0; b < n_seqs; ++b) {
       if (new_tokens[b] < 0 || context[b] < new_tokens[b])
-        return dc::fail(DC_EINVAL, "dc_plan_chunk: sequence %d has %d new tokens in a context of %d", b, new_tokens[b], context[b]);
+        return dc::fail(DC_EINVAL, "%s: sequence %d has %d new tokens in a context of %d", who, b, new_tokens[b], context[b]);
       // (the kernels look a few tiles past a range's end)
-      if (context[b] > INT32_MAX - 65536) return dc::fail(DC_EINVAL, "dc_plan_chunk: sequence %d has too long a context", b);
-      if (int64_t(new_tokens[b]) * n_q > INT32_MAX - dc::kChunkRows) return dc::fail(DC_EINVAL, "dc_plan_chunk: sequence %d has too many new tokens", b);
+      if (context[b] > INT32_MAX - 65536) return dc::fail(DC_EINVAL, "%s: sequence %d has too long a context", who, b);
+      if (int64_t(new_tokens[b]) * n_q > INT32_MAX - dc::kChunkRows) return dc::fail(DC_EINVAL, "%s: sequence %d has too many new tokens", who, b);
+      for (int64_t t = q_tokens; ranges && t < q_tokens + new_tokens[b]; ++t) {
+        const int32_t* r = ranges + 4 * t;
+        if (r[0] < 0 || r[1] < r[0] || r[1] > context[b] || r[2] < 0 || r[3] < r[2] || r[3] > context[b])
+          return dc::fail(DC_EINVAL, "%s: sequence %d has a range outside its context", who, b);
+      }
       q_tokens += new_tokens[b];
     }
-    if (q_tokens > INT32_MAX) return dc::fail(DC_EINVAL, "dc_plan_chunk: too many new tokens");
+    if (q_tokens > INT32_MAX) return dc::fail(DC_EINVAL, "%s: too many new tokens", who);
     std::vector<dc_chunk_item> order;
+    std::vector<std::pair<int32_t, int32_t>> left_out;  // the items' gaps
     std::vector<dc_chunk_merge> joins;
     int64_t parts = 0;
     *few_rows = 0;
@@ -294,9 +301,31 @@ int dc_plan_chunk(const int32_t* new_tokens, const int32_t* context, int32_t n_s
         return new_tokens[b] > 0 && (int64_t(new_tokens[b]) * n_q <= dc::few_row_limit(head_dim)) == few;
       };
       // Row tiles and the steps of their token ranges, streams in order.
+      // A tile takes `near` steps from step begin0, then the rest from step
+      // begin1; its first stretch ends with token end0.
+      struct Reach {
+        int64_t begin0, near, begin1, len;
+        int32_t end0, end1;
+      };
       struct Tile {
         dc_chunk_item item;
         int64_t begin, len;
+        Reach reach;
+      };
+      auto reach_of = [&](const int32_t* r, int64_t tokens) {  // of `tokens` rows of ranges
+        int32_t lo[2] = {INT32_MAX, INT32_MAX}, hi[2] = {0, 0};
+        for (int64_t t = 0; t < tokens; ++t)
+          for (int k = 0; k < 2; ++k) {
+            if (r[4 * t + 2 * k] == r[4 * t + 2 * k + 1]) continue;
+            lo[k] = std::min(lo[k], r[4 * t + 2 * k]);
+            hi[k] = std::max(hi[k], r[4 * t + 2 * k + 1]);
+          }
+        if (lo[0] > lo[1]) std::swap(lo[0], lo[1]), std::swap(hi[0], hi[1]);
+        if (hi[0] == 0) return Reach{0, 0, 0, 1, 0, 1};  // rows that see nothing: zeros have to be written
+        const int64_t b0 = lo[0] / step, e0 = (hi[0] + step - 1) / step, b1 = lo[1] / step, e1 = (hi[1] + step - 1) / step;
+        if (hi[1] == 0) return Reach{0, 0, b0, e0 - b0, 0, hi[0]};
+        if (b1 <= e0) return Reach{0, 0, b0, std::max(e0, e1) - b0, 0, std::max(hi[0], hi[1])};
+        return Reach{b0, e0 - b0, b1, e0 - b0 + e1 - b1, hi[0], hi[1]};
       };
       std::vector<Tile> tiles;
       int64_t total = 0;
@@ -305,12 +334,17 @@ int dc_plan_chunk(const int32_t* new_tokens, const int32_t* context, int32_t n_s
         if (!takes(b)) continue;
         const int32_t rows = new_tokens[b] * n_q, first = context[b] - new_tokens[b];
         if (few) *few_rows = std::max(*few_rows, rows);
+        std::vector<Reach> reach;
+        for (int32_t r = 0; r < rows; r += dc::kChunkRows) {
+          const int32_t r1 = std::min(r + dc::kChunkRows, rows), t0 = r / n_q, t1 = (r1 - 1) / n_q + 1, end = first + t1;
+          reach.push_back(ranges ? reach_of(ranges + 4 * (int64_t(q_begin) + t0), t1 - t0)
+                                 : Reach{0, 0, 0, (int64_t(end) + step - 1) / step, 0, end});
+        }
         for (int32_t h = 0; h < n_kv_heads; ++h)
           for (int32_t r = 0; r < rows; r += dc::kChunkRows) {
-            const int32_t r1 = std::min(r + dc::kChunkRows, rows), end = first + (r1 - 1) / n_q + 1;
-            const int64_t len = (int64_t(end) + step - 1) / step;
-            tiles.push_back({{b, h, q_begin, r, r1, first, 0, end, -1}, total, len});
-            total += len;
+            const Reach& x = reach[r / dc::kChunkRows];
+            tiles.push_back({{b, h, q_begin, r, std::min(r + dc::kChunkRows, rows), first, 0, x.end1, -1}, total, x.len, x});
+            total += x.len;
           }
       }
       if (tiles.empty()) continue;
@@ -394,7 +428,7 @@ int dc_plan_chunk(const int32_t* new_tokens, const int32_t* context, int32_t n_s
         if (of[t].size() < 2) continue;
         const dc_chunk_item& x = tiles[t].item;
         const int64_t rows = x.row_end - x.row_begin, n = int64_t(of[t].size());
-        if (parts + n * rows > INT32_MAX) return dc::fail(DC_EINVAL, "dc_plan_chunk: too many partial results");
+        if (parts + n * rows > INT32_MAX) return dc::fail(DC_EINVAL, "%s: too many partial results", who);
         std::sort(of[t].begin(), of[t].end());
         joins.push_back({x.kv_head, x.q_begin, x.row_begin, x.row_end, int32_t(parts), int32_t(n)});
         for (auto& p : of[t]) {
@@ -406,32 +440,56 @@ int dc_plan_chunk(const int32_t* new_tokens, const int32_t* context, int32_t n_s
         for (const auto& d : die) {
           if (i >= d.size()) {
             order.push_back({-1, 0, 0, 0, 0, 0, 0, 0, -1});
+            left_out.push_back({-1, -1});
             continue;
           }
           const Tile& t = tiles[d[i].tile];
           dc_chunk_item x = t.item;
-          x.kv_begin = int32_t(d[i].begin * step);
-          x.kv_end = int32_t(std::min<int64_t>(d[i].end * step, x.kv_end));
+          const Reach& z = t.reach;
+          const bool from_near = d[i].begin < z.near, to_near = d[i].end <= z.near;
+          x.kv_begin = int32_t((from_near ? z.begin0 + d[i].begin : z.begin1 + d[i].begin - z.near) * step);
+          x.kv_end = int32_t(std::min<int64_t>((to_near ? z.begin0 + d[i].end : z.begin1 + d[i].end - z.near) * step, to_near ? z.end0 : z.end1));
+          left_out.push_back(from_near && !to_near ? std::make_pair(int32_t((z.begin0 + z.near) * step), int32_t(z.begin1 * step))
+                                                   : std::make_pair(-1, -1));
           const auto& p = of[d[i].tile];
           x.partial = int32_t(std::lower_bound(p.begin(), p.end(), std::make_pair(d[i].begin, int64_t(-1)))->second);
           order.push_back(x);
         }
-      while (!order.empty() && order.back().seq < 0) order.pop_back();
-      if (order.size() > INT32_MAX) return dc::fail(DC_EINVAL, "dc_plan_chunk: too many items");
+      while (!order.empty() && order.back().seq < 0) order.pop_back(), left_out.pop_back();
+      if (order.size() > INT32_MAX) return dc::fail(DC_EINVAL, "%s: too many items", who);
       if (few) *n_few = int32_t(order.size());
     }
     *n_items = int32_t(order.size());
     *n_merges = int32_t(joins.size());
     *n_partials = int32_t(parts);
     if (*n_items > max_items || *n_merges > max_merges)
-      return dc::fail(DC_ESPACE, "dc_plan_chunk: need %d items and %d merges", *n_items, *n_merges);
-    if ((!items && *n_items) || (!merges && *n_merges)) return dc::fail(DC_EINVAL, "dc_plan_chunk: null output arrays");
+      return dc::fail(DC_ESPACE, "%s: need %d items and %d merges", who, *n_items, *n_merges);
+    if ((!items && *n_items) || (!merges && *n_merges)) return dc::fail(DC_EINVAL, "%s: null output arrays", who);
     std::copy(order.begin(), order.end(), items);
+    for (size_t i = 0; gaps && i < order.size(); ++i) gaps[2 * i] = left_out[i].first, gaps[2 * i + 1] = left_out[i].second;
     std::copy(joins.begin(), joins.end(), merges);
     return DC_OK;
   } catch (...) {
-    return dc::fail(DC_ESPACE, "dc_plan_chunk: out of memory");
+    return dc::fail(DC_ESPACE, "%s: out of memory", who);
   }
+}
+
+int dc_plan_chunk(const int32_t* new_tokens, const int32_t* context, int32_t n_seqs, int32_t n_kv_heads, int32_t n_q,
+                  int32_t head_dim, int32_t target_items, int32_t min_tokens, dc_chunk_item* items, int32_t max_items,
+                  int32_t* n_items, int32_t* n_few, int32_t* few_rows, dc_chunk_merge* merges, int32_t max_merges,
+                  int32_t* n_merges, int32_t* n_partials) {
+  return plan_chunk("dc_plan_chunk", new_tokens, context, nullptr, n_seqs, n_kv_heads, n_q, head_dim, target_items, min_tokens, items,
+                    nullptr, max_items, n_items, n_few, few_rows, merges, max_merges, n_merges, n_partials);
+}
+
+int dc_plan_chunk_ranges(const int32_t* new_tokens, const int32_t* context, const int32_t* ranges, int32_t n_seqs,
+                         int32_t n_kv_heads, int32_t n_q, int32_t head_dim, int32_t target_items, int32_t min_tokens,
+                         dc_chunk_item* items, int32_t* gaps, int32_t max_items, int32_t* n_items, int32_t* n_few,
+                         int32_t* few_rows, dc_chunk_merge* merges, int32_t max_merges, int32_t* n_merges,
+                         int32_t* n_partials) {
+  if (!ranges || (max_items > 0 && !gaps)) return dc::fail(DC_EINVAL, "dc_plan_chunk_ranges: null pointer");
+  return plan_chunk("dc_plan_chunk_ranges", new_tokens, context, ranges, n_seqs, n_kv_heads, n_q, head_dim, target_items, min_tokens,
+                    items, gaps, max_items, n_items, n_few, few_rows, merges, max_merges, n_merges, n_partials);
 }
 
 }  // extern "C"

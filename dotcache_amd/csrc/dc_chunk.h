@@ -33,6 +33,12 @@ struct ChunkArgs {
   float* part_ml;  // [n_partials][2]
   uint32_t page_mul, page_shift;
   int32_t q_vec, o_vec;  // rows start at multiples of 16 (8) bytes
+  // kernels with a rule (dc_score_rule):
+  float cap;              // cap log2 e, or 0: none
+  float cap_in;           // 2 scale log2 e / cap
+  const float* slopes;    // [n_kv_heads * n_q] or null
+  const int4* ranges;     // [n_tokens] {first, end, first, end}, or null: causal
+  const int2* gaps;       // [n_items] or null
 };
 
 // A work item outside the call's shapes is skipped, not read: a fault guard
@@ -50,6 +56,11 @@ __device__ __forceinline__ bool chunk_merge_ok(const dc_chunk_merge& m, const Ch
          int64_t(m.q_begin) + (m.row_end - 1) / a.n_q < a.n_tokens && m.partial_begin >= 0 && m.count > 0 &&
          int64_t(m.partial_begin) + int64_t(m.count) * (m.row_end - m.row_begin) <= a.n_partials;
 }
+
+// The launches of a call's row tiles and few-row items (the join is apart):
+// `units`, 16-bit queries on pages of 32-channel units.
+int launch_chunks(ChunkArgs a, int32_t n_few, int32_t few_rows, bool units, hipStream_t stream);
+int launch_chunks_rule(ChunkArgs a, int32_t n_few, int32_t few_rows, bool units, hipStream_t stream);
 
 __device__ __forceinline__ void store_value(void* p, int32_t dtype, int64_t i, float x) {
   if (dtype == DC_F32)

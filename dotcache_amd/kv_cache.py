@@ -113,7 +113,7 @@ class DevicePagedKVCache:
         self._host_tables = [None] * L  # the same tables on the host
         self._spec_memo: dict = {}
         self._workspace = None
-        self._chunk_plan = None  # lengths and stream of the last attend_chunk, and its plan
+        self._chunk_plan = None  # lengths and stream of the last attend_chunk, and its plans by mask
 
     # ---- formats -----------------------------------------------------------
     def _page_format(self, kind: str, layer_id: int, kv_head_id: int) -> tuple[int, int]:
@@ -446,10 +446,14 @@ class DevicePagedKVCache:
                 k_table, v_table, counts, _ = self._tables[lid]
                 self._tables[lid] = (k_table, v_table, counts, np.full(B, fill + take, dtype=np.int32))
 
-    def attend_chunk(self, layer_id: int, query_chunk, q_head_to_kv_head=None, *, query_scale: float = 1.0):
-        """Causal attention of ``query_chunk [B, Hq, n, hd]``, the queries of
+    def attend_chunk(self, layer_id: int, query_chunk, q_head_to_kv_head=None, *, query_scale: float = 1.0, mask=None,
+                     cap: float | None = None, slopes=None):
+        """Attention of ``query_chunk [B, Hq, n, hd]``, the queries of
         each sequence's last n cached tokens (append them first): token i
-        attends itself and all before it.  Heads map as in
+        attends itself and all before it, or what ``mask``
+        (:class:`~dotcache_amd.chunk.ChunkMask`, positions counted from the
+        first cached token) says; ``cap`` and ``slopes [Hq]`` shape scores as in
+        :func:`~dotcache_amd.chunk.attend_chunk`.  Heads map as in
         :meth:`decode_layer`.  Returns ``[B, Hq, n, hd]`` in the queries'
         type on the device.  Not to be captured into a graph."""
         lid = self._check_layer(layer_id)
@@ -462,7 +466,7 @@ class DevicePagedKVCache:
             return q.transpose(1, 2).clone()
         k_table, v_table, _, _ = self._layer_tables(lid)
         out = attend_cached(self, q.reshape(B * n, Hq, hd), np.full(B, n, dtype=np.int32), held.astype(np.int32), k_table,
-                            v_table, q_head_to_kv_head, self.q_head_to_kv_head, query_scale)
+                            v_table, q_head_to_kv_head, self.q_head_to_kv_head, query_scale, mask, cap, slopes)
         return out.view(B, n, Hq, hd).transpose(1, 2)
 
     def _held(self, lid: int) -> np.ndarray:

@@ -618,6 +618,44 @@ int dc_attend_chunk(dc_pool k_pool, dc_pool v_pool, const int32_t* k_table, cons
                     const dc_chunk_merge* merges, int32_t n_merges, int32_t n_partials, int32_t n_seqs,
                     int32_t n_kv_heads, int64_t n_tokens, dc_token_rows q, float query_scale, dc_token_rows out, void* workspace, int64_t workspace_bytes, dc_stream_t stream);
 
+/* What the tokens of dc_attend_chunk_rule attend, and how their scores are
+ * shaped.  A score is s = query_scale q . k; then, with a cap, s = cap tanh(s /
+ * cap); then, with slopes, s -= slopes[query head] |i - u| for token i of a
+ * sequence and the token u that it attends.
+ *   ranges : device int32 [n_tokens][4] {first, end, first, end}, 16-byte
+ *            aligned: new token t attends tokens [0], .. [1] - 1 and [2], .. [3] - 1
+ *            of its sequence (the ranges do not overlap; empty ones: a row of
+ *            zeros).  NULL: itself and all before it.
+ *   gaps   : device int32 [n_items][2] beside the items, as
+ *            dc_plan_chunk_ranges wrote them, 8-byte aligned.  NULL: none. */
+typedef struct dc_score_rule {
+  float cap;           /* 0: none                                       */
+  const float* slopes; /* device fp32 [n_kv_heads * n_q]; NULL: none    */
+  const int32_t* ranges;
+  const int32_t* gaps;
+} dc_score_rule;
+
+/* dc_plan_chunk where new token t (of all sequences, one after another) attends
+ * tokens [ranges[t][0], ranges[t][1]) and [ranges[t][2], ranges[t][3]) of its
+ * sequence (host int32, 0 <= first <= end <= the context, apart from each
+ * other): a row tile's items cover what its rows attend, in steps of 128 tokens.
+ * An item that takes tokens of two stretches leaves out [gaps[i][0], gaps[i][1])
+ * between them ({-1, -1}: nothing left out; host [max_items][2]). */
+int dc_plan_chunk_ranges(const int32_t* new_tokens, const int32_t* context, const int32_t* ranges, int32_t n_seqs,
+                         int32_t n_kv_heads, int32_t n_q, int32_t head_dim, int32_t target_items, int32_t min_tokens,
+                         dc_chunk_item* items, int32_t* gaps, int32_t max_items, int32_t* n_items, int32_t* n_few,
+                         int32_t* few_rows, dc_chunk_merge* merges, int32_t max_merges, int32_t* n_merges,
+                         int32_t* n_partials);
+
+/* dc_attend_chunk with a rule; items of dc_plan_chunk, or of
+ * dc_plan_chunk_ranges with the ranges and gaps that belong to them.  Reference
+ * models with windows and capped scores: dotcache/integrations/gemma4.py. */
+int dc_attend_chunk_rule(dc_pool k_pool, dc_pool v_pool, const int32_t* k_table, const int32_t* v_table, int32_t table_stride,
+                         const dc_chunk_item* items, int32_t n_items, int32_t n_few, int32_t few_rows,
+                         const dc_chunk_merge* merges, int32_t n_merges, int32_t n_partials, int32_t n_seqs,
+                         int32_t n_kv_heads, int64_t n_tokens, dc_token_rows q, float query_scale, dc_score_rule rule,
+                         dc_token_rows out, void* workspace, int64_t workspace_bytes, dc_stream_t stream);
+
 /* Process-wide decode kernel choice: 0 (default) runs the MFMA kernel when
  * every page format (M3 fp16 keys and values, M0 4- or 8-bit keys of group
  * 32, M0 4- or 8-bit values of group 32 or 64), head_dim (64/128/256) and
