@@ -226,6 +226,32 @@ __device__ __forceinline__ float capped(const ChunkArgs& a, float s) {
   return fmaf(-2.f * a.cap, __builtin_amdgcn_rcpf(__builtin_amdgcn_exp2f(a.cap_in * s) + 1.f), a.cap);
 }
 
+// The products of a row with blocks of tokens as such exponents: element v of
+// block i is token u + 32 i + 8 (v / 4) + v % 4 (16 elements a block), or token
+// u + 16 i + v (4 elements).
+template <typename V, int N>
+__device__ __forceinline__ void shape_scores(const ChunkArgs& a, float c, const RowRule& r, int u, V (&s)[N]) {
+  constexpr int W = sizeof(V) / 4;
+  if (a.cap > 0.f) {
+#pragma unroll
+    for (int i = 0; i < N; ++i)
+#pragma unroll
+      for (int v = 0; v < W; ++v) s[i][v] = capped(a, s[i][v]);
+  } else {
+#pragma unroll
+    for (int i = 0; i < N; ++i)
+#pragma unroll
+      for (int v = 0; v < W; ++v) s[i][v] *= c;
+  }
+  if (a.slopes) {
+    const float away = r.at - float(u);
+#pragma unroll
+    for (int i = 0; i < N; ++i)
+#pragma unroll
+      for (int v = 0; v < W; ++v) s[i][v] = fmaf(-r.slope, fabsf(away - float((W == 16 ? 32 : 16) * i + 2 * (v & ~3) + v % 4)), s[i][v]);
+  }
+}
+
 // The item's gap: its tiles leave out tokens [x, y).
 __device__ __forceinline__ int2 item_gap(const ChunkArgs& a, uint32_t item) { return a.gaps ? a.gaps[item] : int2{-1, -1}; }
 
@@ -412,26 +438,7 @@ __global__ void __launch_bounds__(256, sizeof(T) == 4 && HDP == 256 ? 1 : 2) att
         }
       }
     }
-    if constexpr (RULE) {
-      if (a.cap > 0.f) {
-#pragma unroll
-        for (int tb = 0; tb < TB; ++tb)
-#pragma unroll
-          for (int v = 0; v < 16; ++v) s[tb][v] = capped(a, s[tb][v]);
-      } else {
-#pragma unroll
-        for (int tb = 0; tb < TB; ++tb)
-#pragma unroll
-          for (int v = 0; v < 16; ++v) s[tb][v] *= c;
-      }
-      if (a.slopes) {
-        const float away = rule.at - float(u0 + 4 * half);
-#pragma unroll
-        for (int tb = 0; tb < TB; ++tb)
-#pragma unroll
-          for (int v = 0; v < 16; ++v) s[tb][v] = fmaf(-rule.slope, fabsf(away - float(32 * tb + 8 * (v / 4) + v % 4)), s[tb][v]);
-      }
-    }
+    if constexpr (RULE) shape_scores(a, c, rule, u0 + 4 * half, s);
     // tokens that do not count, or that this row does not see
     bool masked = RULE ? !mine.whole(u0, KT) : u0 + KT - 1 > sees_all;
 #pragma unroll
@@ -737,7 +744,7 @@ __device__ __forceinline__ uint32_t fold_tokens(uint64_t b) {
 // (head_dim 256, whose queries and output of 32 rows fill the registers).
 // WHOLE: head_dim is HDP, so that no channel is left out and no mask kept for it
 // (12 sequences at head_dim 256 608 -> 597 us, five rows of four long sequences 98 -> 95).
-template <int HDP, int KT, bool UNI, int CS, bool WHOLE>
+template <int HDP, int KT, bool UNI, int CS, bool WHOLE, bool RULE>
 __global__ void __launch_bounds__(512, 2) attend_chunk16_kernel(ChunkArgs a) {
   constexpr int CH = HDP / 8, TB = KT / 32, CB = HDP / 32 / CS, TILE = KT * HDP * 2, QW = HDP / 16;
   constexpr int NT = KT < 64 ? 8 : KT / 8;  // tokens a wavefront turns
@@ -749,7 +756,7 @@ __global__ void __launch_bounds__(512, 2) attend_chunk16_kernel(ChunkArgs a) {
 
   int of_item;
   dc_chunk_item it = block_item(a, CS, &of_item);
-  if (!chunk_item_ok(it, a) || !block_rows(it, of_item, 256 / CS, a.n_q)) return;
+  if (!chunk_item_ok(it, a) || !block_rows(it, of_item, 256 / CS, a.n_q, !RULE || !a.ranges)) return;
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int col = lane & 31, half = lane >> 5;
   const int hd = WHOLE ? HDP : a.kpool.geometry.head_dim, P = a.kpool.geometry.page_capacity;
@@ -762,6 +769,19 @@ __global__ void __launch_bounds__(512, 2) attend_chunk16_kernel(ChunkArgs a) {
   const int sees = has_row ? it.first + tok : -1;
   const int sees_all = it.first + (it.row_begin + rows_at) / a.n_q;
   const int sees_block = it.first + it.row_begin / a.n_q;
+  RowRule rule;
+  Sight mine, all;  // the wavefront's rows' and the block's
+  int gap_tile = INT32_MAX, gap_len = 0;
+  if constexpr (RULE) {
+    rule = row_rule(a, it, has_row, tok, head);
+    mine = sight_of(a, it, it.row_begin + rows_at, min(it.row_begin + rows_at + 32, it.row_end));
+    all = sight_of(a, it, it.row_begin, it.row_end);
+    const int2 gap = item_gap(a, block_index(CS));
+    if (gap.x >= 0) gap_tile = (gap.x - it.kv_begin) / KT, gap_len = gap.y - gap.x;
+  }
+  auto seen = [&](int u) { return RULE ? rule.sees(u) : u <= sees; };
+  // tokens from the item's first to a tile's
+  auto offset = [&](int tile) { return tile * KT + (RULE && tile >= gap_tile ? gap_len : 0); };
 
   // ---- the tiles' way from the pages to LDS
   const int tw = wave % TW, pg = wave / TW;
@@ -769,11 +789,11 @@ __global__ void __launch_bounds__(512, 2) attend_chunk16_kernel(ChunkArgs a) {
   const int lt = UNI ? lane % NT : 0;                           // token within the wavefront's, where they share a page
   const int u_first = it.kv_begin + (UNI ? tw * NT : ut);     // first token of this wavefront's (thread's) of tile 0
   const int64_t table = (int64_t(it.seq) * a.n_kv_heads + it.kv_head) * a.table_stride;
-  const int tiles = (it.kv_end - it.kv_begin + KT - 1) / KT;
+  const int tiles = (it.kv_end - it.kv_begin - gap_len + KT - 1) / KT;
   const bool has = uc < hd;
   const Side ks = make_side(a.kpool, a.k_table + table, lt, uc), vs = make_side(a.vpool, a.v_table + table, lt, uc);
   auto uni = [](int x) { return UNI ? __builtin_amdgcn_readfirstlane(x) : x; };
-  auto page_of = [&](int tile) { return uint32_t((uint64_t(uint32_t(u_first + tile * KT)) * a.page_mul) >> a.page_shift); };
+  auto page_of = [&](int tile) { return uint32_t((uint64_t(uint32_t(u_first + offset(tile))) * a.page_mul) >> a.page_shift); };
   // (a zero in a vector register: ids and descriptors are then read by vector
   // loads, which come back in order; a scalar load in flight would make the next
   // wait for LDS wait for all of LDS and for it)
@@ -791,7 +811,7 @@ __global__ void __launch_bounds__(512, 2) attend_chunk16_kernel(ChunkArgs a) {
   Raw even, odds;  // (of even and of odd tiles)
   auto load_ids = [&](int tile) __attribute__((always_inline)) {
     const uint32_t page = page_of(tile);
-    const bool in = u_first + tile * KT < it.kv_end && page < uint32_t(a.table_stride);
+    const bool in = u_first + offset(tile) < it.kv_end && page < uint32_t(a.table_stride);
     kid = ks.table[(in ? int(page) : 0) + v0];
     vid = vs.table[(in ? int(page) : 0) + v0];
     named = in;
@@ -807,7 +827,7 @@ __global__ void __launch_bounds__(512, 2) attend_chunk16_kernel(ChunkArgs a) {
   // ids of the next ones: those first, since loads come back in order and
   // waiting for them would wait for units issued ahead of them too.
   auto load_units = [&](int tile, Raw& raw) __attribute__((always_inline)) {
-    const int u = u_first + tile * KT, slot = u - int(page_of(tile)) * P;
+    const int u = u_first + offset(tile), slot = u - int(page_of(tile)) * P;
     const auto k = __builtin_bit_cast(dc_page_desc, uint2{uint32_t(uni(kd.x)), uint32_t(uni(kd.y))});
     const auto v = __builtin_bit_cast(dc_page_desc, uint2{uint32_t(uni(vd.x)), uint32_t(uni(vd.y))});
     raw.k_kind = unit_kind(ks, k, P, slot);
@@ -827,7 +847,7 @@ __global__ void __launch_bounds__(512, 2) attend_chunk16_kernel(ChunkArgs a) {
   const int w_at[2] = {lds_at<CH>(ut, uc / 8), lds_at<CH>(ut, uc / 8 + 1)};  // of the unit's chunks in a tile
   auto write_tile = [&](int tile, const Raw& raw) __attribute__((always_inline)) {
     const int buf = tile & 1;
-    const bool zero = !(raw.counts && has), border = it.kv_begin + (tile + 1) * KT - 1 > sees_block;  // (border: uniform)
+    const bool zero = !(raw.counts && has), border = RULE ? !all.whole(it.kv_begin + offset(tile), KT) : it.kv_begin + (tile + 1) * KT - 1 > sees_block;  // (border: uniform)
     uint32_t y[8];
     auto put = [&](uint8_t* to) __attribute__((always_inline)) {
 #pragma unroll
@@ -887,8 +907,8 @@ __global__ void __launch_bounds__(512, 2) attend_chunk16_kernel(ChunkArgs a) {
     }
     const uint8_t* const kt = lds + (i & 1) * TILE;
     const uint8_t* const vt = lds + (2 + (i & 1)) * TILE;
-    const int u0 = it.kv_begin + i * KT;
-    if (u0 + KT - 1 > sees_block) {
+    const int u0 = it.kv_begin + offset(i);
+    if (RULE ? !all.whole(u0, KT) : u0 + KT - 1 > sees_block) {
       const uint32_t* const bad = reinterpret_cast<const uint32_t*>(poison[i & 1][0]);
 #pragma unroll 1
       for (int tb = 0; tb < TB; ++tb)
@@ -908,11 +928,11 @@ __global__ void __launch_bounds__(512, 2) attend_chunk16_kernel(ChunkArgs a) {
 #pragma unroll
             for (int v = 0; v < 16; ++v) {
               const float x = odd[32 * (cb0 + j) + 8 * (v / 4) + kPerm[4 * half + v % 4]];
-              if (u <= sees && !__builtin_isfinite(x)) o[j][v] += x;
+              if (seen(u) && !__builtin_isfinite(x)) o[j][v] += x;
             }
         }
     }
-    if (wave_rows) {
+    if (wave_rows && (!RULE || mine.some(u0, KT))) {
       const uint32_t* const on = reinterpret_cast<const uint32_t*>(live[i & 1]);
       f32x16 s[TB];
 #pragma unroll
@@ -931,7 +951,8 @@ __global__ void __launch_bounds__(512, 2) attend_chunk16_kernel(ChunkArgs a) {
         s[n % TB] = __builtin_amdgcn_mfma_f32_32x32x16_f16(ka[n % kAhead], q[n / TB], s[n % TB], 0, 0, 0);
         if (n + kAhead < QW * TB) ka[n % kAhead] = key(n + kAhead);
       }
-      bool masked = u0 + KT - 1 > sees_all;
+      if constexpr (RULE) shape_scores(a, c, rule, u0 + 4 * half, s);
+      bool masked = RULE ? !mine.whole(u0, KT) : u0 + KT - 1 > sees_all;
 #pragma unroll
       for (int tb = 0; tb < TB; ++tb) masked = masked || on[tb] != ~0u;
       if (masked) {
@@ -941,7 +962,7 @@ __global__ void __launch_bounds__(512, 2) attend_chunk16_kernel(ChunkArgs a) {
 #pragma unroll
           for (int v = 0; v < 16; ++v) {
             const int t = 8 * (v / 4) + v % 4;
-            s[tb][v] = ((bits >> t) & 1) && u0 + 32 * tb + t + 4 * half <= sees ? s[tb][v] : -INFINITY;
+            s[tb][v] = ((bits >> t) & 1) && seen(u0 + 32 * tb + t + 4 * half) ? s[tb][v] : -INFINITY;
           }
         }
       }
@@ -950,7 +971,7 @@ __global__ void __launch_bounds__(512, 2) attend_chunk16_kernel(ChunkArgs a) {
       for (int tb = 0; tb < TB; ++tb)
 #pragma unroll
         for (int v = 0; v < 16; ++v) top = fmaxf(top, s[tb][v]);
-      top = half_max(top) * c;
+      top = half_max(top) * (RULE ? 1.f : c);
       if (__any(top > m + kLazy || (m == -INFINITY && top > m))) {
         const float mn = fmaxf(m, top);
         const float f = m == -INFINITY ? 1.f : __builtin_amdgcn_exp2f(m - mn);
@@ -965,7 +986,7 @@ __global__ void __launch_bounds__(512, 2) attend_chunk16_kernel(ChunkArgs a) {
 #pragma unroll
       for (int tb = 0; tb < TB; ++tb)
 #pragma unroll
-        for (int v = 0; v < 16; ++v) s[tb][v] = __builtin_amdgcn_exp2f(fmaf(s[tb][v], c, -mu));
+        for (int v = 0; v < 16; ++v) s[tb][v] = __builtin_amdgcn_exp2f(RULE ? s[tb][v] - mu : fmaf(s[tb][v], c, -mu));
       const int v_at = fresh(lds_at<CH>(4 * half + ((lane & 15) >> 2), 4 * cb0 + ((lane & 16) >> 3) + ((lane & 3) >> 1)) + 8 * (lane & 1));
       auto value = [&](int n) {
         // token 16 (n / CB) + 4 half + lane % 16 / 4 (+ 8), channel 32 (cb0 + n % CB) + lane / 16 % 2 * 16 + 4 (lane % 4):
@@ -1105,7 +1126,7 @@ __device__ __forceinline__ uint32_t zero_of(int kind, bool affine) {
 // values' operand is read.
 // KW: words of a key operand that are read ahead (4: also fp16 rows; 2: codes
 // only, and fp16 rows when they are needed).  UNI: a tile's tokens lie in one page.
-template <int HDP, int NB, int KW, bool UNI, bool WHOLE>
+template <int HDP, int NB, int KW, bool UNI, bool WHOLE, bool RULE>
 __global__ void __launch_bounds__(64 * kFewWaves, 2) attend_few_kernel(ChunkArgs a) {
   constexpr int CH = HDP / 8, KS = HDP / 32, CB = HDP / 16, TILE = kFewTile * HDP * 2;
   constexpr int VC = HDP / 2, VU = VC / 32;  // a lane's value channels, in units of 32
@@ -1124,6 +1145,14 @@ __global__ void __launch_bounds__(64 * kFewWaves, 2) attend_few_kernel(ChunkArgs
   const int rows = it.row_end - it.row_begin;
 
   int sees[NB];
+  RowRule rule[NB];
+  Sight all;
+  int gap_tile = INT32_MAX, gap_len = 0;
+  if constexpr (RULE) {
+    all = sight_of(a, it, it.row_begin, it.row_end);
+    const int2 gap = item_gap(a, blockIdx.x);
+    if (gap.x >= 0) gap_tile = (gap.x - it.kv_begin) / kFewTile, gap_len = gap.y - gap.x;
+  }
   h8v q[QL ? 1 : NB][QL ? 1 : KS];
   uint8_t* const ql = lds + kFewWaves * TILE;
 #pragma unroll
@@ -1131,6 +1160,7 @@ __global__ void __launch_bounds__(64 * kFewWaves, 2) attend_few_kernel(ChunkArgs
     const int row = it.row_begin + 16 * n + col;
     const bool has_row = row < it.row_end;
     sees[n] = has_row ? it.first + row / a.n_q : -1;
+    if constexpr (RULE) rule[n] = row_rule(a, it, has_row, row / a.n_q, it.kv_head * a.n_q + row % a.n_q);
     const int rr = has_row ? row : it.row_begin, rt = rr / a.n_q;  // (rows that do not exist: the first one's, as zeros)
     const uint16_t* p = reinterpret_cast<const uint16_t*>(a.q) + int64_t(it.q_begin + rt) * a.q_token_stride +
                         int64_t(it.kv_head * a.n_q + rr - rt * a.n_q) * a.q_head_stride;
@@ -1153,6 +1183,9 @@ __global__ void __launch_bounds__(64 * kFewWaves, 2) attend_few_kernel(ChunkArgs
     else
       return q[n][k];
   };
+  auto seen = [&](int n, int u) { return RULE ? rule[n].sees(u) : u <= sees[n]; };
+  // tokens from the item's first to a tile's
+  auto offset = [&](int tile) { return tile * kFewTile + (RULE && tile >= gap_tile ? gap_len : 0); };
   const int sees_first = it.first + it.row_begin / a.n_q;  // the least of the rows'
 
   // ---- the pages: keys of token 16 b + col, channels 32 k + 8 g .. + 7; values of
@@ -1164,7 +1197,7 @@ __global__ void __launch_bounds__(64 * kFewWaves, 2) attend_few_kernel(ChunkArgs
   const uint32_t k_plane = a.kpool.geometry.layout == 0 ? P * kgs / 2 : kgs / 2;  // from a group's codes to the next one's
   const uint32_t v_plane = a.vpool.geometry.layout == 0 ? P * vgs / 2 : vgs / 2;
   auto uni = [](int x) { return UNI ? __builtin_amdgcn_readfirstlane(x) : x; };
-  auto token = [&](int tile, int b) { return it.kv_begin + tile * kFewTile + (UNI ? 0 : 16 * b + col); };
+  auto token = [&](int tile, int b) { return it.kv_begin + offset(tile) + (UNI ? 0 : 16 * b + col); };
   auto page_of = [&](int u) { return uint32_t((uint64_t(uint32_t(u)) * a.page_mul) >> a.page_shift); };
   // (a zero in a vector register: ids and descriptors are then read by vector
   // loads, which come back in order; a scalar load in flight would make the next
@@ -1294,7 +1327,7 @@ __global__ void __launch_bounds__(64 * kFewWaves, 2) attend_few_kernel(ChunkArgs
     }
   };
 
-  const int all = (it.kv_end - it.kv_begin + kFewTile - 1) / kFewTile;
+  const int tiles = (it.kv_end - it.kv_begin - gap_len + kFewTile - 1) / kFewTile;
   uint8_t* const vt = lds + wave * TILE;
   const float c = a.scale * kLog2e;
   float m[NB], l[NB];
@@ -1314,9 +1347,9 @@ __global__ void __launch_bounds__(64 * kFewWaves, 2) attend_few_kernel(ChunkArgs
   load_ids(wave + kFewWaves);
   load_descs();
   load_ids(wave + 2 * kFewWaves);
-  for (int i = wave; i < all; i += kFewWaves) {
-    const int u0 = it.kv_begin + i * kFewTile;
-    const bool border = u0 + kFewTile - 1 > sees_first;  // (uniform)
+  for (int i = wave; i < tiles; i += kFewWaves) {
+    const int u0 = it.kv_begin + offset(i);
+    const bool border = RULE ? !all.whole(u0, kFewTile) : u0 + kFewTile - 1 > sees_first;  // (uniform)
     const uint32_t live = on;
     // ---- values to LDS
     uint32_t bad = 0;
@@ -1421,18 +1454,19 @@ __global__ void __launch_bounds__(64 * kFewWaves, 2) attend_few_kernel(ChunkArgs
     h8v p[NB];
 #pragma unroll
     for (int n = 0; n < NB; ++n) {
+      if constexpr (RULE) shape_scores(a, c, rule[n], u0 + 4 * g, s[n]);
       if (border || live != ~0u) {
 #pragma unroll
         for (int b = 0; b < 2; ++b)
 #pragma unroll
           for (int v = 0; v < 4; ++v) {
             const int t = 16 * b + 4 * g + v;
-            s[n][b][v] = ((live >> t) & 1) && u0 + t <= sees[n] ? s[n][b][v] : -INFINITY;
+            s[n][b][v] = ((live >> t) & 1) && seen(n, u0 + t) ? s[n][b][v] : -INFINITY;
           }
       }
       float top = fmaxf(fmaxf(fmaxf(s[n][0][0], s[n][0][1]), fmaxf(s[n][0][2], s[n][0][3])),
                         fmaxf(fmaxf(s[n][1][0], s[n][1][1]), fmaxf(s[n][1][2], s[n][1][3])));
-      top = quarter_max(top) * c;
+      top = quarter_max(top) * (RULE ? 1.f : c);
       if (__any(top > m[n] + kLazy || (m[n] == -INFINITY && top > m[n]))) {
         const float mn = fmaxf(m[n], top);
         const float f = m[n] == -INFINITY ? 1.f : __builtin_amdgcn_exp2f(m[n] - mn);
@@ -1444,8 +1478,8 @@ __global__ void __launch_bounds__(64 * kFewWaves, 2) attend_few_kernel(ChunkArgs
       const float mu = (m[n] == -INFINITY ? 0.f : m[n]) - kLift;
 #pragma unroll
       for (int v = 0; v < 8; v += 2) {
-        const h2v e = {(_Float16)__builtin_amdgcn_exp2f(fmaf(s[n][v / 4][v % 4], c, -mu)),
-                       (_Float16)__builtin_amdgcn_exp2f(fmaf(s[n][v / 4][v % 4 + 1], c, -mu))};
+        const h2v e = {(_Float16)__builtin_amdgcn_exp2f(RULE ? s[n][v / 4][v % 4] - mu : fmaf(s[n][v / 4][v % 4], c, -mu)),
+                       (_Float16)__builtin_amdgcn_exp2f(RULE ? s[n][v / 4][v % 4 + 1] - mu : fmaf(s[n][v / 4][v % 4 + 1], c, -mu))};
         l[n] = __builtin_amdgcn_fdot2(e, h2v{(_Float16)1.f, (_Float16)1.f}, l[n], false);
         p[n][v] = e[0];
         p[n][v + 1] = e[1];
@@ -1468,7 +1502,7 @@ __global__ void __launch_bounds__(64 * kFewWaves, 2) attend_few_kernel(ChunkArgs
             const float x = odd[wave][16 * j + 8 * (g / 2) + kPerm[4 * (g % 2) + v]];
 #pragma unroll
             for (int n = 0; n < NB; ++n)
-              if (u <= sees[n] && !__builtin_isfinite(x)) o[n][j][v] += x;
+              if (seen(n, u) && !__builtin_isfinite(x)) o[n][j][v] += x;
           }
         __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
       }
@@ -1585,58 +1619,56 @@ static int launch_chunk(const ChunkArgs& a, hipStream_t stream) {
   return check_hip(hipGetLastError(), "attend_chunk_kernel launch");
 }
 
-template <int HDP, int KT, bool UNI, int CS, bool WHOLE>
+template <int HDP, int KT, bool UNI, int CS, bool WHOLE, bool RULE>
 static int launch_chunk16_as(const ChunkArgs& a, hipStream_t stream) {
   constexpr int bytes = 4 * KT * HDP * 2;
   static LdsLimit limit;
-  if (int rc = limit.raise(reinterpret_cast<const void*>(&attend_chunk16_kernel<HDP, KT, UNI, CS, WHOLE>), bytes, "attend_chunk16_kernel LDS")) return rc;
-  hipLaunchKernelGGL((attend_chunk16_kernel<HDP, KT, UNI, CS, WHOLE>), item_grid(a.n_items, CS), dim3(512), bytes, stream, a);
+  if (int rc = limit.raise(reinterpret_cast<const void*>(&attend_chunk16_kernel<HDP, KT, UNI, CS, WHOLE, RULE>), bytes, "attend_chunk16_kernel LDS")) return rc;
+  hipLaunchKernelGGL((attend_chunk16_kernel<HDP, KT, UNI, CS, WHOLE, RULE>), item_grid(a.n_items, CS), dim3(512), bytes, stream, a);
   return check_hip(hipGetLastError(), "attend_chunk16_kernel launch");
 }
 
-template <int HDP, int KT, int CS>
+template <int HDP, int KT, int CS, bool RULE>
 static int launch_chunk16(const ChunkArgs& a, hipStream_t stream) {
-  if (a.kpool.geometry.page_capacity % (KT < 64 ? 8 : KT / 8) != 0) return launch_chunk16_as<HDP, KT, false, CS, false>(a, stream);
-  return a.kpool.geometry.head_dim == HDP ? launch_chunk16_as<HDP, KT, true, CS, true>(a, stream)
-                                          : launch_chunk16_as<HDP, KT, true, CS, false>(a, stream);
+  if (a.kpool.geometry.page_capacity % (KT < 64 ? 8 : KT / 8) != 0) return launch_chunk16_as<HDP, KT, false, CS, false, RULE>(a, stream);
+  return a.kpool.geometry.head_dim == HDP ? launch_chunk16_as<HDP, KT, true, CS, true, RULE>(a, stream)
+                                          : launch_chunk16_as<HDP, KT, true, CS, false, RULE>(a, stream);
 }
 
-template <int HDP, int NB, int KW, bool UNI, bool WHOLE>
+template <int HDP, int NB, int KW, bool UNI, bool WHOLE, bool RULE>
 static int launch_few_as(const ChunkArgs& a, hipStream_t stream) {
   constexpr int tiles = kFewWaves * kFewTile * HDP * 2 + (NB * HDP >= 256 ? 16 * NB * HDP * 2 : 0), joined = 16 * NB * (HDP + 4) * 4, bytes = tiles > joined ? tiles : joined;
   static LdsLimit limit;
-  if (int rc = limit.raise(reinterpret_cast<const void*>(&attend_few_kernel<HDP, NB, KW, UNI, WHOLE>), bytes, "attend_few_kernel LDS")) return rc;
-  hipLaunchKernelGGL((attend_few_kernel<HDP, NB, KW, UNI, WHOLE>), dim3(a.n_items), dim3(64 * kFewWaves), bytes, stream, a);
+  if (int rc = limit.raise(reinterpret_cast<const void*>(&attend_few_kernel<HDP, NB, KW, UNI, WHOLE, RULE>), bytes, "attend_few_kernel LDS")) return rc;
+  hipLaunchKernelGGL((attend_few_kernel<HDP, NB, KW, UNI, WHOLE, RULE>), dim3(a.n_items), dim3(64 * kFewWaves), bytes, stream, a);
   return check_hip(hipGetLastError(), "attend_few_kernel launch");
 }
 
-template <int HDP, int NB, int KW>
+template <int HDP, int NB, int KW, bool RULE>
 static int launch_few(const ChunkArgs& a, hipStream_t stream) {
-  if (a.kpool.geometry.page_capacity % kFewTile != 0) return launch_few_as<HDP, NB, KW, false, false>(a, stream);
-  return a.kpool.geometry.head_dim == HDP ? launch_few_as<HDP, NB, KW, true, true>(a, stream)
-                                          : launch_few_as<HDP, NB, KW, true, false>(a, stream);
+  if (a.kpool.geometry.page_capacity % kFewTile != 0) return launch_few_as<HDP, NB, KW, false, false, RULE>(a, stream);
+  return a.kpool.geometry.head_dim == HDP ? launch_few_as<HDP, NB, KW, true, true, RULE>(a, stream)
+                                          : launch_few_as<HDP, NB, KW, true, false, RULE>(a, stream);
 }
 
 template <bool RULE>
 static int launch_all(ChunkArgs a, int32_t n_few, int32_t few_rows, bool units, hipStream_t st) {
   const int hd = a.kpool.geometry.head_dim;
-  if constexpr (RULE) units = false;
-  if constexpr (!RULE) {
-    if (units && n_few) {
-      ChunkArgs f = a;
-      f.n_items = n_few;
-      const bool one = few_rows <= 16;
-      const int rc = hd <= 64    ? (one ? launch_few<64, 1, 4>(f, st) : launch_few<64, 4, 4>(f, st))
-                     : hd <= 128 ? (one ? launch_few<128, 1, 4>(f, st) : few_rows <= 32 ? launch_few<128, 2, 4>(f, st) : launch_few<128, 3, 2>(f, st))
-                                 : launch_few<256, 1, 2>(f, st);
-      if (rc != DC_OK) return rc;
-      a.items += n_few;
-      a.n_items -= n_few;
-    }
-    if (a.n_items == 0) return DC_OK;
-    if (units)
-      return hd <= 64 ? launch_chunk16<64, 128, 1>(a, st) : hd <= 128 ? launch_chunk16<128, 64, 1>(a, st) : launch_chunk16<256, 32, 2>(a, st);
+  if (units && n_few) {
+    ChunkArgs f = a;
+    f.n_items = n_few;
+    const bool one = few_rows <= 16;
+    const int rc = hd <= 64    ? (one ? launch_few<64, 1, 4, RULE>(f, st) : launch_few<64, 4, 4, RULE>(f, st))
+                   : hd <= 128 ? (one ? launch_few<128, 1, 4, RULE>(f, st) : few_rows <= 32 ? launch_few<128, 2, 4, RULE>(f, st) : launch_few<128, 3, 2, RULE>(f, st))
+                               : launch_few<256, 1, 2, RULE>(f, st);
+    if (rc != DC_OK) return rc;
+    a.items += n_few;
+    if (RULE && a.gaps) a.gaps += n_few;
+    a.n_items -= n_few;
   }
+  if (a.n_items == 0) return DC_OK;
+  if (units)
+    return hd <= 64 ? launch_chunk16<64, 128, 1, RULE>(a, st) : hd <= 128 ? launch_chunk16<128, 64, 1, RULE>(a, st) : launch_chunk16<256, 32, 2, RULE>(a, st);
   if (a.dtype == DC_F32)
     return hd <= 64 ? launch_chunk<float, 64, 64, RULE>(a, st) : hd <= 128 ? launch_chunk<float, 128, 32, RULE>(a, st) : launch_chunk<float, 256, 32, RULE>(a, st);
   return hd <= 64 ? launch_chunk<_Float16, 64, 128, RULE>(a, st) : hd <= 128 ? launch_chunk<_Float16, 128, 64, RULE>(a, st) : launch_chunk<_Float16, 256, 32, RULE>(a, st);
