@@ -72,6 +72,14 @@ class TokenDest(C.Structure):
                 ("n_rows", C.c_int32), ("n_pages", C.c_int32), ("page_tokens", C.c_int32)]
 
 
+class GroupedWeight(C.Structure):
+    _fields_ = [("data", C.c_void_p), ("outputs", C.c_int32), ("inputs", C.c_int32), ("group_size", C.c_int32), ("affine", C.c_int32)]
+
+
+class MatrixRows(C.Structure):
+    _fields_ = [("data", C.c_void_p), ("stride", C.c_int64), ("dtype", C.c_int32)]
+
+
 class ScoreRule(C.Structure):
     _fields_ = [("cap", C.c_float), ("slopes", C.c_void_p), ("ranges", C.c_void_p), ("gaps", C.c_void_p)]
 
@@ -117,6 +125,8 @@ SIGNATURES = {
     "dc_attend_chunk_rule": (C.c_int, [Pool, Pool, C.c_void_p, C.c_void_p, C.c_int32, C.c_void_p, C.c_int32, C.c_int32,
                                        C.c_int32, C.c_void_p, C.c_int32, C.c_int32, C.c_int32, C.c_int32, C.c_int64,
                                        TokenRows, C.c_float, ScoreRule, TokenRows, C.c_void_p, C.c_int64, C.c_void_p]),
+    "dc_grouped_weight_bytes": (C.c_int64, [C.c_int32, C.c_int32, C.c_int32, C.c_int32, C.POINTER(C.c_int64)]),
+    "dc_project": (C.c_int, [GroupedWeight, MatrixRows, MatrixRows, C.c_int64, C.c_void_p]),
     "dc_set_encode_path": (C.c_int, [C.c_int32]),
     "dc_score_pages": (C.c_int, [Pool, C.c_void_p, C.c_void_p, C.c_int32, C.c_void_p, C.c_int32, C.c_void_p, C.c_int64, C.c_void_p]),
     "dc_mix_pages": (C.c_int, [Pool, C.c_void_p, C.c_void_p, C.c_int32, C.c_void_p, C.c_int32, C.c_int64, C.c_void_p, C.c_int32, C.c_void_p]),

@@ -656,6 +656,46 @@ int dc_attend_chunk_rule(dc_pool k_pool, dc_pool v_pool, const int32_t* k_table,
                          int32_t n_kv_heads, int64_t n_tokens, dc_token_rows q, float query_scale, dc_score_rule rule,
                          dc_token_rows out, void* workspace, int64_t workspace_bytes, dc_stream_t stream);
 
+/* ---- products with grouped 4-bit weights ------------------------------- */
+
+/* A weight matrix W [outputs][inputs] of 4-bit codes with a scale (fp16) for
+ * every group of 32, 64 or 128 inputs of an output, and with affine a bias:
+ * W = scale * code + bias, or scale * (code - 7), the page formats' levels.
+ * data (device, 16-byte aligned, dc_grouped_weight_bytes): tiles of 16 outputs x
+ * 128 inputs, [ceil(outputs / 16)][ceil(inputs / 128)], codes and scales of
+ * outputs and inputs past the matrix 0.
+ *   codes  : 64 x 16 bytes a tile; the 16 bytes at l hold output l % 16, word w of
+ *            them inputs 32 w + 8 (l / 16) .. + 7, input j of these eight in
+ *            bits 4 (j / 2 + 4 (j % 2)) ..
+ *   scales : behind the codes of all tiles, for a tile [16][128 / group_size] fp16
+ *            scales, or {scale, bias} pairs */
+typedef struct dc_grouped_weight {
+  const void* data;
+  int32_t outputs;
+  int32_t inputs;
+  int32_t group_size;
+  int32_t affine;
+} dc_grouped_weight;
+
+/* Rows of one dtype at any element stride, their elements contiguous. */
+typedef struct dc_matrix_rows {
+  void* data; /* device */
+  int64_t stride;
+  int32_t dtype;
+} dc_matrix_rows;
+
+/* Bytes of a weight's data and (scales_offset, may be NULL) where its scales
+ * begin; -1 for sizes that none has.  Host only. */
+int64_t dc_grouped_weight_bytes(int32_t outputs, int32_t inputs, int32_t group_size, int32_t affine, int64_t* scales_offset);
+
+/* y[m] = x[m] W^T for `rows` rows x [inputs] and y [outputs] of one dtype
+ * (DC_F32, DC_F16, DC_BF16), sums in fp32, one rounding to y.  y must not
+ * overlap x.  An infinity or NaN among a row's inputs gives infinities or NaN in all
+ * of that row's outputs, and only there.  A weight's levels are those of reference
+ * dotcache/modes/m0_affine.py:15-90; the reference leaves the products around
+ * the cache to its models (dotcache/integrations/llama.py:345-358, :476-481). */
+int dc_project(dc_grouped_weight weight, dc_matrix_rows x, dc_matrix_rows y, int64_t rows, dc_stream_t stream);
+
 /* Process-wide decode kernel choice: 0 (default) runs the MFMA kernel when
  * every page format (M3 fp16 keys and values, M0 4- or 8-bit keys of group
  * 32, M0 4- or 8-bit values of group 32 or 64), head_dim (64/128/256) and
