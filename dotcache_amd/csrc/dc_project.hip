@@ -9,6 +9,8 @@
 // numbers, exactly, with fp32 sums; scales and offsets act on the groups' sums
 // in fp32.  Nothing is rounded before the output.  fp32 rows are three bf16
 // parts each, whose sum they are.
+#include <type_traits>
+
 #include "dc_common.h"
 
 namespace dc {
@@ -56,44 +58,67 @@ __device__ __forceinline__ f32x4 mfma(uint4 a, uint4 b, f32x4 c) {
     return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(b8v, a), __builtin_bit_cast(b8v, b), c, 0, 0, 0);
 }
 
-// Inputs k .. k + 7 of a row as operands (fp32: three parts), zeros past the
-// row's end and for rows that do not exist.
-template <int DT, int PARTS>
-__device__ __forceinline__ void load_x(const ProjectArgs& a, const void* row, bool has, int k, uint4 (&out)[PARTS]) {
-  if constexpr (DT != DC_F32) {
-    const uint16_t* p = static_cast<const uint16_t*>(row);
-    uint32_t w[4];
-    if (a.x_vec) {
-      const uint4 v = *reinterpret_cast<const uint4*>(p + (has && k < a.k ? k : 0));
-      w[0] = v.x; w[1] = v.y; w[2] = v.z; w[3] = v.w;
+// Inputs k .. k + 7 of a row as they lie in memory.  Past the row's end: its
+// first ones (whoever uses them leaves them out).
+template <int DT>
+struct Eight {
+  static constexpr int W = DT == DC_F32 ? 8 : 4;
+  uint32_t w[W];
+};
+template <int DT>
+__device__ __forceinline__ void load_x(const ProjectArgs& a, const void* row, int k, Eight<DT>& x) {
+  typedef std::conditional_t<DT == DC_F32, uint32_t, uint16_t> T;
+  const T* p = static_cast<const T*>(row);
+  if (a.x_vec) {
+    const uint4* v = reinterpret_cast<const uint4*>(p + (k < a.k ? k : 0));
 #pragma unroll
-      for (int i = 0; i < 4; ++i) w[i] = has && k < a.k ? w[i] : 0;
-    } else {
-#pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        const int k0 = k + 2 * i, k1 = k0 + 1;
-        const uint32_t lo = p[k0 < a.k ? k0 : 0], hi = p[k1 < a.k ? k1 : 0];
-        w[i] = (has && k0 < a.k ? lo : 0) | (has && k1 < a.k ? hi << 16 : 0);
-      }
+    for (int i = 0; i < Eight<DT>::W / 4; ++i) {
+      const uint4 y = v[i];
+      x.w[4 * i] = y.x; x.w[4 * i + 1] = y.y; x.w[4 * i + 2] = y.z; x.w[4 * i + 3] = y.w;
     }
-    out[0] = uint4{w[0], w[1], w[2], w[3]};
   } else {
-    const float* p = static_cast<const float*>(row);
-    uint32_t w[3][4];
 #pragma unroll
     for (int i = 0; i < 8; ++i) {
-      float v = p[k + i < a.k ? k + i : 0];
-      v = has && k + i < a.k ? v : 0.f;
-#pragma unroll
-      for (int j = 0; j < 3; ++j) {
-        const uint32_t top = __builtin_bit_cast(uint32_t, v) & 0xffff0000u;  // exact: the next part has what is left
-        v -= __builtin_bit_cast(float, top);
-        w[j][i / 2] = i % 2 ? w[j][i / 2] | top : top >> 16;
-      }
+      const uint32_t v = p[k + i < a.k ? k + i : 0];
+      if constexpr (DT == DC_F32)
+        x.w[i] = v;
+      else
+        x.w[i / 2] = i % 2 ? x.w[i / 2] | v << 16 : v;
     }
-#pragma unroll
-    for (int j = 0; j < 3; ++j) out[j] = uint4{w[j][0], w[j][1], w[j][2], w[j][3]};
   }
+}
+
+// Those past the row's end as zeros.
+template <int DT>
+__device__ __forceinline__ void cut_x(const ProjectArgs& a, int k, Eight<DT>& x) {
+#pragma unroll
+  for (int i = 0; i < Eight<DT>::W; ++i) {
+    if constexpr (DT == DC_F32)
+      x.w[i] = k + i < a.k ? x.w[i] : 0;
+    else
+      x.w[i] &= (k + 2 * i < a.k ? 0xffffu : 0) | (k + 2 * i + 1 < a.k ? 0xffff0000u : 0);
+  }
+}
+
+// Part `part` of them as a matrix operand (fp32 rows have three bf16 parts: the
+// top 16 bits, those of what is left, and the rest).
+template <int DT>
+__device__ __forceinline__ uint4 x_operand(const Eight<DT>& x, int part) {
+  if constexpr (DT != DC_F32) return uint4{x.w[0], x.w[1], x.w[2], x.w[3]};
+  uint32_t out[4];
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    uint32_t top[2];
+#pragma unroll
+    for (int e = 0; e < 2; ++e) {
+      float v = __builtin_bit_cast(float, x.w[(2 * i + e) % Eight<DT>::W]);
+#pragma unroll
+      for (int j = 0; j < part; ++j) v -= __builtin_bit_cast(float, __builtin_bit_cast(uint32_t, v) & 0xffff0000u);  // exact
+      top[e] = __builtin_bit_cast(uint32_t, v);
+    }
+    out[i] = __builtin_amdgcn_perm(top[1], top[0], 0x07060302u);
+  }
+  return uint4{out[0], out[1], out[2], out[3]};
 }
 
 template <int DT>
@@ -106,86 +131,272 @@ __device__ __forceinline__ void store_y(void* y, int64_t i, float v) {
     static_cast<__bf16*>(y)[i] = __bf16(v);
 }
 
-constexpr int kWaves = 4;
-
 }  // namespace
 
-// 16 rows by 16 outputs per block; its wavefronts take the inputs' tiles in turn
-// and join in order.
+// Up to 16 rows by 16 outputs per block.  Bound by reading the weights (few
+// bytes: by the time from a launch to its first word), so its wavefronts split
+// the inputs' tiles among them, in turn, with the next tile's words, scales and
+// rows on their way while one is worked on, and join in order at the end.
 template <int DT, int GS, bool AFFINE>
-__global__ void __launch_bounds__(64 * kWaves) project_rows_kernel(ProjectArgs a) {
-  constexpr int PARTS = DT == DC_F32 ? 3 : 1, OT = DT == DC_F32 ? DC_BF16 : DT, NG = kTileK / GS;
+__global__ void __launch_bounds__(1024) project_few_kernel(ProjectArgs a) {
+  constexpr int PARTS = DT == DC_F32 ? 3 : 1, OT = DT == DC_F32 ? DC_BF16 : DT, SC = kTileK / GS * (AFFINE ? 2 : 1);
   constexpr uint32_t kOne = OT == DC_F16 ? 0x3c003c00u : 0x3f803f80u;
-  __shared__ f32x4 part_sums[kWaves][64];
-  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), col = lane & 15, g = lane >> 4;
+  __shared__ f32x4 joined[16][64];
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), waves = blockDim.x >> 6;
+  const int col = lane & 15, g = lane >> 4;
   const int64_t row0 = int64_t(blockIdx.y) * 16;
-  const bool has = row0 + col < a.rows;
-  const void* const row = static_cast<const char*>(a.x) + (has ? row0 + col : row0) * a.x_stride * (DT == DC_F32 ? 4 : 2);
+  // (rows that do not exist repeat the last one: their sums are not stored)
+  const char* const row = static_cast<const char*>(a.x) + (row0 + col < a.rows ? row0 + col : a.rows - 1) * a.x_stride * (DT == DC_F32 ? 4 : 2);
+  const int64_t tile0 = int64_t(blockIdx.x) * a.k_tiles;
+  const uint4* const words = a.words + tile0 * 64 + lane;
+  const uint16_t* const scales = a.scales + (tile0 * 16 + col) * SC;
+  struct Stage {
+    uint4 w;
+    uint16_t s[SC];
+    Eight<DT> x[4];
+  };
+  auto load = [&](int kt, Stage& st) __attribute__((always_inline)) {
+    const int t = min(kt, a.k_tiles - 1);
+    st.w = words[int64_t(t) * 64];
+    __builtin_memcpy(st.s, __builtin_assume_aligned(scales + int64_t(t) * 16 * SC, 2 * SC), 2 * SC);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) load_x<DT>(a, row, t * kTileK + 32 * i + 8 * g, st.x[i]);
+  };
   const uint4 ones{kOne, kOne, kOne, kOne};
   f32x4 acc{0.f, 0.f, 0.f, 0.f};
-  for (int kt = wave; kt < a.k_tiles; kt += kWaves) {
-    const int64_t tile = int64_t(blockIdx.x) * a.k_tiles + kt;
-    const uint4 r = a.words[tile * 64 + lane];
-    const uint32_t w[4] = {r.x, r.y, r.z, r.w};
-    const uint16_t* const sc = a.scales + (tile * 16 + col) * NG * (AFFINE ? 2 : 1);
-    f32x4 sum{0.f, 0.f, 0.f, 0.f}, xs{0.f, 0.f, 0.f, 0.f};
+  auto take = [&](int kt, Stage& st) __attribute__((always_inline)) {
+    if (kt == a.k_tiles - 1 && a.k % kTileK != 0) {  // (uniform)
+#pragma unroll
+      for (int i = 0; i < 4; ++i) cut_x<DT>(a, kt * kTileK + 32 * i + 8 * g, st.x[i]);
+    }
+    f32x4 sum, xs;
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
-      uint4 x[PARTS];
-      load_x<DT, PARTS>(a, row, has, kt * kTileK + 32 * i + 8 * g, x);
-      const uint4 b = operand<OT>(w[i]);
+      if (i * 32 % GS == 0) sum = xs = f32x4{0.f, 0.f, 0.f, 0.f};
+      const uint4 b = operand<OT>((&st.w.x)[i]);
 #pragma unroll
       for (int j = 0; j < PARTS; ++j) {
-        sum = mfma<OT>(x[j], b, sum);
-        xs = mfma<OT>(x[j], ones, xs);
+        const uint4 x = x_operand<DT>(st.x[i], j);
+        xs = mfma<OT>(x, ones, xs);
+        sum = mfma<OT>(x, b, sum);
       }
       if ((i + 1) * 32 % GS) continue;
       const int gr = i * 32 / GS;
-      const float s = half_of(sc[gr * (AFFINE ? 2 : 1)]);
-      const float off = AFFINE ? half_of(sc[gr * 2 + 1]) - 16.f * s : -23.f * s;
+      const float s = half_of(st.s[gr * (AFFINE ? 2 : 1)]);
+      const float off = AFFINE ? half_of(st.s[(2 * gr + 1) % SC]) - 16.f * s : -23.f * s;
 #pragma unroll
-      for (int v = 0; v < 4; ++v) {
-        acc[v] = fmaf(s, sum[v], fmaf(off, xs[v], acc[v]));
-        sum[v] = xs[v] = 0.f;
-      }
+      for (int v = 0; v < 4; ++v) acc[v] = fmaf(s, sum[v], fmaf(off, xs[v], acc[v]));
+    }
+  };
+  Stage even, odd;
+  if (wave < a.k_tiles) {  // (uniform)
+    load(wave, even);
+    for (int kt = wave; kt < a.k_tiles; kt += 2 * waves) {
+      load(kt + waves, odd);
+      take(kt, even);
+      if (kt + waves >= a.k_tiles) break;
+      load(kt + 2 * waves, even);
+      take(kt + waves, odd);
     }
   }
-  part_sums[wave][lane] = acc;
+  joined[wave][lane] = acc;
   __syncthreads();
   if (wave != 0) return;
-#pragma unroll
-  for (int w = 1; w < kWaves; ++w) acc += part_sums[w][lane];
+  for (int w = 1; w < waves; ++w) acc += joined[w][lane];
   const int out = int(blockIdx.x) * kTileN + col;
 #pragma unroll
   for (int v = 0; v < 4; ++v) {
-    const int64_t m = row0 + 4 * g + v;
-    if (m < a.rows && out < a.n) store_y<DT>(a.y, m * a.y_stride + out, acc[v]);
+    const int64_t r = row0 + 4 * g + v;
+    if (r < a.rows && out < a.n) store_y<DT>(a.y, r * a.y_stride + out, acc[v]);
   }
 }
 
-template <int DT, int GS>
-static int launch_project(const ProjectArgs& a, bool affine, hipStream_t stream) {
-  // (16 rows a block: at most 2^16 - 1 of them in a launch's second dimension)
-  for (int64_t r = 0; r < a.rows; r += 16 * 65535) {
-    ProjectArgs b = a;
-    b.x = static_cast<const char*>(a.x) + r * a.x_stride * (DT == DC_F32 ? 4 : 2);
-    b.y = static_cast<char*>(a.y) + r * a.y_stride * (DT == DC_F32 ? 4 : 2);
-    b.rows = a.rows - r < 16 * 65535 ? a.rows - r : 16 * 65535;
-    const dim3 grid(uint32_t(a.n_tiles), uint32_t((b.rows + 15) / 16));
-    if (affine)
-      hipLaunchKernelGGL((project_rows_kernel<DT, GS, true>), grid, dim3(64 * kWaves), 0, stream, b);
+// Sum of a row's eight 16-bit inputs.
+template <int DT>
+__device__ __forceinline__ float sum8(const uint4& x) {
+  float s = 0.f;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const uint32_t w = (&x.x)[i];
+    if constexpr (DT == DC_F16)
+      s += float(__builtin_bit_cast(_Float16, uint16_t(w))) + float(__builtin_bit_cast(_Float16, uint16_t(w >> 16)));
     else
-      hipLaunchKernelGGL((project_rows_kernel<DT, GS, false>), grid, dim3(64 * kWaves), 0, stream, b);
-    if (int rc = check_hip(hipGetLastError(), "project_rows_kernel launch")) return rc;
+      s += __builtin_bit_cast(float, w << 16) + __builtin_bit_cast(float, w & 0xffff0000u);
+  }
+  return s;
+}
+
+// 16 MB rows by 64 outputs per block, 16-bit rows: four wavefronts, a tile of
+// outputs each, on each half of the inputs' tiles.  A half's rows lie in LDS as
+// the matrix operands that all four read, with their groups' sums, two tiles in
+// turn: while one is worked on the next is written from registers, and the one
+// after it is on its way.
+template <int DT, int GS, bool AFFINE, int MB>
+__global__ void __launch_bounds__(512, 2) project_mid_kernel(ProjectArgs a) {
+  constexpr int NG = kTileK / GS, SC = NG * (AFFINE ? 2 : 1);
+  static_assert(MB <= 4, "a wavefront brings one row block");
+  __shared__ uint4 xt[2][2][MB][4][64];    // [half][turn][row block][32 inputs][lane]
+  __shared__ f32x4 xsum[2][2][MB][NG][4];  // sums of the groups' inputs of four rows
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), half = wave >> 2, mine = wave & 3;
+  const int col = lane & 15, g = lane >> 4;
+  const int64_t row0 = int64_t(blockIdx.y) * (16 * MB);
+  const int n_tile = int(blockIdx.x) * 4 + mine;
+  const int64_t r = row0 + 16 * min(mine, MB - 1) + col;  // the row that this lane brings
+  const char* const row = static_cast<const char*>(a.x) + (r < a.rows ? r : a.rows - 1) * a.x_stride * 2;
+  const int64_t tile0 = int64_t(min(n_tile, a.n_tiles - 1)) * a.k_tiles;
+  const uint4* const words = a.words + tile0 * 64 + lane;
+  const uint16_t* const scales = a.scales + (tile0 * 16 + col) * SC;
+  struct Weights {
+    uint4 w;
+    uint16_t s[SC];
+  };
+  Eight<DT> x[4];
+  auto load_rows = [&](int kt) __attribute__((always_inline)) {
+    const int t = min(kt, a.k_tiles - 1);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) load_x<DT>(a, row, t * kTileK + 32 * i + 8 * g, x[i]);
+  };
+  auto load_weights = [&](int kt, Weights& w) __attribute__((always_inline)) {
+    const int t = min(kt, a.k_tiles - 1);
+    w.w = words[int64_t(t) * 64];
+    __builtin_memcpy(w.s, __builtin_assume_aligned(scales + int64_t(t) * 16 * SC, 2 * SC), 2 * SC);
+  };
+  auto write_rows = [&](int kt, int turn) __attribute__((always_inline)) {
+    if (mine >= MB) return;
+    if (kt >= a.k_tiles - 1 && a.k % kTileK != 0) {
+#pragma unroll
+      for (int i = 0; i < 4; ++i) cut_x<DT>(a, kt * kTileK + 32 * i + 8 * g, x[i]);
+    }
+    float s = 0.f;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const uint4 v = x_operand<DT>(x[i], 0);
+      xt[half][turn][mine][i][lane] = v;
+      s = (i * 32 % GS == 0 ? 0.f : s) + sum8<DT>(v);
+      if ((i + 1) * 32 % GS) continue;
+      s += __shfl_xor(s, 16);
+      s += __shfl_xor(s, 32);
+      if (g == 0) reinterpret_cast<float*>(&xsum[half][turn][mine][i * 32 / GS][0])[col] = s;
+    }
+  };
+  f32x4 acc[MB];
+#pragma unroll
+  for (int m = 0; m < MB; ++m) acc[m] = f32x4{0.f, 0.f, 0.f, 0.f};
+  auto take = [&](const Weights& w, int turn) __attribute__((always_inline)) {
+    f32x4 sum[MB];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const uint4 b = operand<DT>((&w.w.x)[i]);
+#pragma unroll
+      for (int m = 0; m < MB; ++m) {
+        if (i * 32 % GS == 0) sum[m] = f32x4{0.f, 0.f, 0.f, 0.f};
+        sum[m] = mfma<DT>(xt[half][turn][m][i][lane], b, sum[m]);
+      }
+      if ((i + 1) * 32 % GS) continue;
+      const int gr = i * 32 / GS;
+      const float s = half_of(w.s[gr * (AFFINE ? 2 : 1)]);
+      const float off = AFFINE ? half_of(w.s[(2 * gr + 1) % SC]) - 16.f * s : -23.f * s;
+#pragma unroll
+      for (int m = 0; m < MB; ++m) {
+        const f32x4 xs = xsum[half][turn][m][gr][g];
+#pragma unroll
+        for (int v = 0; v < 4; ++v) acc[m][v] = fmaf(s, sum[m][v], fmaf(off, xs[v], acc[m][v]));
+      }
+    }
+  };
+  // half h takes tiles h, h + 2, ...; both run as many turns (the second's last
+  // may be past the end: rows of the last tile, and no sums taken)
+  Weights even, odd;
+  load_rows(half);
+  load_weights(half, even);
+  write_rows(half, 0);
+  load_rows(half + 2);
+  const int turns = (a.k_tiles + 1) / 2;
+  __syncthreads();
+  auto step = [&](int t, const Weights& now, Weights& next) __attribute__((always_inline)) {
+    const int kt = 2 * t + half;
+    load_weights(kt + 2, next);
+    if (t + 1 < turns) {
+      write_rows(kt + 2, (t + 1) & 1);
+      load_rows(kt + 4);
+    }
+    if (kt < a.k_tiles) take(now, t & 1);
+    __syncthreads();
+  };
+  for (int t = 0; t < turns; t += 2) {
+    step(t, even, odd);
+    if (t + 1 < turns) step(t + 1, odd, even);
+  }
+  f32x4* const joined = reinterpret_cast<f32x4*>(xt);  // [4][MB][64]
+  if (half == 1) {
+#pragma unroll
+    for (int m = 0; m < MB; ++m) joined[(mine * MB + m) * 64 + lane] = acc[m];
+  }
+  __syncthreads();
+  if (half == 1) return;
+  const int out = n_tile * kTileN + col;
+#pragma unroll
+  for (int m = 0; m < MB; ++m) {
+    const f32x4 y = acc[m] + joined[(mine * MB + m) * 64 + lane];
+#pragma unroll
+    for (int v = 0; v < 4; ++v) {
+      const int64_t at = row0 + 16 * m + 4 * g + v;
+      if (at < a.rows && out < a.n) store_y<DT>(a.y, at * a.y_stride + out, y[v]);
+    }
+  }
+}
+
+// Wavefronts per block: where blocks alone leave the card's 1024 SIMDs
+// less than four wavefronts each, up to 16, but none without a tile.
+static int waves_of(int64_t blocks, int k_tiles) {
+  int w = 4;
+  while (w < 16 && blocks * w < 4096 && 2 * w <= k_tiles) w *= 2;
+  return w;
+}
+
+// launch(args, grid) for portions of the rows: a launch's second dimension holds
+// 2^16 - 1 blocks of `rows` rows.
+template <typename F>
+static int by_rows(const ProjectArgs& a, int item, int outputs, int rows, const char* what, F launch) {
+  const int64_t most = int64_t(rows) * 65535;
+  for (int64_t r = 0; r < a.rows; r += most) {
+    ProjectArgs b = a;
+    b.x = static_cast<const char*>(a.x) + r * a.x_stride * item;
+    b.y = static_cast<char*>(a.y) + r * a.y_stride * item;
+    b.rows = a.rows - r < most ? a.rows - r : most;
+    launch(b, dim3(uint32_t((a.n + outputs - 1) / outputs), uint32_t((b.rows + rows - 1) / rows)));
+    if (int rc = check_hip(hipGetLastError(), what)) return rc;
   }
   return DC_OK;
 }
 
+template <int DT, int GS, bool AFFINE>
+static int launch_project(const ProjectArgs& a, hipStream_t stream) {
+  if constexpr (DT != DC_F32) {
+    auto mid = [&](auto blocks) {
+      constexpr int MB = decltype(blocks)::value;
+      return by_rows(a, 2, 64, 16 * MB, "project_mid_kernel launch", [&](const ProjectArgs& b, dim3 grid) {
+        hipLaunchKernelGGL((project_mid_kernel<DT, GS, AFFINE, MB>), grid, dim3(512), 0, stream, b);
+      });
+    };
+    if (a.rows > 48) return mid(std::integral_constant<int, 4>{});
+    if (a.rows > 32) return mid(std::integral_constant<int, 3>{});
+    if (a.rows > 16) return mid(std::integral_constant<int, 2>{});
+  }
+  return by_rows(a, DT == DC_F32 ? 4 : 2, 16, 16, "project_few_kernel launch", [&](const ProjectArgs& b, dim3 grid) {
+    hipLaunchKernelGGL((project_few_kernel<DT, GS, AFFINE>), grid, dim3(64 * waves_of(int64_t(grid.x) * grid.y, a.k_tiles)), 0, stream, b);
+  });
+}
+
 template <int DT>
 static int launch_groups(const ProjectArgs& a, int group_size, bool affine, hipStream_t stream) {
-  return group_size == 32 ? launch_project<DT, 32>(a, affine, stream)
-         : group_size == 64 ? launch_project<DT, 64>(a, affine, stream)
-                            : launch_project<DT, 128>(a, affine, stream);
+  if (affine)
+    return group_size == 32   ? launch_project<DT, 32, true>(a, stream)
+           : group_size == 64 ? launch_project<DT, 64, true>(a, stream)
+                              : launch_project<DT, 128, true>(a, stream);
+  return group_size == 32   ? launch_project<DT, 32, false>(a, stream)
+         : group_size == 64 ? launch_project<DT, 64, false>(a, stream)
+                            : launch_project<DT, 128, false>(a, stream);
 }
 
 }  // namespace dc
