@@ -126,7 +126,8 @@ SIGNATURES = {
                                        C.c_int32, C.c_void_p, C.c_int32, C.c_int32, C.c_int32, C.c_int32, C.c_int64,
                                        TokenRows, C.c_float, ScoreRule, TokenRows, C.c_void_p, C.c_int64, C.c_void_p]),
     "dc_grouped_weight_bytes": (C.c_int64, [C.c_int32, C.c_int32, C.c_int32, C.c_int32, C.POINTER(C.c_int64)]),
-    "dc_project": (C.c_int, [GroupedWeight, MatrixRows, MatrixRows, C.c_int64, C.c_void_p]),
+    "dc_project_workspace_bytes": (C.c_int64, [GroupedWeight, C.c_int32, C.c_int64]),
+    "dc_project": (C.c_int, [GroupedWeight, MatrixRows, MatrixRows, C.c_int64, C.c_void_p, C.c_int64, C.c_void_p]),
     "dc_set_encode_path": (C.c_int, [C.c_int32]),
     "dc_score_pages": (C.c_int, [Pool, C.c_void_p, C.c_void_p, C.c_int32, C.c_void_p, C.c_int32, C.c_void_p, C.c_int64, C.c_void_p]),
     "dc_mix_pages": (C.c_int, [Pool, C.c_void_p, C.c_void_p, C.c_int32, C.c_void_p, C.c_int32, C.c_int64, C.c_void_p, C.c_int32, C.c_void_p]),

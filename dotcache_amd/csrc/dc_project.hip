@@ -9,95 +9,43 @@
 // numbers, exactly, with fp32 sums; scales and offsets act on the groups' sums
 // in fp32.  Nothing is rounded before the output.  fp32 rows are three bf16
 // parts each, whose sum they are.
-#include <type_traits>
-
-#include "dc_common.h"
+#include "dc_project.h"
 
 namespace dc {
 
 namespace {
 
-typedef _Float16 h8v __attribute__((ext_vector_type(8)));
-typedef __bf16 b8v __attribute__((ext_vector_type(8)));
-typedef float f32x4 __attribute__((ext_vector_type(4)));
-
-// Weight tiles: 16 outputs x 128 inputs, 1 KiB in the order of the lanes that
-// take them: lane l has output l % 16 and, of the tile's inputs, 32 w + 8 (l / 16)
-// .. + 7 in its word w.  Input j of a word's eight is nibble j / 2 + 4 (j % 2).
-constexpr int kTileN = 16, kTileK = 128;
-
-struct ProjectArgs {
-  const uint4* words;     // [N tiles][K tiles][64]
-  const uint16_t* scales; // [N tiles][K tiles][16][128 / group] scales, or {scale, bias} pairs
-  int32_t n, k, n_tiles, k_tiles;
-  const void* x;
-  void* y;
-  int64_t rows, x_stride, y_stride;
-  int32_t x_vec;  // rows of x start at multiples of 16 bytes, and k is a multiple of 8
-};
-
-__device__ __forceinline__ float half_of(uint16_t h) { return float(__builtin_bit_cast(_Float16, h)); }
-
-// Eight values 16 + code of a word as a matrix operand.
-template <int DT>
-__device__ __forceinline__ uint4 operand(uint32_t r) {
-  if constexpr (DT == DC_F16) {
-    constexpr uint32_t m = 0x03c003c0u, one = 0x4c004c00u;
-    return uint4{((r << 6) & m) | one, ((r << 2) & m) | one, ((r >> 2) & m) | one, ((r >> 6) & m) | one};
-  } else {
-    constexpr uint32_t m = 0x00780078u, one = 0x41804180u;
-    return uint4{((r << 3) & m) | one, ((r >> 1) & m) | one, ((r >> 5) & m) | one, ((r >> 9) & m) | one};
-  }
-}
-
-template <int DT>
-__device__ __forceinline__ f32x4 mfma(uint4 a, uint4 b, f32x4 c) {
-  if constexpr (DT == DC_F16)
-    return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(h8v, a), __builtin_bit_cast(h8v, b), c, 0, 0, 0);
-  else
-    return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(b8v, a), __builtin_bit_cast(b8v, b), c, 0, 0, 0);
-}
-
-// Inputs k .. k + 7 of a row as they lie in memory.  Past the row's end: its
-// first ones (whoever uses them leaves them out).
+// Inputs k .. k + 7 of a row, at any alignment, or the row's last eight where
+// those end behind it: one load whatever the row, with no branch (a register that
+// two branches load would be waited for where they meet).  Rows have eight inputs
+// at least.
 template <int DT>
 struct Eight {
   static constexpr int W = DT == DC_F32 ? 8 : 4;
   uint32_t w[W];
 };
 template <int DT>
-__device__ __forceinline__ void load_x(const ProjectArgs& a, const void* row, int k, Eight<DT>& x) {
-  typedef std::conditional_t<DT == DC_F32, uint32_t, uint16_t> T;
-  const T* p = static_cast<const T*>(row);
-  if (a.x_vec) {
-    const uint4* v = reinterpret_cast<const uint4*>(p + (k < a.k ? k : 0));
-#pragma unroll
-    for (int i = 0; i < Eight<DT>::W / 4; ++i) {
-      const uint4 y = v[i];
-      x.w[4 * i] = y.x; x.w[4 * i + 1] = y.y; x.w[4 * i + 2] = y.z; x.w[4 * i + 3] = y.w;
-    }
-  } else {
-#pragma unroll
-    for (int i = 0; i < 8; ++i) {
-      const uint32_t v = p[k + i < a.k ? k + i : 0];
-      if constexpr (DT == DC_F32)
-        x.w[i] = v;
-      else
-        x.w[i / 2] = i % 2 ? x.w[i / 2] | v << 16 : v;
-    }
-  }
+__device__ __forceinline__ void load_x(const ProjectArgs& a, const char* row, int k, Eight<DT>& x) {
+  constexpr int item = DT == DC_F32 ? 4 : 2;
+  __builtin_memcpy(x.w, __builtin_assume_aligned(row + int64_t(min(k, a.k - 8)) * item, item), sizeof(x.w));
 }
 
-// Those past the row's end as zeros.
+// What load_x read, moved to its place, with zeros behind the row's end (for a last tile
+// that the row does not fill).
 template <int DT>
 __device__ __forceinline__ void cut_x(const ProjectArgs& a, int k, Eight<DT>& x) {
+  constexpr int W = Eight<DT>::W, per = DT == DC_F32 ? 1 : 2;  // inputs a word
+  const int n = a.k - k, d = n >= 8 ? 0 : 8 - n;               // inputs left; how far the load began before k
 #pragma unroll
-  for (int i = 0; i < Eight<DT>::W; ++i) {
-    if constexpr (DT == DC_F32)
-      x.w[i] = k + i < a.k ? x.w[i] : 0;
-    else
-      x.w[i] &= (k + 2 * i < a.k ? 0xffffu : 0) | (k + 2 * i + 1 < a.k ? 0xffff0000u : 0);
+  for (int by = 4; by >= per; by >>= 1)
+#pragma unroll
+    for (int i = 0; i < W; ++i) x.w[i] = d & by ? (i + by / per < W ? x.w[(i + by / per) % W] : 0) : x.w[i];
+  if constexpr (per == 2) {
+#pragma unroll
+    for (int i = 0; i < W; ++i) x.w[i] = d & 1 ? x.w[i] >> 16 | (i + 1 < W ? x.w[(i + 1) % W] << 16 : 0) : x.w[i];
   }
+#pragma unroll
+  for (int i = 0; i < W; ++i) x.w[i] = n > 0 ? x.w[i] : 0;
 }
 
 // Part `part` of them as a matrix operand (fp32 rows have three bf16 parts: the
@@ -111,7 +59,11 @@ __device__ __forceinline__ uint4 x_operand(const Eight<DT>& x, int part) {
     uint32_t top[2];
 #pragma unroll
     for (int e = 0; e < 2; ++e) {
-      float v = __builtin_bit_cast(float, x.w[(2 * i + e) % Eight<DT>::W]);
+      // (a register of its own: built in place, over the loaded ones, the operand
+      // overwrote words that it still needed, as hipcc 7.2 ordered it)
+      uint32_t w = x.w[(2 * i + e) % Eight<DT>::W];
+      asm volatile("" : "+v"(w));
+      float v = __builtin_bit_cast(float, w);
 #pragma unroll
       for (int j = 0; j < part; ++j) v -= __builtin_bit_cast(float, __builtin_bit_cast(uint32_t, v) & 0xffff0000u);  // exact
       top[e] = __builtin_bit_cast(uint32_t, v);
@@ -119,16 +71,6 @@ __device__ __forceinline__ uint4 x_operand(const Eight<DT>& x, int part) {
     out[i] = __builtin_amdgcn_perm(top[1], top[0], 0x07060302u);
   }
   return uint4{out[0], out[1], out[2], out[3]};
-}
-
-template <int DT>
-__device__ __forceinline__ void store_y(void* y, int64_t i, float v) {
-  if constexpr (DT == DC_F32)
-    static_cast<float*>(y)[i] = v;
-  else if constexpr (DT == DC_F16)
-    static_cast<_Float16*>(y)[i] = _Float16(v);
-  else
-    static_cast<__bf16*>(y)[i] = __bf16(v);
 }
 
 }  // namespace
@@ -140,6 +82,7 @@ __device__ __forceinline__ void store_y(void* y, int64_t i, float v) {
 template <int DT, int GS, bool AFFINE>
 __global__ void __launch_bounds__(1024) project_few_kernel(ProjectArgs a) {
   constexpr int PARTS = DT == DC_F32 ? 3 : 1, OT = DT == DC_F32 ? DC_BF16 : DT, SC = kTileK / GS * (AFFINE ? 2 : 1);
+  constexpr int T = DT == DC_F32 ? 1 : 2;  // tiles a round
   constexpr uint32_t kOne = OT == DC_F16 ? 0x3c003c00u : 0x3f803f80u;
   __shared__ f32x4 joined[16][64];
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), waves = blockDim.x >> 6;
@@ -155,8 +98,7 @@ __global__ void __launch_bounds__(1024) project_few_kernel(ProjectArgs a) {
     uint16_t s[SC];
     Eight<DT> x[4];
   };
-  auto load = [&](int kt, Stage& st) __attribute__((always_inline)) {
-    const int t = min(kt, a.k_tiles - 1);
+  auto load = [&](int t, Stage& st) __attribute__((always_inline)) {
     st.w = words[int64_t(t) * 64];
     __builtin_memcpy(st.s, __builtin_assume_aligned(scales + int64_t(t) * 16 * SC, 2 * SC), 2 * SC);
 #pragma unroll
@@ -188,16 +130,16 @@ __global__ void __launch_bounds__(1024) project_few_kernel(ProjectArgs a) {
       for (int v = 0; v < 4; ++v) acc[v] = fmaf(s, sum[v], fmaf(off, xs[v], acc[v]));
     }
   };
-  Stage even, odd;
-  if (wave < a.k_tiles) {  // (uniform)
-    load(wave, even);
-    for (int kt = wave; kt < a.k_tiles; kt += 2 * waves) {
-      load(kt + waves, odd);
-      take(kt, even);
-      if (kt + waves >= a.k_tiles) break;
-      load(kt + 2 * waves, even);
-      take(kt + waves, odd);
-    }
+  // All of a round's loads are under way before its first product; the card's
+  // other wavefronts fill the wait between rounds.
+  for (int kt = wave; kt < a.k_tiles; kt += T * waves) {  // (uniform)
+    Stage st[T];
+#pragma unroll
+    for (int j = 0; j < T; ++j) load(min(kt + j * waves, a.k_tiles - 1), st[j]);
+    __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+    for (int j = 0; j < T; ++j)
+      if (kt + j * waves < a.k_tiles) take(kt + j * waves, st[j]);
   }
   joined[wave][lane] = acc;
   __syncthreads();
@@ -316,16 +258,17 @@ __global__ void __launch_bounds__(512, 2) project_mid_kernel(ProjectArgs a) {
   auto step = [&](int t, const Weights& now, Weights& next) __attribute__((always_inline)) {
     const int kt = 2 * t + half;
     load_weights(kt + 2, next);
-    if (t + 1 < turns) {
-      write_rows(kt + 2, (t + 1) & 1);
-      load_rows(kt + 4);
-    }
+    write_rows(kt + 2, (t + 1) & 1);  // (behind the last: not read)
+    load_rows(kt + 4);
+    __builtin_amdgcn_sched_barrier(0);  // (loads stay ahead of the products)
     if (kt < a.k_tiles) take(now, t & 1);
     __syncthreads();
   };
-  for (int t = 0; t < turns; t += 2) {
+  for (int t = 0;; t += 2) {
     step(t, even, odd);
-    if (t + 1 < turns) step(t + 1, odd, even);
+    if (t + 1 >= turns) break;
+    step(t + 1, odd, even);
+    if (t + 2 >= turns) break;
   }
   f32x4* const joined = reinterpret_cast<f32x4*>(xt);  // [4][MB][64]
   if (half == 1) {
@@ -346,11 +289,29 @@ __global__ void __launch_bounds__(512, 2) project_mid_kernel(ProjectArgs a) {
   }
 }
 
+// Rows of fewer than eight inputs: a thread per output.
+template <int DT>
+__global__ void __launch_bounds__(256) project_short_kernel(ProjectArgs a, int32_t group_size, int32_t affine) {
+  const int out = int(blockIdx.x) * 256 + int(threadIdx.x);
+  const int64_t r = blockIdx.y;
+  if (out >= a.n) return;
+  const uint32_t* w = reinterpret_cast<const uint32_t*>(a.words + int64_t(out / kTileN) * a.k_tiles * 64 + out % kTileN);
+  const uint16_t* sc = a.scales + (int64_t(out / kTileN) * a.k_tiles * 16 + out % kTileN) * (kTileK / group_size) * (affine ? 2 : 1);
+  const float s = half_of(sc[0]), b = affine ? half_of(sc[1]) : -7.f * s;
+  float sum = 0.f, xs = 0.f;
+  for (int k = 0; k < a.k; ++k) {
+    const float x = load_value(a.x, DT, r * a.x_stride + k);
+    sum = fmaf(float(w[0] >> (4 * (k / 2 + 4 * (k % 2))) & 15u), x, sum);
+    xs += x;
+  }
+  store_y<DT>(a.y, r * a.y_stride + out, fmaf(s, sum, b * xs));
+}
+
 // Wavefronts per block: where blocks alone leave the card's 1024 SIMDs
 // less than four wavefronts each, up to 16, but none without a tile.
 static int waves_of(int64_t blocks, int k_tiles) {
   int w = 4;
-  while (w < 16 && blocks * w < 4096 && 2 * w <= k_tiles) w *= 2;
+  while (w < 8 && blocks * w < 4096 && 2 * w <= k_tiles) w *= 2;
   return w;
 }
 
@@ -368,6 +329,13 @@ static int by_rows(const ProjectArgs& a, int item, int outputs, int rows, const 
     if (int rc = check_hip(hipGetLastError(), what)) return rc;
   }
   return DC_OK;
+}
+
+template <int DT>
+static int launch_short(const ProjectArgs& a, int group_size, bool affine, hipStream_t stream) {
+  return by_rows(a, DT == DC_F32 ? 4 : 2, 256, 1, "project_short_kernel launch", [&](const ProjectArgs& b, dim3 grid) {
+    hipLaunchKernelGGL((project_short_kernel<DT>), grid, dim3(256), 0, stream, b, group_size, int32_t(affine));
+  });
 }
 
 template <int DT, int GS, bool AFFINE>
@@ -390,6 +358,7 @@ static int launch_project(const ProjectArgs& a, hipStream_t stream) {
 
 template <int DT>
 static int launch_groups(const ProjectArgs& a, int group_size, bool affine, hipStream_t stream) {
+  if (a.k < 8) return launch_short<DT>(a, group_size, affine, stream);
   if (affine)
     return group_size == 32   ? launch_project<DT, 32, true>(a, stream)
            : group_size == 64 ? launch_project<DT, 64, true>(a, stream)
@@ -408,7 +377,12 @@ extern "C" int64_t dc_grouped_weight_bytes(int32_t outputs, int32_t inputs, int3
   return tiles * (1024 + dc::kTileN * (dc::kTileK / group_size) * (affine ? 4 : 2));
 }
 
-extern "C" int dc_project(dc_grouped_weight weight, dc_matrix_rows x, dc_matrix_rows y, int64_t rows, dc_stream_t stream) {
+extern "C" int64_t dc_project_workspace_bytes(dc_grouped_weight weight, int32_t dtype, int64_t rows) {
+  return dc::project_is_tiled(dtype, rows, weight.outputs, weight.inputs) ? dc::project_tile_workspace(dtype, rows, weight.inputs) : 0;
+}
+
+extern "C" int dc_project(dc_grouped_weight weight, dc_matrix_rows x, dc_matrix_rows y, int64_t rows, void* workspace, int64_t workspace_bytes,
+                          dc_stream_t stream) {
   const char* who = "dc_project";
   int64_t scales = 0;
   if (dc_grouped_weight_bytes(weight.outputs, weight.inputs, weight.group_size, weight.affine, &scales) < 0)
@@ -424,11 +398,15 @@ extern "C" int dc_project(dc_grouped_weight weight, dc_matrix_rows x, dc_matrix_
     return dc::fail(DC_EINVAL, "%s: rows must be aligned to their type", who);
   if (rows > 1 && (y.stride > -int64_t(weight.outputs) && y.stride < int64_t(weight.outputs)))
     return dc::fail(DC_EINVAL, "%s: the output's rows must not overlap", who);
-  dc::ProjectArgs a{static_cast<const uint4*>(weight.data), reinterpret_cast<const uint16_t*>(static_cast<const char*>(weight.data) + scales),
+  const bool tiled = dc::project_is_tiled(x.dtype, rows, weight.outputs, weight.inputs);
+  const int64_t need = tiled ? dc::project_tile_workspace(x.dtype, rows, weight.inputs) : 0;
+  if (workspace_bytes < need || (need && !workspace)) return dc::fail(DC_ESPACE, "%s: workspace too small", who);
+  if (reinterpret_cast<uintptr_t>(workspace) % 16) return dc::fail(DC_EINVAL, "%s: workspace must be 16-byte aligned", who);
+  const dc::ProjectArgs a{static_cast<const uint4*>(weight.data), reinterpret_cast<const uint16_t*>(static_cast<const char*>(weight.data) + scales),
                     weight.outputs, weight.inputs, (weight.outputs + dc::kTileN - 1) / dc::kTileN,
-                    (weight.inputs + dc::kTileK - 1) / dc::kTileK, x.data, y.data, rows, x.stride, y.stride, 0};
-  a.x_vec = reinterpret_cast<uintptr_t>(x.data) % 16 == 0 && (x.stride % 8 == 0 || rows == 1) && weight.inputs % 8 == 0;
+                    (weight.inputs + dc::kTileK - 1) / dc::kTileK, x.data, y.data, rows, x.stride, y.stride};
   const hipStream_t st = hipStream_t(stream);
+  if (tiled) return dc::launch_project_tile(a, x.dtype, weight.group_size, weight.affine, workspace, st);
   return x.dtype == DC_F32   ? dc::launch_groups<DC_F32>(a, weight.group_size, weight.affine, st)
          : x.dtype == DC_F16 ? dc::launch_groups<DC_F16>(a, weight.group_size, weight.affine, st)
                              : dc::launch_groups<DC_BF16>(a, weight.group_size, weight.affine, st);

@@ -10,7 +10,9 @@ the levels of the caches' pages:
     W = scale * (code - 7)           (symmetric, codes 0 .. 14)
 
 Codes, rows and their products are exact as matrix operands and sums are fp32,
-so an output is rounded once, to the rows' type.  The reference leaves these
+so an output is rounded once, to the rows' type; calls of many 16-bit rows, bound by
+the matrix instructions and not by the weights' bytes, round each weight to fp16
+besides.  The reference leaves these
 products to its models (reference ``dotcache/integrations/llama.py:345-358``,
 ``:476-481``); its levels are those of ``dotcache/modes/m0_affine.py:15-90``.
 """
@@ -72,6 +74,9 @@ class GroupedWeight:
                 continue
             if tuple(x.shape) != (N, G) or x.dtype != torch.float16 or x.device != codes.device:
                 raise ValueError(f"{name} must be fp16 [{N}, {G}] on the codes' device")
+        top = max(float(x.float().abs().max()) for x in ((scales * 15, biases, scales * 15 + biases) if biases is not None else (scales * 7,)))
+        if not top <= 65504.0:
+            raise ValueError("scales and biases must be finite, and the levels that they give in fp16's range")
         if int(codes.min()) < 0 or int(codes.max()) > (15 if biases is not None else 14):
             raise ValueError(f"codes must lie in [0, {15 if biases is not None else 14}]")
         data = _new_data(N, K, gs, biases is not None, codes.device)
@@ -174,12 +179,19 @@ def _put(data, N: int, K: int, gs: int, first: int, codes, scales, biases) -> No
             side[at, :, :, :, i] = torch.nn.functional.pad(x, pad).view(-1, _TILE_N, kt, _TILE_K // gs).transpose(1, 2)
 
 
-def project(x, weight: GroupedWeight, *, out=None):
+def workspace_bytes(weight: GroupedWeight, dtype, rows: int) -> int:
+    """Bytes of :func:`project`'s workspace for ``rows`` rows of ``dtype``."""
+    return int(_lib.lib().dc_project_workspace_bytes(weight._c, dtype_code(_torch().empty(0, dtype=dtype)), int(rows)))
+
+
+def project(x, weight: GroupedWeight, *, out=None, workspace=None):
     """``x [..., inputs]`` (fp32, fp16 or bf16; rows at any stride, their
     elements contiguous) times the weight's transpose: ``[..., outputs]`` in the
     same type.  ``out`` (two-dimensional like ``x``, rows at any stride that does
     not overlap) receives it instead; it must not overlap ``x``.  An infinity or
-    NaN in a row makes that row's outputs infinities or NaN."""
+    NaN in a row makes that row's outputs infinities or NaN.  ``workspace``: uint8,
+    :func:`workspace_bytes` at least, 16-byte aligned, not shared by calls that may
+    overlap (default: one of its own where a call needs it)."""
     torch = _torch()
     if x.dim() == 0 or x.shape[-1] != weight.inputs:
         raise ValueError(f"rows must have shape [..., {weight.inputs}]")
@@ -197,10 +209,21 @@ def project(x, weight: GroupedWeight, *, out=None):
             raise ValueError(f"out must have shape [{rows.shape[0]}, {weight.outputs}], the rows' dtype and device")
         if weight.outputs > 1 and y.stride(1) != 1 or y.shape[0] > 1 and y.stride(0) < weight.outputs:
             raise ValueError("out must have contiguous elements, and rows that do not overlap")
-    if rows.shape[0]:
-        call_on(x.device, _lib.lib().dc_project, "dc_project", weight._c,
-                _lib.MatrixRows(rows.data_ptr(), rows.stride(0), code), _lib.MatrixRows(y.data_ptr(), y.stride(0), code), rows.shape[0])
+    n = rows.shape[0]
+    if n:
+        L = _lib.lib()
+        need = L.dc_project_workspace_bytes(weight._c, code, n) if n > 64 else 0
+        if need == 0:
+            workspace = None
+        elif workspace is None:
+            workspace = torch.empty(need, dtype=torch.uint8, device=x.device)
+        elif workspace.numel() * workspace.element_size() < need or not workspace.is_contiguous() or workspace.device != x.device:
+            raise ValueError(f"workspace must be contiguous, {need} bytes at least, on {x.device}")
+        elif workspace.data_ptr() % 16:
+            raise ValueError("workspace must be 16-byte aligned")
+        call_on(x.device, L.dc_project, "dc_project", weight._c, _lib.MatrixRows(rows.data_ptr(), rows.stride(0), code),
+                _lib.MatrixRows(y.data_ptr(), y.stride(0), code), n, None if workspace is None else workspace.data_ptr(), need)
     return y if x.dim() == 2 else y.view(*x.shape[:-1], weight.outputs)
 
 
-__all__ = ["GroupedWeight", "project"]
+__all__ = ["GroupedWeight", "project", "workspace_bytes"]

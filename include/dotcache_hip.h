@@ -688,13 +688,21 @@ typedef struct dc_matrix_rows {
  * begin; -1 for sizes that none has.  Host only. */
 int64_t dc_grouped_weight_bytes(int32_t outputs, int32_t inputs, int32_t group_size, int32_t affine, int64_t* scales_offset);
 
+/* Bytes of the workspace of a dc_project call of `rows` rows of this dtype (0
+ * for most).  Host only. */
+int64_t dc_project_workspace_bytes(dc_grouped_weight weight, int32_t dtype, int64_t rows);
+
 /* y[m] = x[m] W^T for `rows` rows x [inputs] and y [outputs] of one dtype
  * (DC_F32, DC_F16, DC_BF16), sums in fp32, one rounding to y.  y must not
- * overlap x.  An infinity or NaN among a row's inputs gives infinities or NaN in all
- * of that row's outputs, and only there.  A weight's levels are those of reference
+ * overlap x.  Calls of many 16-bit rows round each weight to fp16 (levels past
+ * +-65504 overflow, those below 2^-14 lose bits); the others multiply by the codes as they are.  An infinity or NaN among a
+ * row's inputs gives infinities or NaN in all of that row's outputs, and only
+ * there.  workspace: dc_project_workspace_bytes at least, 16-byte aligned, not
+ * shared by calls that may overlap.  A weight's levels are those of reference
  * dotcache/modes/m0_affine.py:15-90; the reference leaves the products around
  * the cache to its models (dotcache/integrations/llama.py:345-358, :476-481). */
-int dc_project(dc_grouped_weight weight, dc_matrix_rows x, dc_matrix_rows y, int64_t rows, dc_stream_t stream);
+int dc_project(dc_grouped_weight weight, dc_matrix_rows x, dc_matrix_rows y, int64_t rows, void* workspace,
+               int64_t workspace_bytes, dc_stream_t stream);
 
 /* Process-wide decode kernel choice: 0 (default) runs the MFMA kernel when
  * every page format (M3 fp16 keys and values, M0 4- or 8-bit keys of group

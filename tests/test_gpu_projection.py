@@ -32,7 +32,7 @@ def exact_case(M, K, N, gs, affine, dtype, seed=0):
     return x, GroupedWeight.from_codes(codes, scales, biases, group_size=gs), want.to(_dt(dtype)), dense
 
 
-SIZES = [(1, 128, 16), (1, 1, 1), (2, 31, 5), (3, 160, 17), (16, 128, 33), (17, 257, 48), (5, 1000, 777), (33, 1024, 64), (1, 3584, 129), (64, 640, 130),
+SIZES = [(1, 128, 16), (1, 1, 1), (20, 7, 300), (3, 8, 40), (70, 15, 33), (2, 31, 5), (3, 160, 17), (16, 128, 33), (17, 257, 48), (5, 1000, 777), (33, 1024, 64), (1, 3584, 129), (64, 640, 130),
          (65, 512, 100), (130, 96, 257), (128, 64, 256), (300, 448, 272), (513, 130, 16), (257, 2048, 144)]
 
 

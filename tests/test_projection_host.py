@@ -76,7 +76,7 @@ def test_entry_refusals():
         assert L.dc_grouped_weight_bytes(*a, 1, None) == -1
 
     def call(rows=2, data=1 << 20, x=1 << 20, y=1 << 21, xd=0, yd=0, ys=20, gs=32):
-        return L.dc_project(_lib.GroupedWeight(data, 20, 100, gs, 1), _lib.MatrixRows(x, 100, xd), _lib.MatrixRows(y, ys, yd), rows, None)
+        return L.dc_project(_lib.GroupedWeight(data, 20, 100, gs, 1), _lib.MatrixRows(x, 100, xd), _lib.MatrixRows(y, ys, yd), rows, None, 0, None)
 
     for kw in (dict(rows=-1), dict(data=0), dict(x=0), dict(y=0), dict(xd=3), dict(yd=1), dict(ys=19), dict(gs=48), dict(data=(1 << 20) + 8),
                dict(x=(1 << 20) + 2), dict(y=(1 << 20) + 1, xd=1, yd=1)):
