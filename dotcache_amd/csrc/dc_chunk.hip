@@ -101,11 +101,12 @@ __global__ void __launch_bounds__(256) merge_chunk_kernel(ChunkArgs a, const dc_
   }
 }
 
-static int launch_merge_chunk(const ChunkArgs& a, const dc_chunk_merge* merges, int32_t n_merges, hipStream_t stream) {
+// `rows`: of a merge at most.
+static int launch_merge_chunk(const ChunkArgs& a, const dc_chunk_merge* merges, int32_t n_merges, int32_t rows, hipStream_t stream) {
   const int hd = a.kpool.geometry.head_dim;
   const bool vec = hd % 4 == 0;
   const int lanes = vec && hd <= 64 ? 16 : vec && hd <= 128 ? 32 : 64;
-  const dim3 grid(uint32_t(n_merges), kMergeBlocks);
+  const dim3 grid(uint32_t(n_merges), uint32_t(rows < kMergeBlocks ? rows : kMergeBlocks));
   if (vec)
     hipLaunchKernelGGL((merge_chunk_kernel<4>), grid, dim3(256), 0, stream, a, merges, lanes);
   else
@@ -175,7 +176,8 @@ static int attend_chunk(const char* who, dc_pool k_pool, dc_pool v_pool, const i
   }
   const bool units = q.dtype != DC_F32 && units32(k_pool) && units32(v_pool);
   if (int rc = rule ? launch_chunks_rule(a, n_few, few_rows, units, st) : launch_chunks(a, n_few, few_rows, units, st)) return rc;
-  return n_merges ? launch_merge_chunk(a, merges, n_merges, st) : DC_OK;
+  // (items of few rows alone: blocks for those rows)
+  return n_merges ? launch_merge_chunk(a, merges, n_merges, n_few == n_items ? few_rows : kMergeBlocks, st) : DC_OK;
 }
 
 int launch_chunks(ChunkArgs a, int32_t n_few, int32_t few_rows, bool units, hipStream_t stream) {

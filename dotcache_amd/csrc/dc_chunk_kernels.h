@@ -252,6 +252,13 @@ __device__ __forceinline__ void shape_scores(const ChunkArgs& a, float c, const 
   }
 }
 
+// Moves an item's begin past whole tiles of `tile` tokens that none of its rows
+// sees (items begin at multiples of kChunkStep); its gap, if any, stays ahead.
+__device__ __forceinline__ void skip_unseen(dc_chunk_item& it, const Sight& s, int2 gap, int tile) {
+  const int to = min(min(s.any0, s.any20), gap.x >= 0 ? gap.x - tile : it.kv_end - 1);
+  if (to > it.kv_begin) it.kv_begin += (to - it.kv_begin) / tile * tile;
+}
+
 // The item's gap: its tiles leave out tokens [x, y).
 __device__ __forceinline__ int2 item_gap(const ChunkArgs& a, uint32_t item) { return a.gaps ? a.gaps[item] : int2{-1, -1}; }
 
@@ -294,6 +301,7 @@ __global__ void __launch_bounds__(256, sizeof(T) == 4 && HDP == 256 ? 1 : 2) att
     mine = sight_of(a, it, it.row_begin + 32 * wave, min(it.row_begin + 32 * wave + 32, it.row_end));
     all = sight_of(a, it, it.row_begin, it.row_end);
     gap = item_gap(a, block_index(kChunkRows / 128));
+    skip_unseen(it, all, gap, KT);
   }
   auto seen = [&](int u) { return RULE ? rule.sees(u) : u <= sees; };
 
@@ -617,6 +625,10 @@ struct PageLoad {
     if constexpr (UNI) return (__builtin_amdgcn_raw_buffer_load_b16(rsrc(), int(lane), int(ok ? off : 0), 0));
     return *static_cast<const uint16_t*>(at(off, lane));
   }
+  __device__ __forceinline__ uint32_t u32(uint32_t off, uint32_t lane) const {
+    if constexpr (UNI) return __builtin_amdgcn_raw_buffer_load_b32(rsrc(), int(lane), int(ok ? off : 0), 0);
+    return *static_cast<const uint32_t*>(at(off, lane));
+  }
   __device__ __forceinline__ uint2 u64(uint32_t off, uint32_t lane) const {
     if constexpr (UNI) return __builtin_bit_cast(uint2, __builtin_amdgcn_raw_buffer_load_b64(rsrc(), int(lane), int(ok ? off : 0), 0));
     return uint2{static_cast<const uint32_t*>(at(off, lane))[0], static_cast<const uint32_t*>(at(off, lane))[1]};
@@ -777,6 +789,7 @@ __global__ void __launch_bounds__(512, 2) attend_chunk16_kernel(ChunkArgs a) {
     mine = sight_of(a, it, it.row_begin + rows_at, min(it.row_begin + rows_at + 32, it.row_end));
     all = sight_of(a, it, it.row_begin, it.row_end);
     const int2 gap = item_gap(a, block_index(CS));
+    skip_unseen(it, all, gap, KT);
     if (gap.x >= 0) gap_tile = (gap.x - it.kv_begin) / KT, gap_len = gap.y - gap.x;
   }
   auto seen = [&](int u) { return RULE ? rule.sees(u) : u <= sees; };
@@ -1072,6 +1085,11 @@ typedef float f32x4 __attribute__((ext_vector_type(4)));
 constexpr int kFewTile = 32;   // tokens a wavefront takes at a time
 constexpr int kFewWaves = 4;
 
+// Bytes of the wavefronts' joined rows, and whether each has its own: two blocks
+// share a compute unit's 160 KiB.
+constexpr bool few_joined_apart(int hdp, int nb) { return kFewWaves * 16 * nb * (hdp + 4) * 4 <= 72 * 1024; }
+constexpr int few_joined_bytes(int hdp, int nb) { return (few_joined_apart(hdp, nb) ? kFewWaves : 1) * 16 * nb * (hdp + 4) * 4; }
+
 // As lds_at, for tiles whose reads take two chunks of eight tokens at once.
 template <int CH>
 __device__ __forceinline__ int few_at(int t, int ch) {
@@ -1125,19 +1143,25 @@ __device__ __forceinline__ uint32_t zero_of(int kind, bool affine) {
 // K Q^T leaves a row's logits in four lanes, again in the order in which the
 // values' operand is read.
 // KW: words of a key operand that are read ahead (4: also fp16 rows; 2: codes
-// only, and fp16 rows when they are needed).  UNI: a tile's tokens lie in one page.
+// only, and fp16 rows when they are needed; 1: as 2, 4-bit codes only).  UNI: a tile's tokens lie in one page.
+// KW 1 is for pools of 4-bit codes in groups of 32 (and fp16 pages between them):
+// a token's scales lie side by side, and are one load.  The loads' issue is half of
+// a long range's time, so what counts is how few they are: a decode of 8
+// sequences of 32768 tokens at head_dim 256, 336 MB, 172 -> 131 us.
 template <int HDP, int NB, int KW, bool UNI, bool WHOLE, bool RULE>
 __global__ void __launch_bounds__(64 * kFewWaves, 2) attend_few_kernel(ChunkArgs a) {
   constexpr int CH = HDP / 8, KS = HDP / 32, CB = HDP / 16, TILE = kFewTile * HDP * 2;
   constexpr int VC = HDP / 2, VU = VC / 32;  // a lane's value channels, in units of 32
   constexpr int PB = UNI ? 1 : 2;            // pages that a lane follows: its tokens of each 16
   constexpr int COMB = HDP + 4;
+  constexpr bool C4 = KW == 1;
+  static_assert(!C4 || (UNI && WHOLE), "a page's tile, whole rows of scales");
   constexpr bool QL = NB * HDP >= 256;       // the queries stay in LDS (registers are for the output and the next tile)
   extern __shared__ __attribute__((aligned(16))) uint8_t lds[];  // values of each wavefront, then queries; at the end the joined rows
   __shared__ float ml[kFewWaves][16 * NB][2];
   __shared__ float odd[kFewWaves][HDP];
 
-  const dc_chunk_item it = a.items[blockIdx.x];
+  dc_chunk_item it = a.items[blockIdx.x];
   if (!chunk_item_ok(it, a) || it.row_end - it.row_begin > 16 * NB) return;
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int col = lane & 15, g = lane >> 4;
@@ -1151,6 +1175,7 @@ __global__ void __launch_bounds__(64 * kFewWaves, 2) attend_few_kernel(ChunkArgs
   if constexpr (RULE) {
     all = sight_of(a, it, it.row_begin, it.row_end);
     const int2 gap = item_gap(a, blockIdx.x);
+    skip_unseen(it, all, gap, kFewTile);
     if (gap.x >= 0) gap_tile = (gap.x - it.kv_begin) / kFewTile, gap_len = gap.y - gap.x;
   }
   h8v q[QL ? 1 : NB][QL ? 1 : KS];
@@ -1272,8 +1297,26 @@ __global__ void __launch_bounds__(64 * kFewWaves, 2) attend_few_kernel(ChunkArgs
     return x;
   };
   // ... and its words; scales and biases as they are
-  uint32_t kr[2][KS][KW], vr[VU][8];
+  uint32_t kr[2][KS][KW], vr[VU][C4 ? 4 : 8];
   uint16_t k_scale[2][KS], k_bias[2][KS], v_scale[VU], v_bias[VU];
+  uint32_t ks_row[2][KS / 2], kb_row[2][KS / 2], vs_row[(VU + 1) / 2], vb_row[(VU + 1) / 2];  // (C4: in pairs)
+  // N halves side by side, in pairs
+  auto halves = [](const PageLoad<UNI>& p, uint32_t off, uint32_t at, auto n, uint32_t* to) __attribute__((always_inline)) {
+    constexpr int N = decltype(n)::value;
+    if constexpr (N == 1) {
+      to[0] = p.u16(off, at);
+    } else if constexpr (N == 2) {
+      to[0] = p.u32(off, at);
+    } else if constexpr (N == 4) {
+      const uint2 x = p.u64(off, at);
+      to[0] = x.x; to[1] = x.y;
+    } else {
+      const uint4 x = p.u128(off, at);
+      to[0] = x.x; to[1] = x.y; to[2] = x.z; to[3] = x.w;
+    }
+  };
+  // half i of such pairs, twice
+  auto half_of = [](const uint32_t* row, int i) { return __builtin_amdgcn_perm(row[i / 2], row[i / 2], i % 2 ? 0x03020302u : 0x01000100u); };
   // the lane's offsets in a page, from its tile's first token (from its own where its tokens lie in several pages)
   const uint32_t k4 = kt0 * ks.token4 + 4 * g, k_sc = kt0 * ks.groups2, k16 = kt0 * ks.row2 + 16 * g;
   const uint32_t vc0 = VC * (lane >> 5), v16 = vt0 * vs.row2 + 2 * vc0;
@@ -1295,6 +1338,13 @@ __global__ void __launch_bounds__(64 * kFewWaves, 2) attend_few_kernel(ChunkArgs
       const uint32_t sh = x.k_kind == U_B8, lane_at = f16 ? k16 : k4 << sh, lane_s = f16 ? 0 : k_sc;
       const uint32_t codes = f16 ? slot * ks.row2 : (slot * ks.token4) << sh, scales = f16 ? 0 : (ks.scales4 << sh) + slot * ks.groups2;
       const uint32_t gap = x.k_affine && !f16 ? ks.gap : 0;
+      if constexpr (C4) {
+#pragma unroll
+        for (int k = 0; k < KS; ++k) kr[b][k][0] = p.u32(codes + (f16 ? 0 : k * k_plane), f16 ? 0 : k4);
+        halves(p, scales, lane_s, std::integral_constant<int, KS>{}, ks_row[b]);
+        halves(p, scales + gap, lane_s, std::integral_constant<int, KS>{}, kb_row[b]);
+        continue;
+      }
 #pragma unroll
       for (int k = 0; k < KS; ++k) {
         const uint32_t c = 32 * k < hd ? 32 * k : 0, gr = c / kgs;  // (channels past head_dim: the first ones')
@@ -1302,7 +1352,7 @@ __global__ void __launch_bounds__(64 * kFewWaves, 2) attend_few_kernel(ChunkArgs
         if constexpr (KW == 4) {
           const uint4 r = p.u128(o, lane_at);
           kr[b][k][0] = r.x; kr[b][k][1] = r.y; kr[b][k][2] = r.z; kr[b][k][3] = r.w;
-        } else {
+        } else if constexpr (KW == 2) {
           const uint2 r = p.u64(o, lane_at);
           kr[b][k][0] = r.x; kr[b][k][1] = r.y;
         }
@@ -1317,11 +1367,21 @@ __global__ void __launch_bounds__(64 * kFewWaves, 2) attend_few_kernel(ChunkArgs
     const PageLoad<UNI> p{x.v, a.items, x.v_kind != U_NONE && !f16};
     const uint32_t sh = x.v_kind == U_B8, codes = (x.slot * vs.token4) << sh, scales = (vs.scales4 << sh) + x.slot * vs.groups2;
     const uint32_t gap = x.v_affine ? vs.gap : 0;
+    if constexpr (C4) {
+#pragma unroll
+      for (int u = 0; u < VU; ++u) {
+        const uint4 r = p.u128(codes, v4[u]);
+        vr[u][0] = r.x; vr[u][1] = r.y; vr[u][2] = r.z; vr[u][3] = r.w;
+      }
+      halves(p, scales, v_sc[0], std::integral_constant<int, VU>{}, vs_row);
+      halves(p, scales + gap, v_sc[0], std::integral_constant<int, VU>{}, vb_row);
+      return;
+    }
 #pragma unroll
     for (int u = 0; u < VU; ++u) {
       const uint4 r = p.u128(codes, v4[u] << sh), t = p.u128(codes + (sh ? 16 : 0), v4[u] << sh);
       vr[u][0] = r.x; vr[u][1] = r.y; vr[u][2] = r.z; vr[u][3] = r.w;
-      vr[u][4] = t.x; vr[u][5] = t.y; vr[u][6] = t.z; vr[u][7] = t.w;
+      if constexpr (!C4) vr[u][4] = t.x, vr[u][5] = t.y, vr[u][6] = t.z, vr[u][7] = t.w;
       v_scale[u] = p.u16(scales, v_sc[u]);
       v_bias[u] = p.u16(scales + gap, v_sc[u]);
     }
@@ -1362,13 +1422,14 @@ __global__ void __launch_bounds__(64 * kFewWaves, 2) attend_few_kernel(ChunkArgs
       for (int u = 0; u < VU; ++u) {
         uint32_t y[4][4];
         const bool in = int(vc0 + 32 * u) < hd;
-        const h2v s = __builtin_bit_cast(h2v, twice(v_scale[u])), b = __builtin_bit_cast(h2v, x.v_affine ? twice(v_bias[u]) : 0u);
+        const h2v s = __builtin_bit_cast(h2v, C4 ? half_of(vs_row, u) : twice(v_scale[u]));
+        const h2v b = __builtin_bit_cast(h2v, !x.v_affine ? 0u : C4 ? half_of(vb_row, u) : twice(v_bias[u]));
         if (x.v_kind == U_B4) {
 #pragma unroll
           for (int e = 0; e < 4; ++e) eight4(vr[u][e], zero, s, b, y[e]);
-        } else if (x.v_kind == U_B8) {
+        } else if (!C4 && x.v_kind == U_B8) {
 #pragma unroll
-          for (int e = 0; e < 4; ++e) eight8(vr[u][2 * e], vr[u][2 * e + 1], zero, s, b, y[e]);
+          for (int e = 0; e < 4; ++e) eight8(vr[u][2 * e % (C4 ? 4 : 8)], vr[u][(2 * e + 1) % (C4 ? 4 : 8)], zero, s, b, y[e]);
         } else if (x.v_kind == U_F16 && in) {
           const PageLoad<UNI> p{x.v, a.items, true};
 #pragma unroll
@@ -1408,11 +1469,12 @@ __global__ void __launch_bounds__(64 * kFewWaves, 2) attend_few_kernel(ChunkArgs
       if (x.k_kind == U_B4) {
 #pragma unroll
         for (int k = 0; k < KS; ++k)
-          eight4(kr[b][k][0], zero, __builtin_bit_cast(h2v, twice(k_scale[b][k])), __builtin_bit_cast(h2v, x.k_affine ? twice(k_bias[b][k]) : 0u), y[b][k]);
-      } else if (x.k_kind == U_B8) {
+          eight4(kr[b][k][0], zero, __builtin_bit_cast(h2v, C4 ? half_of(ks_row[b], k) : twice(k_scale[b][k])),
+                 __builtin_bit_cast(h2v, !x.k_affine ? 0u : C4 ? half_of(kb_row[b], k) : twice(k_bias[b][k])), y[b][k]);
+      } else if (!C4 && x.k_kind == U_B8) {
 #pragma unroll
         for (int k = 0; k < KS; ++k)
-          eight8(kr[b][k][0], kr[b][k][1], zero, __builtin_bit_cast(h2v, twice(k_scale[b][k])),
+          eight8(kr[b][k][0], kr[b][k][1 % KW], zero, __builtin_bit_cast(h2v, twice(k_scale[b][k])),
                  __builtin_bit_cast(h2v, x.k_affine ? twice(k_bias[b][k]) : 0u), y[b][k]);
       } else if (x.k_kind == U_F16) {
         if constexpr (KW == 4) {
@@ -1538,8 +1600,11 @@ __global__ void __launch_bounds__(64 * kFewWaves, 2) attend_few_kernel(ChunkArgs
     }
   }
   __syncthreads();
-  for (int w = 0; w < kFewWaves; ++w) {
-    if (wave == w) {
+  // (each into rows of its own where those of all four fit, else one after another: a turn
+  // costs a barrier and a pass over LDS, 2 us of a short range's 20 in all)
+  constexpr int APART = few_joined_apart(HDP, NB) ? 16 * NB * COMB : 0;
+  for (int w = 0; w < (APART ? 1 : kFewWaves); ++w) {
+    if (APART || wave == w) {
 #pragma unroll
       for (int n = 0; n < NB; ++n) {
         const int r = 16 * n + col;
@@ -1549,10 +1614,10 @@ __global__ void __launch_bounds__(64 * kFewWaves, 2) attend_few_kernel(ChunkArgs
         for (int j = 0; j < CB; ++j)
 #pragma unroll
           for (int v = 0; v < 4; ++v) {
-            float& x = comb[r * COMB + 16 * j + 8 * (g / 2) + kPerm[4 * (g % 2) + v]];
+            float& x = comb[wave * APART + r * COMB + 16 * j + 8 * (g / 2) + kPerm[4 * (g % 2) + v]];
             // (a wavefront that saw no token holds zeros, or what a value that is not finite left)
             const float y = m[n] == -INFINITY ? o[n][j][v] : o[n][j][v] * f;
-            x = w == 0 ? y : x + y;
+            x = APART || w == 0 ? y : x + y;
           }
       }
     }
@@ -1567,7 +1632,14 @@ __global__ void __launch_bounds__(64 * kFewWaves, 2) attend_few_kernel(ChunkArgs
 #pragma unroll
     for (int w = 0; w < kFewWaves; ++w)
       sum += ml[w][r][0] == -INFINITY ? ml[w][r][1] : ml[w][r][1] * __builtin_amdgcn_exp2f(ml[w][r][0] - top);
-    const float4 x = *reinterpret_cast<const float4*>(comb + r * COMB + ch);
+    float4 x = *reinterpret_cast<const float4*>(comb + r * COMB + ch);
+    if constexpr (APART != 0) {
+#pragma unroll
+      for (int w = 1; w < kFewWaves; ++w) {
+        const float4 y = *reinterpret_cast<const float4*>(comb + w * APART + r * COMB + ch);
+        x.x += y.x; x.y += y.y; x.z += y.z; x.w += y.w;
+      }
+    }
     if (part) {
       const int64_t pr = int64_t(it.partial) + r;
       *reinterpret_cast<float4*>(a.part_o + pr * hd + ch) = x;
@@ -1637,15 +1709,24 @@ static int launch_chunk16(const ChunkArgs& a, hipStream_t stream) {
 
 template <int HDP, int NB, int KW, bool UNI, bool WHOLE, bool RULE>
 static int launch_few_as(const ChunkArgs& a, hipStream_t stream) {
-  constexpr int tiles = kFewWaves * kFewTile * HDP * 2 + (NB * HDP >= 256 ? 16 * NB * HDP * 2 : 0), joined = 16 * NB * (HDP + 4) * 4, bytes = tiles > joined ? tiles : joined;
+  constexpr int tiles = kFewWaves * kFewTile * HDP * 2 + (NB * HDP >= 256 ? 16 * NB * HDP * 2 : 0), joined = few_joined_bytes(HDP, NB), bytes = tiles > joined ? tiles : joined;
   static LdsLimit limit;
   if (int rc = limit.raise(reinterpret_cast<const void*>(&attend_few_kernel<HDP, NB, KW, UNI, WHOLE, RULE>), bytes, "attend_few_kernel LDS")) return rc;
   hipLaunchKernelGGL((attend_few_kernel<HDP, NB, KW, UNI, WHOLE, RULE>), dim3(a.n_items), dim3(64 * kFewWaves), bytes, stream, a);
   return check_hip(hipGetLastError(), "attend_few_kernel launch");
 }
 
+// Whether a pool holds 4-bit codes in groups of 32, and no others.
+static bool codes4(const dc_pool& p) {
+  uint64_t four = 0, others = 0;
+  for (int f : {DC_FMT_M0_AFFINE, DC_FMT_M0_SYMMETRIC}) four |= uint64_t(1) << (f * 9 + 4), others |= uint64_t(1) << (f * 9 + 8);
+  return p.geometry.group_size == 32 && (p.format_mask & four) != 0 && (p.format_mask & others) == 0;
+}
+
 template <int HDP, int NB, int KW, bool RULE>
 static int launch_few(const ChunkArgs& a, hipStream_t stream) {
+  if (a.kpool.geometry.page_capacity % kFewTile == 0 && a.kpool.geometry.head_dim == HDP && codes4(a.kpool) && codes4(a.vpool))
+    return launch_few_as<HDP, NB, 1, true, true, RULE>(a, stream);
   if (a.kpool.geometry.page_capacity % kFewTile != 0) return launch_few_as<HDP, NB, KW, false, false, RULE>(a, stream);
   return a.kpool.geometry.head_dim == HDP ? launch_few_as<HDP, NB, KW, true, true, RULE>(a, stream)
                                           : launch_few_as<HDP, NB, KW, true, false, RULE>(a, stream);

@@ -1,5 +1,5 @@
 // The largest calls of dc_project with 16-bit rows: products of tiles of up to
-// 128 rows by 128 outputs.  Bound by the matrix instructions, so weights are
+// 96 rows by 128 outputs.  Bound by the matrix instructions, so weights are
 // fp16 operands, scale and bias in them (one rounding, 2^-11 of a weight at
 // most), and no sum is touched until the end: 2048 bf16 rows of 3584 x 4608 in 108
 // us, 9 of them the rows' preparation (a library product of dense matrices 66,
@@ -252,13 +252,11 @@ static double rounds(int64_t rows, int32_t n, int mb) {
   return double((blocks + 255) / 256) * (mb ? mb : 3.5);
 }
 
-// Row blocks of a tile: what is done first.  (10 need more registers than two
-// wavefronts on a SIMD have: 172 us where 4 and 8 take 109.)
+// Row blocks of a tile: what is done first.  (8 are never done before 4 and take
+// as long; 10 need more registers than two wavefronts on a SIMD have: 172 us
+// where 4 take 109.)
 static int tile_rows(int64_t rows, int32_t n) {
-  int best = 4;
-  for (int mb : {6, 8})
-    if (rounds(rows, n, mb) < rounds(rows, n, best)) best = mb;
-  return best;
+  return rounds(rows, n, 6) < rounds(rows, n, 4) ? 6 : 4;
 }
 
 bool project_is_tiled(int32_t dtype, int64_t rows, int32_t n, int32_t k) {
@@ -290,7 +288,7 @@ static int launch_tile(const TileArgs& t, hipStream_t stream) {
     return int(DC_OK);
   };
   const int mb = tile_rows(t.p.rows, t.p.n);
-  return mb == 4 ? go(std::integral_constant<int, 4>{}) : mb == 6 ? go(std::integral_constant<int, 6>{}) : go(std::integral_constant<int, 8>{});
+  return mb == 4 ? go(std::integral_constant<int, 4>{}) : go(std::integral_constant<int, 6>{});
 }
 
 template <int DT>
