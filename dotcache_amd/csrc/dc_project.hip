@@ -82,7 +82,7 @@ __device__ __forceinline__ uint4 x_operand(const Eight<DT>& x, int part) {
 template <int DT, int GS, bool AFFINE>
 __global__ void __launch_bounds__(1024) project_few_kernel(ProjectArgs a) {
   constexpr int PARTS = DT == DC_F32 ? 3 : 1, OT = DT == DC_F32 ? DC_BF16 : DT, SC = kTileK / GS * (AFFINE ? 2 : 1);
-  constexpr int T = DT == DC_F32 ? 1 : 2;  // tiles a round
+  constexpr int T = DT == DC_F32 ? 1 : 2;  // tiles a round (4: the same time, more code)
   constexpr uint32_t kOne = OT == DC_F16 ? 0x3c003c00u : 0x3f803f80u;
   __shared__ f32x4 joined[16][64];
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), waves = blockDim.x >> 6;
@@ -371,7 +371,7 @@ static int launch_groups(const ProjectArgs& a, int group_size, bool affine, hipS
 }  // namespace dc
 
 extern "C" int64_t dc_grouped_weight_bytes(int32_t outputs, int32_t inputs, int32_t group_size, int32_t affine, int64_t* scales_offset) {
-  if (outputs <= 0 || inputs <= 0 || (group_size != 32 && group_size != 64 && group_size != 128)) return -1;
+  if (outputs <= 0 || inputs <= 0 || outputs > 1 << 30 || inputs > 1 << 30 || (group_size != 32 && group_size != 64 && group_size != 128)) return -1;
   const int64_t tiles = ((int64_t(outputs) + dc::kTileN - 1) / dc::kTileN) * ((int64_t(inputs) + dc::kTileK - 1) / dc::kTileK);
   if (scales_offset) *scales_offset = tiles * 1024;
   return tiles * (1024 + dc::kTileN * (dc::kTileK / group_size) * (affine ? 4 : 2));

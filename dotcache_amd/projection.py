@@ -74,9 +74,7 @@ class GroupedWeight:
                 continue
             if tuple(x.shape) != (N, G) or x.dtype != torch.float16 or x.device != codes.device:
                 raise ValueError(f"{name} must be fp16 [{N}, {G}] on the codes' device")
-        top = max(float(x.float().abs().max()) for x in ((scales * 15, biases, scales * 15 + biases) if biases is not None else (scales * 7,)))
-        if not top <= 65504.0:
-            raise ValueError("scales and biases must be finite, and the levels that they give in fp16's range")
+        _check_levels(scales, biases)
         if int(codes.min()) < 0 or int(codes.max()) > (15 if biases is not None else 14):
             raise ValueError(f"codes must lie in [0, {15 if biases is not None else 14}]")
         data = _new_data(N, K, gs, biases is not None, codes.device)
@@ -122,6 +120,7 @@ class GroupedWeight:
                 side = [blobs[:, o: o + 2 * P].contiguous().view(torch.float16).reshape(-1)[:n].view(-1, G)
                         for o in range(P * gs // 2, P * gs // 2 + (4 if affine else 2) * P, 2 * P)]
                 codes[:, K:] = 0
+                _check_levels(side[0], side[1] if affine else None)
                 codes = torch.nn.functional.pad(codes, (0, -K % _TILE_K - (G * gs - K), 0, -codes.shape[0] % _TILE_N))
                 _put(data, N, K, gs, r, codes.unflatten(-1, (-1, 8)), side[0], side[1] if affine else None)
         return cls(data, N, K, gs, affine)
@@ -145,6 +144,13 @@ def _group_size(group_size) -> int:
     if group_size not in GROUP_SIZES:
         raise ValueError("group_size must be 32, 64 or 128")
     return int(group_size)
+
+
+def _check_levels(scales, biases) -> None:
+    top = (scales.float() * 7).abs() if biases is None else \
+        _torch().maximum(biases.float().abs(), (scales.float() * 15 + biases.float()).abs()).maximum((scales.float() * 15).abs())
+    if not float(top.max()) <= 65504.0:
+        raise ValueError("a weight's scales, biases and levels must lie in fp16's range")
 
 
 def _new_data(N: int, K: int, gs: int, affine: bool, device):

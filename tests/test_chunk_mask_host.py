@@ -83,6 +83,12 @@ def test_rows_that_attend_nothing_have_an_item():
     assert plan.n_merges == 0
 
 
+def test_a_batch_that_waits():
+    plan = _plan([0, 0], [5, 0], mask=ChunkMask(window=3, documents=[[0, 2], []]))
+    assert plan.n_items == plan.n_tokens == 0 and plan.ranges.shape == (0, 4)
+    assert _plan([0, 0], [5, 0], mask=np.zeros((0, 4), dtype=np.int32)).n_items == 0
+
+
 def test_an_empty_mask_is_the_causal_plan():
     a, b = _plan([700, 1], [900, 5000]), _plan([700, 1], [900, 5000], mask=ChunkMask())
     assert b.ranges is None and np.array_equal(a.host_items, b.host_items) and np.array_equal(a.host_merges, b.host_merges)

@@ -308,3 +308,60 @@ def test_caches_take_masks_and_scores():
     assert len(cache._chunk_plan[1]) == 3
     with pytest.raises(ValueError):
         cache.attend_chunk(0, q, query_scale=0.125, mask=np.zeros((40, 4), dtype=np.int32))
+
+
+@pytest.mark.parametrize("layout", ["group_major", "token_major"])
+@pytest.mark.parametrize("hd,n_q,new", [(64, 3, 5), (64, 7, 9), (128, 7, 1), (128, 4, 6), (128, 7, 6), (256, 4, 1), (256, 5, 3)])
+def test_few_rows_of_4_bit_pages(hd, n_q, new, layout):
+    """Pools of 4-bit pages alone take kernels of their own; once a pool has
+    held an 8-bit page, the same call takes the others: the same outputs, plain and
+    with a rule, tails of fp16 among the pages."""
+    import torch
+
+    rng = np.random.default_rng(hd + n_q)
+    for key, value, tail in (("a4", "s4", True), ("s4", "a4", False), ("a4", "a4", True)):
+        print(f"few rows of 4 bits {hd} {n_q} {new} {layout} {key} {value}", flush=True)
+        batch = _Batch(rng, [700, 65, 32], 2, hd, 32, key, value, layout=layout, tail=tail)
+        n = [new, min(new, 3), 1]
+        calls = [dict(mask=ChunkMask(window=200, sinks=3), cap=5.0, slopes=True), dict()]
+        first = [check_rule(batch, n, n_q, "bf16", rng, **kw) for kw in calls]
+        for p in batch.pools:
+            p.allocate(1, 8, 1)
+        for kw, (q, got, plan) in zip(calls, first):
+            sl = torch.from_numpy(slopes_of(2 * n_q)).cuda() if kw.get("slopes") else None
+            assert torch.equal(batch.attend(q, plan, 1.0 / np.sqrt(hd), cap=kw.get("cap"), slopes=sl), got)
+
+
+def test_block_cache_takes_masks_and_scores():
+    """A serving engine's mixed batch: window and cap over block tables, against
+    the same cache's dense rows."""
+    import torch
+
+    from dotcache_amd.block_cache import DeviceVllmPagedKVCache
+    from dotcache_amd.config import DotCacheConfig
+
+    rng = np.random.default_rng(7)
+    cfg = DotCacheConfig(head_dim=64, group_size=32, bits_k=4, bits_v=4, tokens_per_page=16)
+    cache = DeviceVllmPagedKVCache(config=cfg, num_hidden_layers=1, num_attention_heads=4, num_key_value_heads=2, block_size=16)
+    lens, new = [70, 33], [20, 1]
+    tables = [[7, 2, 9, 4, 0], [5, 1, 3]]
+    for b, n in enumerate(lens):
+        x = [torch.from_numpy(rng.normal(size=(n, 2, 64)).astype(np.float32)).cuda() for _ in range(2)]
+        cache.write_slots(0, *x, [16 * tables[b][t // 16] + t % 16 for t in range(n)])
+    q = torch.from_numpy(rng.normal(size=(21, 4, 64)).astype(np.float32)).cuda()
+    padded = [t + [0] * (5 - len(t)) for t in tables]
+    mask = ChunkMask(window=18, sinks=2, prefix=(60, 0))
+    sl = torch.from_numpy(slopes_of(4)).cuda()
+    got = cache.attend_block_tables(0, q, new, padded, lens, query_scale=0.125, mask=mask, cap=3.0, slopes=sl).double().cpu().numpy()
+    k, v = (y.double().cpu().numpy() for y in cache.read_block_tables(0, padded, lens))
+    t0 = u0 = 0
+    for b, (n, c) in enumerate(zip(new, lens)):
+        ok = sees(mask, b, c)[c - n:]
+        for j in range(4):
+            kk, vv = (y[u0: u0 + c, j // 2] for y in (k, v))
+            s = 3.0 * np.tanh(0.125 * (q[t0: t0 + n, j].double().cpu().numpy() @ kk.T) / 3.0)
+            s = s - float(sl[j]) * np.abs(np.arange(c - n, c)[:, None] - np.arange(c))
+            p = np.exp(np.where(ok, s, -np.inf))
+            # (fp32 throughout, values below 8)
+            assert np.max(np.abs(got[t0: t0 + n, j] - p / p.sum(1, keepdims=True) @ vv)) < 1e-4
+        t0, u0 = t0 + n, u0 + c

@@ -237,3 +237,82 @@ def test_a_layer_of_four_bit_weights_and_pages():
         assert bool(((mixed.double().cpu() - o).abs() <= 2.0 ** -8 * o.abs() + 0.03).all())
         want = mixed.transpose(1, 2).reshape(B, n, -1).double().cpu() @ w_out.dense().double().cpu().t()
         assert bool(((got - want).abs() <= 2.0 ** -8 * want.abs() + 1e-4).all())
+
+
+@pytest.mark.parametrize("dtype", ["f16", "bf16"])
+@pytest.mark.parametrize("gs,affine", [(32, True), (64, True), (128, True), (32, False), (64, False), (128, False)])
+def test_tiles(gs, affine, dtype):
+    """Calls of many rows at both tile heights: outputs that fill no tile, rows
+    at odd addresses and strides, inputs that fill no tile, a workspace of one's own."""
+    import torch
+
+    from dotcache_amd.projection import project, workspace_bytes
+
+    for M, K, N in ((1030, 256, 1100), (1152, 200, 2688), (2000, 384, 640), (1100, 1024, 1031)):
+        print(f"project tiles {M} {K} {N} {gs} {affine} {dtype}", flush=True)
+        x, w, want, _ = exact_case(M, K, N, gs, affine, dtype, M)
+        need = workspace_bytes(w, x.dtype, M)
+        assert (need > 0) == (dtype == "bf16" or K % 128 != 0)
+        assert torch.equal(project(x, w), want)
+        wide = torch.full((M + 1, K + 11), float("nan"), dtype=x.dtype, device="cuda")
+        rows = wide[1:, 3: 3 + K]
+        rows.copy_(x)
+        out = torch.full((M, N + 5), 5.0, dtype=x.dtype, device="cuda")
+        work = torch.empty(max(need, 1), dtype=torch.uint8, device="cuda")
+        got = project(rows, w, out=out[:, 3: 3 + N], workspace=work)
+        assert torch.equal(got, want) and bool((out[:, :3] == 5).all() and (out[:, 3 + N:] == 5).all())
+        if need:
+            for bad in (work[:-1], torch.empty(need + 8, dtype=torch.uint8, device="cuda")[8:], torch.empty(need, dtype=torch.uint8)):
+                with pytest.raises(ValueError):
+                    project(x, w, workspace=bad)
+
+
+@pytest.mark.parametrize("dtype", ["f16", "bf16"])
+def test_tiles_round_weights_once(dtype):
+    """Any values, many rows: a weight is rounded to fp16 (2^-11), its products summed in
+    fp32 (2^-23 for each term); rows apart by 2^60 in size, and rows of zeros."""
+    import torch
+
+    from dotcache_amd.projection import GroupedWeight, project
+
+    M, K, N, gs = 1100, 320, 1100, 64
+    codes, scales, biases, dense = make(N, K, gs, True, 3, "cuda")
+    w = GroupedWeight.from_codes(codes, scales, biases, group_size=gs)
+    r = np.random.default_rng(3)
+    size = 2.0 ** r.integers(-30, 31, size=(M, 1)) if dtype == "bf16" else np.ones((M, 1))
+    x = torch.from_numpy((r.normal(size=(M, K)) * size).astype(np.float32)).to(_dt(dtype)).cuda()
+    x[5] = 0
+    got, xs = project(x, w).double().cpu().numpy(), x.double().cpu().numpy()
+    want = xs @ dense.T
+    terms = np.abs(xs) @ np.abs(dense).T
+    # (below 2^-14 fp16 keeps steps of 2^-24: half of one for a weight near 0)
+    bound = (2.0 ** -11 + (K + 8) * 2.0 ** -23) * terms + 2.0 ** -25 * np.abs(xs).sum(1, keepdims=True) + HALF[dtype] * np.abs(want)
+    assert np.all(np.abs(got - want) <= bound * (1 + 2.0 ** -20) + 1e-30), float(np.nanmax(np.abs(got - want) / (bound + 1e-30)))
+    x[7, 3], x[9, 319] = float("inf"), float("nan")
+    bad = project(x, w)
+    rows = [i for i in range(M) if i not in (7, 9)]
+    assert torch.equal(bad[rows], torch.from_numpy(got).to(bad.dtype).cuda()[rows]) and not torch.isfinite(bad[[7, 9]]).any()
+
+
+def test_tiles_replay():
+    import torch
+
+    from dotcache_amd.projection import project
+
+    x, w, want, dense = exact_case(1030, 256, 1100, 64, True, "bf16", 4)
+    held, out = x.clone(), torch.zeros_like(want)
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        project(held, w, out=out)
+    torch.cuda.current_stream().wait_stream(side)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        project(held, w, out=out)
+    for f in (2.0 ** 40, 0.5, 1.0, -(2.0 ** -50)):
+        held.copy_(x * f)
+        graph.replay()
+        assert torch.equal(out, (x.double() * f @ dense.t().contiguous()).to(out.dtype))
+        out.zero_()
+        torch.cuda.synchronize()

@@ -50,7 +50,8 @@ def test_weight_refusals():
     for c, s, b, gs in ((codes.float(), scales, biases, 32), (codes[0], scales, biases, 32), (codes, scales, biases, 48), (codes, scales.float(), biases, 32),
                         (codes, scales[:, :3], biases, 32), (codes, scales, biases[:5], 32), (codes + 1, scales, biases, 32),
                         (codes.to(torch.int16) - 1, scales, biases, 32), (torch.full_like(codes, 15), scales, None, 32),
-                        (codes[:0], scales[:0], biases[:0], 32), (codes.bool(), scales, biases, 32)):
+                        (codes[:0], scales[:0], biases[:0], 32), (codes.bool(), scales, biases, 32), (codes, scales * float("nan"), biases, 32),
+                        (codes, scales, biases * float("inf"), 32), (codes, torch.full_like(scales, 5000.0), biases, 32)):
         with pytest.raises(ValueError):
             GroupedWeight.from_codes(c, s, b, group_size=gs)
     for w, kw in ((torch.zeros(4, 64), {}), (torch.zeros(4, 64), dict(group_size=16)), (torch.zeros(64), {}), (torch.zeros(4, 0), {})):
@@ -72,7 +73,7 @@ def test_call_refusals():
 
 def test_entry_refusals():
     L = _lib.lib()
-    for a in ((0, 4, 32), (4, 0, 32), (4, 4, 16), (-1, 4, 32)):
+    for a in ((0, 4, 32), (4, 0, 32), (4, 4, 16), (-1, 4, 32), (4, (1 << 30) + 1, 32), ((1 << 30) + 1, 4, 32)):
         assert L.dc_grouped_weight_bytes(*a, 1, None) == -1
 
     def call(rows=2, data=1 << 20, x=1 << 20, y=1 << 21, xd=0, yd=0, ys=20, gs=32):
