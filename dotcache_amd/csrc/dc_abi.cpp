@@ -305,7 +305,7 @@ static int plan_chunk(const char* who, const int32_t* new_tokens, const int32_t*
       // begin1; its first stretch ends with token end0.
       struct Reach {
         int64_t begin0, near, begin1, len;
-        int32_t end0, end1;
+        int32_t end0, end1, low0, low1;
       };
       struct Tile {
         dc_chunk_item item;
@@ -321,11 +321,11 @@ static int plan_chunk(const char* who, const int32_t* new_tokens, const int32_t*
             hi[k] = std::max(hi[k], r[4 * t + 2 * k + 1]);
           }
         if (lo[0] > lo[1]) std::swap(lo[0], lo[1]), std::swap(hi[0], hi[1]);
-        if (hi[0] == 0) return Reach{0, 0, 0, 1, 0, 1};  // rows that see nothing: zeros have to be written
+        if (hi[0] == 0) return Reach{0, 0, 0, 1, 0, 1, 0, 0};  // rows that see nothing: zeros have to be written
         const int64_t b0 = lo[0] / step, e0 = (hi[0] + step - 1) / step, b1 = lo[1] / step, e1 = (hi[1] + step - 1) / step;
-        if (hi[1] == 0) return Reach{0, 0, b0, e0 - b0, 0, hi[0]};
-        if (b1 <= e0) return Reach{0, 0, b0, std::max(e0, e1) - b0, 0, std::max(hi[0], hi[1])};
-        return Reach{b0, e0 - b0, b1, e0 - b0 + e1 - b1, hi[0], hi[1]};
+        if (hi[1] == 0) return Reach{0, 0, b0, e0 - b0, 0, hi[0], 0, lo[0]};
+        if (b1 <= e0) return Reach{0, 0, b0, std::max(e0, e1) - b0, 0, std::max(hi[0], hi[1]), 0, lo[0]};
+        return Reach{b0, e0 - b0, b1, e0 - b0 + e1 - b1, hi[0], hi[1], lo[0], lo[1]};
       };
       std::vector<Tile> tiles;
       int64_t total = 0;
@@ -338,7 +338,7 @@ static int plan_chunk(const char* who, const int32_t* new_tokens, const int32_t*
         for (int32_t r = 0; r < rows; r += dc::kChunkRows) {
           const int32_t r1 = std::min(r + dc::kChunkRows, rows), t0 = r / n_q, t1 = (r1 - 1) / n_q + 1, end = first + t1;
           reach.push_back(ranges ? reach_of(ranges + 4 * (int64_t(q_begin) + t0), t1 - t0)
-                                 : Reach{0, 0, 0, (int64_t(end) + step - 1) / step, 0, end});
+                                 : Reach{0, 0, 0, (int64_t(end) + step - 1) / step, 0, end, 0, 0});
         }
         for (int32_t h = 0; h < n_kv_heads; ++h)
           for (int32_t r = 0; r < rows; r += dc::kChunkRows) {
@@ -449,6 +449,10 @@ static int plan_chunk(const char* who, const int32_t* new_tokens, const int32_t*
           const bool from_near = d[i].begin < z.near, to_near = d[i].end <= z.near;
           x.kv_begin = int32_t((from_near ? z.begin0 + d[i].begin : z.begin1 + d[i].begin - z.near) * step);
           x.kv_end = int32_t(std::min<int64_t>((to_near ? z.begin0 + d[i].end : z.begin1 + d[i].end - z.near) * step, to_near ? z.end0 : z.end1));
+          // (what the range's first rows see may begin later in its step: at a multiple of every
+          // kernel's part of a page; a gap's place counts from the begin, so an item with one stays)
+          const int32_t low = from_near ? z.low0 : z.low1;
+          if ((from_near == to_near || !from_near) && low > x.kv_begin) x.kv_begin = low / 32 * 32;
           left_out.push_back(from_near && !to_near ? std::make_pair(int32_t((z.begin0 + z.near) * step), int32_t(z.begin1 * step))
                                                    : std::make_pair(-1, -1));
           const auto& p = of[d[i].tile];

@@ -7,7 +7,7 @@
 namespace dc {
 
 constexpr int kChunkRows = 256;   // query rows of a work item
-constexpr int kChunkStep = 128;   // token ranges begin at multiples of this (a multiple of every tile)
+constexpr int kChunkStep = 128;   // token ranges begin at multiples of this (a multiple of every tile), or of 32 where nobody sees what is ahead
 constexpr int kChunkXcds = 8;     // consecutive blocks go to consecutive dies, each with an L2 of its own
 
 // Rows of one item of the few-row kernel at most, by what its registers hold.

@@ -252,13 +252,6 @@ __device__ __forceinline__ void shape_scores(const ChunkArgs& a, float c, const 
   }
 }
 
-// Moves an item's begin past whole tiles of `tile` tokens that none of its rows
-// sees (items begin at multiples of kChunkStep); its gap, if any, stays ahead.
-__device__ __forceinline__ void skip_unseen(dc_chunk_item& it, const Sight& s, int2 gap, int tile) {
-  const int to = min(min(s.any0, s.any20), gap.x >= 0 ? gap.x - tile : it.kv_end - 1);
-  if (to > it.kv_begin) it.kv_begin += (to - it.kv_begin) / tile * tile;
-}
-
 // The item's gap: its tiles leave out tokens [x, y).
 __device__ __forceinline__ int2 item_gap(const ChunkArgs& a, uint32_t item) { return a.gaps ? a.gaps[item] : int2{-1, -1}; }
 
@@ -301,7 +294,6 @@ __global__ void __launch_bounds__(256, sizeof(T) == 4 && HDP == 256 ? 1 : 2) att
     mine = sight_of(a, it, it.row_begin + 32 * wave, min(it.row_begin + 32 * wave + 32, it.row_end));
     all = sight_of(a, it, it.row_begin, it.row_end);
     gap = item_gap(a, block_index(kChunkRows / 128));
-    skip_unseen(it, all, gap, KT);
   }
   auto seen = [&](int u) { return RULE ? rule.sees(u) : u <= sees; };
 
@@ -785,11 +777,7 @@ __global__ void __launch_bounds__(512, 2) attend_chunk16_kernel(ChunkArgs a) {
   Sight mine, all;  // the wavefront's rows' and the block's
   int gap_tile = INT32_MAX, gap_len = 0;
   if constexpr (RULE) {
-    rule = row_rule(a, it, has_row, tok, head);
-    mine = sight_of(a, it, it.row_begin + rows_at, min(it.row_begin + rows_at + 32, it.row_end));
-    all = sight_of(a, it, it.row_begin, it.row_end);
     const int2 gap = item_gap(a, block_index(CS));
-    skip_unseen(it, all, gap, KT);
     if (gap.x >= 0) gap_tile = (gap.x - it.kv_begin) / KT, gap_len = gap.y - gap.x;
   }
   auto seen = [&](int u) { return RULE ? rule.sees(u) : u <= sees; };
@@ -891,6 +879,11 @@ __global__ void __launch_bounds__(512, 2) attend_chunk16_kernel(ChunkArgs a) {
   load_ids(1);
   load_units(0, even);
   load_units(1, odds);
+  if constexpr (RULE) {  // (while the pages' rows are on their way)
+    rule = row_rule(a, it, has_row, tok, head);
+    mine = sight_of(a, it, it.row_begin + rows_at, min(it.row_begin + rows_at + 32, it.row_end));
+    all = sight_of(a, it, it.row_begin, it.row_end);
+  }
 
   // ---- queries: row col, channels 16 k + 8 half .. + 7 in LDS order
   h8v q[QW];
@@ -1161,7 +1154,7 @@ __global__ void __launch_bounds__(64 * kFewWaves, 2) attend_few_kernel(ChunkArgs
   __shared__ float ml[kFewWaves][16 * NB][2];
   __shared__ float odd[kFewWaves][HDP];
 
-  dc_chunk_item it = a.items[blockIdx.x];
+  const dc_chunk_item it = a.items[blockIdx.x];
   if (!chunk_item_ok(it, a) || it.row_end - it.row_begin > 16 * NB) return;
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int col = lane & 15, g = lane >> 4;
@@ -1175,7 +1168,6 @@ __global__ void __launch_bounds__(64 * kFewWaves, 2) attend_few_kernel(ChunkArgs
   if constexpr (RULE) {
     all = sight_of(a, it, it.row_begin, it.row_end);
     const int2 gap = item_gap(a, blockIdx.x);
-    skip_unseen(it, all, gap, kFewTile);
     if (gap.x >= 0) gap_tile = (gap.x - it.kv_begin) / kFewTile, gap_len = gap.y - gap.x;
   }
   h8v q[QL ? 1 : NB][QL ? 1 : KS];

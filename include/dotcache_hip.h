@@ -638,7 +638,8 @@ typedef struct dc_score_rule {
 /* dc_plan_chunk where new token t (of all sequences, one after another) attends
  * tokens [ranges[t][0], ranges[t][1]) and [ranges[t][2], ranges[t][3]) of its
  * sequence (host int32, 0 <= first <= end <= the context, apart from each
- * other): a row tile's items cover what its rows attend, in steps of 128 tokens.
+ * other): a row tile's items cover what its rows attend, in steps of 128 tokens (a
+ * first one from a multiple of 32 on).
  * An item that takes tokens of two stretches leaves out [gaps[i][0], gaps[i][1])
  * between them ({-1, -1}: nothing left out; host [max_items][2]). */
 int dc_plan_chunk_ranges(const int32_t* new_tokens, const int32_t* context, const int32_t* ranges, int32_t n_seqs,

@@ -57,7 +57,7 @@ def test_items_cover_what_rows_attend(kw, target):
         x = dict(zip(_lib.CHUNK_ITEM_FIELDS, x))
         if x["seq"] < 0:
             continue
-        assert x["kv_begin"] % 128 == 0 and x["kv_begin"] < x["kv_end"] <= ctx[x["seq"]]
+        assert x["kv_begin"] % (32 if gap == [-1, -1] else 128) == 0 and x["kv_begin"] < x["kv_end"] <= ctx[x["seq"]]
         taken = np.zeros(ctx[x["seq"]], dtype=int)
         taken[x["kv_begin"]: x["kv_end"]] = 1
         if gap != [-1, -1]:
