@@ -26,7 +26,7 @@
 // over 16384 tokens, fp16 keys and 4-bit values, 1.31 ms with the join, 690
 // TFLOP/s of an fp16 library product's 1178; 1.04 ms without the page loads),
 // attend_few_kernel (the same pages, few rows against a long range: 5 rows of 7
-// heads of four sequences to 131072 tokens, 126 MB, 101 us with the join, where
+// heads of four sequences to 131072 tokens, 126 MB, 92 us with the join, where
 // the copy rate would take 27; when it was made 170 us, the 256-row kernel 320) and
 // attend_chunk_kernel (the rest: 3 x 61 rows of 1001 tokens in fp32 83 us and 7
 // for the join; the two calls above, made with 16-bit queries on pools that have
@@ -36,6 +36,13 @@
 // once, by 2^-11 relative, or below 2^-14 (a weight: below 2^-21 of the row's
 // largest) by 2^-25 (2^-32 of the largest).  All of a row's ranges lift their
 // weights alike (kLift), so that joins and the final division cancel it.
+//
+// RULE: tokens of any two ranges a row, and shaped scores (dc_attend_chunk_rule).
+// A tile's products are turned into exponents (cap, slope) where they lie, then
+// masked; a tile that no row of a wavefront sees is none of its work, one that all see
+// whole has no mask.  A cap costs 11 % (2 x 2048 rows at head_dim 256, window
+// 4096: 749 -> 834 us), slopes 25 % (1024 rows of 4096 tokens at head_dim 64: 77
+// -> 97).
 #pragma once
 
 #include <atomic>

@@ -649,8 +649,8 @@ int dc_plan_chunk_ranges(const int32_t* new_tokens, const int32_t* context, cons
                          int32_t* n_partials);
 
 /* dc_attend_chunk with a rule; items of dc_plan_chunk, or of
- * dc_plan_chunk_ranges with the ranges and gaps that belong to them.  Reference
- * models with windows and capped scores: dotcache/integrations/gemma4.py. */
+ * dc_plan_chunk_ranges with the ranges and gaps that belong to them.  The
+ * reference leaves such layers to its models (dotcache/integrations/gemma4.py). */
 int dc_attend_chunk_rule(dc_pool k_pool, dc_pool v_pool, const int32_t* k_table, const int32_t* v_table, int32_t table_stride,
                          const dc_chunk_item* items, int32_t n_items, int32_t n_few, int32_t few_rows,
                          const dc_chunk_merge* merges, int32_t n_merges, int32_t n_partials, int32_t n_seqs,
