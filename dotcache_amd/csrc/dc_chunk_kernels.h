@@ -176,8 +176,8 @@ __device__ __forceinline__ bool block_rows(dc_chunk_item& it, int part, int rows
 // The tokens that a query row sees, first .. first + len - 1 and first2 ..
 // first2 + len2 - 1, its own token and its slope.
 struct RowRule {
-  int first, len, first2, len2;
-  float at, slope;
+  int first, len, first2, len2, at;
+  float slope;
   __device__ __forceinline__ bool sees(int u) const {
     return uint32_t(u - first) < uint32_t(len) || uint32_t(u - first2) < uint32_t(len2);
   }
@@ -191,7 +191,7 @@ __device__ __forceinline__ int4 token_range(const ChunkArgs& a, const dc_chunk_i
 // (a row that does not exist sees nothing)
 __device__ __forceinline__ RowRule row_rule(const ChunkArgs& a, const dc_chunk_item& it, bool has_row, int tok, int head) {
   const int4 r = token_range(a, it, has_row ? tok : it.row_begin / a.n_q);
-  return RowRule{r.z, has_row ? r.w - r.z : 0, r.x, has_row ? r.y - r.x : 0, float(it.first + tok),
+  return RowRule{r.z, has_row ? r.w - r.z : 0, r.x, has_row ? r.y - r.x : 0, it.first + tok,
                  a.slopes && has_row ? a.slopes[head] * kLog2e : 0.f};
 }
 
@@ -251,7 +251,7 @@ __device__ __forceinline__ void shape_scores(const ChunkArgs& a, float c, const 
       for (int v = 0; v < W; ++v) s[i][v] *= c;
   }
   if (a.slopes) {
-    const float away = r.at - float(u);
+    const float away = float(r.at - u);  // (the difference of far tokens is exact, they themselves are not)
 #pragma unroll
     for (int i = 0; i < N; ++i)
 #pragma unroll

@@ -75,13 +75,14 @@ class GroupedWeight:
             if tuple(x.shape) != (N, G) or x.dtype != torch.float16 or x.device != codes.device:
                 raise ValueError(f"{name} must be fp16 [{N}, {G}] on the codes' device")
         _check_levels(scales, biases)
-        if int(codes.min()) < 0 or int(codes.max()) > (15 if biases is not None else 14):
-            raise ValueError(f"codes must lie in [0, {15 if biases is not None else 14}]")
+        most = 15 if biases is not None else 14
         data = _new_data(N, K, gs, biases is not None, codes.device)
         # rows in portions: a portion's codes are widened to 32 bits
         step = max(_TILE_N, (1 << 24) // K // _TILE_N * _TILE_N)
         for r in range(0, N, step):
             part = codes[r: r + step].to(torch.int32)
+            if int(part.min()) < 0 or int(part.max()) > most:
+                raise ValueError(f"codes must lie in [0, {most}]")
             part = torch.nn.functional.pad(part, (0, -K % _TILE_K, 0, -part.shape[0] % _TILE_N))
             _put(data, N, K, gs, r, part.unflatten(-1, (-1, 8)), scales[r: r + step], None if biases is None else biases[r: r + step])
         return cls(data, N, K, gs, biases is not None)

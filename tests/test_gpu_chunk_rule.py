@@ -240,6 +240,30 @@ def test_strides_padding_and_far_tokens():
     check_rule(batch, [3, 40], 2, "f32", rng, slopes=0.01, mask=mask)
 
 
+@pytest.mark.parametrize("dtype", ["f32", "f16"])
+def test_distances_of_far_tokens(dtype):
+    """Past token 2^24 the distance still counts whole tokens: the last ones of
+    a context whose other pages are not there weigh as in a short one."""
+    import torch
+
+    from dotcache_amd.chunk import attend_chunk, plan_chunk
+
+    rng = np.random.default_rng(1)
+    far, P = 2 ** 24 + 3 * 64, 64
+    batch = _Batch(rng, [64], 1, 64, P, "a4", "a4", tail=False)
+    q = torch.from_numpy(rng.normal(size=(3, 2, 64)).astype(np.float32)).to(_dt(dtype)).cuda()
+    sl = torch.tensor([0.9, 0.3], device="cuda")
+    mask = ChunkMask(window=40)
+    near = batch.attend(q, batch.plan([3], 2, mask=mask), 0.125, slopes=sl)
+    tables = [torch.full((1, 1, (far + 64) // P), -1, dtype=torch.int32, device="cuda") for _ in range(2)]
+    for t, kept in zip(tables, batch.tables):
+        t[0, 0, -1] = kept[0, 0, 0]
+    plan = plan_chunk(*batch.pools, [3], [far + 64], kv_heads=1, q_per_kv=2, mask=mask)
+    got = attend_chunk(batch.pools[0], tables[0], batch.pools[1], tables[1], q, plan, query_scale=0.125, slopes=sl)
+    # (the same pages, tokens and distances; the wavefronts may take them in another order)
+    assert float((got.double() - near.double()).abs().max()) <= 4 * torch.finfo(q.dtype).eps * float(near.abs().max())
+
+
 def test_replays_and_streams():
     """A captured call replayed with other queries and slopes, eager work in
     between, and the same call on another stream."""

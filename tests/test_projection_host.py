@@ -43,6 +43,8 @@ def test_layout(N, K, gs, affine):
             inside = n < N and k // gs < scales.shape[1]
             assert s[0] == (scales[n, k // gs] if inside else 0) and (not affine or s[1] == (biases[n, k // gs] if inside else 0))
     assert np.array_equal(w.dense(torch.float64).numpy(), dense.astype(np.float32))
+    for t in (torch.int8, torch.uint16, torch.int64):
+        assert torch.equal(GroupedWeight.from_codes(codes.to(t), scales, biases, group_size=gs).data, w.data)
 
 
 def test_weight_refusals():
