@@ -158,17 +158,19 @@ __global__ void __launch_bounds__(1024) project_few_kernel(ProjectArgs a) {
   }
 }
 
-// Sum of a row's eight 16-bit inputs.
+// Sum of a row's eight 16-bit inputs (products with 1, which are exact; fp32 sums).
 template <int DT>
 __device__ __forceinline__ float sum8(const uint4& x) {
+  typedef _Float16 h2v __attribute__((ext_vector_type(2)));
+  typedef __bf16 b2v __attribute__((ext_vector_type(2)));
   float s = 0.f;
 #pragma unroll
   for (int i = 0; i < 4; ++i) {
     const uint32_t w = (&x.x)[i];
     if constexpr (DT == DC_F16)
-      s += float(__builtin_bit_cast(_Float16, uint16_t(w))) + float(__builtin_bit_cast(_Float16, uint16_t(w >> 16)));
+      s = __builtin_amdgcn_fdot2(__builtin_bit_cast(h2v, w), __builtin_bit_cast(h2v, 0x3c003c00u), s, false);
     else
-      s += __builtin_bit_cast(float, w << 16) + __builtin_bit_cast(float, w & 0xffff0000u);
+      s = __builtin_amdgcn_fdot2_f32_bf16(__builtin_bit_cast(b2v, w), __builtin_bit_cast(b2v, 0x3f803f80u), s, false);
   }
   return s;
 }
