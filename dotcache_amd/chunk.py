@@ -288,7 +288,7 @@ def attend_chunk(pool: DevicePagePool, k_table, v_pool: DevicePagePool | None, v
     if out is None:
         if queries.shape[0] != plan.n_tokens:
             raise ValueError("queries past the plan's tokens (padding) need an out tensor, whose rows there are left")
-        out = torch.empty(queries.shape, dtype=queries.dtype, device=device)
+        out = queries.new_empty(queries.shape)
     elif out.shape != queries.shape or out.dtype != queries.dtype:
         raise ValueError("out must have the queries' shape and dtype")
     q_rows, out_rows = token_rows(queries, "queries", hd, device), token_rows(out, "out", hd, device)
@@ -303,7 +303,7 @@ def attend_chunk(pool: DevicePagePool, k_table, v_pool: DevicePagePool | None, v
     if need == 0:
         workspace = None
     elif workspace is None:
-        workspace = torch.empty(need, dtype=torch.uint8, device=device)
+        workspace = queries.new_empty(need, dtype=torch.uint8)
     elif workspace.numel() * workspace.element_size() < need or not workspace.is_contiguous() or workspace.device != device:
         raise ValueError(f"workspace must be contiguous, {need} bytes at least, on {device}")
     elif workspace.data_ptr() % 16:
