@@ -78,18 +78,20 @@ __device__ __forceinline__ uint4 x_operand(const Eight<DT>& x, int part) {
   return uint4{out[0], out[1], out[2], out[3]};
 }
 
+constexpr int kFewWaves = 8;
+
 }  // namespace
 
 // Up to 16 rows by 16 outputs per block.  Bound by reading the weights (few
 // bytes: by the time from a launch to its first word), so its wavefronts split
-// the inputs' tiles among them, in turn, with the next tile's words, scales and
-// rows on their way while one is worked on, and join in order at the end.
+// the inputs' tiles among them, a few tiles each in a round whose loads are all
+// made first, and join in order at the end.
 template <int DT, int GS, bool AFFINE>
-__global__ void __launch_bounds__(1024) project_few_kernel(ProjectArgs a) {
+__global__ void __launch_bounds__(64 * kFewWaves) project_few_kernel(ProjectArgs a) {
   constexpr int PARTS = DT == DC_F32 ? 3 : 1, OT = DT == DC_F32 ? DC_BF16 : DT, SC = kTileK / GS * (AFFINE ? 2 : 1);
   constexpr int T = DT == DC_F32 ? 1 : 2;  // tiles a round (4: the same time, more code)
   constexpr uint32_t kOne = OT == DC_F16 ? 0x3c003c00u : 0x3f803f80u;
-  __shared__ f32x4 joined[16][64];
+  __shared__ f32x4 joined[kFewWaves][64];
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), waves = blockDim.x >> 6;
   const int col = lane & 15, g = lane >> 4;
   const int64_t row0 = int64_t(blockIdx.y) * 16;
@@ -314,12 +316,11 @@ __global__ void __launch_bounds__(256) project_short_kernel(ProjectArgs a, int32
   store_y<DT>(a.y, r * a.y_stride + out, fmaf(s, sum, b * xs));
 }
 
-// Wavefronts per block: where blocks alone leave the card's 1024 SIMDs
-// less than four wavefronts each, up to 16, but none without a tile.
+// Wavefronts per block of project_few_kernel: where blocks of four leave the
+// card's 1024 SIMDs less than four wavefronts each, kFewWaves, but none without a
+// tile (16 leave a compute unit one block: one row of 3584 x 4608 7.4 us, 8 6.2).
 static int waves_of(int64_t blocks, int k_tiles) {
-  int w = 4;
-  while (w < 8 && blocks * w < 4096 && 2 * w <= k_tiles) w *= 2;
-  return w;
+  return blocks * 4 < 4096 && kFewWaves <= k_tiles ? kFewWaves : 4;
 }
 
 // launch(args, grid) for portions of the rows: a launch's second dimension holds
