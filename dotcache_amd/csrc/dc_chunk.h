@@ -13,6 +13,9 @@ constexpr int kChunkXcds = 8;     // consecutive blocks go to consecutive dies, 
 // Rows of one item of the few-row kernel at most, by what its registers hold.
 constexpr int few_row_limit(int head_dim) { return head_dim <= 64 ? 64 : head_dim <= 128 ? 48 : 16; }
 
+// Kernels of plain causal attention, with a rule, and with a rule and a cap.
+enum { kCausal = 0, kRuled = 1, kCapped = 2 };
+
 struct ChunkArgs {
   dc_pool kpool, vpool;
   const int32_t* k_table;
@@ -34,7 +37,7 @@ struct ChunkArgs {
   uint32_t page_mul, page_shift;
   int32_t q_vec, o_vec;  // rows start at multiples of 16 (8) bytes
   // kernels with a rule (dc_score_rule):
-  float cap;              // cap log2 e, or 0: none
+  float cap;              // cap log2 e (kCapped)
   float cap_in;           // 2 scale log2 e / cap
   const float* slopes;    // [n_kv_heads * n_q] or null
   const int4* ranges;     // [n_tokens] {first, end, first, end}, or null: causal
@@ -61,6 +64,7 @@ __device__ __forceinline__ bool chunk_merge_ok(const dc_chunk_merge& m, const Ch
 // `units`, 16-bit queries on pages of 32-channel units.
 int launch_chunks(ChunkArgs a, int32_t n_few, int32_t few_rows, bool units, hipStream_t stream);
 int launch_chunks_rule(ChunkArgs a, int32_t n_few, int32_t few_rows, bool units, hipStream_t stream);
+int launch_chunks_cap(ChunkArgs a, int32_t n_few, int32_t few_rows, bool units, hipStream_t stream);
 
 __device__ __forceinline__ void store_value(void* p, int32_t dtype, int64_t i, float x) {
   if (dtype == DC_F32)

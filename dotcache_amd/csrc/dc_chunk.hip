@@ -168,20 +168,21 @@ static int attend_chunk(const char* who, dc_pool k_pool, dc_pool v_pool, const i
   a.page_mul = uint32_t(((uint64_t(1) << a.page_shift) + P - 1) / P);
   if (rule) {
     a.cap = rule->cap * kLog2e;
-    a.cap_in = rule->cap > 0.f ? 2.f * a.scale * kLog2e / rule->cap : 0.f;
+    a.cap_in = rule->cap > 0.f ? float(2.0 * a.scale * kLog2e / rule->cap) : 0.f;
     a.slopes = rule->slopes;
     a.ranges = reinterpret_cast<const int4*>(rule->ranges);
     a.gaps = reinterpret_cast<const int2*>(rule->gaps);
     if (!(a.cap <= 3e38f && a.cap_in <= 3e38f)) return fail(DC_EINVAL, "%s: cap is out of range for the scale", who);
   }
   const bool units = q.dtype != DC_F32 && units32(k_pool) && units32(v_pool);
-  if (int rc = rule ? launch_chunks_rule(a, n_few, few_rows, units, st) : launch_chunks(a, n_few, few_rows, units, st)) return rc;
+  const auto launch = !rule ? launch_chunks : rule->cap > 0.f ? launch_chunks_cap : launch_chunks_rule;
+  if (int rc = launch(a, n_few, few_rows, units, st)) return rc;
   // (items of few rows alone: blocks for those rows)
   return n_merges ? launch_merge_chunk(a, merges, n_merges, n_few == n_items ? few_rows : kMergeBlocks, st) : DC_OK;
 }
 
 int launch_chunks(ChunkArgs a, int32_t n_few, int32_t few_rows, bool units, hipStream_t stream) {
-  return launch_all<false>(a, n_few, few_rows, units, stream);
+  return launch_all<kCausal>(a, n_few, few_rows, units, stream);
 }
 
 }  // namespace dc

@@ -37,7 +37,8 @@
 // largest) by 2^-25 (2^-32 of the largest).  All of a row's ranges lift their
 // weights alike (kLift), so that joins and the final division cancel it.
 //
-// RULE: tokens of any two ranges a row, and shaped scores (dc_attend_chunk_rule).
+// RULE, kRuled or kCapped: tokens of any two ranges a row, and shaped scores (dc_attend_chunk_rule),
+// instances with a cap apart (its code took registers that those without it need: 4 % at head_dim 64).
 // A tile's products are turned into exponents (cap, slope) where they lie, then
 // masked; a tile that no row of a wavefront sees is none of its work, one that all see
 // whole has no mask.  A cap costs 11 % (2 x 2048 rows at head_dim 256, window
@@ -227,23 +228,50 @@ __device__ __forceinline__ Sight sight_of(const ChunkArgs& a, const dc_chunk_ite
 }
 
 // A product q . k as the exponent of its weight, in log2, before the maximum:
-// cap tanh(scale q.k / cap) = cap (1 - 2 / (exp2(cap_in q.k) + 1)), which holds
-// at either infinity, or scale q.k (c: scale log2 e).
-__device__ __forceinline__ float capped(const ChunkArgs& a, float s) {
-  return fmaf(-2.f * a.cap, __builtin_amdgcn_rcpf(__builtin_amdgcn_exp2f(a.cap_in * s) + 1.f), a.cap);
+// cap tanh(y), y = scale q.k / cap and x = 2 y log2 e, or (no cap) scale q.k.
+// Where |y| < 1/2 it is x times a polynomial of x^2 for tanh(y) / y (fitted to
+// 2^-26 there), so that the error is a share of the score, whatever the cap.  Beyond,
+// cap (1 - 2 / (exp2(|x|) + 1)) with the sign, which holds at either infinity and cancels little.
+__device__ __forceinline__ float capped(const ChunkArgs& a, float x) {
+  const float t = x * x;
+  float near = a.cap * x * fmaf(t, fmaf(t, fmaf(t, fmaf(t, 1.2437525e-06f, -3.1857868e-05f), 6.6630519e-04f), -1.3875948e-02f), 0.34657359f);
+  float far = fmaf(-2.f * a.cap, __builtin_amdgcn_rcpf(__builtin_amdgcn_exp2f(fabsf(x)) + 1.f), a.cap);
+  asm volatile("" : "+v"(near), "+v"(far));  // (both, and a selection: no branch for each score)
+  return fabsf(x) < 1.44269504f ? near : __builtin_copysignf(far, x);
+}
+
+// The second form alone, for 16-bit queries and caps to kCoarseCap: off by 2^-21 of the cap
+// whatever the score, so a weight by 2^-13, where its own rounding to fp16 and those
+// of its logit's operands are 2^-11 each (2 x 2048 rows at head_dim 256, window 4096: 826 us, the other 945).
+constexpr float kCoarseCap = 256.f;
+__device__ __forceinline__ float capped_coarse(float cap, float x) {
+  return fmaf(-2.f * cap, __builtin_amdgcn_rcpf(__builtin_amdgcn_exp2f(x) + 1.f), cap);
 }
 
 // The products of a row with blocks of tokens as such exponents: element v of
 // block i is token u + 32 i + 8 (v / 4) + v % 4 (16 elements a block), or token
 // u + 16 i + v (4 elements).
-template <typename V, int N>
+template <bool CAP, bool EXACT, typename V, int N>
 __device__ __forceinline__ void shape_scores(const ChunkArgs& a, float c, const RowRule& r, int u, V (&s)[N]) {
   constexpr int W = sizeof(V) / 4;
-  if (a.cap > 0.f) {
+  if constexpr (CAP) {
+    // (factors of its own: products common to both branches would be taken ahead of them, into registers)
+    float cap = a.cap, cap_in = a.cap_in;
+    asm volatile("" : "+s"(cap), "+s"(cap_in));
+    if (!EXACT && cap <= kCoarseCap * kLog2e) {  // (uniform)
 #pragma unroll
-    for (int i = 0; i < N; ++i)
+      for (int i = 0; i < N; ++i)
 #pragma unroll
-      for (int v = 0; v < W; ++v) s[i][v] = capped(a, s[i][v]);
+        for (int v = 0; v < W; ++v) s[i][v] = capped_coarse(cap, cap_in * s[i][v]);
+    } else {
+#pragma unroll
+      for (int i = 0; i < N; ++i)
+#pragma unroll
+        for (int v = 0; v < W; ++v) {
+          s[i][v] = capped(a, a.cap_in * s[i][v]);
+          if (v % 4 == 3) __builtin_amdgcn_sched_barrier(0);  // (four at a time, for the registers)
+        }
+    }
   } else {
 #pragma unroll
     for (int i = 0; i < N; ++i)
@@ -266,7 +294,7 @@ __device__ __forceinline__ int2 item_gap(const ChunkArgs& a, uint32_t item) { re
 
 // T: the matrix operands, _Float16 or float.  HDP: head_dim rounded up to the
 // operands' rows (channels past head_dim are zeros).  KT: tokens per tile.
-template <typename T, int HDP, int KT, bool RULE>
+template <typename T, int HDP, int KT, int RULE>
 __global__ void __launch_bounds__(256, sizeof(T) == 4 && HDP == 256 ? 1 : 2) attend_chunk_kernel(ChunkArgs a) {
   constexpr bool F32 = sizeof(T) == 4;
   constexpr int CH = HDP * int(sizeof(T)) / 16;  // 16-byte chunks of a row
@@ -445,7 +473,7 @@ __global__ void __launch_bounds__(256, sizeof(T) == 4 && HDP == 256 ? 1 : 2) att
         }
       }
     }
-    if constexpr (RULE) shape_scores(a, c, rule, u0 + 4 * half, s);
+    if constexpr (RULE) shape_scores<RULE == kCapped, F32>(a, c, rule, u0 + 4 * half, s);
     // tokens that do not count, or that this row does not see
     bool masked = RULE ? !mine.whole(u0, KT) : u0 + KT - 1 > sees_all;
 #pragma unroll
@@ -755,7 +783,7 @@ __device__ __forceinline__ uint32_t fold_tokens(uint64_t b) {
 // (head_dim 256, whose queries and output of 32 rows fill the registers).
 // WHOLE: head_dim is HDP, so that no channel is left out and no mask kept for it
 // (12 sequences at head_dim 256 608 -> 597 us, five rows of four long sequences 98 -> 95).
-template <int HDP, int KT, bool UNI, int CS, bool WHOLE, bool RULE>
+template <int HDP, int KT, bool UNI, int CS, bool WHOLE, int RULE>
 __global__ void __launch_bounds__(512, 2) attend_chunk16_kernel(ChunkArgs a) {
   constexpr int CH = HDP / 8, TB = KT / 32, CB = HDP / 32 / CS, TILE = KT * HDP * 2, QW = HDP / 16;
   constexpr int NT = KT < 64 ? 8 : KT / 8;  // tokens a wavefront turns
@@ -964,7 +992,7 @@ __global__ void __launch_bounds__(512, 2) attend_chunk16_kernel(ChunkArgs a) {
         s[n % TB] = __builtin_amdgcn_mfma_f32_32x32x16_f16(ka[n % kAhead], q[n / TB], s[n % TB], 0, 0, 0);
         if (n + kAhead < QW * TB) ka[n % kAhead] = key(n + kAhead);
       }
-      if constexpr (RULE) shape_scores(a, c, rule, u0 + 4 * half, s);
+      if constexpr (RULE) shape_scores<RULE == kCapped, false>(a, c, rule, u0 + 4 * half, s);
       bool masked = RULE ? !mine.whole(u0, KT) : u0 + KT - 1 > sees_all;
 #pragma unroll
       for (int tb = 0; tb < TB; ++tb) masked = masked || on[tb] != ~0u;
@@ -1148,7 +1176,7 @@ __device__ __forceinline__ uint32_t zero_of(int kind, bool affine) {
 // a token's scales lie side by side, and are one load.  The loads' issue is half of
 // a long range's time, so what counts is how few they are: a decode of 8
 // sequences of 32768 tokens at head_dim 256, 336 MB, 172 -> 131 us.
-template <int HDP, int NB, int KW, bool UNI, bool WHOLE, bool RULE>
+template <int HDP, int NB, int KW, bool UNI, bool WHOLE, int RULE>
 __global__ void __launch_bounds__(64 * kFewWaves, 2) attend_few_kernel(ChunkArgs a) {
   constexpr int CH = HDP / 8, KS = HDP / 32, CB = HDP / 16, TILE = kFewTile * HDP * 2;
   constexpr int VC = HDP / 2, VU = VC / 32;  // a lane's value channels, in units of 32
@@ -1515,7 +1543,7 @@ __global__ void __launch_bounds__(64 * kFewWaves, 2) attend_few_kernel(ChunkArgs
     h8v p[NB];
 #pragma unroll
     for (int n = 0; n < NB; ++n) {
-      if constexpr (RULE) shape_scores(a, c, rule[n], u0 + 4 * g, s[n]);
+      if constexpr (RULE) shape_scores<RULE == kCapped, false>(a, c, rule[n], u0 + 4 * g, s[n]);
       if (border || live != ~0u) {
 #pragma unroll
         for (int b = 0; b < 2; ++b)
@@ -1681,7 +1709,7 @@ struct LdsLimit {
   }
 };
 
-template <typename T, int HDP, int KT, bool RULE>
+template <typename T, int HDP, int KT, int RULE>
 static int launch_chunk(const ChunkArgs& a, hipStream_t stream) {
   constexpr int bytes = 2 * KT * HDP * int(sizeof(T)) + 16;
   static LdsLimit limit;
@@ -1690,7 +1718,7 @@ static int launch_chunk(const ChunkArgs& a, hipStream_t stream) {
   return check_hip(hipGetLastError(), "attend_chunk_kernel launch");
 }
 
-template <int HDP, int KT, bool UNI, int CS, bool WHOLE, bool RULE>
+template <int HDP, int KT, bool UNI, int CS, bool WHOLE, int RULE>
 static int launch_chunk16_as(const ChunkArgs& a, hipStream_t stream) {
   constexpr int bytes = 4 * KT * HDP * 2;
   static LdsLimit limit;
@@ -1699,14 +1727,14 @@ static int launch_chunk16_as(const ChunkArgs& a, hipStream_t stream) {
   return check_hip(hipGetLastError(), "attend_chunk16_kernel launch");
 }
 
-template <int HDP, int KT, int CS, bool RULE>
+template <int HDP, int KT, int CS, int RULE>
 static int launch_chunk16(const ChunkArgs& a, hipStream_t stream) {
   if (a.kpool.geometry.page_capacity % (KT < 64 ? 8 : KT / 8) != 0) return launch_chunk16_as<HDP, KT, false, CS, false, RULE>(a, stream);
   return a.kpool.geometry.head_dim == HDP ? launch_chunk16_as<HDP, KT, true, CS, true, RULE>(a, stream)
                                           : launch_chunk16_as<HDP, KT, true, CS, false, RULE>(a, stream);
 }
 
-template <int HDP, int NB, int KW, bool UNI, bool WHOLE, bool RULE>
+template <int HDP, int NB, int KW, bool UNI, bool WHOLE, int RULE>
 static int launch_few_as(const ChunkArgs& a, hipStream_t stream) {
   constexpr int tiles = kFewWaves * kFewTile * HDP * 2 + (NB * HDP >= 256 ? 16 * NB * HDP * 2 : 0), joined = few_joined_bytes(HDP, NB), bytes = tiles > joined ? tiles : joined;
   static LdsLimit limit;
@@ -1722,7 +1750,7 @@ static bool codes4(const dc_pool& p) {
   return p.geometry.group_size == 32 && (p.format_mask & four) != 0 && (p.format_mask & others) == 0;
 }
 
-template <int HDP, int NB, int KW, bool RULE>
+template <int HDP, int NB, int KW, int RULE>
 static int launch_few(const ChunkArgs& a, hipStream_t stream) {
   if (a.kpool.geometry.page_capacity % kFewTile == 0 && a.kpool.geometry.head_dim == HDP && codes4(a.kpool) && codes4(a.vpool))
     return launch_few_as<HDP, NB, 1, true, true, RULE>(a, stream);
@@ -1731,7 +1759,7 @@ static int launch_few(const ChunkArgs& a, hipStream_t stream) {
                                           : launch_few_as<HDP, NB, KW, true, false, RULE>(a, stream);
 }
 
-template <bool RULE>
+template <int RULE>
 static int launch_all(ChunkArgs a, int32_t n_few, int32_t few_rows, bool units, hipStream_t st) {
   const int hd = a.kpool.geometry.head_dim;
   if (units && n_few) {
