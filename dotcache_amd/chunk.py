@@ -292,8 +292,8 @@ def attend_chunk(pool: DevicePagePool, k_table, v_pool: DevicePagePool | None, v
     elif out.shape != queries.shape or out.dtype != queries.dtype:
         raise ValueError("out must have the queries' shape and dtype")
     q_rows, out_rows = token_rows(queries, "queries", hd, device), token_rows(out, "out", hd, device)
-    if cap is not None and not (0.0 < float(cap) < float("inf")):
-        raise ValueError("cap must be positive, or None for none")
+    if cap is not None and not (0.0 < C.c_float(cap).value < float("inf")):
+        raise ValueError("cap must be positive in fp32, or None for none")
     if slopes is not None and (slopes.shape != (queries.shape[1],) or slopes.dtype != torch.float32 or slopes.device != device
                                or not slopes.is_contiguous()):
         raise ValueError(f"slopes must be contiguous fp32 [{queries.shape[1]}] on {device}")
