@@ -236,6 +236,12 @@ def _check_pools(pool: DevicePagePool, vpool: DevicePagePool) -> None:
         raise ValueError(f"chunk attention takes head_dim up to {MAX_HEAD_DIM}")
 
 
+def _check_slopes(slopes, heads: int, device) -> None:
+    if slopes is not None and (slopes.shape != (heads,) or slopes.dtype != _torch().float32 or slopes.device != device
+                               or not slopes.is_contiguous()):
+        raise ValueError(f"slopes must be contiguous fp32 [{heads}] on {device}")
+
+
 def workspace_bytes(plan: ChunkPlan, head_dim: int) -> int:
     return int(_lib.lib().dc_chunk_workspace_bytes(plan.n_partials, int(head_dim)))
 
@@ -294,9 +300,7 @@ def attend_chunk(pool: DevicePagePool, k_table, v_pool: DevicePagePool | None, v
     q_rows, out_rows = token_rows(queries, "queries", hd, device), token_rows(out, "out", hd, device)
     if cap is not None and not (0.0 < C.c_float(cap).value < float("inf")):
         raise ValueError("cap must be positive in fp32, or None for none")
-    if slopes is not None and (slopes.shape != (queries.shape[1],) or slopes.dtype != torch.float32 or slopes.device != device
-                               or not slopes.is_contiguous()):
-        raise ValueError(f"slopes must be contiguous fp32 [{queries.shape[1]}] on {device}")
+    _check_slopes(slopes, queries.shape[1], device)
     if validate:
         _validate(pool, vpool, k_table, v_table, plan)
     need = workspace_bytes(plan, hd)
@@ -341,6 +345,7 @@ def attend_cached(cache, queries, new: np.ndarray, context: np.ndarray, k_table,
         raise ValueError("q_head_to_kv_head must give every KV head the same number of query heads")
     if mask is not None and not isinstance(mask, ChunkMask):
         raise ValueError("a cache's mask must be a ChunkMask")
+    _check_slopes(slopes, Hq, cache.k_pool.arena.device)  # (ahead of their reordering)
     key = (new.tobytes(), context.tobytes(), torch.cuda.current_stream(queries.device).cuda_stream if queries.is_cuda else 0)
     if cache._chunk_plan is None or cache._chunk_plan[0] != key:
         cache._chunk_plan = (key, {})
