@@ -1,7 +1,7 @@
 // The largest calls of dc_project with 16-bit rows: products of tiles of up to
 // 96 rows by 128 outputs.  Bound by the matrix instructions, so weights are
 // fp16 operands, scale and bias in them (one rounding, 2^-11 of a weight at
-// most), and no sum is touched until the end: 2048 bf16 rows of 3584 x 4608 in 108
+// most, below 2^-14 2^-25), and no sum is touched until the end: 2048 bf16 rows of 3584 x 4608 in 108
 // us, 9 of them the rows' preparation (a library product of dense matrices 66,
 // project_mid_kernel 154).
 #include "dc_project.h"
@@ -25,19 +25,19 @@ struct TileArgs {
 
 __device__ __forceinline__ uint32_t twice(uint32_t h) { return h | (h << 16); }
 
-// Eight weights of a word: (code - zero) s + t in packed fp16 arithmetic, codes
-// as 16 + code first (exact), zero 8 with t = bias + 8 s (one rounding; it is the levels'
-// middle, so small), or 7 and no t.
+// Eight weights of a word in packed fp16 arithmetic: code s + bias, or (code - 7) s.
+// Codes are 16 + code first and whole numbers then, both exact, so that a weight
+// is rounded once, where it is made.
 template <bool AFFINE>
-__device__ __forceinline__ uint4 weights(uint32_t r, h2v s, h2v t) {
+__device__ __forceinline__ uint4 weights(uint32_t r, h2v s, h2v bias) {
   uint4 out;
 #pragma unroll
   for (int i = 0; i < 4; ++i) {
     const uint32_t sh = i == 0 ? r << 6 : i == 1 ? r << 2 : i == 2 ? r >> 2 : r >> 6;
     const h2v c = __builtin_bit_cast(h2v, (sh & 0x03c003c0u) | 0x4c004c00u);
-    constexpr _Float16 zero = AFFINE ? -24.f : -23.f;
+    constexpr _Float16 zero = AFFINE ? -16.f : -23.f;
     const h2v d = c + h2v{zero, zero};
-    (&out.x)[i] = __builtin_bit_cast(uint32_t, AFFINE ? __builtin_elementwise_fma(d, s, t) : d * s);
+    (&out.x)[i] = __builtin_bit_cast(uint32_t, AFFINE ? __builtin_elementwise_fma(d, s, bias) : d * s);
   }
   return out;
 }
@@ -169,7 +169,7 @@ __global__ void __launch_bounds__(256, 2) project_tile_kernel(TileArgs t) {
     const int gr = i * 32 / GS;
     const h2v s = __builtin_bit_cast(h2v, twice(w.s[n][gr * (AFFINE ? 2 : 1)]));
     const h2v bias = __builtin_bit_cast(h2v, twice(w.s[n][AFFINE ? 2 * gr + 1 : 0]));
-    return weights<AFFINE>((&w.w[n].x)[i], s, AFFINE ? __builtin_elementwise_fma(h2v{(_Float16)8.f, (_Float16)8.f}, s, bias) : bias);
+    return weights<AFFINE>((&w.w[n].x)[i], s, bias);
   };
   auto take = [&](const Weights& w, int turn) __attribute__((always_inline)) {
     auto rows_of = [&](int k) { return xt[turn][k % MB][k / MB][lane]; };
