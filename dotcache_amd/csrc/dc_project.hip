@@ -323,35 +323,43 @@ static int waves_of(int64_t blocks, int k_tiles) {
   return blocks * 4 < 4096 && kFewWaves <= k_tiles ? kFewWaves : 4;
 }
 
-// launch(args, grid) for portions of the rows: a launch's second dimension holds
-// 2^16 - 1 blocks of `rows` rows.
+// launch(args, grid) for portions of the rows and outputs, blocks of `rows` x
+// `outputs` of them: a launch holds 2^16 - 1 blocks in its second dimension, and fewer
+// than 2^32 threads in its first (2^22 blocks of 512).  side: scales and biases of an output in a tile.
 template <typename F>
-static int by_rows(const ProjectArgs& a, int item, int outputs, int rows, const char* what, F launch) {
-  const int64_t most = int64_t(rows) * 65535;
-  for (int64_t r = 0; r < a.rows; r += most) {
-    ProjectArgs b = a;
-    b.x = static_cast<const char*>(a.x) + r * a.x_stride * item;
-    b.y = static_cast<char*>(a.y) + r * a.y_stride * item;
-    b.rows = a.rows - r < most ? a.rows - r : most;
-    launch(b, dim3(uint32_t((a.n + outputs - 1) / outputs), uint32_t((b.rows + rows - 1) / rows)));
-    if (int rc = check_hip(hipGetLastError(), what)) return rc;
+static int by_blocks(const ProjectArgs& a, int item, int side, int outputs, int rows, const char* what, F launch) {
+  const int64_t most = int64_t(rows) * 65535, wide = int64_t(outputs) << 22;
+  for (int64_t n = 0; n < a.n; n += wide) {
+    for (int64_t r = 0; r < a.rows; r += most) {
+      ProjectArgs b = a;
+      b.n = int32_t(a.n - n < wide ? a.n - n : wide);
+      b.n_tiles = (b.n + kTileN - 1) / kTileN;
+      b.words = a.words + n / kTileN * a.k_tiles * 64;
+      b.scales = a.scales + n / kTileN * a.k_tiles * 16 * side;
+      b.x = static_cast<const char*>(a.x) + r * a.x_stride * item;
+      b.y = static_cast<char*>(a.y) + (r * a.y_stride + n) * item;
+      b.rows = a.rows - r < most ? a.rows - r : most;
+      launch(b, dim3(uint32_t((b.n + outputs - 1) / outputs), uint32_t((b.rows + rows - 1) / rows)));
+      if (int rc = check_hip(hipGetLastError(), what)) return rc;
+    }
   }
   return DC_OK;
 }
 
 template <int DT>
 static int launch_short(const ProjectArgs& a, int group_size, bool affine, hipStream_t stream) {
-  return by_rows(a, DT == DC_F32 ? 4 : 2, 256, 1, "project_short_kernel launch", [&](const ProjectArgs& b, dim3 grid) {
+  return by_blocks(a, DT == DC_F32 ? 4 : 2, kTileK / group_size * (affine ? 2 : 1), 256, 1, "project_short_kernel launch", [&](const ProjectArgs& b, dim3 grid) {
     hipLaunchKernelGGL((project_short_kernel<DT>), grid, dim3(256), 0, stream, b, group_size, int32_t(affine));
   });
 }
 
 template <int DT, int GS, bool AFFINE>
 static int launch_project(const ProjectArgs& a, hipStream_t stream) {
+  constexpr int side = kTileK / GS * (AFFINE ? 2 : 1);
   if constexpr (DT != DC_F32) {
     auto mid = [&](auto blocks) {
       constexpr int MB = decltype(blocks)::value;
-      return by_rows(a, 2, 64, 16 * MB, "project_mid_kernel launch", [&](const ProjectArgs& b, dim3 grid) {
+      return by_blocks(a, 2, side, 64, 16 * MB, "project_mid_kernel launch", [&](const ProjectArgs& b, dim3 grid) {
         hipLaunchKernelGGL((project_mid_kernel<DT, GS, AFFINE, MB>), grid, dim3(512), 0, stream, b);
       });
     };
@@ -359,7 +367,7 @@ static int launch_project(const ProjectArgs& a, hipStream_t stream) {
     if (a.rows > 32) return mid(std::integral_constant<int, 3>{});
     if (a.rows > 16) return mid(std::integral_constant<int, 2>{});
   }
-  return by_rows(a, DT == DC_F32 ? 4 : 2, 16, 16, "project_few_kernel launch", [&](const ProjectArgs& b, dim3 grid) {
+  return by_blocks(a, DT == DC_F32 ? 4 : 2, side, 16, 16, "project_few_kernel launch", [&](const ProjectArgs& b, dim3 grid) {
     hipLaunchKernelGGL((project_few_kernel<DT, GS, AFFINE>), grid, dim3(64 * waves_of(int64_t(grid.x) * grid.y, a.k_tiles)), 0, stream, b);
   });
 }

@@ -47,69 +47,72 @@ __device__ __forceinline__ uint4 weights(uint32_t r, h2v s, h2v bias) {
 // Rows as the tiles' kernel takes them: fp16, whole tiles long, bf16 rows
 // divided by the power of two that brings their largest finite value to 2^14 .. 2^15 (what
 // fp16 then drops is below 2^-39 of it).
+constexpr int64_t kPrepareBlocks = 1 << 20;  // (a launch has fewer than 2^32 threads in a dimension)
 template <int DT>
 __global__ void __launch_bounds__(256) project_prepare_kernel(ProjectArgs a, uint16_t* out, int32_t* exps) {
-  // a block per row, eight inputs a thread, up to kRounds loads under way at once
+  // a block per row (and further ones in turn), eight inputs a thread, up to kRounds loads under way at once
   constexpr int kRounds = 4;
   __shared__ float tops[4];
-  const int64_t r = blockIdx.x;
   const int width = a.k_tiles * kTileK;
-  const uint16_t* const row = static_cast<const uint16_t*>(a.x) + r * a.x_stride;
   struct Inputs {
     uint16_t h[8];
   };
-  auto load = [&](int k) {  // (of the row's last ones where it ends sooner)
-    Inputs x;
-    __builtin_memcpy(x.h, __builtin_assume_aligned(row + min(k, a.k - 8), 2), 16);
-    return x;
-  };
-  int e = 0;
-  if constexpr (DT == DC_BF16) {
-    float top = 0.f;
-    for (int k = 8 * int(threadIdx.x); k < a.k; k += kRounds * 2048) {
+  for (int64_t r = blockIdx.x; r < a.rows; r += gridDim.x) {  // (uniform)
+    const uint16_t* const row = static_cast<const uint16_t*>(a.x) + r * a.x_stride;
+    auto load = [&](int k) {  // (of the row's last ones where it ends sooner)
+      Inputs x;
+      __builtin_memcpy(x.h, __builtin_assume_aligned(row + min(k, a.k - 8), 2), 16);
+      return x;
+    };
+    int e = 0;
+    if constexpr (DT == DC_BF16) {
+      float top = 0.f;
+      for (int k = 8 * int(threadIdx.x); k < a.k; k += kRounds * 2048) {
+        Inputs x[kRounds];
+#pragma unroll
+        for (int j = 0; j < kRounds; ++j) x[j] = load(k + 2048 * j);
+#pragma unroll
+        for (int j = 0; j < kRounds; ++j)
+#pragma unroll
+          for (int i = 0; i < 8; ++i) {
+            const float v = fabsf(__builtin_bit_cast(float, uint32_t(x[j].h[i]) << 16));
+            top = __builtin_isfinite(v) ? fmaxf(top, v) : top;
+          }
+      }
+#pragma unroll
+      for (int d = 1; d < 64; d <<= 1) top = fmaxf(top, __shfl_xor(top, d));
+      if (threadIdx.x % 64 == 0) tops[threadIdx.x / 64] = top;
+      __syncthreads();
+      top = fmaxf(fmaxf(tops[0], tops[1]), fmaxf(tops[2], tops[3]));
+      e = top > 0.f ? __builtin_amdgcn_frexp_expf(top) - 15 : 0;  // (frexp: top in [2^(e - 1), 2^e))
+      if (threadIdx.x == 0) exps[r] = e;
+    }
+    for (int k = 8 * int(threadIdx.x); k < width; k += kRounds * 2048) {
       Inputs x[kRounds];
 #pragma unroll
       for (int j = 0; j < kRounds; ++j) x[j] = load(k + 2048 * j);
 #pragma unroll
-      for (int j = 0; j < kRounds; ++j)
+      for (int j = 0; j < kRounds; ++j) {
+        const int at = k + 2048 * j;
+        if (at >= width) break;
+        Inputs y = x[j];
+        if (at + 8 > a.k) {  // (moved to their place, those behind the row's end 0)
 #pragma unroll
-        for (int i = 0; i < 8; ++i) {
-          const float v = fabsf(__builtin_bit_cast(float, uint32_t(x[j].h[i]) << 16));
-          top = __builtin_isfinite(v) ? fmaxf(top, v) : top;
+          for (int i = 0; i < 8; ++i) {
+            y.h[i] = 0;
+#pragma unroll
+            for (int l = i; l < 8; ++l) y.h[i] = at + i == a.k - 8 + l ? x[j].h[l] : y.h[i];
+          }
         }
-    }
+        if constexpr (DT == DC_BF16) {
 #pragma unroll
-    for (int d = 1; d < 64; d <<= 1) top = fmaxf(top, __shfl_xor(top, d));
-    if (threadIdx.x % 64 == 0) tops[threadIdx.x / 64] = top;
-    __syncthreads();
-    top = fmaxf(fmaxf(tops[0], tops[1]), fmaxf(tops[2], tops[3]));
-    e = top > 0.f ? __builtin_amdgcn_frexp_expf(top) - 15 : 0;  // (frexp: top in [2^(e - 1), 2^e))
-    if (threadIdx.x == 0) exps[r] = e;
-  }
-  for (int k = 8 * int(threadIdx.x); k < width; k += kRounds * 2048) {
-    Inputs x[kRounds];
-#pragma unroll
-    for (int j = 0; j < kRounds; ++j) x[j] = load(k + 2048 * j);
-#pragma unroll
-    for (int j = 0; j < kRounds; ++j) {
-      const int at = k + 2048 * j;
-      if (at >= width) break;
-      Inputs y = x[j];
-      if (at + 8 > a.k) {  // (moved to their place, those behind the row's end 0)
-#pragma unroll
-        for (int i = 0; i < 8; ++i) {
-          y.h[i] = 0;
-#pragma unroll
-          for (int l = i; l < 8; ++l) y.h[i] = at + i == a.k - 8 + l ? x[j].h[l] : y.h[i];
+          for (int i = 0; i < 8; ++i)
+            y.h[i] = __builtin_bit_cast(uint16_t, _Float16(__builtin_amdgcn_ldexpf(__builtin_bit_cast(float, uint32_t(y.h[i]) << 16), -e)));
         }
+        *reinterpret_cast<uint4*>(out + r * width + at) = __builtin_bit_cast(uint4, y);
       }
-      if constexpr (DT == DC_BF16) {
-#pragma unroll
-        for (int i = 0; i < 8; ++i)
-          y.h[i] = __builtin_bit_cast(uint16_t, _Float16(__builtin_amdgcn_ldexpf(__builtin_bit_cast(float, uint32_t(y.h[i]) << 16), -e)));
-      }
-      *reinterpret_cast<uint4*>(out + r * width + at) = __builtin_bit_cast(uint4, y);
     }
+    if (r + gridDim.x < a.rows) __syncthreads();  // (the next row writes tops)
   }
 }
 
@@ -308,17 +311,12 @@ int launch_project_tile(const ProjectArgs& a, int32_t dtype, int group_size, boo
     const int64_t width = int64_t(a.k_tiles) * kTileK;
     uint16_t* const rows = static_cast<uint16_t*>(workspace);
     int32_t* const exps = dtype == DC_BF16 ? reinterpret_cast<int32_t*>(rows + a.rows * width) : nullptr;
-    for (int64_t r = 0; r < a.rows; r += 1 << 30) {
-      ProjectArgs b = a;
-      b.x = static_cast<const uint16_t*>(a.x) + r * a.x_stride;
-      b.rows = a.rows - r < (1 << 30) ? a.rows - r : 1 << 30;
-      const dim3 grid(uint32_t(b.rows));
-      if (dtype == DC_BF16)
-        hipLaunchKernelGGL((project_prepare_kernel<DC_BF16>), grid, dim3(256), 0, stream, b, rows + r * width, exps + r);
-      else
-        hipLaunchKernelGGL((project_prepare_kernel<DC_F16>), grid, dim3(256), 0, stream, b, rows + r * width, nullptr);
-      if (int rc = check_hip(hipGetLastError(), "project_prepare_kernel launch")) return rc;
-    }
+    const dim3 grid(uint32_t(a.rows < kPrepareBlocks ? a.rows : kPrepareBlocks));
+    if (dtype == DC_BF16)
+      hipLaunchKernelGGL((project_prepare_kernel<DC_BF16>), grid, dim3(256), 0, stream, a, rows, exps);
+    else
+      hipLaunchKernelGGL((project_prepare_kernel<DC_F16>), grid, dim3(256), 0, stream, a, rows, nullptr);
+    if (int rc = check_hip(hipGetLastError(), "project_prepare_kernel launch")) return rc;
     t.p.x = rows;
     t.p.x_stride = width;
     t.exps = exps;
