@@ -148,8 +148,9 @@ def _group_size(group_size) -> int:
 
 
 def _check_levels(scales, biases) -> None:
-    top = (scales.float() * 7).abs() if biases is None else \
-        _torch().maximum(biases.float().abs(), (scales.float() * 15 + biases.float()).abs()).maximum((scales.float() * 15).abs())
+    """Every level is one that fp16 holds (those between lie within the outer two)."""
+    s = scales.float()
+    top = (s * 7).abs() if biases is None else _torch().maximum(biases.float().abs(), (s * 15 + biases.float()).abs())
     if not float(top.max()) <= 65504.0:
         raise ValueError("a weight's scales, biases and levels must lie in fp16's range")
 

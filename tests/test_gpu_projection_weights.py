@@ -78,3 +78,28 @@ def test_single_weights_of_small_calls(M, dtype):
         off = biases.double().cpu().numpy().T[g] - 16 * s if affine else -23 * s
         bound = 2.0 ** -24 * (31 * np.abs(s) + 2 * np.abs(off) + np.abs(want)) + half * np.abs(want) + 2.0 ** -25 * (dtype == "f16")
         assert np.all(np.abs(got - want) <= bound * (1 + 2.0 ** -10)), float(np.max(np.abs(got - want) / bound))
+
+
+@pytest.mark.parametrize("M", [3, 40, 1152])
+def test_levels_at_the_ends_of_fp16(M):
+    """Levels within fp16's range, of scales that 15 times leave it."""
+    import torch
+
+    from dotcache_amd.projection import GroupedWeight, project
+
+    K, N, gs = 128, 1100, 32
+    r = np.random.default_rng(M)
+    codes = r.integers(0, 16, size=(N, K))
+    flip = r.choice([-1.0, 1.0], size=(N, 4))
+    scales, biases = (flip * r.uniform(8000, 8700, size=(N, 4))).astype(np.float16), (flip * -65504.0).astype(np.float16)
+    g = np.arange(K) // gs
+    dense = codes * scales.astype(np.float64)[:, g] + biases.astype(np.float64)[:, g]
+    assert np.all(np.abs(dense) <= 65504) and np.any(np.abs(15 * scales.astype(np.float64)) > 65504)
+    w = GroupedWeight.from_codes(*(torch.from_numpy(x).cuda() for x in (codes.astype(np.uint8), scales, biases)), group_size=gs)
+    x = torch.zeros(M, K, device="cuda", dtype=torch.float16)
+    at = np.arange(M) % K
+    x[torch.arange(M, device="cuda"), torch.from_numpy(at).cuda()] = 0.5
+    got = project(x, w).double().cpu().numpy()
+    want = 0.5 * dense.T[at]
+    # fp16's rounding of a weight (many rows) and of the output, half a step each; sums of 31 scale in fp32 (a few rows)
+    assert np.all(np.abs(got - want) <= 2.0 ** -10 * np.abs(want) + 8700 * 40 * 2.0 ** -23)
