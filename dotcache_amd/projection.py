@@ -77,13 +77,13 @@ class GroupedWeight:
         _check_levels(scales, biases)
         most = 15 if biases is not None else 14
         data = _new_data(N, K, gs, biases is not None, codes.device)
-        # rows in portions: a portion's codes are widened to 32 bits
+        # rows in portions: a portion's codes are widened (to 64 bits for their check, so that none wraps into the range)
         step = max(_TILE_N, (1 << 24) // K // _TILE_N * _TILE_N)
         for r in range(0, N, step):
-            part = codes[r: r + step].to(torch.int32)
+            part = codes[r: r + step].to(torch.int64)
             if int(part.min()) < 0 or int(part.max()) > most:
                 raise ValueError(f"codes must lie in [0, {most}]")
-            part = torch.nn.functional.pad(part, (0, -K % _TILE_K, 0, -part.shape[0] % _TILE_N))
+            part = torch.nn.functional.pad(part.to(torch.int32), (0, -K % _TILE_K, 0, -part.shape[0] % _TILE_N))
             _put(data, N, K, gs, r, part.unflatten(-1, (-1, 8)), scales[r: r + step], None if biases is None else biases[r: r + step])
         return cls(data, N, K, gs, biases is not None)
 
