@@ -37,12 +37,24 @@ def _torch():
 class GroupedWeight:
     """A weight matrix of 4-bit codes on the device, in the order in which the
     kernels read it (``dc_grouped_weight``).  :meth:`quantize` makes it from a
-    dense matrix, :meth:`from_codes` from a checkpoint's codes."""
+    dense matrix, :meth:`from_codes` from a checkpoint's codes, and the class
+    itself from the ``data`` of another (a saved one's, or moved to another device)."""
 
     def __init__(self, data, outputs: int, inputs: int, group_size: int, affine: bool):
-        self.data, self.outputs, self.inputs = data, int(outputs), int(inputs)
-        self.group_size, self.affine = int(group_size), bool(affine)
-        self._c = _lib.GroupedWeight(data.data_ptr(), self.outputs, self.inputs, self.group_size, int(self.affine))
+        outputs, inputs, gs = int(outputs), int(inputs), _group_size(group_size)
+        need = int(_lib.lib().dc_grouped_weight_bytes(outputs, inputs, gs, int(bool(affine)), None))
+        if need < 0:
+            raise ValueError("a weight needs outputs and inputs, 2^30 of each at most")
+        if data.dtype != _torch().uint8 or data.dim() != 1 or data.numel() != need or not data.is_contiguous() or data.data_ptr() % 16:
+            raise ValueError(f"a weight's data must be {need} contiguous bytes, 16-byte aligned")
+        self._data, self.outputs, self.inputs = data, outputs, inputs
+        self.group_size, self.affine = gs, bool(affine)
+        self._c = _lib.GroupedWeight(data.data_ptr(), outputs, inputs, gs, int(self.affine))
+
+    @property
+    def data(self):
+        """uint8, the bytes of ``dc_grouped_weight`` (read only: the calls keep its address)."""
+        return self._data
 
     @property
     def shape(self) -> tuple[int, int]:
