@@ -120,7 +120,10 @@ class GroupedWeight:
         with torch.cuda.device(weight.device):
             for r in range(0, N, step):
                 # every group as a row of its own, one page after another
-                rows = torch.nn.functional.pad(weight[r: r + step], (0, -K % gs)).reshape(-1, gs)
+                part = weight[r: r + step]
+                if not bool(torch.isfinite(part).all()):
+                    raise ValueError("quantize: the weight must be finite")
+                rows = torch.nn.functional.pad(part, (0, -K % gs)).reshape(-1, gs)
                 n, pages = rows.shape[0], -(-rows.shape[0] // P)
                 pool = DevicePagePool(PoolGeometry(gs, gs, P), device=weight.device, reserve_pages=pages,
                                       reserve_bytes=pages * _lib.page_blob_bytes(*fmt, _lib.geometry(gs, gs, P)))
