@@ -287,8 +287,13 @@ __device__ __forceinline__ void shape_scores(const ChunkArgs& a, float c, const 
   }
 }
 
-// The item's gap: its tiles leave out tokens [x, y).
-__device__ __forceinline__ int2 item_gap(const ChunkArgs& a, uint32_t item) { return a.gaps ? a.gaps[item] : int2{-1, -1}; }
+// The item's gap: its tiles leave out tokens [x, y).  One that does not lie inside
+// the item is none (a fault guard, as chunk_item_ok: the tiles' loop has to
+// end), and costs time only, since ranges say what a row sees.
+__device__ __forceinline__ int2 item_gap(const ChunkArgs& a, const dc_chunk_item& it, uint32_t item) {
+  const int2 g = a.gaps ? a.gaps[item] : int2{-1, -1};
+  return g.x > it.kv_begin && g.y > g.x && g.y < it.kv_end ? g : int2{-1, -1};
+}
 
 }  // namespace
 
@@ -328,7 +333,7 @@ __global__ void __launch_bounds__(256, sizeof(T) == 4 && HDP == 256 ? 1 : 2) att
     rule = row_rule(a, it, has_row, tok, head);
     mine = sight_of(a, it, it.row_begin + 32 * wave, min(it.row_begin + 32 * wave + 32, it.row_end));
     all = sight_of(a, it, it.row_begin, it.row_end);
-    gap = item_gap(a, block_index(kChunkRows / 128));
+    gap = item_gap(a, it, block_index(kChunkRows / 128));
   }
   auto seen = [&](int u) { return RULE ? rule.sees(u) : u <= sees; };
 
@@ -812,7 +817,7 @@ __global__ void __launch_bounds__(512, 2) attend_chunk16_kernel(ChunkArgs a) {
   Sight mine, all;  // the wavefront's rows' and the block's
   int gap_tile = INT32_MAX, gap_len = 0;
   if constexpr (RULE) {
-    const int2 gap = item_gap(a, block_index(CS));
+    const int2 gap = item_gap(a, it, block_index(CS));
     if (gap.x >= 0) gap_tile = (gap.x - it.kv_begin) / KT, gap_len = gap.y - gap.x;
   }
   auto seen = [&](int u) { return RULE ? rule.sees(u) : u <= sees; };
@@ -1202,7 +1207,7 @@ __global__ void __launch_bounds__(64 * kFewWaves, 2) attend_few_kernel(ChunkArgs
   int gap_tile = INT32_MAX, gap_len = 0;
   if constexpr (RULE) {
     all = sight_of(a, it, it.row_begin, it.row_end);
-    const int2 gap = item_gap(a, blockIdx.x);
+    const int2 gap = item_gap(a, it, blockIdx.x);
     if (gap.x >= 0) gap_tile = (gap.x - it.kv_begin) / kFewTile, gap_len = gap.y - gap.x;
   }
   h8v q[QL ? 1 : NB][QL ? 1 : KS];
