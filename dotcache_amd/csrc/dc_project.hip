@@ -316,9 +316,9 @@ __global__ void __launch_bounds__(256) project_short_kernel(ProjectArgs a, int32
   store_y<DT>(a.y, r * a.y_stride + out, fmaf(s, sum, b * xs));
 }
 
-// Wavefronts per block of project_few_kernel: where blocks of four leave the
-// card's 1024 SIMDs less than four wavefronts each, kFewWaves, but none without a
-// tile (16 leave a compute unit one block: one row of 3584 x 4608 7.4 us, 8 6.2).
+// Wavefronts per block of project_few_kernel: kFewWaves where blocks of four leave
+// the card's 1024 SIMDs less than four wavefronts each and there is a tile for each, else
+// four (16 leave a compute unit one block: one row of 3584 x 4608 7.4 us, 8 6.2).
 static int waves_of(int64_t blocks, int k_tiles) {
   return blocks * 4 < 4096 && kFewWaves <= k_tiles ? kFewWaves : 4;
 }

@@ -214,7 +214,7 @@ __global__ void __launch_bounds__(256, 2) project_tile_kernel(TileArgs t) {
     step(kt + 1, odd, even);
     if (kt + 2 >= a.k_tiles) break;
   }
-  // Out by LDS, so that a row's 64 outputs leave in one piece.
+  // Out by LDS, so that a wavefront's 32 outputs of a row leave in one piece.
   uint16_t* const turned = reinterpret_cast<uint16_t*>(&xt[0][0][0][0]) + wave * (16 * kOutRow);
   const int out0 = n0 * kTileN;
 #pragma unroll
