@@ -257,7 +257,7 @@ __device__ __forceinline__ void shape_scores(const ChunkArgs& a, float c, const 
   if constexpr (CAP) {
     // (factors of its own: products common to both branches would be taken ahead of them, into registers)
     float cap = a.cap, cap_in = a.cap_in;
-    asm volatile("" : "+s"(cap), "+s"(cap_in));
+    asm("" : "+s"(cap), "+s"(cap_in));
     if (!EXACT && cap <= kCoarseCap * kLog2e) {  // (uniform)
 #pragma unroll
       for (int i = 0; i < N; ++i)
@@ -269,7 +269,7 @@ __device__ __forceinline__ void shape_scores(const ChunkArgs& a, float c, const 
 #pragma unroll
         for (int v = 0; v < W; ++v) {
           s[i][v] = capped(a, a.cap_in * s[i][v]);
-          if (v % 4 == 3) __builtin_amdgcn_sched_barrier(0);  // (four at a time, for the registers)
+          if (N * W > 16 && v % 4 == 3) __builtin_amdgcn_sched_barrier(0);  // (four at a time, where the registers are short)
         }
     }
   } else {
@@ -1180,7 +1180,10 @@ __device__ __forceinline__ uint32_t zero_of(int kind, bool affine) {
 // KW 1 is for pools of 4-bit codes in groups of 32 (and fp16 pages between them):
 // a token's scales lie side by side, and are one load.  The loads' issue is half of
 // a long range's time, so what counts is how few they are: a decode of 8
-// sequences of 32768 tokens at head_dim 256, 336 MB, 172 -> 131 us.
+// sequences of 32768 tokens at head_dim 256, 336 MB, 172 -> 131 us.  Where such
+// pools hold fp16 pages for the most part, those are read where they are used: 8
+// sequences of 16384 tokens, keys and values both fp16, 34 -> 38 us at head_dim 64 and 56 -> 60
+// at 128, but 151 -> 115 at 256; with one of the two in 4 bits 43 -> 44, 50 -> 48 at 128.
 template <int HDP, int NB, int KW, bool UNI, bool WHOLE, int RULE>
 __global__ void __launch_bounds__(64 * kFewWaves, 2) attend_few_kernel(ChunkArgs a) {
   constexpr int CH = HDP / 8, KS = HDP / 32, CB = HDP / 16, TILE = kFewTile * HDP * 2;
