@@ -55,17 +55,18 @@ def _whole(x, name: str, least: int) -> int:
 
 @dataclass(frozen=True)
 class ChunkMask:
-    """Which tokens of its sequence a token attends: those u that are not
+    """Which tokens of its sequence a token i attends: those u that are not
     behind it (u <= i), or in the sequence's first ``prefix`` tokens with it,
 
     * of its own document (``documents``: for each sequence where its documents
       begin, ascending from 0; None: one document each),
-    * among the last ``window`` tokens up to itself or, of its document, the
-      first ``sinks`` (None: no window).
+    * not ``window`` tokens or more ahead of it (u > i - window: up to itself the
+      last ``window``), or among its document's first ``sinks`` (None: no window).
 
     ``prefix`` is a number for all sequences or one for each; its tokens see
-    each other both ways, so a chunk that ends inside it belongs to no complete
-    prompt and is refused.  Equal masks compare equal."""
+    each other both ways (those behind a token at any distance, a window or not),
+    so a chunk that ends inside it belongs to no complete prompt and is refused.
+    Equal masks compare equal."""
     window: int | None = None
     sinks: int = 0
     prefix: int | tuple | None = None
@@ -264,17 +265,19 @@ def attend_chunk(pool: DevicePagePool, k_table, v_pool: DevicePagePool | None, v
     2^-25 they are zeros.  With fp32 queries everything is fp32.  ``query_scale``
     may have either sign, or be 0.  ``cap`` (positive; None: none) and ``slopes``
     (fp32 device ``[Hq]``, any sign; None: none) shape the scores in fp32, in that
-    order, before the mask.  ``workspace``: uint8, :func:`workspace_bytes`
-    at least, 16-byte aligned, not shared by calls that may overlap (default: one
-    of its own).  ``validate`` reads the tables back and checks them against the
+    order, before the mask; a capped score is off by about 2^-21 of itself, or,
+    with 16-bit queries and a cap up to 256, of the cap.  No gradient flows through
+    the call.  ``workspace``: uint8, :func:`workspace_bytes` at least, 16-byte
+    aligned, not shared by calls that may overlap (default: one of its own).  ``validate`` reads the tables back and checks them against the
     pools (the kernel itself leaves out, and never reads, what a table does not
     name).
 
     The kernel follows from the formats that the pools have ever held.  Once a
     pool has taken a 2- or 3-bit, int8 or fp32 page (a cache's tail, by
     ``escape_dtype``), 16-bit queries take the general kernel, two to six times
-    as long; and a captured call is captured anew once a pool takes pages of a
-    format that it had not."""
+    as long (decodes of long contexts at head_dim 256: fifteen times); and a
+    captured call is captured anew once a pool takes pages of a format that it
+    had not."""
     torch = _torch()
     vpool = pool if v_pool is None else v_pool
     _check_pools(pool, vpool)

@@ -42,8 +42,8 @@
 // A tile's products are turned into exponents (cap, slope) where they lie, then
 // masked; a tile that no row of a wavefront sees is none of its work, one that all see
 // whole has no mask.  A cap costs 11 % (2 x 2048 rows at head_dim 256, window
-// 4096: 749 -> 834 us), slopes 25 % (1024 rows of 4096 tokens at head_dim 64: 77
-// -> 97).
+// 4096: 737 -> 822 us), slopes 25 % (1024 rows of 4096 tokens at head_dim 64: 77
+// -> 95).
 #pragma once
 
 #include <atomic>
@@ -242,7 +242,7 @@ __device__ __forceinline__ float capped(const ChunkArgs& a, float x) {
 
 // The second form alone, for 16-bit queries and caps to kCoarseCap: off by 2^-21 of the cap
 // whatever the score, so a weight by 2^-13, where its own rounding to fp16 and those
-// of its logit's operands are 2^-11 each (2 x 2048 rows at head_dim 256, window 4096: 826 us, the other 945).
+// of its logit's operands are 2^-11 each (2 x 2048 rows at head_dim 256, window 4096: 822 us, the other 935).
 constexpr float kCoarseCap = 256.f;
 __device__ __forceinline__ float capped_coarse(float cap, float x) {
   return fmaf(-2.f * cap, __builtin_amdgcn_rcpf(__builtin_amdgcn_exp2f(x) + 1.f), cap);

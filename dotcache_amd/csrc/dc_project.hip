@@ -10,7 +10,7 @@
 // in fp32.  Nothing is rounded before the output.  fp32 rows are three bf16
 // parts each, whose sum they are.
 //
-// By rows: project_few_kernel to 16 (one row of 3584 x 4608, 9.3 MB, 5.5 us; a launch
+// By rows: project_few_kernel to 16 (one row of 3584 x 4608, 9.3 MB, 5.9 us; a launch
 // with no work 4.2), project_mid_kernel beyond (48 rows of 4096 x 16384, 38 MB, 21
 // us; with the few rows' kernel 59), project_tile_kernel (dc_project_tile.hip)
 // where its rounds of blocks end first.
@@ -318,7 +318,7 @@ __global__ void __launch_bounds__(256) project_short_kernel(ProjectArgs a, int32
 
 // Wavefronts per block of project_few_kernel: kFewWaves where blocks of four leave
 // the card's 1024 SIMDs less than four wavefronts each and there is a tile for each, else
-// four (16 leave a compute unit one block: one row of 3584 x 4608 7.4 us, 8 6.2).
+// four (16 leave a compute unit one block: one row of 3584 x 4608 7.4 us, 8 5.9).
 static int waves_of(int64_t blocks, int k_tiles) {
   return blocks * 4 < 4096 && kFewWaves <= k_tiles ? kFewWaves : 4;
 }

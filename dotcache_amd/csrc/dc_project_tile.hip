@@ -1,8 +1,8 @@
 // The largest calls of dc_project with 16-bit rows: products of tiles of up to
 // 96 rows by 128 outputs.  Bound by the matrix instructions, so weights are
 // fp16 operands, scale and bias in them (one rounding, 2^-11 of a weight at
-// most, below 2^-14 2^-25), and no sum is touched until the end: 2048 bf16 rows of 3584 x 4608 in 108
-// us, 9 of them the rows' preparation (a library product of dense matrices 66,
+// most, below 2^-14 2^-25), and no sum is touched until the end: 2048 bf16 rows of 3584 x 4608 in 107
+// us, 10 of them the rows' preparation (a library product of dense matrices 66,
 // project_mid_kernel 154).
 #include "dc_project.h"
 

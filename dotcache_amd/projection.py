@@ -10,9 +10,13 @@ the levels of the caches' pages:
     W = scale * (code - 7)           (symmetric, codes 0 .. 14)
 
 Codes, rows and their products are exact as matrix operands and sums are fp32,
-so an output is rounded once, to the rows' type; calls of many 16-bit rows, bound by
+so an output is rounded once, to the rows' type.  Calls of many 16-bit rows, bound by
 the matrix instructions and not by the weights' bytes, round each weight to fp16
-besides.  The reference leaves these
+besides (once, 2^-11): those of more than 64 rows for which the tiles' kernel, by rows
+and outputs, is done first.  So fp16 rows among hundreds are less precise than
+alone: off by 2.8e-4 of their size instead of the output's own rounding, 2.1e-4 (bf16
+1.67e-3 instead of 1.66e-3).  For inference: no gradient flows through a
+product.  The reference leaves these
 products to its models (reference ``dotcache/integrations/llama.py:345-358``,
 ``:476-481``); its levels are those of ``dotcache/modes/m0_affine.py:15-90``.
 """
@@ -212,7 +216,9 @@ def project(x, weight: GroupedWeight, *, out=None, workspace=None):
     elements contiguous) times the weight's transpose: ``[..., outputs]`` in the
     same type.  ``out`` (two-dimensional like ``x``, rows at any stride that does
     not overlap) receives it instead; it must not overlap ``x``.  An infinity or
-    NaN in a row makes that row's outputs infinities or NaN.  ``workspace``: uint8,
+    NaN in a row makes that row's outputs infinities or NaN; so may finite values
+    so large that 31 times their sum over a group, or that times the scale, leaves
+    fp32 (from 2^115 on, at scales up to 1).  ``workspace``: uint8,
     :func:`workspace_bytes` at least, 16-byte aligned, not shared by calls that may
     overlap (default: one of its own where a call needs it)."""
     shape = x.shape

@@ -622,6 +622,8 @@ int dc_attend_chunk(dc_pool k_pool, dc_pool v_pool, const int32_t* k_table, cons
  * shaped.  A score is s = query_scale q . k; then, with a cap, s = cap tanh(s /
  * cap); then, with slopes, s -= slopes[query head] |i - u| for token i of a
  * sequence and the token u that it attends.
+ * (A capped score is off by about 2^-21 of itself; with 16-bit queries and a cap
+ * up to 256, of the cap.)
  *   ranges : device int32 [n_tokens][4] {first, end, first, end}, 16-byte
  *            aligned: new token t attends tokens [0], .. [1] - 1 and [2], .. [3] - 1
  *            of its sequence (the ranges do not overlap; empty ones: a row of
@@ -629,7 +631,7 @@ int dc_attend_chunk(dc_pool k_pool, dc_pool v_pool, const int32_t* k_table, cons
  *   gaps   : device int32 [n_items][2] beside the items, as
  *            dc_plan_chunk_ranges wrote them, 8-byte aligned.  NULL: none. */
 typedef struct dc_score_rule {
-  float cap;           /* 0: none                                       */
+  float cap;           /* 0: none; else positive                        */
   const float* slopes; /* device fp32 [n_kv_heads * n_q]; NULL: none    */
   const int32_t* ranges;
   const int32_t* gaps;
@@ -696,10 +698,12 @@ int64_t dc_project_workspace_bytes(dc_grouped_weight weight, int32_t dtype, int6
 /* y[m] = x[m] W^T for `rows` rows x [inputs] and y [outputs] of one dtype
  * (DC_F32, DC_F16, DC_BF16), sums in fp32, one rounding to y.  y must not
  * overlap x.  Calls of many 16-bit rows round each weight to fp16 (levels past
- * +-65504 overflow, those below 2^-14 lose bits); the others multiply by the codes as they are.  An infinity or NaN among a
- * row's inputs gives infinities or NaN in all of that row's outputs, and only
- * there.  workspace: dc_project_workspace_bytes at least, 16-byte aligned, not
- * shared by calls that may overlap.  A weight's levels are those of reference
+ * +-65504 overflow, those below 2^-14 lose bits); the others multiply by the
+ * codes as they are.  An infinity or NaN among a row's inputs gives infinities or
+ * NaN in all of that row's outputs, and only there; so may finite values from 2^115
+ * on (at scales up to 1), since a group's sum of (16 + code) x and its product
+ * with the scale are fp32.  workspace: dc_project_workspace_bytes at least, 16-byte
+ * aligned, not shared by calls that may overlap.  A weight's levels are those of reference
  * dotcache/modes/m0_affine.py:15-90; the reference leaves the products around
  * the cache to its models (dotcache/integrations/llama.py:345-358, :476-481). */
 int dc_project(dc_grouped_weight weight, dc_matrix_rows x, dc_matrix_rows y, int64_t rows, void* workspace,
