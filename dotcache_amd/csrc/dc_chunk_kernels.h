@@ -234,8 +234,8 @@ __device__ __forceinline__ Sight sight_of(const ChunkArgs& a, const dc_chunk_ite
 // cap (1 - 2 / (exp2(|x|) + 1)) with the sign, which holds at either infinity and cancels little.
 __device__ __forceinline__ float capped(const ChunkArgs& a, float x) {
   const float t = x * x;
-  float near = a.cap * x * fmaf(t, fmaf(t, fmaf(t, fmaf(t, 1.2437525e-06f, -3.1857868e-05f), 6.6630519e-04f), -1.3875948e-02f), 0.34657359f);
-  float far = fmaf(-2.f * a.cap, __builtin_amdgcn_rcpf(__builtin_amdgcn_exp2f(fabsf(x)) + 1.f), a.cap);
+  float near = a.cap * (x * fmaf(t, fmaf(t, fmaf(t, fmaf(t, 1.2437525e-06f, -3.1857868e-05f), 6.6630519e-04f), -1.3875948e-02f), 0.34657359f));
+  float far = a.cap * fmaf(-2.f, __builtin_amdgcn_rcpf(__builtin_amdgcn_exp2f(fabsf(x)) + 1.f), 1.f);  // (2 cap may leave fp32)
   asm volatile("" : "+v"(near), "+v"(far));  // (both, and a selection: no branch for each score)
   return fabsf(x) < 1.44269504f ? near : __builtin_copysignf(far, x);
 }

@@ -96,3 +96,27 @@ def test_one_score_by_itself():
         # slope p (1 - p) of the score's 2^-20; exponential, sum and quotient 2^-22
         bound = want * (1 - want) * 2.0 ** -20 * np.abs(x) + 2.0 ** -21 * want
         assert np.all(np.abs(got - want[:, None]) <= bound[:, None]), (cap, float(np.max(np.abs(got - want[:, None]) / bound[:, None])))
+
+
+def test_caps_and_scores_near_the_end_of_fp32():
+    """Scores of 10^38 under a cap of 2 x 10^38, twice which fp32 does not hold:
+    the token of the largest has all the weight, whatever its score's sign or share of the cap."""
+    import torch
+
+    from dotcache_amd.chunk import attend_chunk, plan_chunk
+    from dotcache_amd.page_pool import DevicePagePool, PoolGeometry
+
+    pools = [DevicePagePool(PoolGeometry(64, 32, 16), reserve_bytes=1 << 16, reserve_pages=16) for _ in range(2)]
+    ids = [p.allocate(0, 0, 1, tokens=4) for p in pools]
+    keys = torch.tensor([0.25, -0.5, 1.0, 0.5], device="cuda")[:, None].expand(4, 64).contiguous()
+    values = torch.arange(1.0, 5.0, device="cuda")[:, None].expand(4, 64).contiguous()
+    for p, i, rows in zip(pools, ids, (keys, values)):
+        p.encode_rows(rows, np.repeat(i, 4).astype(np.int32), np.arange(4, dtype=np.int32))
+    tables = [torch.from_numpy(i.reshape(1, 1, 1).astype(np.int32)).cuda() for i in ids]
+    plan = plan_chunk(*pools, [1], [4], kv_heads=1, q_per_kv=1)
+    for sign, want in ((1.0, 3.0), (-1.0, 2.0)):
+        q = torch.full((1, 1, 64), sign * 2.0 ** 120, device="cuda")
+        # 64 x 2^120 = 2^126 (8.5e37) under the largest key; the scale takes it to a quarter, once and twice that
+        for scale in (0.25, 1.0, 2.0):
+            got = attend_chunk(pools[0], tables[0], pools[1], tables[1], q, plan, query_scale=scale, cap=2e38)
+            assert bool((got == want).all()), (sign, scale, got.flatten()[:4])
