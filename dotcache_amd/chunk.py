@@ -238,8 +238,8 @@ def _check_pools(pool: DevicePagePool, vpool: DevicePagePool) -> None:
 
 
 def _check_slopes(slopes, heads: int, device) -> None:
-    if slopes is not None and (slopes.shape != (heads,) or slopes.dtype != _torch().float32 or slopes.device != device
-                               or not slopes.is_contiguous()):
+    if slopes is not None and (not isinstance(slopes, _torch().Tensor) or slopes.shape != (heads,) or slopes.dtype != _torch().float32
+                               or slopes.device != device or not slopes.is_contiguous()):
         raise ValueError(f"slopes must be contiguous fp32 [{heads}] on {device}")
 
 

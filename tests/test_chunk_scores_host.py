@@ -30,7 +30,7 @@ def test_caps_that_it_holds():
 
 @pytest.mark.parametrize("order", [None, [1, 0, 1, 0]])
 @pytest.mark.parametrize("slopes", [torch.zeros(2 * HQ), torch.zeros(HQ - 1), torch.zeros(HQ, 2)[:, 0], torch.zeros(HQ, dtype=torch.float64),
-                                    torch.zeros(1, HQ), torch.zeros(HQ, device="meta")])
+                                    torch.zeros(1, HQ), torch.zeros(HQ, device="meta"), [0.0] * HQ, np.zeros(HQ, np.float32)])
 def test_slopes_of_a_cache_are_checked_in_any_order_of_heads(slopes, order):
     cache = _paged()
     n = np.array([2], dtype=np.int32)
