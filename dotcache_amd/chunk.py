@@ -168,8 +168,9 @@ def plan_chunk(pool: DevicePagePool, v_pool: DevicePagePool | None, new, context
 
     ``mask``: a :class:`ChunkMask` (None: causal), or int32 ``[tokens, 4]``
     for a mask of another kind: new token t attends tokens ``mask[t, 0] ..
-    mask[t, 1] - 1`` and ``mask[t, 2] .. mask[t, 3] - 1`` of its sequence, empty
-    ranges where the two are equal; a token that attends none gets zeros."""
+    mask[t, 1] - 1`` and ``mask[t, 2] .. mask[t, 3] - 1`` of its sequence (once
+    each, where the two overlap), empty ranges where begin and end are equal; a
+    token that attends none gets zeros."""
     torch = _torch()
     vpool = pool if v_pool is None else v_pool
     _check_pools(pool, vpool)

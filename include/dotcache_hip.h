@@ -626,8 +626,8 @@ int dc_attend_chunk(dc_pool k_pool, dc_pool v_pool, const int32_t* k_table, cons
  * up to 256, of the cap.)
  *   ranges : device int32 [n_tokens][4] {first, end, first, end}, 16-byte
  *            aligned: new token t attends tokens [0], .. [1] - 1 and [2], .. [3] - 1
- *            of its sequence (the ranges do not overlap; empty ones: a row of
- *            zeros).  NULL: itself and all before it.
+ *            of its sequence (once each, where the ranges overlap; both empty: a
+ *            row of zeros).  NULL: itself and all before it.
  *   gaps   : device int32 [n_items][2] beside the items, as
  *            dc_plan_chunk_ranges wrote them, 8-byte aligned.  NULL: none. */
 typedef struct dc_score_rule {
@@ -639,9 +639,9 @@ typedef struct dc_score_rule {
 
 /* dc_plan_chunk where new token t (of all sequences, one after another) attends
  * tokens [ranges[t][0], ranges[t][1]) and [ranges[t][2], ranges[t][3]) of its
- * sequence (host int32, 0 <= first <= end <= the context, apart from each
- * other): a row tile's items cover what its rows attend, in steps of 128 tokens (a
- * first one from a multiple of 32 on).
+ * sequence (host int32, 0 <= first <= end <= the context): a row tile's items
+ * cover what its rows attend, in steps of 128 tokens (a first one from a multiple
+ * of 32 on).
  * An item that takes tokens of two stretches leaves out [gaps[i][0], gaps[i][1])
  * between them ({-1, -1}: nothing left out; host [max_items][2]). */
 int dc_plan_chunk_ranges(const int32_t* new_tokens, const int32_t* context, const int32_t* ranges, int32_t n_seqs,

@@ -92,3 +92,23 @@ def test_calls_repeat_their_bits(dtype):
         first = project(x, w)
         for _ in range(4):
             assert torch.equal(project(x, w), first), M
+
+
+def test_two_streams_at_once():
+    """Calls that overlap have workspaces of their own."""
+    import torch
+
+    from dotcache_amd.projection import project
+
+    cases = [exact_case(M, K, 1100, 64, True, "bf16", M) for M, K in ((1100, 300), (1152, 320), (40, 384))]
+    streams = [torch.cuda.Stream() for _ in cases]
+    for s in streams:
+        s.wait_stream(torch.cuda.current_stream())
+    got = [[] for _ in cases]
+    for _ in range(8):
+        for (x, w, _, _), s, out in zip(cases, streams, got):
+            with torch.cuda.stream(s):
+                out.append(project(x, w))
+    torch.cuda.synchronize()
+    for (_, _, want, _), out in zip(cases, got):
+        assert all(torch.equal(y, want) for y in out)
